@@ -1,0 +1,681 @@
+// k_pattn.hip - attention of one new token per request over a paged key-value cache
+// (qllama_paged_attention; semantics in qserve.h).  No counterpart in the reference,
+// whose decode attention (llama.c:554-576) serves one sequence and one dense cache.
+//
+// The work of a call is the key steps of all (request, KV head, 16 query heads) tiles,
+// laid one behind another; every block takes an equal share of them, whatever the
+// lengths are, so ragged batches and one long request fill the chip alike without the
+// host knowing a length.  A share that ends inside a tile leaves its maximum, sum and
+// weighted values in the workspace, and k_paged_join puts a tile's parts together.
+//
+// A wave keeps its tile's queries, running maximum, sum and outputs in registers and
+// takes a step of 16 or 32 keys at a time straight from the pages: no LDS until its
+// share ends.  S^T = K q^T on the matrix cores puts a query head in a lane's column
+// and 4 keys of each 16 in its rows; the same lane's weights are then the operand of
+// O^T += V^T P^T, whose contraction slots are matched to the keys the lane holds, so
+// weights never move between lanes.  A lane loads whole 16-byte pieces of a value row
+// (16 lanes a row), and the pieces of 8 keys are turned by byte permutes.
+//
+// Precision: float queries and weights meet 16-bit keys and values as parts that add up
+// to them (bf16: three parts of 8 bits, f16: two of 11), one MFMA a part; int8 codes
+// are exact in bf16.  fp32 caches use the fp32 MFMA.  At 8 TB/s the parts take a sixth
+// of the bf16 matrix rate.
+#include <hip/hip_runtime.h>
+
+#include "qserve_host.h"
+
+namespace {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+constexpr int kThreads = 256, kWaves = 4;
+constexpr int kBlocks = 512;          // two blocks of four waves a CU
+constexpr int kMinShare = 4;          // steps a block takes at least: one a wave
+constexpr float kNegInf = -__builtin_inff();
+
+struct PaArgs {
+  const char *k, *v;
+  const float *ks, *vs;
+  const float *q;
+  float *o, *lse;
+  const int *table, *lens;
+  float *part;
+  long long pst, hst, sst;            // bytes
+  long long scp, sch, scs;            // floats
+  long long q_stride, o_stride, lse_stride, table_stride;
+  int n_req, n_heads, n_kv, G, tiles, rows, hd, n_pages, page_size, width;
+  float qscale;                       // scale * log2(e)
+};
+
+__host__ __device__ inline int clamp_len(int len, int width, int page_size) {
+  const int most = width * page_size;   // fits: checked by the host
+  return len < 0 ? 0 : len > most ? most : len;
+}
+
+// Page of token `key` and its place there; -1: no page of the cache, or no token.
+__host__ __device__ inline int page_of(const int *table, long long key, int len, int page_size, int n_pages, int *place) {
+  *place = 0;
+  if (key < 0 || key >= len) return -1;
+  const int e = (int)key / page_size, p = table[e];
+  if (p < 0 || p >= n_pages) return -1;
+  *place = (int)key - e * page_size;
+  return p;
+}
+
+// Sum over the block (256 threads) of one int64 a thread.
+__device__ long long block_sum(long long v, long long *lds) {
+  for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  v = 0;
+  for (int i = 0; i < (int)(blockDim.x >> 6); i++) v += lds[i];
+  __syncthreads();
+  return v;
+}
+
+// Steps of a block's share when all tiles together take `units`.
+__device__ inline long long share_of(long long units) {
+  const long long s = (units + kBlocks - 1) / kBlocks;
+  return s < kMinShare ? kMinShare : s;
+}
+
+// What a part with maximum m counts against the maximum of all.  A part without one holds
+// zeros, or the NaN of its scores, which has to stay.
+__device__ inline float part_weight(float m, float top) { return m == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m - top); }
+
+// max of a lane's value with those of lanes l ^ 16, l ^ 32 and l ^ 48
+__device__ inline float max_groups(float x) {
+  const uint32_t u = __float_as_uint(x);
+  u2 r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  const uint32_t y = __float_as_uint(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)));
+  r = __builtin_amdgcn_permlane16_swap(y, y, false, false);
+  return fmaxf(__uint_as_float(r.x), __uint_as_float(r.y));
+}
+__device__ inline float sum_groups(float x) {
+  x += __shfl_xor(x, 16);
+  return x + __shfl_xor(x, 32);
+}
+
+template <int W>
+__device__ inline void load_words(uint32_t (&d)[W], const char *p) {
+  if constexpr (W == 1) {
+    d[0] = *reinterpret_cast<const uint32_t *>(p);
+  } else if constexpr (W == 2) {
+    const u2 x = *reinterpret_cast<const u2 *>(p);
+    d[0] = x.x; d[1] = x.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < W / 4; i++) {
+      const u4 x = *reinterpret_cast<const u4 *>(p + 16 * i);
+      d[4 * i] = x.x; d[4 * i + 1] = x.y; d[4 * i + 2] = x.z; d[4 * i + 3] = x.w;
+    }
+  }
+}
+// 16 bytes of int8 lie on 8-byte boundaries only
+__device__ inline void load_words_8(uint32_t (&d)[4], const char *p) {
+  const u2 x = *reinterpret_cast<const u2 *>(p), y = *reinterpret_cast<const u2 *>(p + 8);
+  d[0] = x.x; d[1] = x.y; d[2] = y.x; d[3] = y.y;
+}
+
+__device__ inline uint32_t hi16s(uint32_t b, uint32_t a) { return __builtin_amdgcn_perm(b, a, 0x07060302); }
+__device__ inline uint32_t lo16s(uint32_t b, uint32_t a) { return __builtin_amdgcn_perm(b, a, 0x05040100); }
+template <int B>
+__device__ inline float byte_f(uint32_t w) { return (float)(int)(int8_t)(w >> (8 * B)); }
+
+// Parts of a float operand of 8 values: sums of the parts are the values (bf16: 24
+// bits by cutting, f16: 22 by rounding to zero).
+struct Parts3 { u4 p[3]; };
+__device__ inline Parts3 cut3(const float (&x)[8]) {
+  Parts3 r;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    float a = x[2 * i], b = x[2 * i + 1];
+#pragma unroll
+    for (int k = 0; k < 3; k++) {
+      r.p[k][i] = hi16s(__float_as_uint(b), __float_as_uint(a));
+      if (k < 2) {
+        a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u);
+        b -= __uint_as_float(__float_as_uint(b) & 0xffff0000u);
+      }
+    }
+  }
+  return r;
+}
+struct Parts2 { u4 p[2]; };
+__device__ inline Parts2 cut2(const float (&x)[8]) {
+  Parts2 r;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const h2 hi = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(x[2 * i], x[2 * i + 1]));
+    const h2 lo = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(x[2 * i] - (float)hi.x, x[2 * i + 1] - (float)hi.y));
+    r.p[0][i] = __builtin_bit_cast(uint32_t, hi);
+    r.p[1][i] = __builtin_bit_cast(uint32_t, lo);
+  }
+  return r;
+}
+
+template <int T>
+__device__ inline f4 mfma16(u4 a, u4 b, f4 c) {
+  if constexpr (T == QLLAMA_KV_F16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
+}
+
+// What a type and a padded head size fix.
+template <int T, int HDP>
+struct Cfg {
+  static constexpr int ES = T == QLLAMA_KV_F32 ? 4 : T == QLLAMA_KV_I8 ? 1 : 2;
+  static constexpr int SUB = T == QLLAMA_KV_F32 ? 1 : 2;       // 16-key groups of a step
+  static constexpr int STEP = 16 * SUB;
+  static constexpr int CH = HDP / 32;                          // 8-dim pieces of a key that a lane loads
+  static constexpr int KW = 8 * ES / 4;                        // words of such a piece
+  static constexpr int DPL = HDP / 16;                         // dims of a value row that a lane loads
+  static constexpr int VW = DPL * ES / 4;
+  static constexpr int PARTS = T == QLLAMA_KV_F16 ? 2 : 3;
+  // 2^SHIFT times the weights: f16 parts then keep 22 bits down to 2^-18 of the largest
+  // weight and the rest to 2^-40
+  static constexpr float SHIFT = T == QLLAMA_KV_F16 ? 15.0f : 0.0f;
+};
+
+template <int T, int HDP>
+struct KTile { uint32_t w[Cfg<T, HDP>::SUB][Cfg<T, HDP>::CH][Cfg<T, HDP>::KW]; };
+template <int T, int HDP>
+struct VTile { uint32_t w[Cfg<T, HDP>::SUB][4][Cfg<T, HDP>::VW]; };
+
+// Where the keys of a wave's steps lie.  UNI (page_size a multiple of 16): lane l holds
+// the page and place of 16-key group first + l, read from the table 64 groups at a
+// time, and a group's address is uniform.  Otherwise lane l holds those of key first +
+// l and they go to the lanes that load the key.  A page outside the cache is -1.
+template <bool UNI>
+struct Window {
+  int first, page, place;
+  __device__ inline void load(const PaArgs &a, const int *table, int from, int len) {
+    first = from;
+    const int lane = threadIdx.x & 63;
+    const long long key = UNI ? ((long long)from + lane) * 16 : (long long)from + lane;
+    page = page_of(table, key, len, a.page_size, a.n_pages, &place);
+  }
+};
+
+template <int T, int HDP, bool UNI>
+__global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaArgs a) {
+  using C = Cfg<T, HDP>;
+  constexpr int SUB = C::SUB, STEP = C::STEP, CH = C::CH, DPL = C::DPL;
+  extern __shared__ float dyn[];                    // [wave][row][HDP] at the end of a share
+  __shared__ long long sums[kWaves];
+  __shared__ float s_m[kWaves][16], s_l[kWaves][16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int n = lane & 15, g = lane >> 4;           // key or query head or value piece; group of 16 lanes
+  const int tiles = a.n_kv * a.tiles;
+
+  // this block's share of all steps, and the request it begins in
+  long long units = 0;
+  for (int r = threadIdx.x; r < a.n_req; r += kThreads)
+    units += (clamp_len(a.lens[r], a.width, a.page_size) + STEP - 1) / STEP;
+  units = block_sum(units, sums) * tiles;
+  const long long share = share_of(units);
+  long long u = blockIdx.x * share;
+  const long long end = u + share < units ? u + share : units;
+  if (u >= end) return;
+  const long long begin = u;
+  int r = 0, steps;
+  long long r_begin = 0;                            // first unit of request r
+  for (;; r++) {                                    // 64 requests at a time, then one by one
+    long long c = 0;
+    const int i = r + lane;
+    if (i < a.n_req) c = (clamp_len(a.lens[i], a.width, a.page_size) + STEP - 1) / STEP;
+    long long s = c;
+    for (int d = 1; d < 64; d <<= 1) {
+      const long long t = __shfl_up(s, d);
+      if (lane >= d) s += t;
+    }
+    const uint64_t past = __ballot(r_begin + s * tiles > u);
+    if (past) {
+      const int at = __builtin_ctzll(past);
+      r_begin += (__shfl(s, at) - __shfl(c, at)) * tiles;
+      steps = (int)__shfl(c, at);
+      r += at;
+      break;
+    }
+    r_begin += __shfl(s, 63) * tiles;
+    r += 63;
+  }
+
+  while (u < end) {
+    const int len = clamp_len(a.lens[r], a.width, a.page_size);
+    steps = (len + STEP - 1) / STEP;
+    if (u >= r_begin + (long long)steps * tiles) {
+      r_begin += (long long)steps * tiles;
+      r++;
+      continue;
+    }
+    const int tile = (int)((u - r_begin) / steps);
+    const int s0 = (int)(u - r_begin - (long long)tile * steps);
+    const int s1 = (int)(end - u < steps - s0 ? s0 + (end - u) : steps);
+    const int kvh = tile / a.tiles, h0 = kvh * a.G + (tile % a.tiles) * 16;
+    const int rows = a.G - (tile % a.tiles) * 16 < 16 ? a.G - (tile % a.tiles) * 16 : 16;
+    const int *table = a.table + r * a.table_stride;
+    const int from = s0 + (s1 - s0) * wave / kWaves, to = s0 + (s1 - s0) * (wave + 1) / kWaves;
+
+    float m = kNegInf, l = 0.0f;                    // of the lane's query head; l over the lane's keys
+    f4 acc[DPL];
+#pragma unroll
+    for (int c = 0; c < DPL; c++) acc[c] = f4{0, 0, 0, 0};
+
+    if (from < to) {
+      // queries: head h0 + n, dims 32 s + 8 g ..; scaled so that weights are powers of two
+      float qf[CH][8];
+      float qmax = 0.0f;
+      const float *q = a.q + r * a.q_stride + (long long)(h0 + n) * a.hd;
+#pragma unroll
+      for (int s = 0; s < CH; s++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const int d = 32 * s + 8 * g + i;
+          qf[s][i] = n < rows && d < a.hd ? q[d] * a.qscale : 0.0f;
+          qmax = fmaxf(qmax, fabsf(qf[s][i]));
+        }
+      u4 qp[C::PARTS][CH];
+      float unscale = 1.0f;
+      if constexpr (T == QLLAMA_KV_F16) {           // into f16's range, by a power of two
+        qmax = max_groups(qmax);
+        const int e = qmax > 0.0f && qmax < __builtin_inff() ? ilogbf(qmax) : 0;
+        unscale = ldexpf(1.0f, e - 13);
+#pragma unroll
+        for (int s = 0; s < CH; s++) {
+#pragma unroll
+          for (int i = 0; i < 8; i++) qf[s][i] = ldexpf(qf[s][i], 13 - e);
+          const Parts2 p = cut2(qf[s]);
+          qp[0][s] = p.p[0]; qp[1][s] = p.p[1];
+        }
+      } else if constexpr (T != QLLAMA_KV_F32) {
+#pragma unroll
+        for (int s = 0; s < CH; s++) {
+          const Parts3 p = cut3(qf[s]);
+          qp[0][s] = p.p[0]; qp[1][s] = p.p[1]; qp[2][s] = p.p[2];
+        }
+      }
+
+      const char *kbase = a.k + kvh * a.hst, *vbase = a.v + kvh * a.hst;
+      int k_off[CH], v_off = n * DPL < a.hd ? n * DPL * C::ES : 0;    // padded dims read dim 0; their products are dropped or with 0
+#pragma unroll
+      for (int s = 0; s < CH; s++) k_off[s] = 32 * s + 8 * g < a.hd ? (32 * s + 8 * g) * C::ES : 0;
+
+      Window<UNI> win;
+      win.load(a, table, UNI ? from * SUB : from * STEP, len);
+
+      // page and place of 16-key group i of step s (UNI), or of its key j
+      auto lookup = [&](int s, int i, int j, int *place) -> int {
+        if constexpr (UNI) {
+          const int at = s * SUB + i - win.first;
+          *place = __builtin_amdgcn_readlane(win.place, at) + j;
+          return __builtin_amdgcn_readlane(win.page, at);
+        } else {
+          const int at = s * STEP + 16 * i + j - win.first;
+          *place = __shfl(win.place, at);
+          return __shfl(win.page, at);
+        }
+      };
+      auto advance = [&](int s) {                   // the window holds step s
+        const int at = UNI ? s * SUB : s * STEP;
+        if (at - win.first >= 64) win.load(a, table, at, len);
+      };
+      auto load_k = [&](int s, KTile<T, HDP> &k) {
+#pragma unroll
+        for (int i = 0; i < SUB; i++) {
+          const char *p;
+          if constexpr (UNI) {
+            int place;
+            int page = lookup(s, i, 0, &place);
+            if (page < 0) { page = 0; place = 0; }
+            p = kbase + page * a.pst + place * a.sst + (unsigned)(n * (int)a.sst);
+          } else {
+            int place;
+            int page = lookup(s, i, n, &place);
+            if (page < 0) { page = 0; place = 0; }
+            p = kbase + page * a.pst + place * a.sst;
+          }
+#pragma unroll
+          for (int c = 0; c < CH; c++) load_words(k.w[i][c], p + k_off[c]);
+        }
+      };
+      auto load_v = [&](int s, VTile<T, HDP> &v) {
+#pragma unroll
+        for (int i = 0; i < SUB; i++) {
+          const char *p = vbase;
+          if constexpr (UNI) {
+            int place;
+            int page = lookup(s, i, 0, &place);
+            if (page < 0) { page = 0; place = 0; }
+            p += page * a.pst + place * a.sst;
+          }
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const char *pj = p;
+            if constexpr (UNI) {
+              pj += (unsigned)((4 * g + j) * (int)a.sst);
+            } else {
+              int place;
+              int page = lookup(s, i, 4 * g + j, &place);
+              if (page < 0) { page = 0; place = 0; }
+              pj += page * a.pst + place * a.sst;
+            }
+            if constexpr (T == QLLAMA_KV_I8 && C::VW == 4) load_words_8(v.w[i][j], pj + v_off);
+            else load_words(v.w[i][j], pj + v_off);
+          }
+        }
+      };
+
+      auto step = [&](int s, KTile<T, HDP> &k, KTile<T, HDP> &k_next) {
+        VTile<T, HDP> v;
+        float ksc[SUB][4], vsc[SUB][4];
+        bool absent = false;                        // some key of the step lies on no page
+        bool out[SUB][4];
+        load_v(s, v);
+#pragma unroll
+        for (int i = 0; i < SUB; i++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            int place, page;
+            if constexpr (UNI) {
+              page = lookup(s, i, 0, &place);
+              place += 4 * g + j;
+            } else {
+              page = lookup(s, i, 4 * g + j, &place);
+            }
+            out[i][j] = page < 0 || s * STEP + 16 * i + 4 * g + j >= len;
+            absent |= out[i][j];
+            if constexpr (T == QLLAMA_KV_I8) {
+              const long long at = out[i][j] ? 0 : page * a.scp + kvh * a.sch + place * a.scs;
+              ksc[i][j] = a.ks[at];
+              vsc[i][j] = a.vs[at];
+            }
+          }
+        if (s + 1 < to) {
+          advance(s + 1);
+          load_k(s + 1, k_next);
+        }
+
+        // scores of 16 SUB keys for the lane's query head
+        float sc[SUB][4];
+#pragma unroll
+        for (int i = 0; i < SUB; i++) {
+          f4 d = {0, 0, 0, 0};
+#pragma unroll
+          for (int c = 0; c < CH; c++) {
+            if constexpr (T == QLLAMA_KV_F32) {
+#pragma unroll
+              for (int e = 0; e < 8; e++) d = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k.w[i][c][e]), qf[c][e], d, 0, 0, 0);
+            } else {
+              u4 kk;
+              if constexpr (T == QLLAMA_KV_I8) {
+#pragma unroll
+                for (int w = 0; w < 2; w++) {
+                  const uint32_t x = k.w[i][c][w];
+                  kk[2 * w] = hi16s(__float_as_uint(byte_f<1>(x)), __float_as_uint(byte_f<0>(x)));
+                  kk[2 * w + 1] = hi16s(__float_as_uint(byte_f<3>(x)), __float_as_uint(byte_f<2>(x)));
+                }
+              } else {
+                kk = u4{k.w[i][c][0], k.w[i][c][1], k.w[i][c][2], k.w[i][c][3]};
+              }
+#pragma unroll
+              for (int p = 0; p < C::PARTS; p++) d = mfma16<T>(kk, qp[p][c], d);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            sc[i][j] = d[j];
+            if constexpr (T == QLLAMA_KV_F16) sc[i][j] *= unscale;
+            if constexpr (T == QLLAMA_KV_I8) sc[i][j] *= ksc[i][j];
+          }
+        }
+        if (__any(absent)) {
+#pragma unroll
+          for (int i = 0; i < SUB; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              if (out[i][j]) {                      // whatever the slot holds, NaN too, counts nothing
+                sc[i][j] = kNegInf;
+                if constexpr (T == QLLAMA_KV_I8) vsc[i][j] = 0.0f;
+#pragma unroll
+                for (int w = 0; w < C::VW; w++) v.w[i][j][w] = 0;
+              }
+            }
+        }
+
+        float top = sc[0][0];
+#pragma unroll
+        for (int i = 0; i < SUB; i++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) top = fmaxf(top, sc[i][j]);
+        top = fmaxf(m, max_groups(top));
+        if (__any(top > m)) {                       // rare after the first steps
+          const float f = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+          l *= f;
+#pragma unroll
+          for (int c = 0; c < DPL; c++) acc[c] *= f;
+          m = top;
+        }
+        const float ref = (m == kNegInf ? 0.0f : m) - C::SHIFT;
+        float p[SUB][4];
+#pragma unroll
+        for (int i = 0; i < SUB; i++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            p[i][j] = __builtin_amdgcn_exp2f(sc[i][j] - ref);
+            l += p[i][j];
+            if constexpr (T == QLLAMA_KV_I8) p[i][j] *= vsc[i][j];
+          }
+
+        if constexpr (T == QLLAMA_KV_F32) {
+#pragma unroll
+          for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int c = 0; c < DPL; c++) acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v.w[0][j][c]), p[0][j], acc[c], 0, 0, 0);
+        } else {
+          const float pf[8] = {p[0][0], p[0][1], p[0][2], p[0][3], p[SUB - 1][0], p[SUB - 1][1], p[SUB - 1][2], p[SUB - 1][3]};
+          u4 pp[C::PARTS];
+          if constexpr (T == QLLAMA_KV_F16) {
+            const Parts2 x = cut2(pf);
+            pp[0] = x.p[0]; pp[1] = x.p[1];
+          } else {
+            const Parts3 x = cut3(pf);
+            pp[0] = x.p[0]; pp[1] = x.p[1]; pp[2] = x.p[2];
+          }
+#pragma unroll
+          for (int c = 0; c < DPL; c++) {
+            u4 vv;                                  // dim c of the lane's piece, 8 keys
+#pragma unroll
+            for (int i = 0; i < SUB; i++)
+#pragma unroll
+              for (int j = 0; j < 2; j++) {
+                const uint32_t *x = v.w[i][2 * j], *y = v.w[i][2 * j + 1];
+                if constexpr (T == QLLAMA_KV_I8) {
+                  const uint32_t xa = x[c / 4] >> (8 * (c % 4)), ya = y[c / 4] >> (8 * (c % 4));
+                  vv[2 * i + j] = hi16s(__float_as_uint(byte_f<0>(ya)), __float_as_uint(byte_f<0>(xa)));
+                } else {
+                  vv[2 * i + j] = c % 2 ? hi16s(y[c / 2], x[c / 2]) : lo16s(y[c / 2], x[c / 2]);
+                }
+              }
+#pragma unroll
+            for (int k = 0; k < C::PARTS; k++) acc[c] = mfma16<T>(vv, pp[k], acc[c]);
+          }
+        }
+      };
+
+      KTile<T, HDP> k0, k1;
+      load_k(from, k0);
+      for (int s = from; s < to; s += 2) {
+        step(s, k0, k1);
+        if (s + 1 < to) step(s + 1, k1, k0);
+      }
+      l = sum_groups(l);
+    }
+
+    // the waves' results together; lane (n, g) holds head n, dims (4 g + i) DPL + c
+    if (g == 0) { s_m[wave][n] = m; s_l[wave][n] = l; }
+    __syncthreads();
+    float top = kNegInf;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) top = fmaxf(top, s_m[w][n]);
+    const float f = part_weight(m, top);
+    if (n < rows) {
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int c = 0; c < DPL; c++) dyn[(wave * a.rows + n) * HDP + (4 * g + i) * DPL + c] = acc[c][i] * f;
+    }
+    __syncthreads();
+    const bool whole = s0 == 0 && s1 == steps;
+    float *part = a.part + (blockIdx.x * 2 + (u == begin ? 0 : 1)) * ((long long)a.rows * (a.hd + 2));
+    for (int i = threadIdx.x; i < rows * a.hd; i += kThreads) {
+      const int row = i / a.hd, d = i - row * a.hd;
+      float t = kNegInf, sum = 0.0f, x = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWaves; w++) t = fmaxf(t, s_m[w][row]);
+#pragma unroll
+      for (int w = 0; w < kWaves; w++) {
+        x += dyn[(w * a.rows + row) * HDP + d];
+        sum += s_l[w][row] * part_weight(s_m[w][row], t);
+      }
+      if (whole) {
+        a.o[r * a.o_stride + (long long)(h0 + row) * a.hd + d] = sum == 0.0f ? 0.0f : x / sum;
+        if (d == 0 && a.lse) a.lse[r * a.lse_stride + h0 + row] = sum == 0.0f ? kNegInf : (t - C::SHIFT + __builtin_amdgcn_logf(sum)) * 0.69314718056f;
+      } else {
+        part[row * (a.hd + 2) + d] = x;
+        if (d == 0) {
+          part[row * (a.hd + 2) + a.hd] = t;
+          part[row * (a.hd + 2) + a.hd + 1] = sum;
+        }
+      }
+    }
+    __syncthreads();
+    u += s1 - s0;
+  }
+}
+
+// One block a request and query head: the parts of its tile put together in the order
+// of their keys; rows without a token are set.
+constexpr int kJoinThreads = 128;
+__global__ __launch_bounds__(kJoinThreads) void k_paged_join(PaArgs a, int step, float shift) {
+  __shared__ long long lds[kJoinThreads / 64];
+  const int r = blockIdx.x, h = blockIdx.y;
+  const int kvh = h / a.G, row = (h - kvh * a.G) % 16, tile = kvh * a.tiles + (h - kvh * a.G) / 16;
+  const int tiles = a.n_kv * a.tiles;
+  long long before = 0, units = 0;
+  for (int i = threadIdx.x; i < a.n_req; i += kJoinThreads) {
+    const long long s = (clamp_len(a.lens[i], a.width, a.page_size) + step - 1) / step;
+    units += s;
+    if (i < r) before += s;
+  }
+  before = block_sum(before, lds) * tiles;
+  units = block_sum(units, lds) * tiles;
+  const int steps = (clamp_len(a.lens[r], a.width, a.page_size) + step - 1) / step;
+  float *o = a.o + r * a.o_stride + (long long)h * a.hd;
+  if (!steps) {
+    for (int d = threadIdx.x; d < a.hd; d += kJoinThreads) o[d] = 0.0f;
+    if (threadIdx.x == 0 && a.lse) a.lse[r * a.lse_stride + h] = kNegInf;
+    return;
+  }
+  const long long share = share_of(units), u0 = before + (long long)tile * steps, u1 = u0 + steps;
+  const int b0 = (int)(u0 / share), b1 = (int)((u1 - 1) / share);
+  if (b0 == b1) return;                              // written by its block
+  const long long one = (long long)a.rows * (a.hd + 2);
+  const float *part = a.part + (long long)row * (a.hd + 2);
+  const int slot0 = u0 == b0 * share ? 0 : 1;        // the first part may follow another tile's in its block
+  float top = kNegInf;
+  for (int b = b0; b <= b1; b++) top = fmaxf(top, part[(2LL * b + (b == b0 ? slot0 : 0)) * one + a.hd]);
+  for (int d = threadIdx.x; d < a.hd; d += kJoinThreads) {
+    float x = 0.0f, sum = 0.0f;
+    for (int b = b0; b <= b1; b++) {
+      const float *p = part + (2LL * b + (b == b0 ? slot0 : 0)) * one;
+      const float f = part_weight(p[a.hd], top);
+      x += p[d] * f;
+      sum += p[a.hd + 1] * f;
+    }
+    o[d] = sum == 0.0f ? 0.0f : x / sum;
+    if (d == 0 && a.lse) a.lse[r * a.lse_stride + h] = sum == 0.0f ? kNegInf : (top - shift + __builtin_amdgcn_logf(sum)) * 0.69314718056f;
+  }
+}
+
+int rows_of(const QPagedKV *c, int n_heads) {
+  const int G = n_heads / c->n_kv;
+  return G < 16 ? G : 16;
+}
+
+template <int T, int HDP>
+int launch(const char *fn, const PaArgs &a, hipStream_t stream) {
+  const size_t lds = (size_t)kWaves * a.rows * HDP * sizeof(float);
+  const bool uni = a.page_size % 16 == 0;
+  if (lds > 60 * 1024) {              // 16 rows of 256 dims: past what a launch may take unasked
+    const void *f = uni ? reinterpret_cast<const void *>(k_paged_attn<T, HDP, true>) : reinterpret_cast<const void *>(k_paged_attn<T, HDP, false>);
+    if (hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) {
+      (void)hipGetLastError();
+      return qs::refuse(fn, "hipFuncSetAttribute failed");
+    }
+  }
+  if (uni) QS_LAUNCH(fn, (k_paged_attn<T, HDP, true>), dim3(kBlocks), dim3(kThreads), lds, stream, a);
+  else QS_LAUNCH(fn, (k_paged_attn<T, HDP, false>), dim3(kBlocks), dim3(kThreads), lds, stream, a);
+  QS_LAUNCH(fn, k_paged_join, dim3(a.n_req, a.n_heads), dim3(kJoinThreads), 0, stream, a, (int)Cfg<T, HDP>::STEP, (float)Cfg<T, HDP>::SHIFT);
+  return 0;
+}
+
+template <int T>
+int launch_hd(const char *fn, const PaArgs &a, hipStream_t stream) {
+  return a.hd <= 64 ? launch<T, 64>(fn, a, stream) : a.hd <= 128 ? launch<T, 128>(fn, a, stream) : launch<T, 256>(fn, a, stream);
+}
+
+}  // namespace
+
+extern "C" int qllama_test_page_of(const int32_t *table, int width, int page_size, int n_pages, int len, long long key, int *place) {
+  return page_of(table, key, clamp_len(len, width, page_size), page_size, n_pages, place);
+}
+
+extern "C" size_t qllama_paged_attention_work(const QPagedKV *c, int n_req, int n_heads) {
+  if (qs::bad_cache(c) || n_req < 0 || n_heads < 1 || n_heads > 65535 || n_heads % c->n_kv) return 0;
+  return (size_t)kBlocks * 2 * rows_of(c, n_heads) * (c->head_dim + 2) * sizeof(float);
+}
+
+extern "C" int qllama_paged_attention(const QPagedKV *c, const QPagedQuery *a, void *stream) {
+  static const char fn[] = "qllama_paged_attention";
+  if (const char *why = qs::bad_cache(c)) return qs::refuse(fn, why);
+  if (!a || a->n_req < 0) return qs::refuse(fn, "null argument or n_req < 0");
+  if (a->n_heads < 1 || a->n_heads > 65535 || a->n_heads % c->n_kv) return qs::refuse(fn, "n_heads must be a multiple of the cache's KV heads");
+  if (a->n_req == 0) return 0;
+  if (!a->q || !a->o || !a->table || !a->lens) return qs::refuse(fn, "null q, o, table or lens");
+  const int64_t qd = (int64_t)a->n_heads * c->head_dim;
+  if (a->q_stride < qd || a->o_stride < qd || (a->lse && a->lse_stride < a->n_heads)) return qs::refuse(fn, "a row stride below the row's length");
+  if (a->width < 1 || a->table_stride < a->width || (int64_t)a->width * c->page_size > INT_MAX)
+    return qs::refuse(fn, "bad table width (width * page_size must fit in 31 bits) or stride");
+  if (!(a->scale >= 0.0f) || a->scale > 3.0e38f) return qs::refuse(fn, "scale must be finite and not negative");
+  if (a->q == a->o) return qs::refuse(fn, "o must not be q");
+  if (qs::misaligned(a->q, 4) || qs::misaligned(a->o, 4) || qs::misaligned(a->lse, 4) || qs::misaligned(a->table, 4) || qs::misaligned(a->lens, 4))
+    return qs::refuse(fn, "a buffer is not aligned to its elements");
+  if (!a->work || qs::misaligned(a->work, 16) || a->work_bytes < qllama_paged_attention_work(c, a->n_req, a->n_heads))
+    return qs::refuse(fn, "work is missing, misaligned or smaller than qllama_paged_attention_work");
+  qs::OnDevice on(c->k, (hipStream_t)stream);
+  if (on.why) return qs::refuse(fn, on.why);
+  const int es = c->type == QLLAMA_KV_F32 ? 4 : c->type == QLLAMA_KV_I8 ? 1 : 2;
+  PaArgs p;
+  p.k = static_cast<const char *>(c->k); p.v = static_cast<const char *>(c->v);
+  p.ks = c->k_scale; p.vs = c->v_scale;
+  p.q = a->q; p.o = a->o; p.lse = a->lse; p.table = a->table; p.lens = a->lens; p.part = static_cast<float *>(a->work);
+  p.pst = c->page_stride * es; p.hst = c->head_stride * es; p.sst = c->slot_stride * es;
+  p.scp = c->scale_page_stride; p.sch = c->scale_head_stride; p.scs = c->scale_slot_stride;
+  p.q_stride = a->q_stride; p.o_stride = a->o_stride; p.lse_stride = a->lse_stride; p.table_stride = a->table_stride;
+  p.n_req = a->n_req; p.n_heads = a->n_heads; p.n_kv = c->n_kv; p.G = a->n_heads / c->n_kv; p.tiles = (p.G + 15) / 16;
+  p.rows = rows_of(c, a->n_heads); p.hd = c->head_dim; p.n_pages = c->n_pages; p.page_size = c->page_size; p.width = a->width;
+  p.qscale = (a->scale > 0.0f ? a->scale : 1.0f / __builtin_sqrtf((float)c->head_dim)) * 1.44269504089f;
+  switch (c->type) {
+    case QLLAMA_KV_F32: return launch_hd<QLLAMA_KV_F32>(fn, p, (hipStream_t)stream);
+    case QLLAMA_KV_F16: return launch_hd<QLLAMA_KV_F16>(fn, p, (hipStream_t)stream);
+    case QLLAMA_KV_BF16: return launch_hd<QLLAMA_KV_BF16>(fn, p, (hipStream_t)stream);
+    default: return launch_hd<QLLAMA_KV_I8>(fn, p, (hipStream_t)stream);
+  }
+}

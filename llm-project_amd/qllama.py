@@ -6,6 +6,7 @@ it is missing: there is no CPU fallback.  Mirrors the reference's quantized API
 """
 import ctypes as C
 import os
+import struct
 
 import numpy as np
 
@@ -67,6 +68,21 @@ class GPT(C.Structure):                        # model.h:19-31
 class KVCache(C.Structure):                    # model.h:124-129 + the device handle
     _fields_ = [(n, C.c_int) for n in ("n_layers", "d_model", "n_heads", "max_seq_len", "len")] + \
                [("K", C.POINTER(Tensor)), ("V", C.POINTER(Tensor)), ("dev", C.c_void_p)]
+
+
+class QPagedKV(C.Structure):                   # qserve.h
+    _fields_ = [(n, C.c_int) for n in ("type", "n_pages", "page_size", "n_kv", "head_dim")] + \
+               [(n, C.c_int64) for n in ("page_stride", "head_stride", "slot_stride")] + \
+               [("k", C.c_void_p), ("v", C.c_void_p)] + \
+               [(n, C.c_int64) for n in ("scale_page_stride", "scale_head_stride", "scale_slot_stride")] + \
+               [("k_scale", C.c_void_p), ("v_scale", C.c_void_p)]
+
+
+# the other structures of qserve.h, packed afresh for every call
+PAGED_PLAN = struct.Struct("@iiiiiqPPPPPPPPPPPP")
+PAGED_ROWS = struct.Struct("@iiPPPPqqqqPPPPiP")
+PAGED_QUERY = struct.Struct("@iiiqqqqPPPPPfPN")
+SAMPLE_ROWS = struct.Struct("@iiqPPPPPPPPPPN")
 
 
 class Rng(C.Structure):
@@ -164,6 +180,14 @@ def lib():
         L.qllama_profile.argtypes = [C.c_int]
         L.qllama_bench_cold.argtypes = [C.c_int]
         L.qllama_profile_read.argtypes = [C.c_char_p, C.c_int, P(C.c_double), P(C.c_longlong), C.c_int]
+        L.qllama_paged_plan.argtypes = [C.c_char_p, C.c_void_p]
+        L.qllama_paged_append.argtypes = [P(QPagedKV), C.c_char_p, C.c_void_p]
+        L.qllama_paged_attention.argtypes = [P(QPagedKV), C.c_char_p, C.c_void_p]
+        L.qllama_paged_attention_work.argtypes = [P(QPagedKV), C.c_int, C.c_int]
+        L.qllama_paged_attention_work.restype = C.c_size_t
+        L.qllama_sample_rows.argtypes = [C.c_char_p, C.c_void_p]
+        L.qllama_sample_rows_work.argtypes = [C.c_int, C.c_int]
+        L.qllama_sample_rows_work.restype = C.c_size_t
         _lib = L
     return _lib
 
@@ -599,3 +623,188 @@ def profile_read():
     n = lib().qllama_profile_read(names, 4096, ms, cnt, 32)
     keys = names.value.decode().split(",")[:max(n, 0)]
     return {k: (ms[i], cnt[i]) for i, k in enumerate(keys)}
+
+
+# ---- qserve.h: one step of many requests over a paged cache ------------------------
+# Buffers are tensors on the GPU (torch's, or anything with is_cuda, dtype, shape,
+# stride() and data_ptr()); stream is a hipStream_t as a number, e.g.
+# torch.cuda.current_stream().cuda_stream, and None the library's own.
+KV_F32, KV_F16, KV_BF16, KV_I8 = 0, 1, 2, 3
+_KV_TYPE = {"float32": KV_F32, "float16": KV_F16, "bfloat16": KV_BF16, "int8": KV_I8}
+_dtypes = {}
+
+
+def _dtype(t):
+    name = _dtypes.get(t.dtype)
+    if name is None:
+        name = _dtypes[t.dtype] = str(t.dtype).replace("torch.", "")
+    return name
+
+
+def _flat(t, name, dtype, size):
+    """Address of a contiguous GPU tensor of `dtype` with at least `size` elements, or 0 for None."""
+    if t is None:
+        return 0
+    if t.is_cuda and _dtypes.get(t.dtype) == dtype and t.numel() >= size and t.is_contiguous():
+        return t.data_ptr()
+    return _ptr(t, name, dtype, size, 8)
+
+
+def _ptr(t, name, dtype, size, inner):
+    """The same where the last `inner` dimensions have to be contiguous."""
+    if not t.is_cuda:
+        raise ValueError(f"{name} is not on the GPU")
+    if _dtype(t) != dtype:
+        raise ValueError(f"{name} must be {dtype}, not {_dtype(t)}")
+    if t.numel() < size:
+        raise ValueError(f"{name} has {t.numel()} elements, {size} are needed")
+    want, strides, shape = 1, t.stride(), t.shape
+    for d in range(len(shape) - 1, max(-1, len(shape) - 1 - inner), -1):
+        if shape[d] != 1 and strides[d] != want:
+            raise ValueError(f"{name} is not contiguous")
+        want *= shape[d]
+    return t.data_ptr()
+
+
+def _row_stride(t, row):
+    return t.stride(0) if t.shape[0] > 1 else row
+
+
+def _stream(stream):
+    return lib().qllama_stream() if stream is None else stream
+
+
+def _work(t):
+    if not t.is_cuda:
+        raise ValueError("work is not on the GPU")
+    return t.data_ptr(), t.numel() * t.element_size()
+
+
+def _done(rc, name):
+    if rc != 0:
+        raise RuntimeError(f"{name} refused the call (its message is on stderr)")
+
+
+class PagedKV:
+    """A view of a paged cache: k and v of shape (pages, KV heads, page size, head_dim) in float32, float16, bfloat16
+    or int8, with any strides whose last is 1; int8 with scales (pages, KV heads, page size).  Keeps the tensors."""
+
+    def __init__(self, k, v, k_scale=None, v_scale=None):
+        kind = _KV_TYPE.get(_dtype(k))
+        if kind is None:
+            raise ValueError(f"no cache of {_dtype(k)}")
+        if len(k.shape) != 4 or tuple(k.shape) != tuple(v.shape) or tuple(k.stride()) != tuple(v.stride()):
+            raise ValueError("k and v must have one shape (pages, KV heads, page size, head_dim) and alike strides")
+        if (k_scale is None) != (kind != KV_I8) or (v_scale is None) != (kind != KV_I8):
+            raise ValueError("an int8 cache, and no other, has scales")
+        pages, n_kv, page, hd = k.shape
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        st = [s if n > 1 else hd for s, n in zip(k.stride(), k.shape)]     # a dimension of one element has any stride
+        self.c = QPagedKV(kind, pages, page, n_kv, hd, st[0], st[1], st[2], _ptr(k, "k", _dtype(k), 0, 1), _ptr(v, "v", _dtype(k), 0, 1))
+        if kind == KV_I8:
+            for s in (k_scale, v_scale):
+                if tuple(s.shape) != (pages, n_kv, page) or tuple(s.stride()) != tuple(k_scale.stride()):
+                    raise ValueError("scales must have the shape (pages, KV heads, page size) and alike strides")
+            st = [s if n > 1 else 1 for s, n in zip(k_scale.stride(), k_scale.shape)]
+            self.c.scale_page_stride, self.c.scale_head_stride, self.c.scale_slot_stride = st
+            self.c.k_scale, self.c.v_scale = _ptr(k_scale, "k_scale", "float32", 0, 0), _ptr(v_scale, "v_scale", "float32", 0, 0)
+        self.ref = C.byref(self.c)
+
+
+def paged_plan(cached, added, table, ring, state, page_size, lens, status, starts, state_out, slots, positions, requests,
+               stream=None):
+    """qllama_paged_plan: pages for the requests' new tokens, and slot, position and request of every new row.  int32
+    tensors; table (requests, width) and ring change in place, the arguments after page_size are outputs."""
+    n, rows = cached.numel(), slots.numel()
+    i32 = "int32"
+    if len(table.shape) != 2 or table.shape[0] < n:
+        raise ValueError("table must have a row for every request")
+    width = table.shape[1]
+    a = PAGED_PLAN.pack(n, width, page_size, ring.numel(), rows, _row_stride(table, width),
+                        _flat(cached, "cached", i32, n), _flat(added, "added", i32, n), _flat(state, "state", i32, 2),
+                        _ptr(table, "table", i32, 0, 1), _flat(ring, "ring", i32, 1), _flat(lens, "lens", i32, n),
+                        _flat(status, "status", i32, n), _flat(starts, "starts", i32, n + 1), _flat(state_out, "state_out", i32, 2),
+                        _flat(slots, "slots", i32, rows), _flat(positions, "positions", i32, rows),
+                        _flat(requests, "requests", i32, rows))
+    _done(lib().qllama_paged_plan(a, _stream(stream)), "qllama_paged_plan")
+
+
+def paged_append(cache, k, v, slots, q=None, q_out=None, positions=None, cos=None, sin=None, bad=None, stream=None):
+    """qllama_paged_append: k, v (rows, KV heads, head_dim) float32 into their slots; with cos and sin (positions,
+    head_dim / 2), keys and the queries q (rows, heads, head_dim) turned by their positions' angles, q into q_out."""
+    c = cache.c
+    rows, hd = slots.numel(), c.head_dim
+    heads = 0
+
+    def take(t, name):
+        if len(t.shape) != 3 or t.shape[0] != rows or t.shape[2] != hd:
+            raise ValueError(f"{name} must have the shape (rows, heads, head_dim)")
+        return _ptr(t, name, "float32", 0, 2), _row_stride(t, t.shape[1] * hd)
+
+    if k.shape[1] != c.n_kv or v.shape[1] != c.n_kv:
+        raise ValueError("k and v must have the cache's KV heads")
+    kp, ks = take(k, "k")
+    vp, vs = take(v, "v")
+    qp = qs = op = os_ = n_pos = 0
+    if q is not None:
+        heads = q.shape[1]
+        if q_out is None or q_out.shape[1] != heads:
+            raise ValueError("q needs q_out of its shape")
+        qp, qs = take(q, "q")
+        op, os_ = take(q_out, "q_out")
+    if cos is not None:
+        n_pos = cos.shape[0]
+        if sin is None or positions is None:
+            raise ValueError("a rotation needs cos, sin and positions")
+    a = PAGED_ROWS.pack(rows, heads, qp, kp, vp, op, qs, ks, vs, os_, _flat(slots, "slots", "int32", rows),
+                        _flat(positions, "positions", "int32", rows), _flat(cos, "cos", "float32", n_pos * hd // 2),
+                        _flat(sin, "sin", "float32", n_pos * hd // 2), n_pos, _flat(bad, "bad", "int32", 1))
+    _done(lib().qllama_paged_append(cache.ref, a, _stream(stream)), "qllama_paged_append")
+
+
+def paged_attention_work(cache, n_req, n_heads):
+    """Bytes of workspace of paged_attention (calls that overlap need one each)."""
+    n = lib().qllama_paged_attention_work(cache.ref, n_req, n_heads)
+    if n == 0:
+        raise ValueError("no such attention over this cache")
+    return n
+
+
+def paged_attention(cache, q, table, lens, o, work, lse=None, scale=0.0, stream=None):
+    """qllama_paged_attention: o (requests, heads, head_dim) and lse (requests, heads) of q over the first lens tokens of
+    every request's pages table (requests, width)."""
+    if len(q.shape) != 3 or len(o.shape) != 3 or len(table.shape) != 2:
+        raise ValueError("q and o must have the shape (requests, heads, head_dim), table (requests, width)")
+    n, heads, hd = q.shape
+    width = table.shape[1]
+    if tuple(o.shape) != (n, heads, hd) or hd != cache.c.head_dim or table.shape[0] < n:
+        raise ValueError("q, o, table and the cache do not fit together")
+    if lse is not None and tuple(lse.shape) != (n, heads):
+        raise ValueError("lse must have the shape (requests, heads)")
+    a = PAGED_QUERY.pack(n, heads, width, _row_stride(q, heads * hd), _row_stride(o, heads * hd),
+                         0 if lse is None else _row_stride(lse, heads), _row_stride(table, width), _ptr(q, "q", "float32", 0, 2),
+                         _ptr(o, "o", "float32", 0, 2), 0 if lse is None else _ptr(lse, "lse", "float32", 0, 1),
+                         _ptr(table, "table", "int32", 0, 1), _flat(lens, "lens", "int32", n), scale, *_work(work))
+    _done(lib().qllama_paged_attention(cache.ref, a, _stream(stream)), "qllama_paged_attention")
+
+
+def sample_rows_work(rows, vocab):
+    """Bytes of workspace of sample_rows (calls that overlap need one each)."""
+    n = lib().qllama_sample_rows_work(rows, vocab)
+    if n == 0:
+        raise ValueError("no such rows of logits")
+    return n
+
+
+def sample_rows(logits, u, token, work, temperature=None, top_k=None, top_p=None, min_p=None, prob=None, kept=None, stream=None):
+    """qllama_sample_rows: a token for every row of logits (rows, vocab) from the numbers u in [0, 1); settings a row
+    each (None: temperature 1, no limit); prob its probability among the kept tokens, kept their number."""
+    if len(logits.shape) != 2:
+        raise ValueError("logits must have the shape (rows, vocab)")
+    n, V = logits.shape
+    a = SAMPLE_ROWS.pack(n, V, _row_stride(logits, V), _ptr(logits, "logits", "float32", 0, 1), _flat(u, "u", "float32", n),
+                         _flat(temperature, "temperature", "float32", n), _flat(top_k, "top_k", "int32", n),
+                         _flat(top_p, "top_p", "float32", n), _flat(min_p, "min_p", "float32", n),
+                         _flat(token, "token", "int32", n), _flat(kept, "kept", "int32", n), _flat(prob, "prob", "float32", n),
+                         *_work(work))
+    _done(lib().qllama_sample_rows(a, _stream(stream)), "qllama_sample_rows")
