@@ -3,18 +3,20 @@
 // whose decode attention (llama.c:554-576) serves one sequence and one dense cache.
 //
 // The work of a call is the key steps of all (request, KV head, 16 query heads) tiles,
-// laid one behind another; every block takes an equal share of them, whatever the
+// laid one behind another; every wave takes an equal share of them, whatever the
 // lengths are, so ragged batches and one long request fill the chip alike without the
 // host knowing a length.  A share that ends inside a tile leaves its maximum, sum and
 // weighted values in the workspace, and k_paged_join puts a tile's parts together.
+// Waves never meet: with four of them on a tile, meeting in LDS at its end, 512 requests
+// of 300 bf16 tokens took XX us against XX.
 //
-// A wave keeps its tile's queries, running maximum, sum and outputs in registers and
-// takes a step of 16 or 32 keys at a time straight from the pages: no LDS until its
-// share ends.  S^T = K q^T on the matrix cores puts a query head in a lane's column
-// and 4 keys of each 16 in its rows; the same lane's weights are then the operand of
-// O^T += V^T P^T, whose contraction slots are matched to the keys the lane holds, so
-// weights never move between lanes.  A lane loads whole 16-byte pieces of a value row
-// (16 lanes a row), and the pieces of 8 keys are turned by byte permutes.
+// A wave keeps its running maximum, sum and outputs in registers, its queries in LDS, and
+// takes a step of 16 or 32 keys at a time straight from the pages into registers.
+// S^T = K q^T on the matrix cores puts a query head in a lane's column and 4 keys of
+// each 16 in its rows; the same lane's weights are then the operand of O^T += V^T P^T,
+// whose contraction slots are matched to the keys the lane holds, so weights never move
+// between lanes.  A lane loads whole pieces of a value row (16 lanes a row), and the
+// pieces of 8 keys are turned by byte permutes.
 //
 // Precision: float queries and weights meet 16-bit keys and values as parts that add up
 // to them (bf16: three parts of 8 bits, f16: two of 11), one MFMA a part; int8 codes
@@ -35,7 +37,8 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256, kWaves = 4;
 constexpr int kBlocks = 512;          // two blocks of four waves a CU
-constexpr int kMinShare = 4;          // steps a block takes at least: one a wave
+constexpr int kShares = kBlocks * kWaves;
+constexpr int kMinShare = 2;          // steps a wave takes at least
 constexpr float kNegInf = -__builtin_inff();
 
 struct PaArgs {
@@ -67,7 +70,7 @@ __host__ __device__ inline int page_of(const int *table, long long key, int len,
   return p;
 }
 
-// Sum over the block (256 threads) of one int64 a thread.
+// Sum over the block of one int64 a thread.
 __device__ long long block_sum(long long v, long long *lds) {
   for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
   if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
@@ -78,9 +81,9 @@ __device__ long long block_sum(long long v, long long *lds) {
   return v;
 }
 
-// Steps of a block's share when all tiles together take `units`.
+// Steps of a wave's share when all tiles together take `units`.
 __device__ inline long long share_of(long long units) {
-  const long long s = (units + kBlocks - 1) / kBlocks;
+  const long long s = (units + kShares - 1) / kShares;
   return s < kMinShare ? kMinShare : s;
 }
 
@@ -116,12 +119,6 @@ __device__ inline void load_words(uint32_t (&d)[W], const char *p) {
     }
   }
 }
-// 16 bytes of int8 lie on 8-byte boundaries only
-__device__ inline void load_words_8(uint32_t (&d)[4], const char *p) {
-  const u2 x = *reinterpret_cast<const u2 *>(p), y = *reinterpret_cast<const u2 *>(p + 8);
-  d[0] = x.x; d[1] = x.y; d[2] = y.x; d[3] = y.y;
-}
-
 __device__ inline uint32_t hi16s(uint32_t b, uint32_t a) { return __builtin_amdgcn_perm(b, a, 0x07060302); }
 __device__ inline uint32_t lo16s(uint32_t b, uint32_t a) { return __builtin_amdgcn_perm(b, a, 0x05040100); }
 template <int B>
@@ -177,7 +174,11 @@ struct Cfg {
   static constexpr int KW = 8 * ES / 4;                        // words of such a piece
   static constexpr int DPL = HDP / 16;                         // dims of a value row that a lane loads
   static constexpr int VW = DPL * ES / 4;
-  static constexpr int PARTS = T == QLLAMA_KV_F16 ? 2 : 3;
+  static constexpr int PIECES = DPL > 8 ? 2 : 1, PW = VW / PIECES;    // a piece: at most 8 dims, as head_dim is a multiple of 8
+  static constexpr int PARTS = T == QLLAMA_KV_F32 ? 1 : T == QLLAMA_KV_F16 ? 2 : 3;
+  // a query row in LDS: its parts' values, and 64 bytes that spread rows over the banks
+  static constexpr int QES = T == QLLAMA_KV_F32 ? 4 : 2;
+  static constexpr int QROW = HDP * QES + 64;
   // 2^SHIFT times the weights: f16 parts then keep 22 bits down to 2^-18 of the largest
   // weight and the rest to 2^-40
   static constexpr float SHIFT = T == QLLAMA_KV_F16 ? 15.0f : 0.0f;
@@ -186,7 +187,7 @@ struct Cfg {
 template <int T, int HDP>
 struct KTile { uint32_t w[Cfg<T, HDP>::SUB][Cfg<T, HDP>::CH][Cfg<T, HDP>::KW]; };
 template <int T, int HDP>
-struct VTile { uint32_t w[Cfg<T, HDP>::SUB][4][Cfg<T, HDP>::VW]; };
+struct VTile { uint32_t w[Cfg<T, HDP>::SUB][4][Cfg<T, HDP>::PIECES][Cfg<T, HDP>::PW]; };
 
 // Where the keys of a wave's steps lie.  UNI (page_size a multiple of 16): lane l holds
 // the page and place of 16-key group first + l, read from the table 64 groups at a
@@ -207,364 +208,386 @@ template <int T, int HDP, bool UNI>
 __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaArgs a) {
   using C = Cfg<T, HDP>;
   constexpr int SUB = C::SUB, STEP = C::STEP, CH = C::CH, DPL = C::DPL;
-  extern __shared__ float dyn[];                    // [wave][row][HDP] at the end of a share
-  __shared__ long long sums[kWaves];
-  __shared__ float s_m[kWaves][16], s_l[kWaves][16];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int n = lane & 15, g = lane >> 4;           // key or query head or value piece; group of 16 lanes
+  extern __shared__ __align__(16) char dyn[];       // a wave's queries: [part][row]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int n = lane & 15, g = lane >> 4;           // key, query head or value piece; group of 16 lanes
   const int tiles = a.n_kv * a.tiles;
+  char *q_lds = dyn + wave * (C::PARTS * a.rows * C::QROW);
 
-  // this block's share of all steps, and the request it begins in
-  long long units = 0;
-  for (int r = threadIdx.x; r < a.n_req; r += kThreads)
-    units += (clamp_len(a.lens[r], a.width, a.page_size) + STEP - 1) / STEP;
-  units = block_sum(units, sums) * tiles;
+  // this wave's share of all steps; shares of one block lie far apart, so that few of
+  // them are spread over the CUs
+  int mine = 0, all = 0;                            // steps of request `lane` of the last 64; of all
+  for (int r = 0; r < a.n_req; r += 64) {
+    mine = r + lane < a.n_req ? (clamp_len(a.lens[r + lane], a.width, a.page_size) + STEP - 1) / STEP : 0;
+    all += mine;
+  }
+  for (int d = 32; d; d >>= 1) all += __shfl_xor(all, d);
+  const long long units = (long long)__builtin_amdgcn_readfirstlane(all) * tiles;
   const long long share = share_of(units);
-  long long u = blockIdx.x * share;
+  const int id = wave * kBlocks + blockIdx.x;
+  long long u = id * share;
   const long long end = u + share < units ? u + share : units;
   if (u >= end) return;
   const long long begin = u;
-  int r = 0, steps;
-  long long r_begin = 0;                            // first unit of request r
-  for (;; r++) {                                    // 64 requests at a time, then one by one
-    long long c = 0;
-    const int i = r + lane;
-    if (i < a.n_req) c = (clamp_len(a.lens[i], a.width, a.page_size) + STEP - 1) / STEP;
-    long long s = c;
+  int r = 0;                                        // the request it begins in, and that one's first unit
+  long long r_begin = 0;
+  for (;; r += 64) {
+    if (a.n_req > 64) mine = r + lane < a.n_req ? (clamp_len(a.lens[r + lane], a.width, a.page_size) + STEP - 1) / STEP : 0;
+    int s = mine;
     for (int d = 1; d < 64; d <<= 1) {
-      const long long t = __shfl_up(s, d);
+      const int t = __shfl_up(s, d);
       if (lane >= d) s += t;
     }
-    const uint64_t past = __ballot(r_begin + s * tiles > u);
+    const uint64_t past = __ballot(r_begin + (long long)s * tiles > u);
     if (past) {
       const int at = __builtin_ctzll(past);
-      r_begin += (__shfl(s, at) - __shfl(c, at)) * tiles;
-      steps = (int)__shfl(c, at);
+      r_begin += (long long)(__builtin_amdgcn_readlane(s, at) - __builtin_amdgcn_readlane(mine, at)) * tiles;
       r += at;
       break;
     }
-    r_begin += __shfl(s, 63) * tiles;
-    r += 63;
+    r_begin += (long long)__builtin_amdgcn_readlane(s, 63) * tiles;
   }
 
   while (u < end) {
     const int len = clamp_len(a.lens[r], a.width, a.page_size);
-    steps = (len + STEP - 1) / STEP;
+    const int steps = (len + STEP - 1) / STEP;
     if (u >= r_begin + (long long)steps * tiles) {
       r_begin += (long long)steps * tiles;
       r++;
       continue;
     }
-    const int tile = (int)((u - r_begin) / steps);
-    const int s0 = (int)(u - r_begin - (long long)tile * steps);
-    const int s1 = (int)(end - u < steps - s0 ? s0 + (end - u) : steps);
+    const unsigned long long at = u - r_begin;
+    const int tile = at >> 32 ? (int)(at / (unsigned)steps) : (int)((unsigned)at / (unsigned)steps);
+    const int from = (int)(at - (unsigned long long)tile * steps);
+    const int to = (int)(end - u < steps - from ? from + (end - u) : steps);
     const int kvh = tile / a.tiles, h0 = kvh * a.G + (tile % a.tiles) * 16;
     const int rows = a.G - (tile % a.tiles) * 16 < 16 ? a.G - (tile % a.tiles) * 16 : 16;
     const int *table = a.table + r * a.table_stride;
-    const int from = s0 + (s1 - s0) * wave / kWaves, to = s0 + (s1 - s0) * (wave + 1) / kWaves;
+    const int row = n % rows;                       // columns past the tile's heads repeat them
+
+    Window<UNI> win;
+    win.load(a, table, UNI ? from * SUB : from * STEP, len);
+
+    // queries: head h0 + row, dims 32 c + 8 g ..; scaled so that weights are powers of two
+    float unscale = 1.0f;
+    {
+      float qf[CH][8];
+      float qmax = 0.0f;
+      const float *q = a.q + r * a.q_stride + (long long)(h0 + row) * a.hd;
+#pragma unroll
+      for (int c = 0; c < CH; c++) {
+        const int d = 32 * c + 8 * g;
+        __builtin_memcpy(qf[c], q + (d < a.hd ? d : 0), sizeof qf[c]);     // 4-byte aligned; head_dim is a multiple of 8
+      }
+#pragma unroll
+      for (int c = 0; c < CH; c++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          qf[c][i] = 32 * c + 8 * g < a.hd ? qf[c][i] * a.qscale : 0.0f;
+          qmax = fmaxf(qmax, fabsf(qf[c][i]));
+        }
+      int e = 0;
+      if constexpr (T == QLLAMA_KV_F16) {           // into f16's range, by a power of two
+        qmax = max_groups(qmax);
+        e = qmax > 0.0f && qmax < __builtin_inff() ? ilogbf(qmax) - 13 : 0;
+        unscale = ldexpf(1.0f, e);
+      }
+      __builtin_amdgcn_wave_barrier();              // the last tile's reads come first
+#pragma unroll
+      for (int c = 0; c < CH; c++) {
+        char *to_lds = q_lds + row * C::QROW + (32 * c + 8 * g) * C::QES;
+        if constexpr (T == QLLAMA_KV_F32) {
+          if (n < rows) __builtin_memcpy(__builtin_assume_aligned(to_lds, 16), qf[c], sizeof qf[c]);
+        } else if constexpr (T == QLLAMA_KV_F16) {
+#pragma unroll
+          for (int i = 0; i < 8; i++) qf[c][i] = ldexpf(qf[c][i], -e);
+          const Parts2 x = cut2(qf[c]);
+#pragma unroll
+          for (int p = 0; p < 2; p++)
+            if (n < rows) *reinterpret_cast<u4 *>(to_lds + p * a.rows * C::QROW) = x.p[p];
+        } else {
+          const Parts3 x = cut3(qf[c]);
+#pragma unroll
+          for (int p = 0; p < 3; p++)
+            if (n < rows) *reinterpret_cast<u4 *>(to_lds + p * a.rows * C::QROW) = x.p[p];
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+    const char *q_mine = q_lds + row * C::QROW + 8 * g * C::QES;
 
     float m = kNegInf, l = 0.0f;                    // of the lane's query head; l over the lane's keys
     f4 acc[DPL];
 #pragma unroll
     for (int c = 0; c < DPL; c++) acc[c] = f4{0, 0, 0, 0};
 
-    if (from < to) {
-      // queries: head h0 + n, dims 32 s + 8 g ..; scaled so that weights are powers of two
-      float qf[CH][8];
-      float qmax = 0.0f;
-      const float *q = a.q + r * a.q_stride + (long long)(h0 + n) * a.hd;
+    const char *kbase = a.k + kvh * a.hst, *vbase = a.v + kvh * a.hst;
+    int k_off[CH], v_off[C::PIECES];                // padded dims read dim 0: their products are dropped, or with 0
 #pragma unroll
-      for (int s = 0; s < CH; s++)
+    for (int c = 0; c < CH; c++) k_off[c] = 32 * c + 8 * g < a.hd ? (32 * c + 8 * g) * C::ES : 0;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const int d = 32 * s + 8 * g + i;
-          qf[s][i] = n < rows && d < a.hd ? q[d] * a.qscale : 0.0f;
-          qmax = fmaxf(qmax, fabsf(qf[s][i]));
-        }
-      u4 qp[C::PARTS][CH];
-      float unscale = 1.0f;
-      if constexpr (T == QLLAMA_KV_F16) {           // into f16's range, by a power of two
-        qmax = max_groups(qmax);
-        const int e = qmax > 0.0f && qmax < __builtin_inff() ? ilogbf(qmax) : 0;
-        unscale = ldexpf(1.0f, e - 13);
-#pragma unroll
-        for (int s = 0; s < CH; s++) {
-#pragma unroll
-          for (int i = 0; i < 8; i++) qf[s][i] = ldexpf(qf[s][i], 13 - e);
-          const Parts2 p = cut2(qf[s]);
-          qp[0][s] = p.p[0]; qp[1][s] = p.p[1];
-        }
-      } else if constexpr (T != QLLAMA_KV_F32) {
-#pragma unroll
-        for (int s = 0; s < CH; s++) {
-          const Parts3 p = cut3(qf[s]);
-          qp[0][s] = p.p[0]; qp[1][s] = p.p[1]; qp[2][s] = p.p[2];
-        }
+    for (int i = 0; i < C::PIECES; i++) v_off[i] = n * DPL + 8 * i < a.hd ? (n * DPL + 8 * i) * C::ES : 0;
+
+    // page and place of 16-key group i of step s (UNI), or of its key j
+    auto lookup = [&](int s, int i, int j, int *place) -> int {
+      if constexpr (UNI) {
+        const int at = s * SUB + i - win.first;
+        *place = __builtin_amdgcn_readlane(win.place, at) + j;
+        return __builtin_amdgcn_readlane(win.page, at);
+      } else {
+        const int at = s * STEP + 16 * i + j - win.first;
+        *place = __shfl(win.place, at);
+        return __shfl(win.page, at);
       }
-
-      const char *kbase = a.k + kvh * a.hst, *vbase = a.v + kvh * a.hst;
-      int k_off[CH], v_off = n * DPL < a.hd ? n * DPL * C::ES : 0;    // padded dims read dim 0; their products are dropped or with 0
+    };
+    auto advance = [&](int s) {                     // the window holds step s
+      const int at = UNI ? s * SUB : s * STEP;
+      if (at - win.first >= 64) win.load(a, table, at, len);
+    };
+    auto load_k = [&](int s, KTile<T, HDP> &k) {
 #pragma unroll
-      for (int s = 0; s < CH; s++) k_off[s] = 32 * s + 8 * g < a.hd ? (32 * s + 8 * g) * C::ES : 0;
-
-      Window<UNI> win;
-      win.load(a, table, UNI ? from * SUB : from * STEP, len);
-
-      // page and place of 16-key group i of step s (UNI), or of its key j
-      auto lookup = [&](int s, int i, int j, int *place) -> int {
+      for (int i = 0; i < SUB; i++) {
+        int place;
+        int page = lookup(s, i, UNI ? 0 : n, &place);
+        if (page < 0) { page = 0; place = 0; }
+        const char *p = kbase + page * a.pst + place * a.sst;
+        if constexpr (UNI) p += (unsigned)(n * (int)a.sst);
+#pragma unroll
+        for (int c = 0; c < CH; c++) load_words(k.w[i][c], p + k_off[c]);
+      }
+    };
+    auto load_v = [&](int s, VTile<T, HDP> &v) {
+#pragma unroll
+      for (int i = 0; i < SUB; i++) {
+        const char *p = vbase;
         if constexpr (UNI) {
-          const int at = s * SUB + i - win.first;
-          *place = __builtin_amdgcn_readlane(win.place, at) + j;
-          return __builtin_amdgcn_readlane(win.page, at);
-        } else {
-          const int at = s * STEP + 16 * i + j - win.first;
-          *place = __shfl(win.place, at);
-          return __shfl(win.page, at);
+          int place;
+          int page = lookup(s, i, 0, &place);
+          if (page < 0) { page = 0; place = 0; }
+          p += page * a.pst + place * a.sst;
         }
-      };
-      auto advance = [&](int s) {                   // the window holds step s
-        const int at = UNI ? s * SUB : s * STEP;
-        if (at - win.first >= 64) win.load(a, table, at, len);
-      };
-      auto load_k = [&](int s, KTile<T, HDP> &k) {
 #pragma unroll
-        for (int i = 0; i < SUB; i++) {
-          const char *p;
+        for (int j = 0; j < 4; j++) {
+          const char *pj = p;
           if constexpr (UNI) {
-            int place;
-            int page = lookup(s, i, 0, &place);
-            if (page < 0) { page = 0; place = 0; }
-            p = kbase + page * a.pst + place * a.sst + (unsigned)(n * (int)a.sst);
+            pj += (unsigned)((4 * g + j) * (int)a.sst);
           } else {
             int place;
-            int page = lookup(s, i, n, &place);
+            int page = lookup(s, i, 4 * g + j, &place);
             if (page < 0) { page = 0; place = 0; }
-            p = kbase + page * a.pst + place * a.sst;
+            pj += page * a.pst + place * a.sst;
           }
 #pragma unroll
-          for (int c = 0; c < CH; c++) load_words(k.w[i][c], p + k_off[c]);
+          for (int x = 0; x < C::PIECES; x++) load_words(v.w[i][j][x], pj + v_off[x]);
         }
-      };
-      auto load_v = [&](int s, VTile<T, HDP> &v) {
-#pragma unroll
-        for (int i = 0; i < SUB; i++) {
-          const char *p = vbase;
-          if constexpr (UNI) {
-            int place;
-            int page = lookup(s, i, 0, &place);
-            if (page < 0) { page = 0; place = 0; }
-            p += page * a.pst + place * a.sst;
-          }
-#pragma unroll
-          for (int j = 0; j < 4; j++) {
-            const char *pj = p;
-            if constexpr (UNI) {
-              pj += (unsigned)((4 * g + j) * (int)a.sst);
-            } else {
-              int place;
-              int page = lookup(s, i, 4 * g + j, &place);
-              if (page < 0) { page = 0; place = 0; }
-              pj += page * a.pst + place * a.sst;
-            }
-            if constexpr (T == QLLAMA_KV_I8 && C::VW == 4) load_words_8(v.w[i][j], pj + v_off);
-            else load_words(v.w[i][j], pj + v_off);
-          }
-        }
-      };
+      }
+    };
 
-      auto step = [&](int s, KTile<T, HDP> &k, KTile<T, HDP> &k_next) {
-        VTile<T, HDP> v;
-        float ksc[SUB][4], vsc[SUB][4];
-        bool absent = false;                        // some key of the step lies on no page
-        bool out[SUB][4];
-        load_v(s, v);
+    auto step = [&](int s, KTile<T, HDP> &k, KTile<T, HDP> &k_next) {
+      VTile<T, HDP> v;
+      float ksc[SUB][4], vsc[SUB][4];
+      bool out[SUB][4];                             // a key behind the last, or on no page
+      bool absent = (s + 1) * STEP > len;
 #pragma unroll
-        for (int i = 0; i < SUB; i++)
+      for (int i = 0; i < SUB; i++) {
+        int page[4], place[4];
+        if constexpr (UNI) page[0] = lookup(s, i, 0, &place[0]);
 #pragma unroll
-          for (int j = 0; j < 4; j++) {
-            int place, page;
-            if constexpr (UNI) {
-              page = lookup(s, i, 0, &place);
-              place += 4 * g + j;
-            } else {
-              page = lookup(s, i, 4 * g + j, &place);
-            }
-            out[i][j] = page < 0 || s * STEP + 16 * i + 4 * g + j >= len;
-            absent |= out[i][j];
-            if constexpr (T == QLLAMA_KV_I8) {
-              const long long at = out[i][j] ? 0 : page * a.scp + kvh * a.sch + place * a.scs;
+        for (int j = 0; j < 4; j++) {
+          if constexpr (UNI) {
+            page[j] = page[0];
+            place[j] = place[0] + 4 * g + j;
+          } else {
+            page[j] = lookup(s, i, 4 * g + j, &place[j]);
+          }
+          out[i][j] = page[j] < 0 || s * STEP + 16 * i + 4 * g + j >= len;
+          absent |= page[j] < 0;
+        }
+        if constexpr (T == QLLAMA_KV_I8) {
+          if (UNI && a.scs == 1) {                  // 4 keys' scales beside each other, on any 4-byte boundary
+            const long long at = (page[0] < 0 ? 4 * g : page[0] * a.scp + place[0]) + kvh * a.sch;
+            __builtin_memcpy(ksc[i], a.ks + at, sizeof ksc[i]);
+            __builtin_memcpy(vsc[i], a.vs + at, sizeof vsc[i]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              const long long at = out[i][j] ? 0 : page[j] * a.scp + kvh * a.sch + place[j] * a.scs;
               ksc[i][j] = a.ks[at];
               vsc[i][j] = a.vs[at];
             }
           }
-        if (s + 1 < to) {
-          advance(s + 1);
-          load_k(s + 1, k_next);
         }
+      }
+      load_v(s, v);
+      if (s + 1 < to) {
+        advance(s + 1);
+        load_k(s + 1, k_next);
+      }
 
-        // scores of 16 SUB keys for the lane's query head
-        float sc[SUB][4];
+      // scores of 16 SUB keys for the lane's query head
+      f4 d[SUB];
 #pragma unroll
-        for (int i = 0; i < SUB; i++) {
-          f4 d = {0, 0, 0, 0};
+      for (int i = 0; i < SUB; i++) d[i] = f4{0, 0, 0, 0};
+      asm volatile("" ::: "memory");                // the queries are read from LDS in every step, not kept in registers
 #pragma unroll
-          for (int c = 0; c < CH; c++) {
-            if constexpr (T == QLLAMA_KV_F32) {
+      for (int c = 0; c < CH; c++) {
+        const char *qc = q_mine + 32 * c * C::QES;
+        if constexpr (T == QLLAMA_KV_F32) {
+          const f4 q0 = *reinterpret_cast<const f4 *>(qc), q1 = *reinterpret_cast<const f4 *>(qc + 16);
 #pragma unroll
-              for (int e = 0; e < 8; e++) d = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k.w[i][c][e]), qf[c][e], d, 0, 0, 0);
-            } else {
-              u4 kk;
-              if constexpr (T == QLLAMA_KV_I8) {
+          for (int e = 0; e < 8; e++) d[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k.w[0][c][e]), e < 4 ? q0[e % 4] : q1[e % 4], d[0], 0, 0, 0);
+        } else {
+          u4 qp[C::PARTS];
 #pragma unroll
-                for (int w = 0; w < 2; w++) {
-                  const uint32_t x = k.w[i][c][w];
-                  kk[2 * w] = hi16s(__float_as_uint(byte_f<1>(x)), __float_as_uint(byte_f<0>(x)));
-                  kk[2 * w + 1] = hi16s(__float_as_uint(byte_f<3>(x)), __float_as_uint(byte_f<2>(x)));
-                }
-              } else {
-                kk = u4{k.w[i][c][0], k.w[i][c][1], k.w[i][c][2], k.w[i][c][3]};
+          for (int p = 0; p < C::PARTS; p++) qp[p] = *reinterpret_cast<const u4 *>(qc + p * a.rows * C::QROW);
+#pragma unroll
+          for (int i = 0; i < SUB; i++) {
+            u4 kk;
+            if constexpr (T == QLLAMA_KV_I8) {
+#pragma unroll
+              for (int w = 0; w < 2; w++) {
+                const uint32_t x = k.w[i][c][w];
+                kk[2 * w] = hi16s(__float_as_uint(byte_f<1>(x)), __float_as_uint(byte_f<0>(x)));
+                kk[2 * w + 1] = hi16s(__float_as_uint(byte_f<3>(x)), __float_as_uint(byte_f<2>(x)));
               }
-#pragma unroll
-              for (int p = 0; p < C::PARTS; p++) d = mfma16<T>(kk, qp[p][c], d);
+            } else {
+              kk = u4{k.w[i][c][0], k.w[i][c][1], k.w[i][c][2], k.w[i][c][3]};
             }
+#pragma unroll
+            for (int p = 0; p < C::PARTS; p++) d[i] = mfma16<T>(kk, qp[p], d[i]);
           }
+        }
+      }
+      float sc[SUB][4];
+#pragma unroll
+      for (int i = 0; i < SUB; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          sc[i][j] = d[i][j];
+          if constexpr (T == QLLAMA_KV_F16) sc[i][j] *= unscale;
+          if constexpr (T == QLLAMA_KV_I8) sc[i][j] *= ksc[i][j];
+        }
+      if (__any(absent)) {
+#pragma unroll
+        for (int i = 0; i < SUB; i++)
 #pragma unroll
           for (int j = 0; j < 4; j++) {
-            sc[i][j] = d[j];
-            if constexpr (T == QLLAMA_KV_F16) sc[i][j] *= unscale;
-            if constexpr (T == QLLAMA_KV_I8) sc[i][j] *= ksc[i][j];
+            if (out[i][j]) {                        // whatever the slot holds, NaN too, counts nothing
+              sc[i][j] = kNegInf;
+              if constexpr (T == QLLAMA_KV_I8) vsc[i][j] = 0.0f;
+#pragma unroll
+              for (int x = 0; x < C::PIECES; x++)
+#pragma unroll
+                for (int w = 0; w < C::PW; w++) v.w[i][j][x][w] = 0;
+            }
           }
+      }
+
+      float top = sc[0][0];
+#pragma unroll
+      for (int i = 0; i < SUB; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) top = fmaxf(top, sc[i][j]);
+      top = fmaxf(m, max_groups(top));
+      if (__any(top > m)) {                         // rare after the first steps
+        const float f = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+        l *= f;
+#pragma unroll
+        for (int c = 0; c < DPL; c++) acc[c] *= f;
+        m = top;
+      }
+      const float ref = (m == kNegInf ? 0.0f : m) - C::SHIFT;
+      float p[SUB][4];
+#pragma unroll
+      for (int i = 0; i < SUB; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          p[i][j] = __builtin_amdgcn_exp2f(sc[i][j] - ref);
+          l += p[i][j];
+          if constexpr (T == QLLAMA_KV_I8) p[i][j] *= vsc[i][j];
         }
-        if (__any(absent)) {
+
+      if constexpr (T == QLLAMA_KV_F32) {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+          for (int c = 0; c < DPL; c++)
+            acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v.w[0][j][c / 8][c % 8]), p[0][j], acc[c], 0, 0, 0);
+      } else {
+        const float pf[8] = {p[0][0], p[0][1], p[0][2], p[0][3], p[SUB - 1][0], p[SUB - 1][1], p[SUB - 1][2], p[SUB - 1][3]};
+        u4 pp[C::PARTS];
+        if constexpr (T == QLLAMA_KV_F16) {
+          const Parts2 x = cut2(pf);
+          pp[0] = x.p[0]; pp[1] = x.p[1];
+        } else {
+          const Parts3 x = cut3(pf);
+          pp[0] = x.p[0]; pp[1] = x.p[1]; pp[2] = x.p[2];
+        }
+#pragma unroll
+        for (int c = 0; c < DPL; c++) {
+          u4 vv;                                    // dim c of the lane's piece, 8 keys
 #pragma unroll
           for (int i = 0; i < SUB; i++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-              if (out[i][j]) {                      // whatever the slot holds, NaN too, counts nothing
-                sc[i][j] = kNegInf;
-                if constexpr (T == QLLAMA_KV_I8) vsc[i][j] = 0.0f;
-#pragma unroll
-                for (int w = 0; w < C::VW; w++) v.w[i][j][w] = 0;
+            for (int j = 0; j < 2; j++) {
+              const uint32_t *x = v.w[i][2 * j][c / 8], *y = v.w[i][2 * j + 1][c / 8];
+              if constexpr (T == QLLAMA_KV_I8) {
+                const uint32_t xa = x[c % 8 / 4] >> (8 * (c % 4)), ya = y[c % 8 / 4] >> (8 * (c % 4));
+                vv[2 * i + j] = hi16s(__float_as_uint(byte_f<0>(ya)), __float_as_uint(byte_f<0>(xa)));
+              } else {
+                vv[2 * i + j] = c % 2 ? hi16s(y[c % 8 / 2], x[c % 8 / 2]) : lo16s(y[c % 8 / 2], x[c % 8 / 2]);
               }
             }
+#pragma unroll
+          for (int k = 0; k < C::PARTS; k++) acc[c] = mfma16<T>(vv, pp[k], acc[c]);
         }
-
-        float top = sc[0][0];
-#pragma unroll
-        for (int i = 0; i < SUB; i++)
-#pragma unroll
-          for (int j = 0; j < 4; j++) top = fmaxf(top, sc[i][j]);
-        top = fmaxf(m, max_groups(top));
-        if (__any(top > m)) {                       // rare after the first steps
-          const float f = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - top);
-          l *= f;
-#pragma unroll
-          for (int c = 0; c < DPL; c++) acc[c] *= f;
-          m = top;
-        }
-        const float ref = (m == kNegInf ? 0.0f : m) - C::SHIFT;
-        float p[SUB][4];
-#pragma unroll
-        for (int i = 0; i < SUB; i++)
-#pragma unroll
-          for (int j = 0; j < 4; j++) {
-            p[i][j] = __builtin_amdgcn_exp2f(sc[i][j] - ref);
-            l += p[i][j];
-            if constexpr (T == QLLAMA_KV_I8) p[i][j] *= vsc[i][j];
-          }
-
-        if constexpr (T == QLLAMA_KV_F32) {
-#pragma unroll
-          for (int j = 0; j < 4; j++)
-#pragma unroll
-            for (int c = 0; c < DPL; c++) acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v.w[0][j][c]), p[0][j], acc[c], 0, 0, 0);
-        } else {
-          const float pf[8] = {p[0][0], p[0][1], p[0][2], p[0][3], p[SUB - 1][0], p[SUB - 1][1], p[SUB - 1][2], p[SUB - 1][3]};
-          u4 pp[C::PARTS];
-          if constexpr (T == QLLAMA_KV_F16) {
-            const Parts2 x = cut2(pf);
-            pp[0] = x.p[0]; pp[1] = x.p[1];
-          } else {
-            const Parts3 x = cut3(pf);
-            pp[0] = x.p[0]; pp[1] = x.p[1]; pp[2] = x.p[2];
-          }
-#pragma unroll
-          for (int c = 0; c < DPL; c++) {
-            u4 vv;                                  // dim c of the lane's piece, 8 keys
-#pragma unroll
-            for (int i = 0; i < SUB; i++)
-#pragma unroll
-              for (int j = 0; j < 2; j++) {
-                const uint32_t *x = v.w[i][2 * j], *y = v.w[i][2 * j + 1];
-                if constexpr (T == QLLAMA_KV_I8) {
-                  const uint32_t xa = x[c / 4] >> (8 * (c % 4)), ya = y[c / 4] >> (8 * (c % 4));
-                  vv[2 * i + j] = hi16s(__float_as_uint(byte_f<0>(ya)), __float_as_uint(byte_f<0>(xa)));
-                } else {
-                  vv[2 * i + j] = c % 2 ? hi16s(y[c / 2], x[c / 2]) : lo16s(y[c / 2], x[c / 2]);
-                }
-              }
-#pragma unroll
-            for (int k = 0; k < C::PARTS; k++) acc[c] = mfma16<T>(vv, pp[k], acc[c]);
-          }
-        }
-      };
-
-      KTile<T, HDP> k0, k1;
-      load_k(from, k0);
-      for (int s = from; s < to; s += 2) {
-        step(s, k0, k1);
-        if (s + 1 < to) step(s + 1, k1, k0);
       }
-      l = sum_groups(l);
-    }
+    };
 
-    // the waves' results together; lane (n, g) holds head n, dims (4 g + i) DPL + c
-    if (g == 0) { s_m[wave][n] = m; s_l[wave][n] = l; }
-    __syncthreads();
-    float top = kNegInf;
-#pragma unroll
-    for (int w = 0; w < kWaves; w++) top = fmaxf(top, s_m[w][n]);
-    const float f = part_weight(m, top);
+    KTile<T, HDP> k0, k1;
+    load_k(from, k0);
+    for (int s = from; s < to; s += 2) {
+      step(s, k0, k1);
+      if (s + 1 < to) step(s + 1, k1, k0);
+    }
+    l = sum_groups(l);
+
+    // lane (n, g) holds head n, dims (4 g + i) DPL + c
+    const bool whole = from == 0 && to == steps;
+    float *o = a.part + ((long long)id * 2 + (u == begin ? 0 : 1)) * (a.rows * (a.hd + 2)) + row * (a.hd + 2), by = 1.0f;
+    if (whole) {
+      o = a.o + r * a.o_stride + (long long)(h0 + row) * a.hd;
+      by = l == 0.0f ? 0.0f : 1.0f / l;
+    }
     if (n < rows) {
 #pragma unroll
       for (int i = 0; i < 4; i++)
 #pragma unroll
-        for (int c = 0; c < DPL; c++) dyn[(wave * a.rows + n) * HDP + (4 * g + i) * DPL + c] = acc[c][i] * f;
-    }
-    __syncthreads();
-    const bool whole = s0 == 0 && s1 == steps;
-    float *part = a.part + (blockIdx.x * 2 + (u == begin ? 0 : 1)) * ((long long)a.rows * (a.hd + 2));
-    for (int i = threadIdx.x; i < rows * a.hd; i += kThreads) {
-      const int row = i / a.hd, d = i - row * a.hd;
-      float t = kNegInf, sum = 0.0f, x = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kWaves; w++) t = fmaxf(t, s_m[w][row]);
-#pragma unroll
-      for (int w = 0; w < kWaves; w++) {
-        x += dyn[(w * a.rows + row) * HDP + d];
-        sum += s_l[w][row] * part_weight(s_m[w][row], t);
-      }
-      if (whole) {
-        a.o[r * a.o_stride + (long long)(h0 + row) * a.hd + d] = sum == 0.0f ? 0.0f : x / sum;
-        if (d == 0 && a.lse) a.lse[r * a.lse_stride + h0 + row] = sum == 0.0f ? kNegInf : (t - C::SHIFT + __builtin_amdgcn_logf(sum)) * 0.69314718056f;
-      } else {
-        part[row * (a.hd + 2) + d] = x;
-        if (d == 0) {
-          part[row * (a.hd + 2) + a.hd] = t;
-          part[row * (a.hd + 2) + a.hd + 1] = sum;
+        for (int c = 0; c < DPL; c += 4) {
+          const float x[4] = {acc[c][i] * by, acc[c + 1][i] * by, acc[c + 2][i] * by, acc[c + 3][i] * by};
+          if ((4 * g + i) * DPL + c < a.hd) __builtin_memcpy(o + (4 * g + i) * DPL + c, x, sizeof x);
+        }
+      if (g == 0) {
+        if (!whole) {
+          o[a.hd] = m;
+          o[a.hd + 1] = l;
+        } else if (a.lse) {
+          a.lse[r * a.lse_stride + h0 + row] = l == 0.0f ? kNegInf : (m - C::SHIFT + __builtin_amdgcn_logf(l)) * 0.69314718056f;
         }
       }
     }
-    __syncthreads();
-    u += s1 - s0;
+    u += to - from;
   }
 }
 
 // One block a request and query head: the parts of its tile put together in the order
-// of their keys; rows without a token are set.
+// of their keys; requests without a token are set.
 constexpr int kJoinThreads = 128;
 __global__ __launch_bounds__(kJoinThreads) void k_paged_join(PaArgs a, int step, float shift) {
   __shared__ long long lds[kJoinThreads / 64];
+  __shared__ float weight[kShares], total[kShares], tops[kJoinThreads / 64];
   const int r = blockIdx.x, h = blockIdx.y;
   const int kvh = h / a.G, row = (h - kvh * a.G) % 16, tile = kvh * a.tiles + (h - kvh * a.G) / 16;
   const int tiles = a.n_kv * a.tiles;
@@ -585,23 +608,33 @@ __global__ __launch_bounds__(kJoinThreads) void k_paged_join(PaArgs a, int step,
   }
   const long long share = share_of(units), u0 = before + (long long)tile * steps, u1 = u0 + steps;
   const int b0 = (int)(u0 / share), b1 = (int)((u1 - 1) / share);
-  if (b0 == b1) return;                              // written by its block
-  const long long one = (long long)a.rows * (a.hd + 2);
-  const float *part = a.part + (long long)row * (a.hd + 2);
-  const int slot0 = u0 == b0 * share ? 0 : 1;        // the first part may follow another tile's in its block
+  if (b0 == b1) return;                              // written by its wave
+  const int one = a.rows * (a.hd + 2);
+  // the first part may follow another tile's in its share
+  const float *part = a.part + (2LL * b0) * one + row * (a.hd + 2);
+  const int first = u0 == b0 * share ? 0 : one, parts = b1 - b0 + 1;
   float top = kNegInf;
-  for (int b = b0; b <= b1; b++) top = fmaxf(top, part[(2LL * b + (b == b0 ? slot0 : 0)) * one + a.hd]);
-  for (int d = threadIdx.x; d < a.hd; d += kJoinThreads) {
-    float x = 0.0f, sum = 0.0f;
-    for (int b = b0; b <= b1; b++) {
-      const float *p = part + (2LL * b + (b == b0 ? slot0 : 0)) * one;
-      const float f = part_weight(p[a.hd], top);
-      x += p[d] * f;
-      sum += p[a.hd + 1] * f;
-    }
-    o[d] = sum == 0.0f ? 0.0f : x / sum;
-    if (d == 0 && a.lse) a.lse[r * a.lse_stride + h] = sum == 0.0f ? kNegInf : (top - shift + __builtin_amdgcn_logf(sum)) * 0.69314718056f;
+  for (int i = threadIdx.x; i < parts; i += kJoinThreads) {
+    const float *p = part + 2LL * i * one + (i ? 0 : first) + a.hd;
+    weight[i] = p[0];
+    total[i] = p[1];
+    top = fmaxf(top, p[0]);
   }
+  for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+  __syncthreads();
+  for (int i = 0; i < kJoinThreads / 64; i++) top = fmaxf(top, tops[i]);
+  for (int i = threadIdx.x; i < parts; i += kJoinThreads) weight[i] = part_weight(weight[i], top);
+  __syncthreads();
+  float sum = 0.0f;
+  for (int i = 0; i < parts; i++) sum += total[i] * weight[i];
+  for (int d = threadIdx.x; d < a.hd; d += kJoinThreads) {
+    float x = part[first + d] * weight[0];
+#pragma unroll 8
+    for (int i = 1; i < parts; i++) x += part[2LL * i * one + d] * weight[i];
+    o[d] = sum == 0.0f ? 0.0f : x / sum;
+  }
+  if (threadIdx.x == 0 && a.lse) a.lse[r * a.lse_stride + h] = sum == 0.0f ? kNegInf : (top - shift + __builtin_amdgcn_logf(sum)) * 0.69314718056f;
 }
 
 int rows_of(const QPagedKV *c, int n_heads) {
@@ -611,9 +644,9 @@ int rows_of(const QPagedKV *c, int n_heads) {
 
 template <int T, int HDP>
 int launch(const char *fn, const PaArgs &a, hipStream_t stream) {
-  const size_t lds = (size_t)kWaves * a.rows * HDP * sizeof(float);
+  const size_t lds = (size_t)kWaves * Cfg<T, HDP>::PARTS * a.rows * Cfg<T, HDP>::QROW;
   const bool uni = a.page_size % 16 == 0;
-  if (lds > 60 * 1024) {              // 16 rows of 256 dims: past what a launch may take unasked
+  if (lds > 64 * 1024) {              // past what a launch may take unasked
     const void *f = uni ? reinterpret_cast<const void *>(k_paged_attn<T, HDP, true>) : reinterpret_cast<const void *>(k_paged_attn<T, HDP, false>);
     if (hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) {
       (void)hipGetLastError();
@@ -639,7 +672,7 @@ extern "C" int qllama_test_page_of(const int32_t *table, int width, int page_siz
 
 extern "C" size_t qllama_paged_attention_work(const QPagedKV *c, int n_req, int n_heads) {
   if (qs::bad_cache(c) || n_req < 0 || n_heads < 1 || n_heads > 65535 || n_heads % c->n_kv) return 0;
-  return (size_t)kBlocks * 2 * rows_of(c, n_heads) * (c->head_dim + 2) * sizeof(float);
+  return (size_t)kShares * 2 * rows_of(c, n_heads) * (c->head_dim + 2) * sizeof(float);
 }
 
 extern "C" int qllama_paged_attention(const QPagedKV *c, const QPagedQuery *a, void *stream) {
@@ -653,6 +686,8 @@ extern "C" int qllama_paged_attention(const QPagedKV *c, const QPagedQuery *a, v
   if (a->q_stride < qd || a->o_stride < qd || (a->lse && a->lse_stride < a->n_heads)) return qs::refuse(fn, "a row stride below the row's length");
   if (a->width < 1 || a->table_stride < a->width || (int64_t)a->width * c->page_size > INT_MAX)
     return qs::refuse(fn, "bad table width (width * page_size must fit in 31 bits) or stride");
+  if ((int64_t)a->n_req * (((int64_t)a->width * c->page_size + 15) / 16) > INT_MAX)
+    return qs::refuse(fn, "n_req * width * page_size is too large");
   if (!(a->scale >= 0.0f) || a->scale > 3.0e38f) return qs::refuse(fn, "scale must be finite and not negative");
   if (a->q == a->o) return qs::refuse(fn, "o must not be q");
   if (qs::misaligned(a->q, 4) || qs::misaligned(a->o, 4) || qs::misaligned(a->lse, 4) || qs::misaligned(a->table, 4) || qs::misaligned(a->lens, 4))
