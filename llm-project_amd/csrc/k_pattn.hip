@@ -48,6 +48,7 @@ struct PaArgs {
   float *o, *lse;
   const int *table, *lens;
   float *part;
+  int4 *split;
   long long pst, hst, sst;            // bytes
   long long scp, sch, scs;            // floats
   long long q_stride, o_stride, lse_stride, table_stride;
@@ -68,17 +69,6 @@ __host__ __device__ inline int page_of(const int *table, long long key, int len,
   if (p < 0 || p >= n_pages) return -1;
   *place = (int)key - e * page_size;
   return p;
-}
-
-// Sum over the block of one int64 a thread.
-__device__ long long block_sum(long long v, long long *lds) {
-  for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = 0;
-  for (int i = 0; i < (int)(blockDim.x >> 6); i++) v += lds[i];
-  __syncthreads();
-  return v;
 }
 
 // Steps of a wave's share when all tiles together take `units`.
@@ -104,21 +94,19 @@ __device__ inline float sum_groups(float x) {
   return x + __shfl_xor(x, 32);
 }
 
-template <int W>
+// W words of a row; STREAM: read once, so past the caches' retention
+template <bool STREAM, int W>
 __device__ inline void load_words(uint32_t (&d)[W], const char *p) {
+  typedef uint32_t vec __attribute__((ext_vector_type(W), aligned(W > 2 ? 8 : 4)));
   if constexpr (W == 1) {
     d[0] = *reinterpret_cast<const uint32_t *>(p);
-  } else if constexpr (W == 2) {
-    const u2 x = *reinterpret_cast<const u2 *>(p);
-    d[0] = x.x; d[1] = x.y;
   } else {
+    const vec x = STREAM ? __builtin_nontemporal_load(reinterpret_cast<const vec *>(p)) : *reinterpret_cast<const vec *>(p);
 #pragma unroll
-    for (int i = 0; i < W / 4; i++) {
-      const u4 x = *reinterpret_cast<const u4 *>(p + 16 * i);
-      d[4 * i] = x.x; d[4 * i + 1] = x.y; d[4 * i + 2] = x.z; d[4 * i + 3] = x.w;
-    }
+    for (int i = 0; i < W; i++) d[i] = x[i];
   }
 }
+
 __device__ inline uint32_t hi16s(uint32_t b, uint32_t a) { return __builtin_amdgcn_perm(b, a, 0x07060302); }
 __device__ inline uint32_t lo16s(uint32_t b, uint32_t a) { return __builtin_amdgcn_perm(b, a, 0x05040100); }
 template <int B>
@@ -170,13 +158,14 @@ struct Cfg {
   static constexpr int ES = T == QLLAMA_KV_F32 ? 4 : T == QLLAMA_KV_I8 ? 1 : 2;
   static constexpr int SUB = T == QLLAMA_KV_F32 ? 1 : 2;       // 16-key groups of a step
   static constexpr int STEP = 16 * SUB;
-  static constexpr int CH = HDP / 32;                          // 8-dim pieces of a key that a lane loads
-  static constexpr int KW = 8 * ES / 4;                        // words of such a piece
-  static constexpr int DPL = HDP / 16;                         // dims of a value row that a lane loads
-  static constexpr int VW = DPL * ES / 4;
-  static constexpr int PIECES = DPL > 8 ? 2 : 1, PW = VW / PIECES;    // a piece: at most 8 dims, as head_dim is a multiple of 8
+  // a key's row: load x takes bytes 64 x + 16 g .. of it in lane (key, g), EL elements
+  static constexpr int KL = HDP * ES / 64, EL = 16 / ES;
+  // a value row: piece x of lane (n, g) takes dims 16 PD x + PD n .. of key 4 g + j
+  static constexpr int PB0 = HDP * ES / 16, PB1 = PB0 < 16 ? PB0 : 16, PB = PB1 < 8 * ES ? PB1 : 8 * ES;
+  static constexpr int PD = PB / ES, PIECES = HDP / (16 * PD), PW = PB / 4;
+  static constexpr int DPL = HDP / 16;                         // dims of a value row in a lane
   static constexpr int PARTS = T == QLLAMA_KV_F32 ? 1 : T == QLLAMA_KV_F16 ? 2 : 3;
-  // a query row in LDS: its parts' values, and 64 bytes that spread rows over the banks
+  // a query row in LDS: a part's values, and 64 bytes that spread rows over the banks
   static constexpr int QES = T == QLLAMA_KV_F32 ? 4 : 2;
   static constexpr int QROW = HDP * QES + 64;
   // 2^SHIFT times the weights: f16 parts then keep 22 bits down to 2^-18 of the largest
@@ -185,7 +174,7 @@ struct Cfg {
 };
 
 template <int T, int HDP>
-struct KTile { uint32_t w[Cfg<T, HDP>::SUB][Cfg<T, HDP>::CH][Cfg<T, HDP>::KW]; };
+struct KTile { uint32_t w[Cfg<T, HDP>::SUB][Cfg<T, HDP>::KL][4]; };
 template <int T, int HDP>
 struct VTile { uint32_t w[Cfg<T, HDP>::SUB][4][Cfg<T, HDP>::PIECES][Cfg<T, HDP>::PW]; };
 
@@ -204,10 +193,10 @@ struct Window {
   }
 };
 
-template <int T, int HDP, bool UNI>
+template <int T, int HDP, bool UNI, bool STREAM>
 __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaArgs a) {
   using C = Cfg<T, HDP>;
-  constexpr int SUB = C::SUB, STEP = C::STEP, CH = C::CH, DPL = C::DPL;
+  constexpr int SUB = C::SUB, STEP = C::STEP, CH = HDP / 32, DPL = C::DPL;
   extern __shared__ __align__(16) char dyn[];       // a wave's queries: [part][row]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;           // key, query head or value piece; group of 16 lanes
@@ -227,11 +216,11 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
   const int id = wave * kBlocks + blockIdx.x;
   long long u = id * share;
   const long long end = u + share < units ? u + share : units;
-  if (u >= end) return;
+  if (lane == 0) a.split[id] = make_int4(0, 0, 0, 0);
   const long long begin = u;
   int r = 0;                                        // the request it begins in, and that one's first unit
   long long r_begin = 0;
-  for (;; r += 64) {
+  for (; u < end; r += 64) {
     if (a.n_req > 64) mine = r + lane < a.n_req ? (clamp_len(a.lens[r + lane], a.width, a.page_size) + STEP - 1) / STEP : 0;
     int s = mine;
     for (int d = 1; d < 64; d <<= 1) {
@@ -316,7 +305,7 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
       __builtin_amdgcn_wave_barrier();
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
-    const char *q_mine = q_lds + row * C::QROW + 8 * g * C::QES;
+    const char *q_mine = q_lds + row * C::QROW;
 
     float m = kNegInf, l = 0.0f;                    // of the lane's query head; l over the lane's keys
     f4 acc[DPL];
@@ -324,11 +313,11 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
     for (int c = 0; c < DPL; c++) acc[c] = f4{0, 0, 0, 0};
 
     const char *kbase = a.k + kvh * a.hst, *vbase = a.v + kvh * a.hst;
-    int k_off[CH], v_off[C::PIECES];                // padded dims read dim 0: their products are dropped, or with 0
+    int k_off[C::KL], v_off[C::PIECES];             // padded dims read dim 0: their products are dropped, or with 0
 #pragma unroll
-    for (int c = 0; c < CH; c++) k_off[c] = 32 * c + 8 * g < a.hd ? (32 * c + 8 * g) * C::ES : 0;
+    for (int x = 0; x < C::KL; x++) k_off[x] = 64 * x + 16 * g < a.hd * C::ES ? 64 * x + 16 * g : 0;
 #pragma unroll
-    for (int i = 0; i < C::PIECES; i++) v_off[i] = n * DPL + 8 * i < a.hd ? (n * DPL + 8 * i) * C::ES : 0;
+    for (int x = 0; x < C::PIECES; x++) v_off[x] = 16 * C::PD * x + C::PD * n < a.hd ? (16 * C::PD * x + C::PD * n) * C::ES : 0;
 
     // page and place of 16-key group i of step s (UNI), or of its key j
     auto lookup = [&](int s, int i, int j, int *place) -> int {
@@ -355,7 +344,16 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
         const char *p = kbase + page * a.pst + place * a.sst;
         if constexpr (UNI) p += (unsigned)(n * (int)a.sst);
 #pragma unroll
-        for (int c = 0; c < CH; c++) load_words(k.w[i][c], p + k_off[c]);
+        for (int x = 0; x < C::KL; x++) {
+          if (T != QLLAMA_KV_I8 || a.hd % 16 == 0) {
+            load_words<STREAM>(k.w[i][x], p + k_off[x]);
+          } else {                                  // the row may end within the 16 bytes
+            uint32_t lo[2], hi[2];
+            load_words<STREAM>(lo, p + k_off[x]);
+            load_words<STREAM>(hi, p + (64 * x + 16 * g + 8 < a.hd ? k_off[x] + 8 : 0));
+            k.w[i][x][0] = lo[0]; k.w[i][x][1] = lo[1]; k.w[i][x][2] = hi[0]; k.w[i][x][3] = hi[1];
+          }
+        }
       }
     };
     auto load_v = [&](int s, VTile<T, HDP> &v) {
@@ -380,7 +378,7 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
             pj += page * a.pst + place * a.sst;
           }
 #pragma unroll
-          for (int x = 0; x < C::PIECES; x++) load_words(v.w[i][j][x], pj + v_off[x]);
+          for (int x = 0; x < C::PIECES; x++) load_words<STREAM>(v.w[i][j][x], pj + v_off[x]);
         }
       }
     };
@@ -432,31 +430,34 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
       for (int i = 0; i < SUB; i++) d[i] = f4{0, 0, 0, 0};
       asm volatile("" ::: "memory");                // the queries are read from LDS in every step, not kept in registers
 #pragma unroll
-      for (int c = 0; c < CH; c++) {
-        const char *qc = q_mine + 32 * c * C::QES;
+      for (int x = 0; x < C::KL; x++) {
         if constexpr (T == QLLAMA_KV_F32) {
-          const f4 q0 = *reinterpret_cast<const f4 *>(qc), q1 = *reinterpret_cast<const f4 *>(qc + 16);
+          const f4 q = *reinterpret_cast<const f4 *>(q_mine + 64 * x + 16 * g);
 #pragma unroll
-          for (int e = 0; e < 8; e++) d[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k.w[0][c][e]), e < 4 ? q0[e % 4] : q1[e % 4], d[0], 0, 0, 0);
+          for (int e = 0; e < 4; e++) d[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k.w[0][x][e]), q[e], d[0], 0, 0, 0);
         } else {
-          u4 qp[C::PARTS];
 #pragma unroll
-          for (int p = 0; p < C::PARTS; p++) qp[p] = *reinterpret_cast<const u4 *>(qc + p * a.rows * C::QROW);
+          for (int h = 0; h < C::EL / 8; h++) {     // 8 dims an MFMA
+            u4 qp[C::PARTS];
 #pragma unroll
-          for (int i = 0; i < SUB; i++) {
-            u4 kk;
-            if constexpr (T == QLLAMA_KV_I8) {
+            for (int p = 0; p < C::PARTS; p++)
+              qp[p] = *reinterpret_cast<const u4 *>(q_mine + p * a.rows * C::QROW + ((64 * x + 16 * g) / C::ES + 8 * h) * 2);
 #pragma unroll
-              for (int w = 0; w < 2; w++) {
-                const uint32_t x = k.w[i][c][w];
-                kk[2 * w] = hi16s(__float_as_uint(byte_f<1>(x)), __float_as_uint(byte_f<0>(x)));
-                kk[2 * w + 1] = hi16s(__float_as_uint(byte_f<3>(x)), __float_as_uint(byte_f<2>(x)));
+            for (int i = 0; i < SUB; i++) {
+              u4 kk;
+              if constexpr (T == QLLAMA_KV_I8) {
+#pragma unroll
+                for (int w = 0; w < 2; w++) {
+                  const uint32_t b = k.w[i][x][2 * h + w];
+                  kk[2 * w] = hi16s(__float_as_uint(byte_f<1>(b)), __float_as_uint(byte_f<0>(b)));
+                  kk[2 * w + 1] = hi16s(__float_as_uint(byte_f<3>(b)), __float_as_uint(byte_f<2>(b)));
+                }
+              } else {
+                kk = u4{k.w[i][x][0], k.w[i][x][1], k.w[i][x][2], k.w[i][x][3]};
               }
-            } else {
-              kk = u4{k.w[i][c][0], k.w[i][c][1], k.w[i][c][2], k.w[i][c][3]};
-            }
 #pragma unroll
-            for (int p = 0; p < C::PARTS; p++) d[i] = mfma16<T>(kk, qp[p], d[i]);
+              for (int p = 0; p < C::PARTS; p++) d[i] = mfma16<T>(kk, qp[p], d[i]);
+            }
           }
         }
       }
@@ -514,7 +515,7 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
         for (int j = 0; j < 4; j++)
 #pragma unroll
           for (int c = 0; c < DPL; c++)
-            acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v.w[0][j][c / 8][c % 8]), p[0][j], acc[c], 0, 0, 0);
+            acc[c] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v.w[0][j][c / C::PD][c % C::PD]), p[0][j], acc[c], 0, 0, 0);
       } else {
         const float pf[8] = {p[0][0], p[0][1], p[0][2], p[0][3], p[SUB - 1][0], p[SUB - 1][1], p[SUB - 1][2], p[SUB - 1][3]};
         u4 pp[C::PARTS];
@@ -532,12 +533,13 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
           for (int i = 0; i < SUB; i++)
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-              const uint32_t *x = v.w[i][2 * j][c / 8], *y = v.w[i][2 * j + 1][c / 8];
+              const uint32_t *x = v.w[i][2 * j][c / C::PD], *y = v.w[i][2 * j + 1][c / C::PD];
+              constexpr int PD = C::PD;
               if constexpr (T == QLLAMA_KV_I8) {
-                const uint32_t xa = x[c % 8 / 4] >> (8 * (c % 4)), ya = y[c % 8 / 4] >> (8 * (c % 4));
+                const uint32_t xa = x[c % PD / 4] >> (8 * (c % 4)), ya = y[c % PD / 4] >> (8 * (c % 4));
                 vv[2 * i + j] = hi16s(__float_as_uint(byte_f<0>(ya)), __float_as_uint(byte_f<0>(xa)));
               } else {
-                vv[2 * i + j] = c % 2 ? hi16s(y[c % 8 / 2], x[c % 8 / 2]) : lo16s(y[c % 8 / 2], x[c % 8 / 2]);
+                vv[2 * i + j] = c % 2 ? hi16s(y[c % PD / 2], x[c % PD / 2]) : lo16s(y[c % PD / 2], x[c % PD / 2]);
               }
             }
 #pragma unroll
@@ -554,7 +556,7 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
     }
     l = sum_groups(l);
 
-    // lane (n, g) holds head n, dims (4 g + i) DPL + c
+    // lane (n, g) holds head n; acc[c][i] is dim c mod PD of the piece of lane 4 g + i
     const bool whole = from == 0 && to == steps;
     float *o = a.part + ((long long)id * 2 + (u == begin ? 0 : 1)) * (a.rows * (a.hd + 2)) + row * (a.hd + 2), by = 1.0f;
     if (whole) {
@@ -567,7 +569,8 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
 #pragma unroll
         for (int c = 0; c < DPL; c += 4) {
           const float x[4] = {acc[c][i] * by, acc[c + 1][i] * by, acc[c + 2][i] * by, acc[c + 3][i] * by};
-          if ((4 * g + i) * DPL + c < a.hd) __builtin_memcpy(o + (4 * g + i) * DPL + c, x, sizeof x);
+          const int d = 16 * C::PD * (c / C::PD) + C::PD * (4 * g + i) + c % C::PD;
+          if (d < a.hd) __builtin_memcpy(o + d, x, sizeof x);
         }
       if (g == 0) {
         if (!whole) {
@@ -578,61 +581,73 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
         }
       }
     }
+    if (from == 0 && !whole && lane == 0)            // the tile goes on in the shares behind this one
+      a.split[id] = make_int4(1 + (int)((steps - to + share - 1) / share), r, tile, u == begin ? 0 : 1);
     u += to - from;
   }
+
+  // a request without a token has no tile: its outputs are set here
+  for (int e = id; e < a.n_req; e += kShares)
+    if (a.lens[e] <= 0)
+      for (int i = lane; i < a.n_heads * a.hd; i += 64) {
+        a.o[e * a.o_stride + i] = 0.0f;
+        if (a.lse && i < a.n_heads) a.lse[e * a.lse_stride + i] = kNegInf;
+      }
 }
 
-// One block a request and query head: the parts of its tile put together in the order
-// of their keys; requests without a token are set.
-constexpr int kJoinThreads = 128;
-__global__ __launch_bounds__(kJoinThreads) void k_paged_join(PaArgs a, int step, float shift) {
-  __shared__ long long lds[kJoinThreads / 64];
-  __shared__ float weight[kShares], total[kShares], tops[kJoinThreads / 64];
-  const int r = blockIdx.x, h = blockIdx.y;
-  const int kvh = h / a.G, row = (h - kvh * a.G) % 16, tile = kvh * a.tiles + (h - kvh * a.G) / 16;
-  const int tiles = a.n_kv * a.tiles;
-  long long before = 0, units = 0;
-  for (int i = threadIdx.x; i < a.n_req; i += kJoinThreads) {
-    const long long s = (clamp_len(a.lens[i], a.width, a.page_size) + step - 1) / step;
-    units += s;
-    if (i < r) before += s;
-  }
-  before = block_sum(before, lds) * tiles;
-  units = block_sum(units, lds) * tiles;
-  const int steps = (clamp_len(a.lens[r], a.width, a.page_size) + step - 1) / step;
-  float *o = a.o + r * a.o_stride + (long long)h * a.hd;
-  if (!steps) {
-    for (int d = threadIdx.x; d < a.hd; d += kJoinThreads) o[d] = 0.0f;
-    if (threadIdx.x == 0 && a.lse) a.lse[r * a.lse_stride + h] = kNegInf;
-    return;
-  }
-  const long long share = share_of(units), u0 = before + (long long)tile * steps, u1 = u0 + steps;
-  const int b0 = (int)(u0 / share), b1 = (int)((u1 - 1) / share);
-  if (b0 == b1) return;                              // written by its wave
+// One block a share and row: where a tile begins in the share and goes on behind it, its
+// parts put together in the order of their keys, 8 (hd <= 128) or 4 side by side.
+constexpr int kJoinThreads = 256;
+__global__ __launch_bounds__(kJoinThreads) void k_paged_join(PaArgs a, float shift) {
+  __shared__ float weight[kShares], lds[kJoinThreads / 32][256], red[2][kJoinThreads / 64];
+  const int4 s = a.split[blockIdx.x];
+  const int parts = s.x, r = s.y, tile = s.z, row = blockIdx.y;
+  const int kvh = tile / a.tiles, h = kvh * a.G + (tile % a.tiles) * 16 + row;
+  if (!parts || h >= (kvh + 1) * a.G) return;
   const int one = a.rows * (a.hd + 2);
   // the first part may follow another tile's in its share
-  const float *part = a.part + (2LL * b0) * one + row * (a.hd + 2);
-  const int first = u0 == b0 * share ? 0 : one, parts = b1 - b0 + 1;
+  const float *part = a.part + 2LL * blockIdx.x * one + row * (a.hd + 2);
+  const int first = s.w * one;
   float top = kNegInf;
   for (int i = threadIdx.x; i < parts; i += kJoinThreads) {
-    const float *p = part + 2LL * i * one + (i ? 0 : first) + a.hd;
-    weight[i] = p[0];
-    total[i] = p[1];
-    top = fmaxf(top, p[0]);
+    weight[i] = part[2LL * i * one + (i ? 0 : first) + a.hd];
+    top = fmaxf(top, weight[i]);
   }
   for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-  if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+  if ((threadIdx.x & 63) == 0) red[0][threadIdx.x >> 6] = top;
   __syncthreads();
-  for (int i = 0; i < kJoinThreads / 64; i++) top = fmaxf(top, tops[i]);
-  for (int i = threadIdx.x; i < parts; i += kJoinThreads) weight[i] = part_weight(weight[i], top);
-  __syncthreads();
+  for (int i = 0; i < kJoinThreads / 64; i++) top = fmaxf(top, red[0][i]);
   float sum = 0.0f;
-  for (int i = 0; i < parts; i++) sum += total[i] * weight[i];
-  for (int d = threadIdx.x; d < a.hd; d += kJoinThreads) {
-    float x = part[first + d] * weight[0];
+  for (int i = threadIdx.x; i < parts; i += kJoinThreads) {
+    weight[i] = part_weight(weight[i], top);
+    sum += part[2LL * i * one + (i ? 0 : first) + a.hd + 1] * weight[i];
+  }
+  for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+  if ((threadIdx.x & 63) == 0) red[1][threadIdx.x >> 6] = sum;
+  __syncthreads();
+  sum = 0.0f;
+  for (int i = 0; i < kJoinThreads / 64; i++) sum += red[1][i];
+
+  const int width = a.hd <= 128 ? 32 : 64, groups = kJoinThreads / width;
+  const int group = threadIdx.x / width, d = threadIdx.x % width * 4;
+  if (d < a.hd) {
+    float x[4] = {0, 0, 0, 0};
 #pragma unroll 8
-    for (int i = 1; i < parts; i++) x += part[2LL * i * one + d] * weight[i];
-    o[d] = sum == 0.0f ? 0.0f : x / sum;
+    for (int i = group; i < parts; i += groups) {
+      float y[4];
+      __builtin_memcpy(y, part + 2LL * i * one + (i ? 0 : first) + d, sizeof y);
+#pragma unroll
+      for (int c = 0; c < 4; c++) x[c] += y[c] * weight[i];
+    }
+#pragma unroll
+    for (int c = 0; c < 4; c++) lds[group][d + c] = x[c];
+  }
+  __syncthreads();
+  const float by = sum == 0.0f ? 0.0f : 1.0f / sum;
+  for (int i = threadIdx.x; i < a.hd; i += kJoinThreads) {
+    float x = 0.0f;
+    for (int j = 0; j < groups; j++) x += lds[j][i];
+    a.o[r * a.o_stride + (long long)h * a.hd + i] = x * by;
   }
   if (threadIdx.x == 0 && a.lse) a.lse[r * a.lse_stride + h] = sum == 0.0f ? kNegInf : (top - shift + __builtin_amdgcn_logf(sum)) * 0.69314718056f;
 }
@@ -645,17 +660,19 @@ int rows_of(const QPagedKV *c, int n_heads) {
 template <int T, int HDP>
 int launch(const char *fn, const PaArgs &a, hipStream_t stream) {
   const size_t lds = (size_t)kWaves * Cfg<T, HDP>::PARTS * a.rows * Cfg<T, HDP>::QROW;
-  const bool uni = a.page_size % 16 == 0;
-  if (lds > 64 * 1024) {              // past what a launch may take unasked
-    const void *f = uni ? reinterpret_cast<const void *>(k_paged_attn<T, HDP, true>) : reinterpret_cast<const void *>(k_paged_attn<T, HDP, false>);
-    if (hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) {
-      (void)hipGetLastError();
-      return qs::refuse(fn, "hipFuncSetAttribute failed");
-    }
+  const bool uni = a.page_size % 16 == 0, once = a.tiles == 1;
+  void (*f)(PaArgs) = uni ? once ? k_paged_attn<T, HDP, true, true> : k_paged_attn<T, HDP, true, false>
+                          : once ? k_paged_attn<T, HDP, false, true> : k_paged_attn<T, HDP, false, false>;
+  if (lds > 64 * 1024 &&              // past what a launch may take unasked
+      hipFuncSetAttribute(reinterpret_cast<const void *>(f), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) {
+    (void)hipGetLastError();
+    return qs::refuse(fn, "hipFuncSetAttribute failed");
   }
-  if (uni) QS_LAUNCH(fn, (k_paged_attn<T, HDP, true>), dim3(kBlocks), dim3(kThreads), lds, stream, a);
-  else QS_LAUNCH(fn, (k_paged_attn<T, HDP, false>), dim3(kBlocks), dim3(kThreads), lds, stream, a);
-  QS_LAUNCH(fn, k_paged_join, dim3(a.n_req, a.n_heads), dim3(kJoinThreads), 0, stream, a, (int)Cfg<T, HDP>::STEP, (float)Cfg<T, HDP>::SHIFT);
+  QS_LAUNCH(fn, f, dim3(kBlocks), dim3(kThreads), lds, stream, a);
+  // shares that can hold a step, by the room of the tables
+  const long long most = (long long)a.n_req * a.n_kv * a.tiles * (((long long)a.width * a.page_size + Cfg<T, HDP>::STEP - 1) / Cfg<T, HDP>::STEP);
+  const int shares = most / kMinShare + 1 < kShares ? (int)(most / kMinShare + 1) : kShares;
+  QS_LAUNCH(fn, k_paged_join, dim3(shares, a.rows), dim3(kJoinThreads), 0, stream, a, (float)Cfg<T, HDP>::SHIFT);
   return 0;
 }
 
@@ -672,7 +689,7 @@ extern "C" int qllama_test_page_of(const int32_t *table, int width, int page_siz
 
 extern "C" size_t qllama_paged_attention_work(const QPagedKV *c, int n_req, int n_heads) {
   if (qs::bad_cache(c) || n_req < 0 || n_heads < 1 || n_heads > 65535 || n_heads % c->n_kv) return 0;
-  return (size_t)kShares * 2 * rows_of(c, n_heads) * (c->head_dim + 2) * sizeof(float);
+  return kShares * (sizeof(int4) + (size_t)2 * rows_of(c, n_heads) * (c->head_dim + 2) * sizeof(float));
 }
 
 extern "C" int qllama_paged_attention(const QPagedKV *c, const QPagedQuery *a, void *stream) {
@@ -700,7 +717,8 @@ extern "C" int qllama_paged_attention(const QPagedKV *c, const QPagedQuery *a, v
   PaArgs p;
   p.k = static_cast<const char *>(c->k); p.v = static_cast<const char *>(c->v);
   p.ks = c->k_scale; p.vs = c->v_scale;
-  p.q = a->q; p.o = a->o; p.lse = a->lse; p.table = a->table; p.lens = a->lens; p.part = static_cast<float *>(a->work);
+  p.q = a->q; p.o = a->o; p.lse = a->lse; p.table = a->table; p.lens = a->lens; p.split = static_cast<int4 *>(a->work);
+  p.part = reinterpret_cast<float *>(p.split + kShares);
   p.pst = c->page_stride * es; p.hst = c->head_stride * es; p.sst = c->slot_stride * es;
   p.scp = c->scale_page_stride; p.sch = c->scale_head_stride; p.scs = c->scale_slot_stride;
   p.q_stride = a->q_stride; p.o_stride = a->o_stride; p.lse_stride = a->lse_stride; p.table_stride = a->table_stride;
