@@ -157,7 +157,7 @@ int qllama_test_page_of(const int32_t *table, int width, int page_size, int n_pa
 // l_0) / temperature), and the first n tokens are kept, where n is the smallest of
 //   top_k (0 < top_k < vocab, else no limit),
 //   the first n whose e add up to at least top_p of all (0 < top_p < 1, else no limit),
-//   the number of tokens with e_i >= min_p (min_p > 0, else no limit; above 1 as 1);
+//   the number of tokens with e_i >= min_p (min_p > 2^-43, else no limit; above 1 as 1);
 // the token is the first j whose e_0 + .. + e_j reach u times the kept sum.
 // temperature <= 0 or NaN: the first index of the largest logit.  u outside [0, 1)
 // counts as the nearest inside, NaN as 0; a NaN setting is no limit.  Logits of -inf
@@ -169,7 +169,7 @@ int qllama_test_page_of(const int32_t *table, int width, int page_size, int n_pa
 // settings' arrays may be NULL: temperature 1, no limit.  work: qllama_sample_rows_work
 // bytes, 16-byte aligned.
 typedef struct {
-  int rows, vocab;                            // vocab 1 .. 1048576
+  int rows, vocab;                            // rows up to 65535, vocab 1 .. 1048576
   int64_t stride;                             // floats between rows of logits, >= vocab
   const float *logits, *u;
   const float *temperature;

@@ -2,77 +2,196 @@
 // qserve.h): sample_token (sampler.c:54-143) for many rows with settings and random
 // numbers of their own, and min-p.
 //
-// No row is sorted.  A token's weight e = exp((l - max) / T) is held as a whole number
-// of 2^-43 in 64 bits, so sums are exact in any order and LDS atomics give the same
-// bits every time; a histogram over log2 e with the number and the weight of the tokens
-// in each bin tells in which bin the kept set ends, and in which the drawn token lies;
-// only that bin's tokens are put in order.  A bin that holds too many of them (equal or
-// nearly equal logits) is divided by the bits of (logit, index) until few are left.
+// No row is sorted.  With u = 16 log2(e) l / T, a token's weight 2^(u / 16) is that of
+// its cell floor(u) of a grid that all rows of one temperature share, times 2^(f / 16), f
+// = u - floor(u) in [0, 1).  Only the second factor, between 1 and 1.045, needs a token's
+// own arithmetic (six terms), and in a histogram over the cells it adds up as a whole
+// number of 2^-38 beside the number of tokens in one 64-bit word: sums are exact in any
+// order, so LDS atomics give the same bits every time, and slices of a row add up without
+// knowing its maximum.  k_sample_slices reads a row once, a slice a block, and leaves
+// each slice's histogram of 768 cells (48 powers of two).  k_sample_pick puts a row's
+// histograms together, finds in which cell the kept set ends and in which the drawn token
+// lies, and reads only those cells' tokens again, from the slices that hold some.  A
+// cell's range of (logit, index) is divided into up to 512 parts until the one where the
+// search ends holds 64 tokens at most, which a wave puts in order.
 #include <hip/hip_runtime.h>
 
 #include "qserve_host.h"
 
 namespace {
 
-constexpr int kThreads = 1024;
-constexpr int kBins = 2048;
-constexpr int kList = 2048;           // tokens of a bin that are put in order at once
-constexpr double kUnit = 8796093022208.0;   // 2^43
-constexpr double kLog2e = 1.4426950408889634074;
-
 typedef unsigned long long u64;
 
-// A logit and its index as one number, larger for earlier in the order; 0: masked.
+constexpr int kSliceThreads = 256;
+constexpr int kBins = 768;            // cells of a histogram: the tokens past it weigh less than 2^-47 of the largest
+constexpr double kGrid = 16.0;        // cells a power of two
+constexpr int kPickThreads = kBins;   // one a cell
+constexpr int kParts = 512;           // parts of a divided range
+constexpr int kList = 2048;           // tokens of a cell that are kept in LDS
+constexpr int kUnitBits = 43;         // a row's weights are whole numbers of 2^-43
+constexpr int kFractionBits = 38;
+constexpr double kLog2e = 1.4426950408889634074;
+constexpr int kCountShift = 48;       // a histogram word: number of tokens, sum of 2^38 (2^(f / 16) - 1)
+
+// A slice of a row in the workspace, followed by the others' and by all histograms.
+struct Slice {
+  u64 best;                           // token_key of the first largest logit, 0: all masked
+  uint32_t n;                         // tokens that are not masked
+  uint32_t pad;
+};
+
+// A logit and its index (20 bits) as one number, larger for earlier in the order; 0: masked.
 __device__ inline u64 token_key(float l, int i) {
   if (!(l > -__builtin_inff())) return 0;               // -inf and NaN
   const uint32_t b = __float_as_uint(l + 0.0f);         // -0 as 0
   const uint32_t o = b & 0x80000000u ? ~b : b | 0x80000000u;
-  return (u64)o << 32 | (0xffffffffu - (uint32_t)i);
+  return (u64)o << 20 | (0xfffffu - (uint32_t)i);
 }
 __device__ inline float key_logit(u64 k) {
-  const uint32_t o = (uint32_t)(k >> 32);
+  const uint32_t o = (uint32_t)(k >> 20);
   return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
 }
-__device__ inline int key_index(u64 k) { return (int)(0xffffffffu - (uint32_t)k); }
+__device__ inline int key_index(u64 k) { return (int)(0xfffffu - (uint32_t)(k & 0xfffffu)); }
+__device__ inline u64 smallest_key(float l) { return token_key(l, 0xfffff); }   // of all tokens with this logit
 
-// -log2 of a token's weight
-__device__ inline double depth(float l, float top, double per) { return l == top ? 0.0 : ((double)top - (double)l) * per; }
+// 2^38 (2^(f / 16) - 1), 0 <= f <= 1, rounded to whole: six terms of the exponential's
+// series (the seventh is 2^-6 at most), and 2^52 whose addition rounds
+struct Series {
+  double a[6];
+  __device__ inline Series() {
+    constexpr double x = 0.69314718055994530942 / kGrid, s = (double)(1ull << kFractionBits);
+    a[0] = s * x; a[1] = a[0] * x / 2; a[2] = a[1] * x / 3; a[3] = a[2] * x / 4; a[4] = a[3] * x / 5; a[5] = a[4] * x / 6;
+  }
+  __device__ inline u64 operator()(double f) const {
+    double s = a[5];
+#pragma unroll
+    for (int i = 4; i >= 0; i--) s = fma(s, f, a[i]);
+    return __builtin_bit_cast(u64, fma(s, f, 4503599627370496.0)) & 0xfffffffffffffull;
+  }
+};
 
-// 2^-t, 0 <= t: the nearest power of two times the Taylor series of the rest (|r| <=
-// 0.35, its 13th term 2e-16); 0 past t = 64
-__device__ inline double weight(double t) {
-  if (!(t <= 64.0)) return 0.0;
-  const double k = rint(t), r = (k - t) * 0.69314718055994530942;
-  double s = 1.0 / 479001600.0;
-  s = fma(s, r, 1.0 / 39916800.0);
-  s = fma(s, r, 1.0 / 3628800.0);
-  s = fma(s, r, 1.0 / 362880.0);
-  s = fma(s, r, 1.0 / 40320.0);
-  s = fma(s, r, 1.0 / 5040.0);
-  s = fma(s, r, 1.0 / 720.0);
-  s = fma(s, r, 1.0 / 120.0);
-  s = fma(s, r, 1.0 / 24.0);
-  s = fma(s, r, 1.0 / 6.0);
-  s = fma(s, r, 0.5);
-  s = fma(s, r, 1.0);
-  s = fma(s, r, 1.0);
-  return ldexp(s, -(int)k);
+// A token below `top`: its cell's distance from top's (kBins: past the last) and f.  per: 16
+// log2(e) / T.  Tokens equal to top share its cell whatever it is, infinity too.
+struct Place { int bin; double f; };
+__device__ inline Place place_of(float l, float top, double cell_top, double per) {
+  const double u = (double)l * per, cell = floor(u), d = cell_top - cell;
+  if (l == top && !(u - cell >= 0.0)) return {0, 0.0};
+  return {d < kBins ? (int)d : kBins, u - cell};
 }
-__device__ inline u64 units(double t) { return (u64)(weight(t) * kUnit + 0.5); }
+__device__ inline double cell_of(float l, double per) { return floor((double)l * per); }
 
-// bins of equal width in log2; tokens without weight in the last
-__device__ inline int bin_of(double t) { return t < 44.5 ? (int)(t * 46.0) : kBins - 1; }
+// n tokens of a cell, x of whose fractions: their weight against 2^(cell of the row's
+// largest / 16) in units.  In bin 0 exact, so equal largest logits weigh alike, alone and
+// together; elsewhere rounded.
+__device__ inline u64 units(int bin, u64 n, u64 x) {
+  const u64 raw = (n << kFractionBits) + x;
+  if (bin == 0) return raw << (kUnitBits - kFractionBits);
+  return bin < kBins ? (u64)((double)raw * exp2(kUnitBits - kFractionBits - bin * (1.0 / kGrid)) + 0.5) : 0;
+}
+__device__ inline u64 units(Place p) { return units(p.bin, 1, Series()(p.f)); }
+// A token's weight unrounded, in units
+__device__ inline double weight(Place p) { return exp2(kUnitBits + (p.f - p.bin) * (1.0 / kGrid)); }
+
+// What one row asks for.
+struct Ask {
+  double per;                         // 16 log2(e) / T
+  bool greedy;
+};
+__device__ inline Ask ask_of(const QSampleRows &a, int r) {
+  const float T = a.temperature ? a.temperature[r] : 1.0f;
+  return {kGrid * kLog2e / (double)T, !(T > 0.0f)};
+}
+
+// A slice of 1024 Q tokens in registers: the only reading of most of a row.
+template <int Q>
+__global__ __launch_bounds__(kSliceThreads) void k_sample_slices(QSampleRows a, Slice *slices, u64 *hist) {
+  __shared__ u64 h[kBins], bests[kSliceThreads / 64];
+  __shared__ uint32_t counts[kSliceThreads / 64];
+  const int r = blockIdx.y, t = threadIdx.x;
+  const size_t at = (size_t)r * gridDim.x + blockIdx.x;
+  const float *row = a.logits + r * a.stride;
+  const int i0 = blockIdx.x * (1024 * Q);
+  float l[Q][4];
+#pragma unroll
+  for (int j = 0; j < Q; j++) {
+    const int i = i0 + (j * kSliceThreads + t) * 4;
+    if (i + 4 <= a.vocab) {
+      __builtin_memcpy(l[j], row + i, sizeof l[j]);      // any 4-byte boundary
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; c++) l[j][c] = i + c < a.vocab ? row[i + c] : -__builtin_inff();
+    }
+  }
+  const Ask ask = ask_of(a, r);
+  for (int b = t; b < kBins; b += kSliceThreads) h[b] = 0;
+  float most = -__builtin_inff();
+  uint32_t count = 0;
+#pragma unroll
+  for (int j = 0; j < Q; j++)
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+      most = fmaxf(most, l[j][c]);                       // of a NaN and a number the number
+      count += l[j][c] > -__builtin_inff();
+    }
+  u64 best = token_key(most, 0);
+  if (ask.greedy) {                                      // its index counts
+#pragma unroll
+    for (int j = Q - 1; j >= 0; j--)
+#pragma unroll
+      for (int c = 3; c >= 0; c--)
+        if (l[j][c] == most) best = token_key(most, i0 + (j * kSliceThreads + t) * 4 + c);
+  }
+  for (int d = 32; d; d >>= 1) {
+    const u64 o = __shfl_xor(best, d);
+    best = o > best ? o : best;
+    count += __shfl_xor(count, d);
+  }
+  if ((t & 63) == 0) { bests[t >> 6] = best; counts[t >> 6] = count; }
+  __syncthreads();
+  count = 0;
+#pragma unroll
+  for (int i = 0; i < kSliceThreads / 64; i++) {
+    best = bests[i] > best ? bests[i] : best;
+    count += counts[i];
+  }
+  if (t == 0) slices[at] = {best, count, 0};
+  if (ask.greedy || !best) return;                       // no histogram is read
+
+  const float top = key_logit(best);
+  const double cell_top = cell_of(top, ask.per);
+  Series whole;
+#pragma unroll
+  for (int i = 0; i < 6; i++) asm volatile("" : "+v"(whole.a[i]));     // kept in registers, not moved there for every token
+  if (fabs(cell_top) < 1e15) {
+#pragma unroll
+    for (int j = 0; j < Q; j++)
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        const double u = (double)l[j][c] * ask.per, cell = floor(u), d = cell_top - cell;
+        if (d < kBins) atomicAdd(&h[(int)d], whole(u - cell) | 1ull << kCountShift);      // NaN and -inf are not
+      }
+  } else {                                               // infinite or enormous logits
+    for (int i = i0 + t; i < min(i0 + 1024 * Q, a.vocab); i += kSliceThreads) {
+      const float x = row[i];
+      const Place p = place_of(x, top, cell_top, ask.per);
+      if (x > -__builtin_inff() && p.bin < kBins) atomicAdd(&h[p.bin], whole(p.f) | 1ull << kCountShift);
+    }
+  }
+  __syncthreads();
+  for (int b = t; b < kBins; b += kSliceThreads) hist[at * kBins + b] = h[b];
+}
 
 struct Mass { u64 w; uint32_t n; };
 
 struct Shared {
-  u64 w[kBins];
-  uint32_t n[kBins];
-  u64 list[kList];
-  u64 part_w[kThreads / 64];
-  uint32_t part_n[kThreads / 64];
-  uint32_t fill;
+  u64 w[kParts];
+  uint32_t n[kParts];
+  u64 list[kList], few[64];
+  u64 part_w[kPickThreads / 64];
+  uint32_t part_n[kPickThreads / 64];
+  uint32_t fill, n_some;
   int found;
+  u64 key;
 };
 
 // Inclusive sums over the block's threads.
@@ -90,220 +209,322 @@ __device__ Mass scan(Mass v, Shared &s) {
   return v;
 }
 
-__device__ void clear(Shared &s) {
+// Smallest index over the block for which a thread says so (each its own smallest).
+__device__ int first_of(int at, Shared &s) {
+  if (threadIdx.x == 0) s.found = INT_MAX;
   __syncthreads();
-  for (int b = threadIdx.x; b < kBins; b += kThreads) { s.w[b] = 0; s.n[b] = 0; }
-  __syncthreads();
-}
-
-// w and n become inclusive sums from bin 0 on.
-__device__ void accumulate(Shared &s) {
-  __syncthreads();
-  const int b = 2 * threadIdx.x;
-  const u64 w0 = s.w[b], w1 = s.w[b + 1];
-  const uint32_t n0 = s.n[b], n1 = s.n[b + 1];
-  const Mass v = scan({w0 + w1, n0 + n1}, s);
-  s.w[b] = v.w - w1; s.w[b + 1] = v.w;
-  s.n[b] = v.n - n1; s.n[b + 1] = v.n;
-  __syncthreads();
-}
-
-// The first bin (sums accumulated, on top of `before`) where n tokens or the weight are
-// reached; the last one that holds a token where they never are.
-__device__ int find_bin(Shared &s, Mass before, uint32_t n, double w) {
-  if (threadIdx.x == 0) s.found = kBins;
-  __syncthreads();
-  const uint32_t all = s.n[kBins - 1];
-  int at = kBins;
-  for (int b = 2 * threadIdx.x + 1; b >= 2 * (int)threadIdx.x; b--)
-    if (s.n[b] && (before.n + s.n[b] >= n || (double)(before.w + s.w[b]) >= w || s.n[b] == all)) at = b;
-  if (at < kBins) atomicMin(&s.found, at);
+  for (int d = 32; d; d >>= 1) at = min(at, __shfl_xor(at, d));
+  if ((threadIdx.x & 63) == 0) atomicMin(&s.found, at);
   __syncthreads();
   return s.found;
 }
 
+// Where a search ends: at the first token at which n tokens or the weight w are reached,
+// before the first one whose key is below `floor`, or at the last.
+struct Goal { uint32_t n; double w; u64 floor; };
+__device__ inline bool reached(Mass m, Goal g) { return m.n >= g.n || (double)m.w >= g.w; }
+
 struct Row {
   const float *l;
-  int V;
+  int V, slices, slice;         // tokens, slices, tokens of a slice
   float top;
-  double per;                   // log2(e) / T
+  double cell_top, per;
+  const int *offs;              // bin of the row that is each slice's first (LDS); kBins: none is
+  int *some;                    // slices that hold tokens of a bin (LDS)
+  const u64 *hist;              // of each slice
 };
 
-struct Found { Mass upto; u64 key; };   // number and weight up to and with a token, and the token
+struct Found { Mass upto; u64 key; };   // number and weight up to and with a token, and the token (0: none below `before`)
 
-// The token at which, in order, n tokens or the weight are reached first.  s.w and s.n
-// hold the accumulated first histogram; they are changed.
-__device__ Found locate(const Row &row, Shared &s, uint32_t n, double w) {
-  Mass before = {0, 0};
-  const int bin = find_bin(s, before, n, w);
-  uint32_t inside = s.n[bin] - (bin ? s.n[bin - 1] : 0);
-  if (bin) before = {s.w[bin - 1], s.n[bin - 1]};
-  u64 prefix = 0;
-  int shift = 64;               // of the bits that are settled
-  while (inside > kList) {
-    const int next = shift > 11 ? shift - 11 : 0;
-    clear(s);
-    for (int i = threadIdx.x; i < row.V; i += kThreads) {
-      const float l = row.l[i];
-      const u64 k = token_key(l, i);
-      if (!k) continue;
-      const double t = depth(l, row.top, row.per);
-      if (bin_of(t) != bin || (shift < 64 && k >> shift != prefix)) continue;
-      const int d = kBins - 1 - (int)((k >> next) & (kBins - 1));
-      atomicAdd(&s.w[d], units(t));
-      atomicAdd(&s.n[d], 1u);
-    }
-    accumulate(s);
-    const int d = find_bin(s, before, n, w);
-    inside = s.n[d] - (d ? s.n[d - 1] : 0);
-    if (d) { before.w += s.w[d - 1]; before.n += s.n[d - 1]; }
-    prefix = (shift < 64 ? prefix << (shift - next) : 0) | (u64)(kBins - 1 - d);   // the last digit repeats settled bits
-    shift = next;
-  }
-
-  __syncthreads();
-  if (threadIdx.x == 0) s.fill = 0;
-  int pow2 = 64;
-  while (pow2 < (int)inside) pow2 <<= 1;
-  for (int i = threadIdx.x; i < pow2; i += kThreads) s.list[i] = 0;
-  __syncthreads();
-  for (int i = threadIdx.x; i < row.V; i += kThreads) {
-    const float l = row.l[i];
-    const u64 k = token_key(l, i);
-    if (!k || bin_of(depth(l, row.top, row.per)) != bin || (shift < 64 && k >> shift != prefix)) continue;
-    s.list[atomicAdd(&s.fill, 1u)] = k;
-  }
-  for (int size = 2; size <= pow2; size <<= 1)
-    for (int d = size >> 1; d; d >>= 1) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < pow2 / 2; i += kThreads) {
-        const int a = 2 * i - (i & (d - 1)), b = a + d;
-        const u64 x = s.list[a], y = s.list[b];
-        if ((x < y) == ((a & size) == 0)) { s.list[a] = y; s.list[b] = x; }
-      }
-    }
-  __syncthreads();
-
-  const int i0 = 2 * threadIdx.x;
-  u64 k[2], m[2];
-  for (int i = 0; i < 2; i++) {
-    k[i] = i0 + i < pow2 ? s.list[i0 + i] : 0;
-    m[i] = k[i] ? units(depth(key_logit(k[i]), row.top, row.per)) : 0;
-  }
-  const Mass v = scan({m[0] + m[1], (uint32_t)(k[0] != 0) + (k[1] != 0)}, s);
-  if (threadIdx.x == 0) s.found = kList;
-  __syncthreads();
-  for (int i = 1; i >= 0; i--) {
-    const Mass u = {before.w + v.w - (i ? 0 : m[1]), before.n + v.n - (i ? 0 : k[1] != 0)};
-    if (k[i] && (u.n >= n || (double)u.w >= w || u.n == before.n + inside)) atomicMin(&s.found, i0 + i);
-  }
-  __syncthreads();
-  const int at = s.found;
-  if (i0 <= at && at < i0 + 2) {                  // its thread tells the others
-    const int i = at - i0;
-    s.part_w[0] = before.w + v.w - (i ? 0 : m[1]);
-    s.part_n[0] = before.n + v.n - (i ? 0 : k[1] != 0);
-  }
-  __syncthreads();
-  const Found f = {{s.part_w[0], s.part_n[0]}, s.list[at]};
-  __syncthreads();
-  return f;
+// The smallest logit whose cell is at least `cell` (per > 0)
+__device__ float first_of_cell(double cell, double per) {
+  const float lowest = -3.4028234663852886e38f, inf = __builtin_inff();
+  const double x = cell / per;
+  float c = x > lowest ? (float)x : lowest;             // past the largest float: infinity
+  for (int i = 0; i < 4 && c < inf && cell_of(c, per) < cell; i++) c = nextafterf(c, inf);
+  for (int i = 0; i < 4 && c > lowest && cell_of(nextafterf(c, lowest), per) >= cell; i++) c = nextafterf(c, lowest);
+  return c;
 }
 
-__global__ __launch_bounds__(kThreads) void k_sample_rows(QSampleRows a) {
+// Every token of bin `bin` with a key in [lo, hi), as f(key, place).
+template <typename F>
+__device__ void for_tokens(const Row &row, Shared &s, int bin, u64 lo, u64 hi, F f) {
+  __syncthreads();
+  if (threadIdx.x == 0) s.n_some = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < row.slices; i += kPickThreads) {
+    const int b = bin - row.offs[i];
+    if (b >= 0 && row.hist[(size_t)i * kBins + b]) row.some[atomicAdd(&s.n_some, 1u)] = i;
+  }
+  __syncthreads();
+  // keys below -inf's and above inf's are no logits
+  const float least = lo >> 20 > 0x007fffffu ? key_logit(lo) : -__builtin_inff(), most = hi >> 20 < 0xff800000u ? key_logit(hi) : __builtin_inff();
+  const int fours = row.slice / 4, all = (int)s.n_some * fours;       // a power of two, so the division is a shift
+  const int bits = 31 - __builtin_clz(fours);
+  for (int q0 = threadIdx.x; q0 < all; q0 += 8 * kPickThreads) {
+    float l[8][4];
+    int at[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const int q = q0 + j * kPickThreads;
+      at[j] = q < all ? row.some[q >> bits] * row.slice + (q & (fours - 1)) * 4 : row.V;
+      if (at[j] + 4 <= row.V) {
+        __builtin_memcpy(l[j], row.l + at[j], sizeof l[j]);
+      } else {
+#pragma unroll
+        for (int c = 0; c < 4; c++) l[j][c] = at[j] + c < row.V ? row.l[at[j] + c] : -__builtin_inff();
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++)
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        if (!(l[j][c] >= least && l[j][c] <= most)) continue;         // most of them, at two comparisons
+        const u64 k = token_key(l[j][c], at[j] + c);
+        const Place p = place_of(l[j][c], row.top, row.cell_top, row.per);
+        if (k >= lo && k < hi && k && p.bin == bin) f(k, p);
+      }
+  }
+  __syncthreads();
+}
+
+// Divide the range [lo, hi) of keys, in which `inside` tokens lie and before which
+// `before` is, and go to the part where the search ends.  each(f) calls f(key, place) for
+// the range's tokens.
+template <typename E>
+__device__ void divide(Shared &s, Goal goal, u64 &lo, u64 &hi, Mass &before, uint32_t &inside, E each) {
+  const int span = 64 - __builtin_clzll((hi - lo - 1) | 1), shift = span > 9 ? span - 9 : 0;
+  const int t = threadIdx.x;
+  __syncthreads();
+  if (t < kParts) { s.w[t] = 0; s.n[t] = 0; }
+  __syncthreads();
+  each([&](u64 k, Place p) {
+    const int d = (int)((hi - 1 - k) >> shift);
+    atomicAdd(&s.w[d], units(p));
+    atomicAdd(&s.n[d], 1u);
+  });
+  __syncthreads();
+  const Mass own = t < kParts ? Mass{s.w[t], s.n[t]} : Mass{0, 0};
+  const Mass upto = scan(own, s);
+  const bool ends = own.n && (reached({before.w + upto.w, before.n + upto.n}, goal) || upto.n == inside);
+  const bool floor_here = goal.floor && t < kParts && (goal.floor >= hi ? t == 0 : goal.floor >= lo && (int)((hi - 1 - goal.floor) >> shift) == t);
+  const int d = first_of(ends || floor_here ? t : INT_MAX, s);
+  if (t == d) {                 // its thread tells the others
+    s.part_w[0] = upto.w - own.w;
+    s.part_n[0] = upto.n - own.n;
+    s.fill = own.n;
+  }
+  __syncthreads();
+  before.w += s.part_w[0];
+  before.n += s.part_n[0];
+  inside = s.fill;
+  const u64 top = hi - ((u64)d << shift), bottom = hi - lo > (u64)(d + 1) << shift ? hi - ((u64)(d + 1) << shift) : lo;
+  lo = bottom;
+  hi = top;
+  __syncthreads();
+}
+
+// The token at which a search ends that has `before` behind it and lies in bin `bin` of
+// `inside` tokens.  list_bin: the bin all of whose tokens s.list holds, or -1.
+__device__ Found locate(const Row &row, Shared &s, Goal goal, int bin, Mass before, uint32_t inside, int &list_bin) {
+  if (!inside) return {before, 0};
+  const int t = threadIdx.x;
+  // a cell's logits are an interval; where the arithmetic has no room for its ends
+  // (infinite or enormous logits or temperatures) the range is that of all
+  u64 lo = 0, hi = 1ull << 52;
+  if (row.per > 0.0 && fabs(row.cell_top) < 1e15) {
+    lo = smallest_key(first_of_cell(row.cell_top - bin, row.per));
+    hi = smallest_key(first_of_cell(row.cell_top - bin + 1.0, row.per));
+  }
+  if (list_bin != bin) {
+    list_bin = bin;
+    while (inside > kList) {
+      divide(s, goal, lo, hi, before, inside, [&](auto f) { for_tokens(row, s, bin, lo, hi, f); });
+      list_bin = -1;
+    }
+    if (!inside) return {before, 0};
+    if (t == 0) s.fill = 0;     // for_tokens synchronizes
+    for_tokens(row, s, bin, lo, hi, [&](u64 k, Place) { s.list[atomicAdd(&s.fill, 1u)] = k; });
+  }
+  const uint32_t listed = inside;
+  const auto in_list = [&](auto f) {
+    for (uint32_t i = t; i < listed; i += kPickThreads) {
+      const u64 k = s.list[i];
+      if (k >= lo && k < hi) f(k, place_of(key_logit(k), row.top, row.cell_top, row.per));
+    }
+  };
+  while (inside > 64) divide(s, goal, lo, hi, before, inside, in_list);
+  if (!inside) return {before, 0};
+
+  __syncthreads();
+  if (t == 0) s.fill = 0;
+  __syncthreads();
+  in_list([&](u64 k, Place) { s.few[atomicAdd(&s.fill, 1u)] = k; });
+  __syncthreads();
+  if (t < 64) {                 // a wave puts them in order: every lane counts the keys before its own
+    u64 k = t < (int)inside ? s.few[t] : 0;
+    int rank = 0;
+    for (int i = 0; i < (int)inside; i++) rank += s.few[i] > k;
+    __builtin_amdgcn_wave_barrier();
+    if (k) s.few[rank] = k;
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    if (k) k = s.few[t];
+    Mass m = {k ? units(place_of(key_logit(k), row.top, row.cell_top, row.per)) : 0, k != 0};
+    for (int d = 1; d < 64; d <<= 1) {
+      const u64 w = __shfl_up(m.w, d);
+      const uint32_t n = __shfl_up(m.n, d);
+      if (t >= d) { m.w += w; m.n += n; }
+    }
+    const u64 next = __shfl_down(k, 1);
+    m = {before.w + m.w, before.n + m.n};
+    const uint64_t stops = __ballot(k && (reached(m, goal) || t + 1 == (int)inside || next < goal.floor));
+    const bool none = __shfl(k, 0) < goal.floor;          // not even the first of them
+    if (none ? t == 0 : t == __builtin_ctzll(stops)) {
+      s.part_w[0] = none ? before.w : m.w;
+      s.part_n[0] = none ? before.n : m.n;
+      s.key = none ? 0 : k;
+    }
+  }
+  __syncthreads();
+  const Found found = {{s.part_w[0], s.part_n[0]}, s.key};
+  __syncthreads();
+  return found;
+}
+
+// The smallest logit l with exp((l - top) / T) >= m (0 < m <= 1); per: 16 log2(e) / T.
+__device__ float smallest_passing(float m, float top, double per) {
+  if (top == __builtin_inff() || m >= 1.0f) return top;
+  const double least = -1.7976931348623157e308, x = per > 0.0 ? (double)top + log2((double)m) * kGrid / per : least;
+  const auto passes = [&](float l) { return exp2(((double)l - (double)top) * per / kGrid) >= (double)m; };
+  const float lowest = -3.4028234663852886e38f;
+  float c = x > lowest ? (float)x : lowest;
+  if (c > top) c = top;
+  for (int i = 0; i < 4 && c < top && !passes(c); i++) c = nextafterf(c, top);
+  for (int i = 0; i < 4 && c > lowest && passes(nextafterf(c, lowest)); i++) c = nextafterf(c, lowest);
+  return c;
+}
+
+__global__ __launch_bounds__(kPickThreads) void k_sample_pick(QSampleRows a, int slices, int slice, const Slice *recs, const u64 *hist) {
+  extern __shared__ __align__(8) char dyn[];
+  float *tops = reinterpret_cast<float *>(dyn);            // largest logits of the slices
+  int *offs = reinterpret_cast<int *>(tops + slices), *some = offs + slices;
   __shared__ Shared s;
-  const int r = blockIdx.x;
-  Row row = {a.logits + r * a.stride, a.vocab, 0.0f, 0.0};
-  const float T = a.temperature ? a.temperature[r] : 1.0f;
-  const bool greedy = !(T > 0.0f);
+  const int r = blockIdx.x, t = threadIdx.x;
+  const Ask ask = ask_of(a, r);
+  recs += (size_t)r * slices;
+  hist += (size_t)r * slices * kBins;
 
   u64 best = 0;
-  for (int i = threadIdx.x; i < row.V; i += kThreads) {
-    const u64 k = token_key(row.l[i], i);
-    best = k > best ? k : best;
+  uint32_t all_n = 0;
+  for (int i = t; i < slices; i += kPickThreads) {
+    const Slice x = recs[i];
+    tops[i] = x.best ? key_logit(x.best) : -__builtin_inff();
+    best = x.best > best ? x.best : best;
+    all_n += x.n;
   }
   for (int d = 32; d; d >>= 1) {
     const u64 o = __shfl_xor(best, d);
     best = o > best ? o : best;
+    all_n += __shfl_xor(all_n, d);
   }
-  if ((threadIdx.x & 63) == 0) s.part_w[threadIdx.x >> 6] = best;
+  if ((t & 63) == 0) { s.part_w[t >> 6] = best; s.part_n[t >> 6] = all_n; }
   __syncthreads();
-  for (int i = 0; i < kThreads / 64; i++) best = s.part_w[i] > best ? s.part_w[i] : best;
-  if (!best || greedy) {
-    if (threadIdx.x == 0) {
+  all_n = 0;
+  for (int i = 0; i < kPickThreads / 64; i++) {
+    best = s.part_w[i] > best ? s.part_w[i] : best;
+    all_n += s.part_n[i];
+  }
+  if (!best || ask.greedy) {
+    if (t == 0) {
       a.token[r] = best ? key_index(best) : -1;
       if (a.prob) a.prob[r] = best ? 1.0f : 0.0f;
       if (a.kept) a.kept[r] = best ? 1 : 0;
     }
     return;
   }
-  row.top = key_logit(best);
-  row.per = kLog2e / (double)T;
+  Row row = {a.logits + r * a.stride, a.vocab, slices, slice, key_logit(best), 0.0, ask.per, offs, some, hist};
+  row.cell_top = cell_of(row.top, row.per);
+  for (int i = t; i < slices; i += kPickThreads)
+    offs[i] = tops[i] > -__builtin_inff() ? place_of(tops[i], row.top, row.cell_top, row.per).bin : kBins;
+  __syncthreads();
 
-  // min-p limits the number of tokens: e >= min_p, that is depth <= -log2(min_p)
-  float mp = a.min_p ? a.min_p[r] : 0.0f;
-  const bool by_min = mp > 0.0f;
-  if (mp > 1.0f) mp = 1.0f;
-  clear(s);
-  uint32_t passing = 0;
-  for (int i = threadIdx.x; i < row.V; i += kThreads) {
-    const float l = row.l[i];
-    if (!(l > -__builtin_inff())) continue;
-    const double t = depth(l, row.top, row.per), e = weight(t);
-    const int b = bin_of(t);
-    const u64 w = (u64)(e * kUnit + 0.5);
-    if (w) atomicAdd(&s.w[b], w);
-    atomicAdd(&s.n[b], 1u);
-    passing += by_min && e >= (double)mp;
+  // this thread's cell of the row
+  u64 x = 0;
+  Mass own = {0, 0};
+#pragma unroll 8
+  for (int i = 0; i < slices; i++) {
+    const int b = t - offs[i];
+    const u64 y = b >= 0 ? hist[(size_t)i * kBins + b] : 0;
+    own.n += (uint32_t)(y >> kCountShift);
+    x += y & ((1ull << kCountShift) - 1);
   }
-  accumulate(s);
-  const u64 all_w = s.w[kBins - 1];
-  const uint32_t all_n = s.n[kBins - 1];
-  if (by_min) {
-    for (int d = 32; d; d >>= 1) passing += __shfl_xor(passing, d);
-    if ((threadIdx.x & 63) == 0) s.part_n[threadIdx.x >> 6] = passing;
+  own.w = units(t, own.n, x);
+  const Mass upto = scan(own, s);
+  const Mass before = {upto.w - own.w, upto.n - own.n};
+  if (t == kPickThreads - 1) { s.part_w[0] = upto.w; s.part_n[0] = upto.n; }
+  __syncthreads();
+  const Mass held = {s.part_w[0], s.part_n[0]};            // tokens behind the last bin weigh nothing
+  __syncthreads();
+
+  int list_bin = -1;
+  auto search = [&](Goal goal) -> Found {
+    const float fl = key_logit(goal.floor);
+    const int floor_bin = goal.floor ? place_of(fl, row.top, row.cell_top, row.per).bin : kBins;
+    const bool ends = own.n && (reached(upto, goal) || upto.n == held.n);
+    const int bin = first_of(ends || t == floor_bin ? t : INT_MAX, s);
+    if (t == bin) { s.part_w[0] = before.w; s.part_n[0] = before.n; s.fill = own.n; }
     __syncthreads();
-    passing = 0;
-    for (int i = 0; i < kThreads / 64; i++) passing += s.part_n[i];
-  }
+    const Mass b = {s.part_w[0], s.part_n[0]};
+    const uint32_t inside = s.fill;
+    __syncthreads();
+    return locate(row, s, goal, bin, b, inside, list_bin);
+  };
+
   const int k = a.top_k ? a.top_k[r] : 0;
   const float p = a.top_p ? a.top_p[r] : 0.0f;
-  uint32_t n = all_n;
-  if (k > 0 && (uint32_t)k < n) n = k;
-  if (by_min && passing < n) n = passing;
-  if (n < 1) n = 1;
-  const bool by_mass = p > 0.0f && p < 1.0f;
-
-  // the histogram is used twice: kept aside in registers while the first search changes it
-  const u64 w0 = s.w[2 * threadIdx.x], w1 = s.w[2 * threadIdx.x + 1];
-  const uint32_t n0 = s.n[2 * threadIdx.x], n1 = s.n[2 * threadIdx.x + 1];
-  Mass kept = {all_w, all_n};
-  if (n < all_n || by_mass) {
-    kept = locate(row, s, n, by_mass ? (double)p * (double)all_w : __builtin_inf()).upto;
-    s.w[2 * threadIdx.x] = w0; s.w[2 * threadIdx.x + 1] = w1;
-    s.n[2 * threadIdx.x] = n0; s.n[2 * threadIdx.x + 1] = n1;
-    __syncthreads();
-  }
+  const float mp = a.min_p ? a.min_p[r] : 0.0f;
+  const bool by_min = mp > 0x1p-43f;
+  const bool by_mass = p > 0.0f && p < 1.0f, by_count = k > 0 && (uint32_t)k < all_n;
+  Mass kept = {held.w, by_count ? (uint32_t)k : all_n};    // a limit among the tokens that weigh nothing needs no search
+  if ((by_count && kept.n < held.n) || by_mass || by_min)
+    kept = search({kept.n, by_mass ? (double)p * (double)held.w : __builtin_inf(),
+                   by_min ? smallest_key(smallest_passing(mp, row.top, row.per)) : 0}).upto;
   float u = a.u[r];
   u = u > 0.0f ? (u < 1.0f ? u : 0x1.fffffep-1f) : 0.0f;
-  const Found f = locate(row, s, kept.n, (double)u * (double)kept.w);
-  if (threadIdx.x == 0) {
+  const Found f = search({kept.n, (double)u * (double)kept.w, 0});
+  if (t == 0) {
     a.token[r] = key_index(f.key);
-    if (a.prob) a.prob[r] = (float)(weight(depth(key_logit(f.key), row.top, row.per)) * kUnit / (double)kept.w);
+    if (a.prob) a.prob[r] = (float)(weight(place_of(key_logit(f.key), row.top, row.cell_top, row.per)) / (double)kept.w);
     if (a.kept) a.kept[r] = (int)kept.n;
   }
+}
+
+// Slices of 8192 tokens; of 4096 where the former would leave CUs idle.
+int quads_of(int rows, int vocab) { return (long long)rows * ((vocab + 8191) / 8192) >= 256 ? 8 : 4; }
+
+template <int Q>
+int launch(const char *fn, const QSampleRows &s, hipStream_t stream) {
+  const int slices = (s.vocab + 1024 * Q - 1) / (1024 * Q);
+  u64 *hist = static_cast<u64 *>(s.work);
+  Slice *recs = reinterpret_cast<Slice *>(hist + (size_t)s.rows * slices * kBins);
+  QS_LAUNCH(fn, k_sample_slices<Q>, dim3(slices, s.rows), dim3(kSliceThreads), 0, stream, s, recs, hist);
+  QS_LAUNCH(fn, k_sample_pick, dim3(s.rows), dim3(kPickThreads), slices * 12, stream, s, slices, 1024 * Q, recs, hist);
+  return 0;
 }
 
 }  // namespace
 
 extern "C" size_t qllama_sample_rows_work(int rows, int vocab) {
-  if (rows < 0 || vocab < 1 || vocab > (1 << 20)) return 0;
-  return 16;
+  if (rows < 0 || rows > 65535 || vocab < 1 || vocab > (1 << 20)) return 0;
+  const int slice = 1024 * quads_of(rows, vocab);
+  return 16 + (size_t)rows * ((vocab + slice - 1) / slice) * (kBins * sizeof(u64) + sizeof(Slice));
 }
 
 extern "C" int qllama_sample_rows(const QSampleRows *s, void *stream) {
   static const char fn[] = "qllama_sample_rows";
-  if (!s || s->rows < 0) return qs::refuse(fn, "null argument or rows < 0");
+  if (!s || s->rows < 0 || s->rows > 65535) return qs::refuse(fn, "null argument, or rows not 0 .. 65535");
   if (s->vocab < 1 || s->vocab > (1 << 20) || s->stride < s->vocab) return qs::refuse(fn, "vocab must be 1 .. 1048576, stride at least vocab");
   if (s->rows == 0) return 0;
   if (!s->logits || !s->u || !s->token) return qs::refuse(fn, "null logits, u or token");
@@ -314,6 +535,5 @@ extern "C" int qllama_sample_rows(const QSampleRows *s, void *stream) {
     return qs::refuse(fn, "work is missing, misaligned or smaller than qllama_sample_rows_work");
   qs::OnDevice on(s->logits, (hipStream_t)stream);
   if (on.why) return qs::refuse(fn, on.why);
-  QS_LAUNCH(fn, k_sample_rows, dim3(s->rows), dim3(kThreads), 0, (hipStream_t)stream, *s);
-  return 0;
+  return quads_of(s->rows, s->vocab) == 8 ? launch<8>(fn, *s, (hipStream_t)stream) : launch<4>(fn, *s, (hipStream_t)stream);
 }
