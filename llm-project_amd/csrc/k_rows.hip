@@ -181,42 +181,57 @@ __global__ __launch_bounds__(kSliceThreads) void k_sample_slices(QSampleRows a, 
   for (int b = t; b < kBins; b += kSliceThreads) hist[at * kBins + b] = h[b];
 }
 
+constexpr int kPickWaves = kPickThreads / 64;
+
 struct Mass { u64 w; uint32_t n; };
 
+// Sets of what waves tell each other, used in turn: a set is written again only after the
+// barrier behind the next one's writing, when all have read it.
 struct Shared {
   u64 w[kParts];
   uint32_t n[kParts];
   u64 list[kList], few[64];
-  u64 part_w[kPickThreads / 64];
-  uint32_t part_n[kPickThreads / 64];
-  uint32_t fill, n_some;
-  int found;
-  u64 key;
+  u64 scan_w[2][kPickWaves], hit_w[2][kPickWaves], hit_mask[2][kPickWaves];
+  uint32_t scan_n[2][kPickWaves], hit_n[2][kPickWaves], hit_inside[2][kPickWaves];
+  int hit_at[2][kPickWaves];
+  u64 found_w[2], found_key[2];
+  uint32_t found_n[2], fill;
+  int some[64], n_some;
 };
 
 // Inclusive sums over the block's threads.
-__device__ Mass scan(Mass v, Shared &s) {
+__device__ Mass scan(Mass v, Shared &s, int &turn) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  turn ^= 1;
   for (int d = 1; d < 64; d <<= 1) {
     const u64 w = __shfl_up(v.w, d);
     const uint32_t n = __shfl_up(v.n, d);
     if (lane >= d) { v.w += w; v.n += n; }
   }
+  if (lane == 63) { s.scan_w[turn][wave] = v.w; s.scan_n[turn][wave] = v.n; }
   __syncthreads();
-  if (lane == 63) { s.part_w[wave] = v.w; s.part_n[wave] = v.n; }
-  __syncthreads();
-  for (int i = 0; i < wave; i++) { v.w += s.part_w[i]; v.n += s.part_n[i]; }
+  for (int i = 0; i < wave; i++) { v.w += s.scan_w[turn][i]; v.n += s.scan_n[turn][i]; }
   return v;
 }
 
-// Smallest index over the block for which a thread says so (each its own smallest).
-__device__ int first_of(int at, Shared &s) {
-  if (threadIdx.x == 0) s.found = INT_MAX;
+// The first thread that says so, and what it has: its place, what lies before it, and
+// the tokens inside.
+struct Hit { int at; Mass before; uint32_t inside; u64 mask; };
+__device__ Hit first_of(bool here, int at, Mass before, uint32_t inside, u64 mask, Shared &s, int &turn) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  turn ^= 1;
+  const uint64_t b = __ballot(here);
+  if (lane == (b ? __builtin_ctzll(b) : 0)) {
+    s.hit_at[turn][wave] = b ? at : -1;
+    s.hit_w[turn][wave] = before.w;
+    s.hit_n[turn][wave] = before.n;
+    s.hit_inside[turn][wave] = inside;
+    s.hit_mask[turn][wave] = mask;
+  }
   __syncthreads();
-  for (int d = 32; d; d >>= 1) at = min(at, __shfl_xor(at, d));
-  if ((threadIdx.x & 63) == 0) atomicMin(&s.found, at);
-  __syncthreads();
-  return s.found;
+  int w = 0;
+  while (w < kPickWaves - 1 && s.hit_at[turn][w] < 0) w++;
+  return {s.hit_at[turn][w], {s.hit_w[turn][w], s.hit_n[turn][w]}, s.hit_inside[turn][w], s.hit_mask[turn][w]};
 }
 
 // Where a search ends: at the first token at which n tokens or the weight w are reached,
@@ -226,48 +241,69 @@ __device__ inline bool reached(Mass m, Goal g) { return m.n >= g.n || (double)m.
 
 struct Row {
   const float *l;
-  int V, slices, slice;         // tokens, slices, tokens of a slice
+  int V, bits;                  // tokens; log2 of a quarter of the tokens that a bit of a mask stands for
   float top;
   double cell_top, per;
-  const int *offs;              // bin of the row that is each slice's first (LDS); kBins: none is
-  int *some;                    // slices that hold tokens of a bin (LDS)
-  const u64 *hist;              // of each slice
 };
 
 struct Found { Mass upto; u64 key; };   // number and weight up to and with a token, and the token (0: none below `before`)
 
-// The smallest logit whose cell is at least `cell` (per > 0)
-__device__ float first_of_cell(double cell, double per) {
-  const float lowest = -3.4028234663852886e38f, inf = __builtin_inff();
-  const double x = cell / per;
-  float c = x > lowest ? (float)x : lowest;             // past the largest float: infinity
-  for (int i = 0; i < 4 && c < inf && cell_of(c, per) < cell; i++) c = nextafterf(c, inf);
-  for (int i = 0; i < 4 && c > lowest && cell_of(nextafterf(c, lowest), per) >= cell; i++) c = nextafterf(c, lowest);
-  return c;
+constexpr uint32_t kOrdLowest = 0x00800000u, kOrdInf = 0xff800000u;    // of the lowest finite float, and infinity
+__device__ inline uint32_t ord_of(float l) {
+  const uint32_t b = __float_as_uint(l);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ inline float of_ord(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
+
+// The smallest float that passes a test which a larger one passes too, near c: a wave
+// tries 64 (half: 32, in each half of the wave) neighbours at once.  0: it is not among them.
+__device__ inline uint32_t neighbour(float c, int n) {
+  const long long o = (long long)ord_of(c) + (int)(threadIdx.x & (n - 1)) - n / 2;
+  return o < kOrdLowest ? kOrdLowest : o > kOrdInf ? kOrdInf : (uint32_t)o;
+}
+__device__ inline float finite(double x) { return (float)fmin(fmax(x, -3.4028234663852886e38), 3.4028234663852886e38); }
+
+// Range of the keys of a cell's tokens.  Where the arithmetic has no room for its ends
+// (infinite or enormous logits or temperatures) it is that of all.
+__device__ void range_of(const Row &row, int bin, u64 &lo, u64 &hi) {
+  lo = 0;
+  hi = 1ull << 52;
+  if (!(row.per > 0.0 && fabs(row.cell_top) < 1e15)) return;
+  const double want = row.cell_top - bin + (threadIdx.x >> 5 & 1);
+  const uint32_t o = neighbour(finite(want / row.per), 32);
+  const uint64_t pass = __ballot(cell_of(of_ord(o), row.per) >= want);
+  const uint32_t below = (uint32_t)pass, above = (uint32_t)(pass >> 32);
+  if (below && !(below & 1) && above && !(above & 1)) {
+    lo = (u64)__shfl(o, __builtin_ctz(below)) << 20;
+    hi = (u64)__shfl(o, 32 + __builtin_ctz(above)) << 20;
+  }
 }
 
-// Every token of bin `bin` with a key in [lo, hi), as f(key, place).
+// The key below which tokens weigh less than m (0 < m <= 1) of the largest.
+__device__ u64 floor_of(float m, const Row &row) {
+  if (!(fabsf(row.top) < __builtin_inff()) || m >= 1.0f) return smallest_key(row.top);
+  if (!(row.per > 0.0)) return 1;                         // all weigh alike
+  const uint32_t o = neighbour(finite((double)row.top + log2((double)m) * kGrid / row.per), 64);
+  const float l = of_ord(o);
+  const uint64_t pass = __ballot(l >= row.top || exp2(((double)l - (double)row.top) * row.per / kGrid) >= (double)m);
+  return (u64)__shfl(o, pass ? __builtin_ctzll(pass) : 63) << 20;
+}
+
+// Every token of bin `bin` with a key in [lo, hi), as f(key, place), among the slices in
+// s.some.
 template <typename F>
 __device__ void for_tokens(const Row &row, Shared &s, int bin, u64 lo, u64 hi, F f) {
-  __syncthreads();
-  if (threadIdx.x == 0) s.n_some = 0;
-  __syncthreads();
-  for (int i = threadIdx.x; i < row.slices; i += kPickThreads) {
-    const int b = bin - row.offs[i];
-    if (b >= 0 && row.hist[(size_t)i * kBins + b]) row.some[atomicAdd(&s.n_some, 1u)] = i;
-  }
-  __syncthreads();
   // keys below -inf's and above inf's are no logits
-  const float least = lo >> 20 > 0x007fffffu ? key_logit(lo) : -__builtin_inff(), most = hi >> 20 < 0xff800000u ? key_logit(hi) : __builtin_inff();
-  const int fours = row.slice / 4, all = (int)s.n_some * fours;       // a power of two, so the division is a shift
-  const int bits = 31 - __builtin_clz(fours);
+  const float least = lo >> 20 >= kOrdLowest ? of_ord((uint32_t)(lo >> 20)) : -__builtin_inff(),
+              most = hi >> 20 < kOrdInf ? of_ord((uint32_t)(hi >> 20)) : __builtin_inff();
+  const int all = s.n_some << row.bits, in = (1 << row.bits) - 1;
   for (int q0 = threadIdx.x; q0 < all; q0 += 8 * kPickThreads) {
     float l[8][4];
     int at[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) {
       const int q = q0 + j * kPickThreads;
-      at[j] = q < all ? row.some[q >> bits] * row.slice + (q & (fours - 1)) * 4 : row.V;
+      at[j] = q < all ? (s.some[q >> row.bits] << row.bits | (q & in)) * 4 : row.V;
       if (at[j] + 4 <= row.V) {
         __builtin_memcpy(l[j], row.l + at[j], sizeof l[j]);
       } else {
@@ -290,12 +326,11 @@ __device__ void for_tokens(const Row &row, Shared &s, int bin, u64 lo, u64 hi, F
 
 // Divide the range [lo, hi) of keys, in which `inside` tokens lie and before which
 // `before` is, and go to the part where the search ends.  each(f) calls f(key, place) for
-// the range's tokens.
+// the range's tokens, and synchronizes.
 template <typename E>
-__device__ void divide(Shared &s, Goal goal, u64 &lo, u64 &hi, Mass &before, uint32_t &inside, E each) {
+__device__ void divide(Shared &s, int &turn, Goal goal, u64 &lo, u64 &hi, Mass &before, uint32_t &inside, E each) {
   const int span = 64 - __builtin_clzll((hi - lo - 1) | 1), shift = span > 9 ? span - 9 : 0;
   const int t = threadIdx.x;
-  __syncthreads();
   if (t < kParts) { s.w[t] = 0; s.n[t] = 0; }
   __syncthreads();
   each([&](u64 k, Place p) {
@@ -303,47 +338,41 @@ __device__ void divide(Shared &s, Goal goal, u64 &lo, u64 &hi, Mass &before, uin
     atomicAdd(&s.w[d], units(p));
     atomicAdd(&s.n[d], 1u);
   });
-  __syncthreads();
   const Mass own = t < kParts ? Mass{s.w[t], s.n[t]} : Mass{0, 0};
-  const Mass upto = scan(own, s);
+  const Mass upto = scan(own, s, turn);
   const bool ends = own.n && (reached({before.w + upto.w, before.n + upto.n}, goal) || upto.n == inside);
   const bool floor_here = goal.floor && t < kParts && (goal.floor >= hi ? t == 0 : goal.floor >= lo && (int)((hi - 1 - goal.floor) >> shift) == t);
-  const int d = first_of(ends || floor_here ? t : INT_MAX, s);
-  if (t == d) {                 // its thread tells the others
-    s.part_w[0] = upto.w - own.w;
-    s.part_n[0] = upto.n - own.n;
-    s.fill = own.n;
-  }
-  __syncthreads();
-  before.w += s.part_w[0];
-  before.n += s.part_n[0];
-  inside = s.fill;
-  const u64 top = hi - ((u64)d << shift), bottom = hi - lo > (u64)(d + 1) << shift ? hi - ((u64)(d + 1) << shift) : lo;
+  const Hit h = first_of(ends || floor_here, t, {upto.w - own.w, upto.n - own.n}, own.n, 0, s, turn);
+  before.w += h.before.w;
+  before.n += h.before.n;
+  inside = h.inside;
+  const u64 top = hi - ((u64)h.at << shift), bottom = hi - lo > (u64)(h.at + 1) << shift ? hi - ((u64)(h.at + 1) << shift) : lo;
   lo = bottom;
   hi = top;
-  __syncthreads();
 }
 
-// The token at which a search ends that has `before` behind it and lies in bin `bin` of
-// `inside` tokens.  list_bin: the bin all of whose tokens s.list holds, or -1.
-__device__ Found locate(const Row &row, Shared &s, Goal goal, int bin, Mass before, uint32_t inside, int &list_bin) {
+// The token at which a search ends that lies in bin h.at.  list_bin: the bin all of
+// whose tokens s.list holds, or -1.
+__device__ Found locate(const Row &row, Shared &s, int &turn, Goal goal, const Hit &h, int &list_bin) {
+  const int t = threadIdx.x, bin = h.at;
+  Mass before = h.before;
+  uint32_t inside = h.inside;
   if (!inside) return {before, 0};
-  const int t = threadIdx.x;
-  // a cell's logits are an interval; where the arithmetic has no room for its ends
-  // (infinite or enormous logits or temperatures) the range is that of all
-  u64 lo = 0, hi = 1ull << 52;
-  if (row.per > 0.0 && fabs(row.cell_top) < 1e15) {
-    lo = smallest_key(first_of_cell(row.cell_top - bin, row.per));
-    hi = smallest_key(first_of_cell(row.cell_top - bin + 1.0, row.per));
-  }
+  u64 lo, hi;
+  range_of(row, bin, lo, hi);
   if (list_bin != bin) {
+    if (t < 64) {               // the slices that hold some of them
+      const uint64_t below = h.mask & ((1ull << t) - 1);
+      if (h.mask >> t & 1) s.some[__builtin_popcountll(below)] = t;
+      if (t == 0) { s.n_some = __builtin_popcountll(h.mask); s.fill = 0; }
+    }
+    __syncthreads();
     list_bin = bin;
     while (inside > kList) {
-      divide(s, goal, lo, hi, before, inside, [&](auto f) { for_tokens(row, s, bin, lo, hi, f); });
+      divide(s, turn, goal, lo, hi, before, inside, [&](auto f) { for_tokens(row, s, bin, lo, hi, f); });
       list_bin = -1;
     }
     if (!inside) return {before, 0};
-    if (t == 0) s.fill = 0;     // for_tokens synchronizes
     for_tokens(row, s, bin, lo, hi, [&](u64 k, Place) { s.list[atomicAdd(&s.fill, 1u)] = k; });
   }
   const uint32_t listed = inside;
@@ -352,25 +381,26 @@ __device__ Found locate(const Row &row, Shared &s, Goal goal, int bin, Mass befo
       const u64 k = s.list[i];
       if (k >= lo && k < hi) f(k, place_of(key_logit(k), row.top, row.cell_top, row.per));
     }
+    __syncthreads();
   };
-  while (inside > 64) divide(s, goal, lo, hi, before, inside, in_list);
-  if (!inside) return {before, 0};
-
-  __syncthreads();
-  if (t == 0) s.fill = 0;
-  __syncthreads();
-  in_list([&](u64 k, Place) { s.few[atomicAdd(&s.fill, 1u)] = k; });
-  __syncthreads();
+  const u64 *few = s.list;
+  if (listed > 64) {
+    while (inside > 64) divide(s, turn, goal, lo, hi, before, inside, in_list);
+    if (!inside) return {before, 0};
+    if (t == 0) s.fill = 0;
+    __syncthreads();
+    in_list([&](u64 k, Place) { s.few[atomicAdd(&s.fill, 1u)] = k; });
+    few = s.few;
+  }
+  turn ^= 1;
   if (t < 64) {                 // a wave puts them in order: every lane counts the keys before its own
-    u64 k = t < (int)inside ? s.few[t] : 0;
+    const u64 mine = t < (int)inside ? few[t] : 0;
+    const auto of_lane = [&](int i) { return (u64)__builtin_amdgcn_readlane((int)(mine >> 32), i) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)mine, i); };
     int rank = 0;
-    for (int i = 0; i < (int)inside; i++) rank += s.few[i] > k;
-    __builtin_amdgcn_wave_barrier();
-    if (k) s.few[rank] = k;
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    if (k) k = s.few[t];
+    for (int i = 0; i < (int)inside; i++) rank += of_lane(i) > mine;
+    u64 k = 0;                  // lane `rank` takes the key
+    for (int i = 0; i < (int)inside; i++)
+      if (__builtin_amdgcn_readlane(rank, i) == t) k = of_lane(i);
     Mass m = {k ? units(place_of(key_logit(k), row.top, row.cell_top, row.per)) : 0, k != 0};
     for (int d = 1; d < 64; d <<= 1) {
       const u64 w = __shfl_up(m.w, d);
@@ -382,45 +412,34 @@ __device__ Found locate(const Row &row, Shared &s, Goal goal, int bin, Mass befo
     const uint64_t stops = __ballot(k && (reached(m, goal) || t + 1 == (int)inside || next < goal.floor));
     const bool none = __shfl(k, 0) < goal.floor;          // not even the first of them
     if (none ? t == 0 : t == __builtin_ctzll(stops)) {
-      s.part_w[0] = none ? before.w : m.w;
-      s.part_n[0] = none ? before.n : m.n;
-      s.key = none ? 0 : k;
+      s.found_w[turn] = none ? before.w : m.w;
+      s.found_n[turn] = none ? before.n : m.n;
+      s.found_key[turn] = none ? 0 : k;
     }
   }
   __syncthreads();
-  const Found found = {{s.part_w[0], s.part_n[0]}, s.key};
-  __syncthreads();
-  return found;
+  return {{s.found_w[turn], s.found_n[turn]}, s.found_key[turn]};
 }
 
-// The smallest logit l with exp((l - top) / T) >= m (0 < m <= 1); per: 16 log2(e) / T.
-__device__ float smallest_passing(float m, float top, double per) {
-  if (top == __builtin_inff() || m >= 1.0f) return top;
-  const double least = -1.7976931348623157e308, x = per > 0.0 ? (double)top + log2((double)m) * kGrid / per : least;
-  const auto passes = [&](float l) { return exp2(((double)l - (double)top) * per / kGrid) >= (double)m; };
-  const float lowest = -3.4028234663852886e38f;
-  float c = x > lowest ? (float)x : lowest;
-  if (c > top) c = top;
-  for (int i = 0; i < 4 && c < top && !passes(c); i++) c = nextafterf(c, top);
-  for (int i = 0; i < 4 && c > lowest && passes(nextafterf(c, lowest)); i++) c = nextafterf(c, lowest);
-  return c;
-}
-
-__global__ __launch_bounds__(kPickThreads) void k_sample_pick(QSampleRows a, int slices, int slice, const Slice *recs, const u64 *hist) {
-  extern __shared__ __align__(8) char dyn[];
-  float *tops = reinterpret_cast<float *>(dyn);            // largest logits of the slices
-  int *offs = reinterpret_cast<int *>(tops + slices), *some = offs + slices;
+// A row's token from its slices' histograms.  A chain of short steps, each a barrier or a
+// trip to memory behind the one before.
+__global__ __launch_bounds__(kPickThreads) void k_sample_pick(QSampleRows a, int slices, int bits, int group, const Slice *recs, const u64 *hist) {
+  extern __shared__ int offs[];                            // the row's bin that is a slice's first; kBins: none is
   __shared__ Shared s;
   const int r = blockIdx.x, t = threadIdx.x;
   const Ask ask = ask_of(a, r);
+  const float u_given = a.u[r], p = a.top_p ? a.top_p[r] : 0.0f, mp = a.min_p ? a.min_p[r] : 0.0f;
+  const int k = a.top_k ? a.top_k[r] : 0;
   recs += (size_t)r * slices;
   hist += (size_t)r * slices * kBins;
+  int turn = 0;
 
+  // every wave reduces the slices' records
   u64 best = 0;
   uint32_t all_n = 0;
-  for (int i = t; i < slices; i += kPickThreads) {
+  for (int i = t & 63; i < slices; i += 64) {
     const Slice x = recs[i];
-    tops[i] = x.best ? key_logit(x.best) : -__builtin_inff();
+    if (t < 64) offs[i] = __float_as_int(x.best ? key_logit(x.best) : -__builtin_inff());    // for now its largest logit
     best = x.best > best ? x.best : best;
     all_n += x.n;
   }
@@ -428,13 +447,6 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(QSampleRows a, int
     const u64 o = __shfl_xor(best, d);
     best = o > best ? o : best;
     all_n += __shfl_xor(all_n, d);
-  }
-  if ((t & 63) == 0) { s.part_w[t >> 6] = best; s.part_n[t >> 6] = all_n; }
-  __syncthreads();
-  all_n = 0;
-  for (int i = 0; i < kPickThreads / 64; i++) {
-    best = s.part_w[i] > best ? s.part_w[i] : best;
-    all_n += s.part_n[i];
   }
   if (!best || ask.greedy) {
     if (t == 0) {
@@ -444,55 +456,47 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(QSampleRows a, int
     }
     return;
   }
-  Row row = {a.logits + r * a.stride, a.vocab, slices, slice, key_logit(best), 0.0, ask.per, offs, some, hist};
+  Row row = {a.logits + r * a.stride, a.vocab, bits, key_logit(best), 0.0, ask.per};
   row.cell_top = cell_of(row.top, row.per);
-  for (int i = t; i < slices; i += kPickThreads)
-    offs[i] = tops[i] > -__builtin_inff() ? place_of(tops[i], row.top, row.cell_top, row.per).bin : kBins;
+  if (t < 64)
+    for (int i = t; i < slices; i += 64) {
+      const float top = __int_as_float(offs[i]);
+      offs[i] = top > -__builtin_inff() ? place_of(top, row.top, row.cell_top, row.per).bin : kBins;
+    }
   __syncthreads();
 
-  // this thread's cell of the row
-  u64 x = 0;
+  // this thread's cell of the row, and the groups of slices that have tokens of it
+  u64 x = 0, mask = 0;
   Mass own = {0, 0};
-#pragma unroll 8
+#pragma unroll 16
   for (int i = 0; i < slices; i++) {
     const int b = t - offs[i];
-    const u64 y = b >= 0 ? hist[(size_t)i * kBins + b] : 0;
+    u64 y = hist[(size_t)i * kBins + (b < 0 ? 0 : b)];
+    y = b < 0 ? 0 : y;
     own.n += (uint32_t)(y >> kCountShift);
     x += y & ((1ull << kCountShift) - 1);
+    mask |= (u64)(y != 0) << (i >> group);
   }
   own.w = units(t, own.n, x);
-  const Mass upto = scan(own, s);
+  const Mass upto = scan(own, s, turn);
   const Mass before = {upto.w - own.w, upto.n - own.n};
-  if (t == kPickThreads - 1) { s.part_w[0] = upto.w; s.part_n[0] = upto.n; }
+  if (t == kPickThreads - 1) { s.found_w[0] = upto.w; s.found_n[0] = upto.n; }
   __syncthreads();
-  const Mass held = {s.part_w[0], s.part_n[0]};            // tokens behind the last bin weigh nothing
-  __syncthreads();
+  const Mass held = {s.found_w[0], s.found_n[0]};          // tokens behind the last bin weigh nothing
 
   int list_bin = -1;
-  auto search = [&](Goal goal) -> Found {
-    const float fl = key_logit(goal.floor);
-    const int floor_bin = goal.floor ? place_of(fl, row.top, row.cell_top, row.per).bin : kBins;
+  const auto search = [&](Goal goal) -> Found {
+    const int floor_bin = goal.floor ? place_of(key_logit(goal.floor), row.top, row.cell_top, row.per).bin : kBins;
     const bool ends = own.n && (reached(upto, goal) || upto.n == held.n);
-    const int bin = first_of(ends || t == floor_bin ? t : INT_MAX, s);
-    if (t == bin) { s.part_w[0] = before.w; s.part_n[0] = before.n; s.fill = own.n; }
-    __syncthreads();
-    const Mass b = {s.part_w[0], s.part_n[0]};
-    const uint32_t inside = s.fill;
-    __syncthreads();
-    return locate(row, s, goal, bin, b, inside, list_bin);
+    return locate(row, s, turn, goal, first_of(ends || t == floor_bin, t, before, own.n, mask, s, turn), list_bin);
   };
 
-  const int k = a.top_k ? a.top_k[r] : 0;
-  const float p = a.top_p ? a.top_p[r] : 0.0f;
-  const float mp = a.min_p ? a.min_p[r] : 0.0f;
   const bool by_min = mp > 0x1p-43f;
   const bool by_mass = p > 0.0f && p < 1.0f, by_count = k > 0 && (uint32_t)k < all_n;
   Mass kept = {held.w, by_count ? (uint32_t)k : all_n};    // a limit among the tokens that weigh nothing needs no search
   if ((by_count && kept.n < held.n) || by_mass || by_min)
-    kept = search({kept.n, by_mass ? (double)p * (double)held.w : __builtin_inf(),
-                   by_min ? smallest_key(smallest_passing(mp, row.top, row.per)) : 0}).upto;
-  float u = a.u[r];
-  u = u > 0.0f ? (u < 1.0f ? u : 0x1.fffffep-1f) : 0.0f;
+    kept = search({kept.n, by_mass ? (double)p * (double)held.w : __builtin_inf(), by_min ? floor_of(mp, row) : 0}).upto;
+  const float u = u_given > 0.0f ? (u_given < 1.0f ? u_given : 0x1.fffffep-1f) : 0.0f;
   const Found f = search({kept.n, (double)u * (double)kept.w, 0});
   if (t == 0) {
     a.token[r] = key_index(f.key);
@@ -510,7 +514,10 @@ int launch(const char *fn, const QSampleRows &s, hipStream_t stream) {
   u64 *hist = static_cast<u64 *>(s.work);
   Slice *recs = reinterpret_cast<Slice *>(hist + (size_t)s.rows * slices * kBins);
   QS_LAUNCH(fn, k_sample_slices<Q>, dim3(slices, s.rows), dim3(kSliceThreads), 0, stream, s, recs, hist);
-  QS_LAUNCH(fn, k_sample_pick, dim3(s.rows), dim3(kPickThreads), slices * 12, stream, s, slices, 1024 * Q, recs, hist);
+  int group = 0;                      // 2^group slices share a bit of a mask of 64
+  while ((slices - 1) >> group > 63) group++;
+  const int bits = 8 + (Q == 8 ? 3 : 2) + group;
+  QS_LAUNCH(fn, k_sample_pick, dim3(s.rows), dim3(kPickThreads), slices * sizeof(float), stream, s, slices, bits, group, recs, hist);
   return 0;
 }
 
