@@ -80,15 +80,34 @@ __device__ inline Place place_of(float l, float top, double cell_top, double per
 }
 __device__ inline double cell_of(float l, double per) { return floor((double)l * per); }
 
-// n tokens of a cell, x of whose fractions: their weight against 2^(cell of the row's
-// largest / 16) in units.  In bin 0 exact, so equal largest logits weigh alike, alone and
-// together; elsewhere rounded.
-__device__ inline u64 units(int bin, u64 n, u64 x) {
-  const u64 raw = (n << kFractionBits) + x;
-  if (bin == 0) return raw << (kUnitBits - kFractionBits);
-  return bin < kBins ? (u64)((double)raw * exp2(kUnitBits - kFractionBits - bin * (1.0 / kGrid)) + 0.5) : 0;
+// 2^(5 - bin / 16): a histogram's 2^-38 as units of 2^-43, and the cell's weight.  The
+// sixteenths by the exponential's series (0.65^16 / 16! is 5e-17).
+__device__ inline double scale_of(int bin) {
+  const double x = (bin & 15) * (-0.69314718055994530942 / kGrid);
+  double s = 1.0 / 1307674368000.0;
+  s = fma(s, x, 1.0 / 87178291200.0);
+  s = fma(s, x, 1.0 / 6227020800.0);
+  s = fma(s, x, 1.0 / 479001600.0);
+  s = fma(s, x, 1.0 / 39916800.0);
+  s = fma(s, x, 1.0 / 3628800.0);
+  s = fma(s, x, 1.0 / 362880.0);
+  s = fma(s, x, 1.0 / 40320.0);
+  s = fma(s, x, 1.0 / 5040.0);
+  s = fma(s, x, 1.0 / 720.0);
+  s = fma(s, x, 1.0 / 120.0);
+  s = fma(s, x, 1.0 / 24.0);
+  s = fma(s, x, 1.0 / 6.0);
+  s = fma(s, x, 0.5);
+  s = fma(s, x, 1.0);
+  s = fma(s, x, 1.0);
+  return ldexp(s, kUnitBits - kFractionBits - (bin >> 4));
 }
-__device__ inline u64 units(Place p) { return units(p.bin, 1, Series()(p.f)); }
+// n tokens of a cell, x of whose fractions: their weight in units.  In bin 0 exact, so
+// equal largest logits weigh alike, alone and together; elsewhere rounded.
+__device__ inline u64 units(int bin, double scale, u64 n, u64 x) {
+  const u64 raw = (n << kFractionBits) + x;
+  return bin == 0 ? raw << (kUnitBits - kFractionBits) : (u64)((double)raw * scale + 0.5);
+}
 // A token's weight unrounded, in units
 __device__ inline double weight(Place p) { return exp2(kUnitBits + (p.f - p.bin) * (1.0 / kGrid)); }
 
@@ -185,53 +204,73 @@ constexpr int kPickWaves = kPickThreads / 64;
 
 struct Mass { u64 w; uint32_t n; };
 
+// Where a search stands: a place (a bin, a part), what lies before it, the tokens inside,
+// the groups of slices that hold them, the scale of the bin.
+struct Hit { int at; Mass before; uint32_t inside; u64 mask; double scale; };
+
 // Sets of what waves tell each other, used in turn: a set is written again only after the
 // barrier behind the next one's writing, when all have read it.
 struct Shared {
   u64 w[kParts];
   uint32_t n[kParts];
   u64 list[kList], few[64];
-  u64 scan_w[2][kPickWaves], hit_w[2][kPickWaves], hit_mask[2][kPickWaves];
-  uint32_t scan_n[2][kPickWaves], hit_n[2][kPickWaves], hit_inside[2][kPickWaves];
+  u64 scan_w[2][kPickWaves];
+  uint32_t scan_n[2][kPickWaves];
+  Hit hit[2][kPickWaves];
   int hit_at[2][kPickWaves];
   u64 found_w[2], found_key[2];
   uint32_t found_n[2], fill;
   int some[64], n_some;
 };
 
+template <int CTRL, int ROWS>
+__device__ inline uint32_t from_lane(uint32_t x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false); }
+template <int CTRL, int ROWS = 0xf>
+__device__ inline void add_from(Mass &v) {
+  const uint32_t lo = from_lane<CTRL, ROWS>((uint32_t)v.w), hi = from_lane<CTRL, ROWS>((uint32_t)(v.w >> 32));
+  v.n += from_lane<CTRL, ROWS>(v.n);
+  v.w += (u64)hi << 32 | lo;
+}
+// Inclusive sums over a wave: within rows of 16 lanes, then from row to row.
+__device__ inline Mass wave_scan(Mass v) {
+  add_from<0x111>(v);           // row_shr 1, 2, 4, 8
+  add_from<0x112>(v);
+  add_from<0x114>(v);
+  add_from<0x118>(v);
+  add_from<0x142, 0xa>(v);      // row_bcast 15 to rows 1 and 3, 31 to rows 2 and 3
+  add_from<0x143, 0xc>(v);
+  return v;
+}
+
 // Inclusive sums over the block's threads.
 __device__ Mass scan(Mass v, Shared &s, int &turn) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   turn ^= 1;
-  for (int d = 1; d < 64; d <<= 1) {
-    const u64 w = __shfl_up(v.w, d);
-    const uint32_t n = __shfl_up(v.n, d);
-    if (lane >= d) { v.w += w; v.n += n; }
-  }
+  v = wave_scan(v);
   if (lane == 63) { s.scan_w[turn][wave] = v.w; s.scan_n[turn][wave] = v.n; }
   __syncthreads();
-  for (int i = 0; i < wave; i++) { v.w += s.scan_w[turn][i]; v.n += s.scan_n[turn][i]; }
+#pragma unroll
+  for (int i = 0; i < kPickWaves - 1; i++) {
+    v.w += i < wave ? s.scan_w[turn][i] : 0;
+    v.n += i < wave ? s.scan_n[turn][i] : 0;
+  }
   return v;
 }
 
-// The first thread that says so, and what it has: its place, what lies before it, and
-// the tokens inside.
-struct Hit { int at; Mass before; uint32_t inside; u64 mask; };
-__device__ Hit first_of(bool here, int at, Mass before, uint32_t inside, u64 mask, Shared &s, int &turn) {
+// What the first thread has that says so.
+__device__ Hit first_of(bool here, const Hit &mine, Shared &s, int &turn) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   turn ^= 1;
   const uint64_t b = __ballot(here);
   if (lane == (b ? __builtin_ctzll(b) : 0)) {
-    s.hit_at[turn][wave] = b ? at : -1;
-    s.hit_w[turn][wave] = before.w;
-    s.hit_n[turn][wave] = before.n;
-    s.hit_inside[turn][wave] = inside;
-    s.hit_mask[turn][wave] = mask;
+    s.hit_at[turn][wave] = b ? mine.at : -1;
+    s.hit[turn][wave] = mine;
   }
   __syncthreads();
   int w = 0;
-  while (w < kPickWaves - 1 && s.hit_at[turn][w] < 0) w++;
-  return {s.hit_at[turn][w], {s.hit_w[turn][w], s.hit_n[turn][w]}, s.hit_inside[turn][w], s.hit_mask[turn][w]};
+#pragma unroll
+  for (int i = kPickWaves - 1; i >= 0; i--) w = s.hit_at[turn][i] >= 0 ? i : w;
+  return s.hit[turn][w];
 }
 
 // Where a search ends: at the first token at which n tokens or the weight w are reached,
@@ -243,7 +282,7 @@ struct Row {
   const float *l;
   int V, bits;                  // tokens; log2 of a quarter of the tokens that a bit of a mask stands for
   float top;
-  double cell_top, per;
+  double cell_top, per, inverse;   // 1 / per
 };
 
 struct Found { Mass upto; u64 key; };   // number and weight up to and with a token, and the token (0: none below `before`)
@@ -270,7 +309,7 @@ __device__ void range_of(const Row &row, int bin, u64 &lo, u64 &hi) {
   hi = 1ull << 52;
   if (!(row.per > 0.0 && fabs(row.cell_top) < 1e15)) return;
   const double want = row.cell_top - bin + (threadIdx.x >> 5 & 1);
-  const uint32_t o = neighbour(finite(want / row.per), 32);
+  const uint32_t o = neighbour(finite(want * row.inverse), 32);
   const uint64_t pass = __ballot(cell_of(of_ord(o), row.per) >= want);
   const uint32_t below = (uint32_t)pass, above = (uint32_t)(pass >> 32);
   if (below && !(below & 1) && above && !(above & 1)) {
@@ -283,7 +322,7 @@ __device__ void range_of(const Row &row, int bin, u64 &lo, u64 &hi) {
 __device__ u64 floor_of(float m, const Row &row) {
   if (!(fabsf(row.top) < __builtin_inff()) || m >= 1.0f) return smallest_key(row.top);
   if (!(row.per > 0.0)) return 1;                         // all weigh alike
-  const uint32_t o = neighbour(finite((double)row.top + log2((double)m) * kGrid / row.per), 64);
+  const uint32_t o = neighbour(finite((double)row.top + log2((double)m) * kGrid * row.inverse), 64);
   const float l = of_ord(o);
   const uint64_t pass = __ballot(l >= row.top || exp2(((double)l - (double)row.top) * row.per / kGrid) >= (double)m);
   return (u64)__shfl(o, pass ? __builtin_ctzll(pass) : 63) << 20;
@@ -297,29 +336,31 @@ __device__ void for_tokens(const Row &row, Shared &s, int bin, u64 lo, u64 hi, F
   const float least = lo >> 20 >= kOrdLowest ? of_ord((uint32_t)(lo >> 20)) : -__builtin_inff(),
               most = hi >> 20 < kOrdInf ? of_ord((uint32_t)(hi >> 20)) : __builtin_inff();
   const int all = s.n_some << row.bits, in = (1 << row.bits) - 1;
+  const auto first = [&](int q) { return q < all ? (s.some[q >> row.bits] << row.bits | (q & in)) * 4 : row.V; };
   for (int q0 = threadIdx.x; q0 < all; q0 += 8 * kPickThreads) {
     float l[8][4];
-    int at[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-      const int q = q0 + j * kPickThreads;
-      at[j] = q < all ? (s.some[q >> row.bits] << row.bits | (q & in)) * 4 : row.V;
-      if (at[j] + 4 <= row.V) {
-        __builtin_memcpy(l[j], row.l + at[j], sizeof l[j]);
+      const int at = first(q0 + j * kPickThreads);
+      if (at + 4 <= row.V) {
+        __builtin_memcpy(l[j], row.l + at, sizeof l[j]);
       } else {
 #pragma unroll
-        for (int c = 0; c < 4; c++) l[j][c] = at[j] + c < row.V ? row.l[at[j] + c] : -__builtin_inff();
+        for (int c = 0; c < 4; c++) l[j][c] = at + c < row.V ? row.l[at + c] : -__builtin_inff();
       }
     }
+    uint32_t in_range = 0;      // few: read again one by one, which keeps the code short (it runs once, from a cold cache)
 #pragma unroll
     for (int j = 0; j < 8; j++)
 #pragma unroll
-      for (int c = 0; c < 4; c++) {
-        if (!(l[j][c] >= least && l[j][c] <= most)) continue;         // most of them, at two comparisons
-        const u64 k = token_key(l[j][c], at[j] + c);
-        const Place p = place_of(l[j][c], row.top, row.cell_top, row.per);
-        if (k >= lo && k < hi && k && p.bin == bin) f(k, p);
-      }
+      for (int c = 0; c < 4; c++) in_range |= (uint32_t)(l[j][c] >= least && l[j][c] <= most) << (4 * j + c);
+    for (; in_range; in_range &= in_range - 1) {
+      const int b = __builtin_ctz(in_range), at = first(q0 + (b >> 2) * kPickThreads) + (b & 3);
+      const float x = at < row.V ? row.l[at] : -__builtin_inff();
+      const u64 k = token_key(x, at);
+      const Place p = place_of(x, row.top, row.cell_top, row.per);
+      if (k >= lo && k < hi && k && p.bin == bin) f(k, p);
+    }
   }
   __syncthreads();
 }
@@ -328,21 +369,21 @@ __device__ void for_tokens(const Row &row, Shared &s, int bin, u64 lo, u64 hi, F
 // `before` is, and go to the part where the search ends.  each(f) calls f(key, place) for
 // the range's tokens, and synchronizes.
 template <typename E>
-__device__ void divide(Shared &s, int &turn, Goal goal, u64 &lo, u64 &hi, Mass &before, uint32_t &inside, E each) {
+__device__ void divide(Shared &s, int &turn, Goal goal, const Hit &bin, u64 &lo, u64 &hi, Mass &before, uint32_t &inside, E each) {
   const int span = 64 - __builtin_clzll((hi - lo - 1) | 1), shift = span > 9 ? span - 9 : 0;
   const int t = threadIdx.x;
   if (t < kParts) { s.w[t] = 0; s.n[t] = 0; }
   __syncthreads();
   each([&](u64 k, Place p) {
     const int d = (int)((hi - 1 - k) >> shift);
-    atomicAdd(&s.w[d], units(p));
+    atomicAdd(&s.w[d], units(bin.at, bin.scale, 1, Series()(p.f)));
     atomicAdd(&s.n[d], 1u);
   });
   const Mass own = t < kParts ? Mass{s.w[t], s.n[t]} : Mass{0, 0};
   const Mass upto = scan(own, s, turn);
   const bool ends = own.n && (reached({before.w + upto.w, before.n + upto.n}, goal) || upto.n == inside);
   const bool floor_here = goal.floor && t < kParts && (goal.floor >= hi ? t == 0 : goal.floor >= lo && (int)((hi - 1 - goal.floor) >> shift) == t);
-  const Hit h = first_of(ends || floor_here, t, {upto.w - own.w, upto.n - own.n}, own.n, 0, s, turn);
+  const Hit h = first_of(ends || floor_here, {t, {upto.w - own.w, upto.n - own.n}, own.n, 0, 0.0}, s, turn);
   before.w += h.before.w;
   before.n += h.before.n;
   inside = h.inside;
@@ -369,7 +410,7 @@ __device__ Found locate(const Row &row, Shared &s, int &turn, Goal goal, const H
     __syncthreads();
     list_bin = bin;
     while (inside > kList) {
-      divide(s, turn, goal, lo, hi, before, inside, [&](auto f) { for_tokens(row, s, bin, lo, hi, f); });
+      divide(s, turn, goal, h, lo, hi, before, inside, [&](auto f) { for_tokens(row, s, bin, lo, hi, f); });
       list_bin = -1;
     }
     if (!inside) return {before, 0};
@@ -385,7 +426,7 @@ __device__ Found locate(const Row &row, Shared &s, int &turn, Goal goal, const H
   };
   const u64 *few = s.list;
   if (listed > 64) {
-    while (inside > 64) divide(s, turn, goal, lo, hi, before, inside, in_list);
+    while (inside > 64) divide(s, turn, goal, h, lo, hi, before, inside, in_list);
     if (!inside) return {before, 0};
     if (t == 0) s.fill = 0;
     __syncthreads();
@@ -401,12 +442,8 @@ __device__ Found locate(const Row &row, Shared &s, int &turn, Goal goal, const H
     u64 k = 0;                  // lane `rank` takes the key
     for (int i = 0; i < (int)inside; i++)
       if (__builtin_amdgcn_readlane(rank, i) == t) k = of_lane(i);
-    Mass m = {k ? units(place_of(key_logit(k), row.top, row.cell_top, row.per)) : 0, k != 0};
-    for (int d = 1; d < 64; d <<= 1) {
-      const u64 w = __shfl_up(m.w, d);
-      const uint32_t n = __shfl_up(m.n, d);
-      if (t >= d) { m.w += w; m.n += n; }
-    }
+    Mass m = {k ? units(bin, h.scale, 1, Series()(place_of(key_logit(k), row.top, row.cell_top, row.per).f)) : 0, k != 0};
+    m = wave_scan(m);
     const u64 next = __shfl_down(k, 1);
     m = {before.w + m.w, before.n + m.n};
     const uint64_t stops = __ballot(k && (reached(m, goal) || t + 1 == (int)inside || next < goal.floor));
@@ -456,7 +493,7 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(QSampleRows a, int
     }
     return;
   }
-  Row row = {a.logits + r * a.stride, a.vocab, bits, key_logit(best), 0.0, ask.per};
+  Row row = {a.logits + r * a.stride, a.vocab, bits, key_logit(best), 0.0, ask.per, 1.0 / ask.per};
   row.cell_top = cell_of(row.top, row.per);
   if (t < 64)
     for (int i = t; i < slices; i += 64) {
@@ -477,27 +514,36 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(QSampleRows a, int
     x += y & ((1ull << kCountShift) - 1);
     mask |= (u64)(y != 0) << (i >> group);
   }
-  own.w = units(t, own.n, x);
+  const double scale = scale_of(t);
+  own.w = units(t, scale, own.n, x);
   const Mass upto = scan(own, s, turn);
   const Mass before = {upto.w - own.w, upto.n - own.n};
   if (t == kPickThreads - 1) { s.found_w[0] = upto.w; s.found_n[0] = upto.n; }
   __syncthreads();
   const Mass held = {s.found_w[0], s.found_n[0]};          // tokens behind the last bin weigh nothing
 
-  int list_bin = -1;
-  const auto search = [&](Goal goal) -> Found {
-    const int floor_bin = goal.floor ? place_of(key_logit(goal.floor), row.top, row.cell_top, row.per).bin : kBins;
-    const bool ends = own.n && (reached(upto, goal) || upto.n == held.n);
-    return locate(row, s, turn, goal, first_of(ends || t == floor_bin, t, before, own.n, mask, s, turn), list_bin);
-  };
-
   const bool by_min = mp > 0x1p-43f;
   const bool by_mass = p > 0.0f && p < 1.0f, by_count = k > 0 && (uint32_t)k < all_n;
-  Mass kept = {held.w, by_count ? (uint32_t)k : all_n};    // a limit among the tokens that weigh nothing needs no search
-  if ((by_count && kept.n < held.n) || by_mass || by_min)
-    kept = search({kept.n, by_mass ? (double)p * (double)held.w : __builtin_inf(), by_min ? floor_of(mp, row) : 0}).upto;
   const float u = u_given > 0.0f ? (u_given < 1.0f ? u_given : 0x1.fffffep-1f) : 0.0f;
-  const Found f = search({kept.n, (double)u * (double)kept.w, 0});
+  Mass kept = {held.w, by_count ? (uint32_t)k : all_n};    // a limit among the tokens that weigh nothing needs no search
+  Found f = {{0, 0}, 0};
+  int list_bin = -1;
+  // first where the kept set ends, then the token; one code for both, as it runs from a cold cache
+#pragma unroll 1
+  for (int pass = (by_count && kept.n < held.n) || by_mass || by_min ? 0 : 1; pass < 2; pass++) {
+    Goal goal = {kept.n, (double)u * (double)kept.w, 0};
+    int floor_bin = kBins;
+    if (pass == 0) {
+      goal.w = by_mass ? (double)p * (double)held.w : __builtin_inf();
+      if (by_min) {
+        goal.floor = floor_of(mp, row);
+        floor_bin = place_of(key_logit(goal.floor), row.top, row.cell_top, row.per).bin;
+      }
+    }
+    const bool ends = own.n && (reached(upto, goal) || upto.n == held.n);
+    f = locate(row, s, turn, goal, first_of(ends || t == floor_bin, {t, before, own.n, mask, scale}, s, turn), list_bin);
+    if (pass == 0) kept = f.upto;
+  }
   if (t == 0) {
     a.token[r] = key_index(f.key);
     if (a.prob) a.prob[r] = (float)(weight(place_of(key_logit(f.key), row.top, row.cell_top, row.per)) / (double)kept.w);
