@@ -61,14 +61,28 @@ __host__ __device__ inline int clamp_len(int len, int width, int page_size) {
   return len < 0 ? 0 : len > most ? most : len;
 }
 
-// Page of token `key` and its place there; -1: no page of the cache, or no token.
-__host__ __device__ inline int page_of(const int *table, long long key, int len, int page_size, int n_pages, int *place) {
-  *place = 0;
-  if (key < 0 || key >= len) return -1;
-  const int e = (int)key / page_size, p = table[e];
-  if (p < 0 || p >= n_pages) return -1;
-  *place = (int)key - e * page_size;
-  return p;
+// Where a token lies: its table entry (of the last token for one behind it, so that the
+// entry can always be read; len > 0) and its place there; then the entry's page, -1 for
+// no page of the cache or no token.
+__host__ __device__ inline int entry_of(long long key, int len, int page_size, int *place) {
+  const int k = key < len ? (int)key : len - 1, e = k / page_size;
+  *place = k - e * page_size;
+  return e;
+}
+__host__ __device__ inline int page_of(int entry, long long key, int len, int n_pages) {
+  return key < len && entry >= 0 && entry < n_pages ? entry : -1;
+}
+
+// Inclusive sums over a wave: within rows of 16 lanes, then from row to row.
+template <int CTRL, int ROWS>
+__device__ inline int from_lane(int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false); }
+__device__ inline int wave_scan(int x) {
+  x += from_lane<0x111, 0xf>(x);        // row_shr 1, 2, 4, 8
+  x += from_lane<0x112, 0xf>(x);
+  x += from_lane<0x114, 0xf>(x);
+  x += from_lane<0x118, 0xf>(x);
+  x += from_lane<0x142, 0xa>(x);        // row_bcast 15 to rows 1 and 3, 31 to rows 2 and 3
+  return x + from_lane<0x143, 0xc>(x);
 }
 
 // Steps of a wave's share when all tiles together take `units`.
@@ -185,12 +199,12 @@ struct VTile { uint32_t w[Cfg<T, HDP>::SUB][4][Cfg<T, HDP>::PIECES][Cfg<T, HDP>:
 template <bool UNI>
 struct Window {
   int first, page, place;
-  __device__ inline void load(const PaArgs &a, const int *table, int from, int len) {
+  __device__ inline long long key() const { return UNI ? ((long long)first + (threadIdx.x & 63)) * 16 : (long long)first + (threadIdx.x & 63); }
+  __device__ inline void request(const PaArgs &a, const int *table, int from, int len) {
     first = from;
-    const int lane = threadIdx.x & 63;
-    const long long key = UNI ? ((long long)from + lane) * 16 : (long long)from + lane;
-    page = page_of(table, key, len, a.page_size, a.n_pages, &place);
+    page = table[entry_of(key(), len, a.page_size, &place)];
   }
+  __device__ inline void settle(const PaArgs &a, int len) { page = page_of(page, key(), len, a.n_pages); }
 };
 
 template <int T, int HDP, bool UNI, bool STREAM>
@@ -205,13 +219,12 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
 
   // this wave's share of all steps; shares of one block lie far apart, so that few of
   // them are spread over the CUs
-  int mine = 0, all = 0;                            // steps of request `lane` of the last 64; of all
-  for (int r = 0; r < a.n_req; r += 64) {
-    mine = r + lane < a.n_req ? (clamp_len(a.lens[r + lane], a.width, a.page_size) + STEP - 1) / STEP : 0;
-    all += mine;
-  }
-  for (int d = 32; d; d >>= 1) all += __shfl_xor(all, d);
-  const long long units = (long long)__builtin_amdgcn_readfirstlane(all) * tiles;
+  const auto len_of = [&](int r) { return r < a.n_req ? clamp_len(a.lens[r], a.width, a.page_size) : 0; };
+  int len = len_of(lane);                           // of request `lane` of the 64 in hand, then of the one at work
+  int upto = wave_scan((len + STEP - 1) / STEP);    // steps of those up to it
+  long long units = (long long)__builtin_amdgcn_readlane(upto, 63) * tiles;
+  for (int r = 64; r < a.n_req; r += 64)
+    units += (long long)__builtin_amdgcn_readlane(wave_scan((len_of(r + lane) + STEP - 1) / STEP), 63) * tiles;
   const long long share = share_of(units);
   const int id = wave * kBlocks + blockIdx.x;
   long long u = id * share;
@@ -221,28 +234,26 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
   int r = 0;                                        // the request it begins in, and that one's first unit
   long long r_begin = 0;
   for (; u < end; r += 64) {
-    if (a.n_req > 64) mine = r + lane < a.n_req ? (clamp_len(a.lens[r + lane], a.width, a.page_size) + STEP - 1) / STEP : 0;
-    int s = mine;
-    for (int d = 1; d < 64; d <<= 1) {
-      const int t = __shfl_up(s, d);
-      if (lane >= d) s += t;
+    if (r) {
+      len = len_of(r + lane);
+      upto = wave_scan((len + STEP - 1) / STEP);
     }
-    const uint64_t past = __ballot(r_begin + (long long)s * tiles > u);
+    const uint64_t past = __ballot(r_begin + (long long)upto * tiles > u);
     if (past) {
       const int at = __builtin_ctzll(past);
-      r_begin += (long long)(__builtin_amdgcn_readlane(s, at) - __builtin_amdgcn_readlane(mine, at)) * tiles;
+      len = __builtin_amdgcn_readlane(len, at);
+      r_begin += (long long)(__builtin_amdgcn_readlane(upto, at) - (len + STEP - 1) / STEP) * tiles;
       r += at;
       break;
     }
-    r_begin += (long long)__builtin_amdgcn_readlane(s, 63) * tiles;
+    r_begin += (long long)__builtin_amdgcn_readlane(upto, 63) * tiles;
   }
 
   while (u < end) {
-    const int len = clamp_len(a.lens[r], a.width, a.page_size);
     const int steps = (len + STEP - 1) / STEP;
     if (u >= r_begin + (long long)steps * tiles) {
       r_begin += (long long)steps * tiles;
-      r++;
+      len = len_of(++r);
       continue;
     }
     const unsigned long long at = u - r_begin;
@@ -255,7 +266,7 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
     const int row = n % rows;                       // columns past the tile's heads repeat them
 
     Window<UNI> win;
-    win.load(a, table, UNI ? from * SUB : from * STEP, len);
+    win.request(a, table, UNI ? from * SUB : from * STEP, len);
 
     // queries: head h0 + row, dims 32 c + 8 g ..; scaled so that weights are powers of two
     float unscale = 1.0f;
@@ -306,6 +317,7 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
       __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
     const char *q_mine = q_lds + row * C::QROW;
+    win.settle(a, len);
 
     float m = kNegInf, l = 0.0f;                    // of the lane's query head; l over the lane's keys
     f4 acc[DPL];
@@ -333,7 +345,10 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
     };
     auto advance = [&](int s) {                     // the window holds step s
       const int at = UNI ? s * SUB : s * STEP;
-      if (at - win.first >= 64) win.load(a, table, at, len);
+      if (at - win.first >= 64) {
+        win.request(a, table, at, len);
+        win.settle(a, len);
+      }
     };
     auto load_k = [&](int s, KTile<T, HDP> &k) {
 #pragma unroll
@@ -597,7 +612,7 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
 
 // One block a share and row: where a tile begins in the share and goes on behind it, its
 // parts put together in the order of their keys, 8 (hd <= 128) or 4 side by side.
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 256, kAhead = 4;
 __global__ __launch_bounds__(kJoinThreads) void k_paged_join(PaArgs a, float shift) {
   __shared__ float weight[kShares], lds[kJoinThreads / 32][256], red[2][kJoinThreads / 64];
   const int4 s = a.split[blockIdx.x];
@@ -608,9 +623,21 @@ __global__ __launch_bounds__(kJoinThreads) void k_paged_join(PaArgs a, float shi
   // the first part may follow another tile's in its share
   const float *part = a.part + 2LL * blockIdx.x * one + row * (a.hd + 2);
   const int first = s.w * one;
-  float top = kNegInf;
+  const int width = a.hd <= 128 ? 32 : 64, groups = kJoinThreads / width;
+  const int group = threadIdx.x / width, d = threadIdx.x % width * 4;
+  // a thread's first values are under way while the weights are formed
+  float y[kAhead][4];
+#pragma unroll
+  for (int j = 0; j < kAhead; j++) {
+    const int i = group + j * groups;
+    const float *p = part + (i < parts && d < a.hd ? 2LL * i * one + (i ? 0 : first) + d : first);
+    __builtin_memcpy(y[j], p, sizeof y[j]);
+  }
+  float top = kNegInf, l = 0.0f;
   for (int i = threadIdx.x; i < parts; i += kJoinThreads) {
-    weight[i] = part[2LL * i * one + (i ? 0 : first) + a.hd];
+    const float *p = part + 2LL * i * one + (i ? 0 : first) + a.hd;
+    weight[i] = p[0];
+    if (i < kJoinThreads) l = p[1];
     top = fmaxf(top, weight[i]);
   }
   for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
@@ -620,7 +647,7 @@ __global__ __launch_bounds__(kJoinThreads) void k_paged_join(PaArgs a, float shi
   float sum = 0.0f;
   for (int i = threadIdx.x; i < parts; i += kJoinThreads) {
     weight[i] = part_weight(weight[i], top);
-    sum += part[2LL * i * one + (i ? 0 : first) + a.hd + 1] * weight[i];
+    sum += (i < kJoinThreads ? l : part[2LL * i * one + a.hd + 1]) * weight[i];
   }
   for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
   if ((threadIdx.x & 63) == 0) red[1][threadIdx.x >> 6] = sum;
@@ -628,16 +655,23 @@ __global__ __launch_bounds__(kJoinThreads) void k_paged_join(PaArgs a, float shi
   sum = 0.0f;
   for (int i = 0; i < kJoinThreads / 64; i++) sum += red[1][i];
 
-  const int width = a.hd <= 128 ? 32 : 64, groups = kJoinThreads / width;
-  const int group = threadIdx.x / width, d = threadIdx.x % width * 4;
   if (d < a.hd) {
     float x[4] = {0, 0, 0, 0};
-#pragma unroll 8
-    for (int i = group; i < parts; i += groups) {
-      float y[4];
-      __builtin_memcpy(y, part + 2LL * i * one + (i ? 0 : first) + d, sizeof y);
 #pragma unroll
-      for (int c = 0; c < 4; c++) x[c] += y[c] * weight[i];
+    for (int j = 0; j < kAhead; j++) {
+      const int i = group + j * groups;
+      if (i < parts) {
+        const float f = weight[i];
+#pragma unroll
+        for (int c = 0; c < 4; c++) x[c] += y[j][c] * f;
+      }
+    }
+#pragma unroll 8
+    for (int i = group + kAhead * groups; i < parts; i += groups) {
+      float z[4];
+      __builtin_memcpy(z, part + 2LL * i * one + d, sizeof z);
+#pragma unroll
+      for (int c = 0; c < 4; c++) x[c] += z[c] * weight[i];
     }
 #pragma unroll
     for (int c = 0; c < 4; c++) lds[group][d + c] = x[c];
@@ -684,7 +718,12 @@ int launch_hd(const char *fn, const PaArgs &a, hipStream_t stream) {
 }  // namespace
 
 extern "C" int qllama_test_page_of(const int32_t *table, int width, int page_size, int n_pages, int len, long long key, int *place) {
-  return page_of(table, key, clamp_len(len, width, page_size), page_size, n_pages, place);
+  len = clamp_len(len, width, page_size);
+  *place = 0;
+  if (key < 0 || len == 0) return -1;
+  const int page = page_of(table[entry_of(key, len, page_size, place)], key, len, n_pages);
+  if (page < 0) *place = 0;
+  return page;
 }
 
 extern "C" size_t qllama_paged_attention_work(const QPagedKV *c, int n_req, int n_heads) {
