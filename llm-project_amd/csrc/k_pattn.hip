@@ -38,7 +38,7 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 constexpr int kThreads = 256, kWaves = 4;
 constexpr int kBlocks = 512;          // two blocks of four waves a CU
 constexpr int kShares = kBlocks * kWaves;
-constexpr int kMinShare = 2;          // steps a wave takes at least
+constexpr int kMinShare = 1;          // steps a wave takes at least
 constexpr float kNegInf = -__builtin_inff();
 
 struct PaArgs {
@@ -233,6 +233,7 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
   const long long begin = u;
   int r = 0;                                        // the request it begins in, and that one's first unit
   long long r_begin = 0;
+  int steps = 0, tile = 0, from = 0;                // of the request; in it; in that
   for (; u < end; r += 64) {
     if (r) {
       len = len_of(r + lane);
@@ -249,80 +250,39 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
     r_begin += (long long)__builtin_amdgcn_readlane(upto, 63) * tiles;
   }
 
-  while (u < end) {
-    const int steps = (len + STEP - 1) / STEP;
-    if (u >= r_begin + (long long)steps * tiles) {
-      r_begin += (long long)steps * tiles;
-      len = len_of(++r);
-      continue;
-    }
+  if (u < end) {
     const unsigned long long at = u - r_begin;
-    const int tile = at >> 32 ? (int)(at / (unsigned)steps) : (int)((unsigned)at / (unsigned)steps);
-    const int from = (int)(at - (unsigned long long)tile * steps);
+    steps = (len + STEP - 1) / STEP;
+    tile = at >> 32 ? (int)(at / (unsigned)steps) : (int)((unsigned)at / (unsigned)steps);
+    from = (int)(at - (unsigned long long)tile * steps);
+  }
+  Window<UNI> win;
+  win.first = -1;
+
+  while (u < end) {
+    if (tile == tiles) {                            // the next request that has tokens
+      do len = len_of(++r); while (len == 0);
+      steps = (len + STEP - 1) / STEP;
+      tile = 0;
+      win.first = -1;
+    }
     const int to = (int)(end - u < steps - from ? from + (end - u) : steps);
-    const int kvh = tile / a.tiles, h0 = kvh * a.G + (tile % a.tiles) * 16;
-    const int rows = a.G - (tile % a.tiles) * 16 < 16 ? a.G - (tile % a.tiles) * 16 : 16;
+    const int kvh = a.tiles == 1 ? tile : tile / a.tiles, part = a.tiles == 1 ? 0 : tile - kvh * a.tiles;
+    const int h0 = kvh * a.G + part * 16, rows = a.G - part * 16 < 16 ? a.G - part * 16 : 16;
     const int *table = a.table + r * a.table_stride;
     const int row = n % rows;                       // columns past the tile's heads repeat them
+    const bool fresh = win.first != (UNI ? from * SUB : from * STEP);    // a request's tiles read the same pages
+    if (fresh) win.request(a, table, UNI ? from * SUB : from * STEP, len);
 
-    Window<UNI> win;
-    win.request(a, table, UNI ? from * SUB : from * STEP, len);
-
-    // queries: head h0 + row, dims 32 c + 8 g ..; scaled so that weights are powers of two
-    float unscale = 1.0f;
-    {
-      float qf[CH][8];
-      float qmax = 0.0f;
-      const float *q = a.q + r * a.q_stride + (long long)(h0 + row) * a.hd;
+    // queries: head h0 + row, dims 32 c + 8 g ..
+    float qf[CH][8];
+    const float *q = a.q + r * a.q_stride + (long long)(h0 + row) * a.hd;
 #pragma unroll
-      for (int c = 0; c < CH; c++) {
-        const int d = 32 * c + 8 * g;
-        __builtin_memcpy(qf[c], q + (d < a.hd ? d : 0), sizeof qf[c]);     // 4-byte aligned; head_dim is a multiple of 8
-      }
-#pragma unroll
-      for (int c = 0; c < CH; c++)
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          qf[c][i] = 32 * c + 8 * g < a.hd ? qf[c][i] * a.qscale : 0.0f;
-          qmax = fmaxf(qmax, fabsf(qf[c][i]));
-        }
-      int e = 0;
-      if constexpr (T == QLLAMA_KV_F16) {           // into f16's range, by a power of two
-        qmax = max_groups(qmax);
-        e = qmax > 0.0f && qmax < __builtin_inff() ? ilogbf(qmax) - 13 : 0;
-        unscale = ldexpf(1.0f, e);
-      }
-      __builtin_amdgcn_wave_barrier();              // the last tile's reads come first
-#pragma unroll
-      for (int c = 0; c < CH; c++) {
-        char *to_lds = q_lds + row * C::QROW + (32 * c + 8 * g) * C::QES;
-        if constexpr (T == QLLAMA_KV_F32) {
-          if (n < rows) __builtin_memcpy(__builtin_assume_aligned(to_lds, 16), qf[c], sizeof qf[c]);
-        } else if constexpr (T == QLLAMA_KV_F16) {
-#pragma unroll
-          for (int i = 0; i < 8; i++) qf[c][i] = ldexpf(qf[c][i], -e);
-          const Parts2 x = cut2(qf[c]);
-#pragma unroll
-          for (int p = 0; p < 2; p++)
-            if (n < rows) *reinterpret_cast<u4 *>(to_lds + p * a.rows * C::QROW) = x.p[p];
-        } else {
-          const Parts3 x = cut3(qf[c]);
-#pragma unroll
-          for (int p = 0; p < 3; p++)
-            if (n < rows) *reinterpret_cast<u4 *>(to_lds + p * a.rows * C::QROW) = x.p[p];
-        }
-      }
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    for (int c = 0; c < CH; c++) {
+      const int d = 32 * c + 8 * g;
+      __builtin_memcpy(qf[c], q + (d < a.hd ? d : 0), sizeof qf[c]);       // 4-byte aligned; head_dim is a multiple of 8
     }
-    const char *q_mine = q_lds + row * C::QROW;
-    win.settle(a, len);
-
-    float m = kNegInf, l = 0.0f;                    // of the lane's query head; l over the lane's keys
-    f4 acc[DPL];
-#pragma unroll
-    for (int c = 0; c < DPL; c++) acc[c] = f4{0, 0, 0, 0};
+    if (fresh) win.settle(a, len);
 
     const char *kbase = a.k + kvh * a.hst, *vbase = a.v + kvh * a.hst;
     int k_off[C::KL], v_off[C::PIECES];             // padded dims read dim 0: their products are dropped, or with 0
@@ -397,6 +357,57 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
         }
       }
     };
+
+    KTile<T, HDP> k0, k1;
+    load_k(from, k0);
+
+    // into LDS, scaled so that weights are powers of two
+    float unscale = 1.0f;
+    {
+      float qmax = 0.0f;
+#pragma unroll
+      for (int c = 0; c < CH; c++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          qf[c][i] = 32 * c + 8 * g < a.hd ? qf[c][i] * a.qscale : 0.0f;
+          qmax = fmaxf(qmax, fabsf(qf[c][i]));
+        }
+      int e = 0;
+      if constexpr (T == QLLAMA_KV_F16) {           // into f16's range, by a power of two
+        qmax = max_groups(qmax);
+        e = qmax > 0.0f && qmax < __builtin_inff() ? ilogbf(qmax) - 13 : 0;
+        unscale = ldexpf(1.0f, e);
+      }
+      __builtin_amdgcn_wave_barrier();              // the last tile's reads come first
+#pragma unroll
+      for (int c = 0; c < CH; c++) {
+        char *to_lds = q_lds + row * C::QROW + (32 * c + 8 * g) * C::QES;
+        if constexpr (T == QLLAMA_KV_F32) {
+          if (n < rows) __builtin_memcpy(__builtin_assume_aligned(to_lds, 16), qf[c], sizeof qf[c]);
+        } else if constexpr (T == QLLAMA_KV_F16) {
+#pragma unroll
+          for (int i = 0; i < 8; i++) qf[c][i] = ldexpf(qf[c][i], -e);
+          const Parts2 x = cut2(qf[c]);
+#pragma unroll
+          for (int p = 0; p < 2; p++)
+            if (n < rows) *reinterpret_cast<u4 *>(to_lds + p * a.rows * C::QROW) = x.p[p];
+        } else {
+          const Parts3 x = cut3(qf[c]);
+#pragma unroll
+          for (int p = 0; p < 3; p++)
+            if (n < rows) *reinterpret_cast<u4 *>(to_lds + p * a.rows * C::QROW) = x.p[p];
+        }
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+    const char *q_mine = q_lds + row * C::QROW;
+
+    float m = kNegInf, l = 0.0f;                    // of the lane's query head; l over the lane's keys
+    f4 acc[DPL];
+#pragma unroll
+    for (int c = 0; c < DPL; c++) acc[c] = f4{0, 0, 0, 0};
 
     auto step = [&](int s, KTile<T, HDP> &k, KTile<T, HDP> &k_next) {
       VTile<T, HDP> v;
@@ -563,8 +574,6 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
       }
     };
 
-    KTile<T, HDP> k0, k1;
-    load_k(from, k0);
     for (int s = from; s < to; s += 2) {
       step(s, k0, k1);
       if (s + 1 < to) step(s + 1, k1, k0);
@@ -599,6 +608,8 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
     if (from == 0 && !whole && lane == 0)            // the tile goes on in the shares behind this one
       a.split[id] = make_int4(1 + (int)((steps - to + share - 1) / share), r, tile, u == begin ? 0 : 1);
     u += to - from;
+    from = 0;
+    tile++;
   }
 
   // a request without a token has no tile: its outputs are set here
