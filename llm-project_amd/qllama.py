@@ -652,6 +652,8 @@ def _flat(t, name, dtype, size):
 
 def _ptr(t, name, dtype, size, inner):
     """The same where the last `inner` dimensions have to be contiguous."""
+    if t.is_cuda and _dtypes.get(t.dtype) == dtype and size == 0 and inner == 1 and t.stride(-1) == 1:
+        return t.data_ptr()
     if not t.is_cuda:
         raise ValueError(f"{name} is not on the GPU")
     if _dtype(t) != dtype:
@@ -729,29 +731,30 @@ def paged_plan(cached, added, table, ring, state, page_size, lens, status, start
     _done(lib().qllama_paged_plan(a, _stream(stream)), "qllama_paged_plan")
 
 
+def _heads(t, name, rows, heads, hd):
+    """Address and row stride of a float32 GPU tensor (rows, heads, hd) whose rows are contiguous."""
+    shape, (s0, s1, s2) = t.shape, t.stride()
+    if tuple(shape) != (rows, heads, hd):
+        raise ValueError(f"{name} must have the shape {(rows, heads, hd)}, not {tuple(shape)}")
+    if not t.is_cuda or _dtypes.get(t.dtype) != "float32" or (hd != 1 and s2 != 1) or (heads != 1 and s1 != hd):
+        _ptr(t, name, "float32", 0, 2)
+    return t.data_ptr(), s0 if rows > 1 else heads * hd
+
+
 def paged_append(cache, k, v, slots, q=None, q_out=None, positions=None, cos=None, sin=None, bad=None, stream=None):
     """qllama_paged_append: k, v (rows, KV heads, head_dim) float32 into their slots; with cos and sin (positions,
     head_dim / 2), keys and the queries q (rows, heads, head_dim) turned by their positions' angles, q into q_out."""
-    c = cache.c
-    rows, hd = slots.numel(), c.head_dim
-    heads = 0
-
-    def take(t, name):
-        if len(t.shape) != 3 or t.shape[0] != rows or t.shape[2] != hd:
-            raise ValueError(f"{name} must have the shape (rows, heads, head_dim)")
-        return _ptr(t, name, "float32", 0, 2), _row_stride(t, t.shape[1] * hd)
-
-    if k.shape[1] != c.n_kv or v.shape[1] != c.n_kv:
-        raise ValueError("k and v must have the cache's KV heads")
-    kp, ks = take(k, "k")
-    vp, vs = take(v, "v")
-    qp = qs = op = os_ = n_pos = 0
+    n_kv, hd = cache.c.n_kv, cache.c.head_dim
+    rows = slots.numel()
+    heads = qp = qs = op = os_ = n_pos = 0
+    kp, ks = _heads(k, "k", rows, n_kv, hd)
+    vp, vs = _heads(v, "v", rows, n_kv, hd)
     if q is not None:
-        heads = q.shape[1]
-        if q_out is None or q_out.shape[1] != heads:
+        if q_out is None:
             raise ValueError("q needs q_out of its shape")
-        qp, qs = take(q, "q")
-        op, os_ = take(q_out, "q_out")
+        heads = q.shape[1]
+        qp, qs = _heads(q, "q", rows, heads, hd)
+        op, os_ = _heads(q_out, "q_out", rows, heads, hd)
     if cos is not None:
         n_pos = cos.shape[0]
         if sin is None or positions is None:
@@ -773,18 +776,19 @@ def paged_attention_work(cache, n_req, n_heads):
 def paged_attention(cache, q, table, lens, o, work, lse=None, scale=0.0, stream=None):
     """qllama_paged_attention: o (requests, heads, head_dim) and lse (requests, heads) of q over the first lens tokens of
     every request's pages table (requests, width)."""
-    if len(q.shape) != 3 or len(o.shape) != 3 or len(table.shape) != 2:
-        raise ValueError("q and o must have the shape (requests, heads, head_dim), table (requests, width)")
     n, heads, hd = q.shape
+    if len(table.shape) != 2 or table.shape[0] < n or hd != cache.c.head_dim:
+        raise ValueError("q, table and the cache do not fit together")
     width = table.shape[1]
-    if tuple(o.shape) != (n, heads, hd) or hd != cache.c.head_dim or table.shape[0] < n:
-        raise ValueError("q, o, table and the cache do not fit together")
-    if lse is not None and tuple(lse.shape) != (n, heads):
-        raise ValueError("lse must have the shape (requests, heads)")
-    a = PAGED_QUERY.pack(n, heads, width, _row_stride(q, heads * hd), _row_stride(o, heads * hd),
-                         0 if lse is None else _row_stride(lse, heads), _row_stride(table, width), _ptr(q, "q", "float32", 0, 2),
-                         _ptr(o, "o", "float32", 0, 2), 0 if lse is None else _ptr(lse, "lse", "float32", 0, 1),
-                         _ptr(table, "table", "int32", 0, 1), _flat(lens, "lens", "int32", n), scale, *_work(work))
+    qp, qs = _heads(q, "q", n, heads, hd)
+    op, os_ = _heads(o, "o", n, heads, hd)
+    lp = ls = 0
+    if lse is not None:
+        if tuple(lse.shape) != (n, heads):
+            raise ValueError("lse must have the shape (requests, heads)")
+        lp, ls = _ptr(lse, "lse", "float32", 0, 1), _row_stride(lse, heads)
+    a = PAGED_QUERY.pack(n, heads, width, qs, os_, ls, _row_stride(table, width), qp, op, lp, _ptr(table, "table", "int32", 0, 1),
+                         _flat(lens, "lens", "int32", n), scale, *_work(work))
     _done(lib().qllama_paged_attention(cache.ref, a, _stream(stream)), "qllama_paged_attention")
 
 
