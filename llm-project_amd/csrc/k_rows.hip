@@ -213,7 +213,7 @@ struct Hit { int at; Mass before; uint32_t inside; u64 mask; double scale; };
 struct Shared {
   u64 w[kParts];
   uint32_t n[kParts];
-  u64 list[kList], few[64];
+  u64 list[kList], few[64], order[64];
   u64 scan_w[2][kPickWaves];
   uint32_t scan_n[2][kPickWaves];
   Hit hit[2][kPickWaves];
@@ -439,9 +439,11 @@ __device__ Found locate(const Row &row, Shared &s, int &turn, Goal goal, const H
     const auto of_lane = [&](int i) { return (u64)__builtin_amdgcn_readlane((int)(mine >> 32), i) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)mine, i); };
     int rank = 0;
     for (int i = 0; i < (int)inside; i++) rank += of_lane(i) > mine;
-    u64 k = 0;                  // lane `rank` takes the key
-    for (int i = 0; i < (int)inside; i++)
-      if (__builtin_amdgcn_readlane(rank, i) == t) k = of_lane(i);
+    if (mine) s.order[rank] = mine;
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    const u64 k = mine ? s.order[t] : 0;
     Mass m = {k ? units(bin, h.scale, 1, Series()(place_of(key_logit(k), row.top, row.cell_top, row.per).f)) : 0, k != 0};
     m = wave_scan(m);
     const u64 next = __shfl_down(k, 1);
