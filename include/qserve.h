@@ -82,7 +82,7 @@ typedef struct {
 typedef struct {
   int n_req;              // 0 .. 8192
   int width;              // table entries of a request
-  int page_size, ring_size;
+  int page_size, ring_size;                  // ring_size and max_rows: up to 2^30
   int max_rows;           // room for rows in slots, positions and requests
   int64_t table_stride;   // entries between two rows of table, >= width
   const int32_t *cached, *added, *state;     // n_req, n_req, 2

@@ -281,7 +281,8 @@ extern "C" int qllama_paged_plan(const QPagedPlan *p, void *stream) {
   if (p->n_req < 0 || p->n_req > kPlanMaxReq) return qs::refuse(fn, "n_req must be 0 .. 8192");
   if (p->width < 1 || p->page_size < 1 || (int64_t)p->width * p->page_size > INT_MAX)
     return qs::refuse(fn, "bad width or page size (width * page_size must fit in 31 bits)");
-  if (p->ring_size < 1 || p->max_rows < 0 || p->table_stride < p->width) return qs::refuse(fn, "bad ring size, max_rows or table stride");
+  if (p->ring_size < 1 || p->ring_size > (1 << 30) || p->max_rows < 0 || p->max_rows > (1 << 30) || p->table_stride < p->width)
+    return qs::refuse(fn, "bad ring size, max_rows (each up to 2^30) or table stride");
   if (!p->state || !p->ring || !p->starts || !p->state_out || (p->n_req && (!p->cached || !p->added || !p->table || !p->lens || !p->status)) ||
       (p->max_rows && (!p->slots || !p->positions || !p->requests)))
     return qs::refuse(fn, "null buffer");

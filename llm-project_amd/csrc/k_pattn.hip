@@ -416,13 +416,13 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
       bool absent = (s + 1) * STEP > len;
 #pragma unroll
       for (int i = 0; i < SUB; i++) {
-        int page[4], place[4];
-        if constexpr (UNI) page[0] = lookup(s, i, 0, &place[0]);
+        int page[4], place[4], group_place = 0;
+        const int group_page = UNI ? lookup(s, i, 0, &group_place) : 0;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
           if constexpr (UNI) {
-            page[j] = page[0];
-            place[j] = place[0] + 4 * g + j;
+            page[j] = group_page;
+            place[j] = group_place + 4 * g + j;
           } else {
             page[j] = lookup(s, i, 4 * g + j, &place[j]);
           }

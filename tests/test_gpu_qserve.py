@@ -352,7 +352,7 @@ SHAPES = [(6, 2, 48), (32, 8, 64), (8, 2, 128), (4, 4, 128), (5, 1, 8), (20, 1, 
 
 @pytest.mark.parametrize("typ", ["f32", "f16", "bf16", "i8"])
 @pytest.mark.parametrize("H,KVH,hd", SHAPES)
-@pytest.mark.parametrize("page,order", [(16, "head"), (5, "slot")])
+@pytest.mark.parametrize("page,order", [(16, "head"), (5, "slot"), (48, "slot"), (1, "head")])
 def test_attention_matches_the_definition(Q, typ, H, KVH, hd, page, order):
     """Lengths of none, one, at and around the steps of 16 and 32 keys and the pages, in one ragged batch."""
     lens = [0, 1, 2, 15, 16, 17, 31, 32, 33, 47, 64, 65, 100, 257, -4]

@@ -111,6 +111,7 @@ BAD_CACHE = [({"k": None}, "null"), ({"v": None}, "null"), ({"type": 4}, "type")
 REFUSED = [("plan", kw, w) for kw, w in [
     ({"n_req": -1}, "n_req"), ({"n_req": 8193}, "n_req"), ({"width": 0}, "width"), ({"page_size": 0}, "page size"),
     ({"width": 1 << 20, "page_size": 1 << 11, "table_stride": 1 << 20}, "31 bits"), ({"ring_size": 0}, "ring"), ({"max_rows": -1}, "max_rows"),
+    ({"ring_size": (1 << 30) + 1}, "ring"), ({"max_rows": (1 << 30) + 1}, "max_rows"),
     ({"table_stride": 3}, "stride"), ({"state": 0}, "null"), ({"ring": 0}, "null"), ({"cached": 0}, "null"), ({"added": 0}, "null"),
     ({"table": 0}, "null"), ({"lens": 0}, "null"), ({"starts": 0}, "null"), ({"state_out": 0}, "null"), ({"slots": 0}, "null"),
     ({"positions": 0}, "null"), ({"requests": 0}, "null"), ({"state_out": A + 4096 * 2}, "output"), ({"lens": A}, "output"),
