@@ -460,6 +460,53 @@ def test_attention_large_scores_and_nan(Q):
         assert torch.equal(o2[0, [0, 2, 3]], o[0, [0, 2, 3]]) and torch.equal(o2[1], o[1])
 
 
+@pytest.mark.parametrize("typ", ["f32", "i8"])
+def test_attention_many_requests_most_of_them_empty(Q, typ):
+    """700 requests, runs of empty ones among them longer than what a wave looks at at once, the last ones empty too."""
+    g = torch.Generator(device="cuda").manual_seed(11)
+    r = random.Random(5)
+    lens = [r.choice([1, 17, 90]) if r.random() < 0.1 and not 200 < i < 420 and i < 690 else 0 for i in range(700)]
+    need = sum(-(-x // 16) for x in lens)
+    kv = make_cache(Q, typ, need, 2, 16, 64, "head", g)
+    q = torch.randn((700, 2, 64), generator=g, device="cuda")
+    check(Q, kv, q, pages_for(lens, 16, 6, need, 1), cuda_i32(lens))
+    o, lse = attend(Q, kv, q, pages_for([0] * 700, 16, 6, need, 1), cuda_i32([0] * 700))
+    assert bool((o == 0).all()) and bool(torch.isinf(lse).all())
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16", "i8"])
+def test_attention_shared_pages_and_equal_requests(Q, typ):
+    """Requests that share a prefix's pages, and the same request twice: equal bits where equal work is asked of equal places
+    in a share, and the definition's values anyway."""
+    g = torch.Generator(device="cuda").manual_seed(14)
+    kv = make_cache(Q, typ, 12, 2, 32, 128, "head", g)
+    table = cuda_i32([[0, 1, 2, 3], [0, 1, 4, 5], [0, 1, 2, 3], [7, 7, 7, 7]])
+    q = torch.randn((4, 4, 128), generator=g, device="cuda")
+    q[2] = q[0]
+    check(Q, kv, q, table, cuda_i32([128, 100, 128, 97]))
+
+
+def test_attention_16_heads_a_group_of_256_in_a_graph(Q):
+    """The largest queries in LDS (set as the launch's own size) under capture."""
+    g = torch.Generator(device="cuda").manual_seed(15)
+    kv = make_cache(Q, "bf16", 30, 1, 16, 256, "head", g)
+    lens = [300, 77]
+    table = pages_for(lens, 16, 19, 30, 1)
+    q, n = torch.randn((2, 16, 256), generator=g, device="cuda"), cuda_i32(lens)
+    want = attend(Q, kv, q, table, n)
+    o, lse = torch.zeros_like(q), torch.zeros((2, 16), device="cuda")
+    work = torch.empty(Q.paged_attention_work(kv, 2, 16), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        Q.paged_attention(kv, q, table, n, o, work, lse=lse, stream=stream())
+    for _ in range(3):
+        o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o, want[0]) and torch.equal(lse, want[1])
+
+
 def test_attention_scale_strides_and_sentinels(Q):
     """A given scale; queries inside packed rows, outputs with room behind every row, a table inside a larger one."""
     g = torch.Generator(device="cuda").manual_seed(2)
@@ -578,6 +625,28 @@ def test_sample_rows_match_the_definition(Q, kind, V):
         want = sample_ref(x[i].numpy(), f(t[i]), k[i], f(p[i]), f(m[i]), u[i])
         assert (token[i], kept[i]) == want[:2], (i, SETTINGS[i % len(SETTINGS)], u[i])
         assert abs(prob[i] - want[2]) <= 2.0 ** -20 * want[2]
+
+
+@pytest.mark.parametrize("kind", ["normal", "equal", "ties"])
+def test_sample_rows_of_the_largest_vocabulary(Q, kind):
+    """2^20 tokens: more slices than a mask has bits, and cells of a million equal tokens."""
+    x = rows_of(kind, 3, 1 << 20, 2)
+    t, k, p, m = [1.0, 0.7, 1.5], [0, 50, 0], [0.9, 1.0, 1.0], [0.0, 0.0, 0.01]
+    u = [float(np.float32(y)) for y in (0.77, 0.2, 0.999)]
+    token, kept, _ = sample_run(Q, x.cuda(), u, t, k, p, m)
+    f = lambda y: float(np.float32(y))  # noqa: E731
+    for i in range(3):
+        assert (token[i], kept[i]) == sample_ref(x[i].numpy(), f(t[i]), k[i], f(p[i]), f(m[i]), u[i])[:2], i
+
+
+@pytest.mark.parametrize("n", [1, 31, 33, 300])
+def test_sample_rows_batches_around_the_slice_rule(Q, n):
+    """Numbers of rows that take slices of either length give the same tokens for the same row."""
+    x = rows_of("peaked", 1, 70001, 3)
+    u = float(np.float32(0.61))
+    want = sample_ref(x[0].numpy(), float(np.float32(0.9)), 0, float(np.float32(0.97)), 0.0, u)
+    token, kept, _ = sample_run(Q, x.expand(n, -1).contiguous().cuda(), [u] * n, [0.9] * n, None, [0.97] * n)
+    assert token == [want[0]] * n and kept == [want[1]] * n
 
 
 def test_sample_rows_settings_out_of_range(Q):
