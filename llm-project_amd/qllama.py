@@ -628,7 +628,8 @@ def profile_read():
 # ---- qserve.h: one step of many requests over a paged cache ------------------------
 # Buffers are tensors on the GPU (torch's, or anything with is_cuda, dtype, shape,
 # stride() and data_ptr()); stream is a hipStream_t as a number, e.g.
-# torch.cuda.current_stream().cuda_stream, and None the library's own.
+# torch.cuda.current_stream().cuda_stream, and None the library's own.  torch brings a HIP
+# runtime of its own: import it before the library is loaded, so that both share it.
 KV_F32, KV_F16, KV_BF16, KV_I8 = 0, 1, 2, 3
 _KV_TYPE = {"float32": KV_F32, "float16": KV_F16, "bfloat16": KV_BF16, "int8": KV_I8}
 _dtypes = {}
@@ -641,19 +642,21 @@ def _dtype(t):
     return name
 
 
-def _flat(t, name, dtype, size):
-    """Address of a contiguous GPU tensor of `dtype` with at least `size` elements, or 0 for None."""
-    if t is None:
-        return 0
-    if t.is_cuda and _dtypes.get(t.dtype) == dtype and t.numel() >= size and t.is_contiguous():
-        return t.data_ptr()
-    return _ptr(t, name, dtype, size, 8)
+def _flat(dtype, *tensors):
+    """Addresses of contiguous GPU tensors of `dtype`, given as (tensor, name, elements that are needed); 0 for None."""
+    at, known = [], _dtypes.get
+    for t, name, size in tensors:
+        if t is None:
+            at.append(0)
+        elif t.is_cuda and known(t.dtype) == dtype and t.numel() >= size and t.is_contiguous():
+            at.append(t.data_ptr())
+        else:
+            at.append(_ptr(t, name, dtype, size, 8))
+    return at
 
 
 def _ptr(t, name, dtype, size, inner):
-    """The same where the last `inner` dimensions have to be contiguous."""
-    if t.is_cuda and _dtypes.get(t.dtype) == dtype and size == 0 and inner == 1 and t.stride(-1) == 1:
-        return t.data_ptr()
+    """Address of a GPU tensor whose last `inner` dimensions have to be contiguous."""
     if not t.is_cuda:
         raise ValueError(f"{name} is not on the GPU")
     if _dtype(t) != dtype:
@@ -668,8 +671,15 @@ def _ptr(t, name, dtype, size, inner):
     return t.data_ptr()
 
 
-def _row_stride(t, row):
-    return t.stride(0) if t.shape[0] > 1 else row
+def _rows(t, name, dtype, shape):
+    """Address and row stride of a GPU tensor of `dtype` and `shape` whose rows are contiguous."""
+    if t.shape != shape:
+        raise ValueError(f"{name} must have the shape {tuple(shape)}, not {tuple(t.shape)}")
+    st = t.stride()
+    row = shape[1] if len(shape) == 2 else shape[1] * shape[2]
+    if not (t.is_cuda and _dtypes.get(t.dtype) == dtype and st[-1] == 1 and (len(shape) == 2 or st[1] == shape[2])):
+        _ptr(t, name, dtype, 0, len(shape) - 1)
+    return t.data_ptr(), st[0] if shape[0] > 1 else row
 
 
 def _stream(stream):
@@ -710,6 +720,7 @@ class PagedKV:
             st = [s if n > 1 else 1 for s, n in zip(k_scale.stride(), k_scale.shape)]
             self.c.scale_page_stride, self.c.scale_head_stride, self.c.scale_slot_stride = st
             self.c.k_scale, self.c.v_scale = _ptr(k_scale, "k_scale", "float32", 0, 0), _ptr(v_scale, "v_scale", "float32", 0, 0)
+        self.n_kv, self.head_dim = n_kv, hd
         self.ref = C.byref(self.c)
 
 
@@ -718,51 +729,40 @@ def paged_plan(cached, added, table, ring, state, page_size, lens, status, start
     """qllama_paged_plan: pages for the requests' new tokens, and slot, position and request of every new row.  int32
     tensors; table (requests, width) and ring change in place, the arguments after page_size are outputs."""
     n, rows = cached.numel(), slots.numel()
-    i32 = "int32"
-    if len(table.shape) != 2 or table.shape[0] < n:
+    tn, width = table.shape
+    if tn < n:
         raise ValueError("table must have a row for every request")
-    width = table.shape[1]
-    a = PAGED_PLAN.pack(n, width, page_size, ring.numel(), rows, _row_stride(table, width),
-                        _flat(cached, "cached", i32, n), _flat(added, "added", i32, n), _flat(state, "state", i32, 2),
-                        _ptr(table, "table", i32, 0, 1), _flat(ring, "ring", i32, 1), _flat(lens, "lens", i32, n),
-                        _flat(status, "status", i32, n), _flat(starts, "starts", i32, n + 1), _flat(state_out, "state_out", i32, 2),
-                        _flat(slots, "slots", i32, rows), _flat(positions, "positions", i32, rows),
-                        _flat(requests, "requests", i32, rows))
-    _done(lib().qllama_paged_plan(a, _stream(stream)), "qllama_paged_plan")
-
-
-def _heads(t, name, rows, heads, hd):
-    """Address and row stride of a float32 GPU tensor (rows, heads, hd) whose rows are contiguous."""
-    shape, (s0, s1, s2) = t.shape, t.stride()
-    if tuple(shape) != (rows, heads, hd):
-        raise ValueError(f"{name} must have the shape {(rows, heads, hd)}, not {tuple(shape)}")
-    if not t.is_cuda or _dtypes.get(t.dtype) != "float32" or (hd != 1 and s2 != 1) or (heads != 1 and s1 != hd):
-        _ptr(t, name, "float32", 0, 2)
-    return t.data_ptr(), s0 if rows > 1 else heads * hd
+    tp, ts = _rows(table, "table", "int32", table.shape)
+    at = _flat("int32", (cached, "cached", n), (added, "added", n), (state, "state", 2), (ring, "ring", 1), (lens, "lens", n),
+               (status, "status", n), (starts, "starts", n + 1), (state_out, "state_out", 2), (slots, "slots", rows),
+               (positions, "positions", rows), (requests, "requests", rows))
+    a = PAGED_PLAN.pack(n, width, page_size, ring.numel(), rows, ts, at[0], at[1], at[2], tp, *at[3:])
+    _done((_lib or lib()).qllama_paged_plan(a, _stream(stream)), "qllama_paged_plan")
 
 
 def paged_append(cache, k, v, slots, q=None, q_out=None, positions=None, cos=None, sin=None, bad=None, stream=None):
     """qllama_paged_append: k, v (rows, KV heads, head_dim) float32 into their slots; with cos and sin (positions,
     head_dim / 2), keys and the queries q (rows, heads, head_dim) turned by their positions' angles, q into q_out."""
-    n_kv, hd = cache.c.n_kv, cache.c.head_dim
-    rows = slots.numel()
+    hd, rows = cache.head_dim, slots.numel()
+    shape = (rows, cache.n_kv, hd)
     heads = qp = qs = op = os_ = n_pos = 0
-    kp, ks = _heads(k, "k", rows, n_kv, hd)
-    vp, vs = _heads(v, "v", rows, n_kv, hd)
+    kp, ks = _rows(k, "k", "float32", shape)
+    vp, vs = _rows(v, "v", "float32", shape)
     if q is not None:
         if q_out is None:
             raise ValueError("q needs q_out of its shape")
         heads = q.shape[1]
-        qp, qs = _heads(q, "q", rows, heads, hd)
-        op, os_ = _heads(q_out, "q_out", rows, heads, hd)
+        shape = (rows, heads, hd)
+        qp, qs = _rows(q, "q", "float32", shape)
+        op, os_ = _rows(q_out, "q_out", "float32", shape)
     if cos is not None:
         n_pos = cos.shape[0]
         if sin is None or positions is None:
             raise ValueError("a rotation needs cos, sin and positions")
-    a = PAGED_ROWS.pack(rows, heads, qp, kp, vp, op, qs, ks, vs, os_, _flat(slots, "slots", "int32", rows),
-                        _flat(positions, "positions", "int32", rows), _flat(cos, "cos", "float32", n_pos * hd // 2),
-                        _flat(sin, "sin", "float32", n_pos * hd // 2), n_pos, _flat(bad, "bad", "int32", 1))
-    _done(lib().qllama_paged_append(cache.ref, a, _stream(stream)), "qllama_paged_append")
+    sp, pp, bp = _flat("int32", (slots, "slots", rows), (positions, "positions", rows), (bad, "bad", 1))
+    cp, np_ = _flat("float32", (cos, "cos", n_pos * hd // 2), (sin, "sin", n_pos * hd // 2))
+    a = PAGED_ROWS.pack(rows, heads, qp, kp, vp, op, qs, ks, vs, os_, sp, pp, cp, np_, n_pos, bp)
+    _done((_lib or lib()).qllama_paged_append(cache.ref, a, _stream(stream)), "qllama_paged_append")
 
 
 def paged_attention_work(cache, n_req, n_heads):
@@ -776,20 +776,16 @@ def paged_attention_work(cache, n_req, n_heads):
 def paged_attention(cache, q, table, lens, o, work, lse=None, scale=0.0, stream=None):
     """qllama_paged_attention: o (requests, heads, head_dim) and lse (requests, heads) of q over the first lens tokens of
     every request's pages table (requests, width)."""
-    n, heads, hd = q.shape
-    if len(table.shape) != 2 or table.shape[0] < n or hd != cache.c.head_dim:
+    n, heads, hd = shape = q.shape
+    tn, width = table.shape
+    if tn < n or hd != cache.head_dim:
         raise ValueError("q, table and the cache do not fit together")
-    width = table.shape[1]
-    qp, qs = _heads(q, "q", n, heads, hd)
-    op, os_ = _heads(o, "o", n, heads, hd)
-    lp = ls = 0
-    if lse is not None:
-        if tuple(lse.shape) != (n, heads):
-            raise ValueError("lse must have the shape (requests, heads)")
-        lp, ls = _ptr(lse, "lse", "float32", 0, 1), _row_stride(lse, heads)
-    a = PAGED_QUERY.pack(n, heads, width, qs, os_, ls, _row_stride(table, width), qp, op, lp, _ptr(table, "table", "int32", 0, 1),
-                         _flat(lens, "lens", "int32", n), scale, *_work(work))
-    _done(lib().qllama_paged_attention(cache.ref, a, _stream(stream)), "qllama_paged_attention")
+    qp, qs = _rows(q, "q", "float32", shape)
+    op, os_ = _rows(o, "o", "float32", shape)
+    tp, ts = _rows(table, "table", "int32", table.shape)
+    lp, ls = (0, 0) if lse is None else _rows(lse, "lse", "float32", shape[:2])
+    a = PAGED_QUERY.pack(n, heads, width, qs, os_, ls, ts, qp, op, lp, tp, _flat("int32", (lens, "lens", n))[0], scale, *_work(work))
+    _done((_lib or lib()).qllama_paged_attention(cache.ref, a, _stream(stream)), "qllama_paged_attention")
 
 
 def sample_rows_work(rows, vocab):
@@ -803,12 +799,10 @@ def sample_rows_work(rows, vocab):
 def sample_rows(logits, u, token, work, temperature=None, top_k=None, top_p=None, min_p=None, prob=None, kept=None, stream=None):
     """qllama_sample_rows: a token for every row of logits (rows, vocab) from the numbers u in [0, 1); settings a row
     each (None: temperature 1, no limit); prob its probability among the kept tokens, kept their number."""
-    if len(logits.shape) != 2:
-        raise ValueError("logits must have the shape (rows, vocab)")
     n, V = logits.shape
-    a = SAMPLE_ROWS.pack(n, V, _row_stride(logits, V), _ptr(logits, "logits", "float32", 0, 1), _flat(u, "u", "float32", n),
-                         _flat(temperature, "temperature", "float32", n), _flat(top_k, "top_k", "int32", n),
-                         _flat(top_p, "top_p", "float32", n), _flat(min_p, "min_p", "float32", n),
-                         _flat(token, "token", "int32", n), _flat(kept, "kept", "int32", n), _flat(prob, "prob", "float32", n),
-                         *_work(work))
-    _done(lib().qllama_sample_rows(a, _stream(stream)), "qllama_sample_rows")
+    lp, ls = _rows(logits, "logits", "float32", logits.shape)
+    up, tp, pp, mp, op = _flat("float32", (u, "u", n), (temperature, "temperature", n), (top_p, "top_p", n), (min_p, "min_p", n),
+                               (prob, "prob", n))
+    kp, ip, np_ = _flat("int32", (top_k, "top_k", n), (token, "token", n), (kept, "kept", n))
+    a = SAMPLE_ROWS.pack(n, V, ls, lp, up, tp, kp, pp, mp, ip, np_, op, *_work(work))
+    _done((_lib or lib()).qllama_sample_rows(a, _stream(stream)), "qllama_sample_rows")
