@@ -2,13 +2,17 @@
 // (qllama_paged_attention; semantics in qserve.h).  No counterpart in the reference,
 // whose decode attention (llama.c:554-576) serves one sequence and one dense cache.
 //
+// Memory bound: every key and value row is read once, 2 n_kv hd element bytes a token,
+// and each byte takes part in n_heads / n_kv multiply-adds (4 at the shapes below).
+//
 // The work of a call is the key steps of all (request, KV head, 16 query heads) tiles,
 // laid one behind another; every wave takes an equal share of them, whatever the
 // lengths are, so ragged batches and one long request fill the chip alike without the
 // host knowing a length.  A share that ends inside a tile leaves its maximum, sum and
 // weighted values in the workspace, and k_paged_join puts a tile's parts together.
 // Waves never meet: with four of them on a tile, meeting in LDS at its end, 512 requests
-// of 300 bf16 tokens took XX us against XX.
+// of up to 300 f16 tokens (8 KV heads of 128, pages of 16) took 167 us, with shares of
+// their own 134 (100 with all that follows here).
 //
 // A wave keeps its running maximum, sum and outputs in registers, its queries in LDS, and
 // takes a step of 16 or 32 keys at a time straight from the pages into registers.
@@ -18,10 +22,26 @@
 // between lanes.  A lane loads whole pieces of a value row (16 lanes a row), and the
 // pieces of 8 keys are turned by byte permutes.
 //
+// What is under way carries the bandwidth: two waves a SIMD, a step's values and the next
+// step's keys in registers.  Loading the values a step ahead too took 82 us against 76
+// at the first row below, three waves a SIMD (with fewer registers) 110 against 84 at the
+// time, twice the blocks 92.
+//
 // Precision: float queries and weights meet 16-bit keys and values as parts that add up
 // to them (bf16: three parts of 8 bits, f16: two of 11), one MFMA a part; int8 codes
 // are exact in bf16.  fp32 caches use the fp32 MFMA.  At 8 TB/s the parts take a sixth
 // of the bf16 matrix rate.
+//
+// Measured (both kernels, 32 query and 8 KV heads; a 1 GiB copy moves 5.1 TB/s):
+//   64 ragged requests of up to 2560 tokens, bf16, hd 128     73.7 us   4.8 TB/s
+//   2 requests, up to 120000 tokens, f16, hd 128             134   us   5.5 TB/s
+//   128 requests of up to 4100 tokens, int8, hd 128          132   us   4.3 TB/s
+//   24 requests of up to 768 tokens, f32, hd 64               17.1 us   2.1 TB/s
+//   1 request of 2060 tokens, bf16, hd 128                    12.5 us   0.7 TB/s
+// The short ones are two launches and a chain of dependent trips to memory (lengths,
+// table, keys, values, parts).  int8 rows take three times a 16-bit row's vector
+// instructions a byte: 34 thousand a SIMD at the third row, which with the MFMAs keep it
+// some 0.6 of the time.
 #include <hip/hip_runtime.h>
 
 #include "qserve_host.h"
@@ -38,7 +58,7 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 constexpr int kThreads = 256, kWaves = 4;
 constexpr int kBlocks = 512;          // two blocks of four waves a CU
 constexpr int kShares = kBlocks * kWaves;
-constexpr int kMinShare = 1;          // steps a wave takes at least
+constexpr int kMinShare = 1;          // steps a wave takes at least; one request of 200 tokens took 7.6 us, with 2 or 4 9.1
 constexpr float kNegInf = -__builtin_inff();
 
 struct PaArgs {
@@ -108,7 +128,9 @@ __device__ inline float sum_groups(float x) {
   return x + __shfl_xor(x, 32);
 }
 
-// W words of a row; STREAM: read once, so past the caches' retention
+// W words of a row; STREAM: read once (one tile of query heads a KV head), so past the
+// caches' retention: 84 -> 77 us at 64 ragged bf16 requests, together with whole 64-byte
+// runs a load; more tiles of a KV head find the rows in L2
 template <bool STREAM, int W>
 __device__ inline void load_words(uint32_t (&d)[W], const char *p) {
   typedef uint32_t vec __attribute__((ext_vector_type(W), aligned(W > 2 ? 8 : 4)));
@@ -622,7 +644,10 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
 }
 
 // One block a share and row: where a tile begins in the share and goes on behind it, its
-// parts put together in the order of their keys, 8 (hd <= 128) or 4 side by side.
+// parts put together in the order of their keys, 8 (hd <= 128) or 4 side by side.  A
+// trip to the descriptor and one to the parts, with a launch in front: 3.8 us for two
+// tiles of 13 parts, 7.1 at 64 ragged requests (512 tiles of some 4 parts), 12.3 where
+// 2048 shares make 16 tiles.
 constexpr int kJoinThreads = 256, kAhead = 4;
 __global__ __launch_bounds__(kJoinThreads) void k_paged_join(PaArgs a, float shift) {
   __shared__ float weight[kShares], lds[kJoinThreads / 32][256], red[2][kJoinThreads / 64];

@@ -121,7 +121,9 @@ __device__ inline Ask ask_of(const QSampleRows &a, int r) {
   return {kGrid * kLog2e / (double)T, !(T > 0.0f)};
 }
 
-// A slice of 1024 Q tokens in registers: the only reading of most of a row.
+// A slice of 1024 Q tokens in registers: the only reading of most of a row.  Memory bound
+// for many rows: 192 rows of 128256 tokens 25.4 us, 98 MB read and 19 MB of histograms
+// written (4.6 TB/s); 4 rows 4.5 us.
 template <int Q>
 __global__ __launch_bounds__(kSliceThreads) void k_sample_slices(QSampleRows a, Slice *slices, u64 *hist) {
   __shared__ u64 h[kBins], bests[kSliceThreads / 64];
@@ -461,7 +463,9 @@ __device__ Found locate(const Row &row, Shared &s, int &turn, Goal goal, const H
 }
 
 // A row's token from its slices' histograms.  A chain of short steps, each a barrier or a
-// trip to memory behind the one before.
+// trip to memory behind the one before: 16 us for 4 rows with top-k 40 and top-p 0.95.
+// Of 192 rows with settings of their own (36 us) those without a limit end in cells that
+// every slice has tokens of, and read a good part of the row again.
 __global__ __launch_bounds__(kPickThreads) void k_sample_pick(QSampleRows a, int slices, int bits, int group, const Slice *recs, const u64 *hist) {
   extern __shared__ int offs[];                            // the row's bin that is a slice's first; kBins: none is
   __shared__ Shared s;
@@ -553,7 +557,9 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(QSampleRows a, int
   }
 }
 
-// Slices of 8192 tokens; of 4096 where the former would leave CUs idle.
+// Slices of 8192 tokens; of 4096 where the former would leave CUs idle.  192 rows of
+// 128256 tokens took 74.6 us with 8192, 77.8 with 4096 (twice the histograms), 79.3 with
+// 16384 (fewer loads under way).
 int quads_of(int rows, int vocab) { return (long long)rows * ((vocab + 8191) / 8192) >= 256 ? 8 : 4; }
 
 template <int Q>
