@@ -163,7 +163,7 @@ int qllama_test_page_of(const int32_t *table, int width, int page_size, int n_pa
 // counts as the nearest inside, NaN as 0; a NaN setting is no limit.  Logits of -inf
 // and NaN are masked: never kept; a row with nothing else gives token -1, kept 0 and
 // prob 0.  Logits of +inf share the row between them.
-// Sums and comparisons in 64 bits (each e to 2^-44 of the largest), so a token differs
+// Sums and comparisons in 64 bits (each e to 2^-39 of the largest), so a token differs
 // from sample_token's only where that one's float rounding decides.
 // prob: the token's probability among the kept ones; kept: n.  Both may be NULL.  The
 // settings' arrays may be NULL: temperature 1, no limit.  work: qllama_sample_rows_work

@@ -732,9 +732,48 @@ def test_sample_rows_of_the_largest_vocabulary(Q, kind):
         assert (token[i], kept[i]) == sample_ref(x[i].numpy(), f(t[i]), k[i], f(p[i]), f(m[i]), u[i])[:2], i
 
 
+@pytest.mark.parametrize("kind", ["normal", "ties", "equal"])
+@pytest.mark.parametrize("V", [300, 8193, 40000])
+def test_sample_rows_around_64_kept_tokens(Q, kind, V):
+    """As many tokens kept as a wave orders at once, and a few more or fewer, by each of the limits; one cell or many."""
+    x1 = rows_of(kind, 1, V, 5)
+    if kind == "normal":
+        x1[0, ::V // 70] = torch.linspace(9.0, 12.0, len(x1[0, ::V // 70]))
+    k = list(range(55, 74)) + [0] * 30
+    p = [1.0] * 19 + [0.80 + 0.01 * i for i in range(15)] + [1.0] * 15
+    m = [0.0] * 34 + [0.001 * 1.6 ** i for i in range(15)]
+    r = random.Random(V)
+    u = [float(np.float32(r.random())) for _ in k]
+    n = len(k)
+    token, kept, prob = sample_run(Q, x1.expand(n, V).contiguous(), u, [1.1] * n, k, p, m)
+    f = lambda y: float(np.float32(y))  # noqa: E731
+    for i in range(n):
+        want = sample_ref(x1[0].numpy(), f(1.1), k[i], f(p[i]), f(m[i]), u[i])
+        assert (token[i], kept[i]) == want[:2], (i, k[i], p[i], m[i], u[i])
+        assert abs(prob[i] - want[2]) <= 2.0 ** -20 * want[2]
+
+
+def test_sample_rows_of_enormous_logits(Q):
+    """Logits and temperatures whose cells are no numbers of their own: the ends of a cell are searched among all floats."""
+    x = torch.full((6, 9000), -1e38)
+    x[0, 70:80], x[0, 4000:4100] = 3e38, 2.9e38
+    x[1, 5:500] = 1e25
+    x[2] = torch.linspace(-3e38, 3e38, 9000)
+    x[3, ::3] = 1e-3
+    x[4, 10], x[4, 8999] = float("inf"), 3e38
+    x[5, 100:200] = -1e30
+    t = [1.0, 0.5, 1e38, 1e-38, 1.0, float("inf")]
+    k, p, m = [0, 30, 100, 0, 0, 0], [0.55, 1.0, 0.9, 0.3, 0.9, 0.5], [0.0, 0.0, 0.0, 0.5, 0.0, 0.0]
+    u = [0.77, 0.41, 0.62, 0.37, 0.5, 0.83]
+    f = lambda y: float(np.float32(y))  # noqa: E731
+    token, kept, _ = sample_run(Q, x, u, t, k, p, m)
+    for i in range(6):
+        assert (token[i], kept[i]) == sample_ref(x[i].numpy(), f(t[i]), k[i], f(p[i]), f(m[i]), f(u[i]))[:2], i
+
+
 @pytest.mark.parametrize("n", [1, 31, 33, 300])
-def test_sample_rows_batches_around_the_slice_rule(Q, n):
-    """Numbers of rows that take slices of either length give the same tokens for the same row."""
+def test_sample_rows_batches_of_one_row(Q, n):
+    """Every row of a batch of equal rows gets the same token."""
     x = rows_of("peaked", 1, 70001, 3)
     u = float(np.float32(0.61))
     want = sample_ref(x[0].numpy(), float(np.float32(0.9)), 0, float(np.float32(0.97)), 0.0, u)
