@@ -107,7 +107,7 @@ int qllama_paged_plan(const QPagedPlan *p, void *stream);
 // is increased by their number.  Slots of one call must differ.  A NaN becomes code 0
 // in an int8 row, and does not count for its scale.
 typedef struct {
-  int rows, n_heads;                          // n_heads: query heads (with q)
+  int rows, n_heads;                          // rows up to 2^23; n_heads: query heads (with q)
   const float *q, *k, *v;
   float *q_out;
   int64_t q_stride, k_stride, v_stride, q_out_stride;

@@ -313,7 +313,7 @@ static int append_launch(const char *fn, const AppArgs &a, bool vec, hipStream_t
 extern "C" int qllama_paged_append(const QPagedKV *c, const QPagedRows *r, void *stream) {
   static const char fn[] = "qllama_paged_append";
   if (const char *why = qs::bad_cache(c)) return qs::refuse(fn, why);
-  if (!r || r->rows < 0) return qs::refuse(fn, "null argument or rows < 0");
+  if (!r || r->rows < 0 || r->rows > (1 << 23)) return qs::refuse(fn, "null argument, or rows not 0 .. 2^23");
   if (r->rows == 0) return 0;
   if (!r->k || !r->v || !r->slots) return qs::refuse(fn, "null k, v or slots");
   const int H = r->q ? r->n_heads : 0;

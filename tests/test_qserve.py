@@ -117,7 +117,8 @@ REFUSED = [("plan", kw, w) for kw, w in [
     ({"positions": 0}, "null"), ({"requests": 0}, "null"), ({"state_out": A + 4096 * 2}, "output"), ({"lens": A}, "output"),
     ({"status": A + 4096}, "output")]]
 REFUSED += [("rows", kw, w) for kw, w in [
-    ({"rows": -1}, "rows"), ({"k": 0}, "null"), ({"v": 0}, "null"), ({"slots": 0}, "null"), ({"q_out": 0}, "q_out"), ({"n_heads": 0}, "q_out"),
+    ({"rows": -1}, "rows"), ({"rows": (1 << 23) + 1}, "rows"), ({"k": 0}, "null"), ({"v": 0}, "null"), ({"slots": 0}, "null"),
+    ({"q_out": 0}, "q_out"), ({"n_heads": 0}, "q_out"),
     ({"sin_t": 0}, "rotation"), ({"positions": 0}, "rotation"), ({"n_pos": 0}, "rotation"), ({"k_stride": 127}, "stride"),
     ({"v_stride": 0}, "stride"), ({"q_stride": 255}, "stride"), ({"q_out_stride": 255}, "stride"), ({"k": A + 2}, "aligned")]]
 REFUSED += [("query", kw, w) for kw, w in [
