@@ -78,7 +78,9 @@ typedef struct {
 //     and request; rows behind the last get slot -1, position 0, request -1.
 //   * state_out is the ring's new state.  state outside the ring counts as position 0
 //     and as many pages as the ring has places, respectively.
-// table and ring change in place; no other output may be one of the inputs.
+// table and ring change in place; no other output may be one of the inputs.  A page that
+// two requests hold (a shared beginning) is returned by each of them: such pages are the
+// caller's to count, and to leave out of the rows of ended requests.
 typedef struct {
   int n_req;              // 0 .. 8192
   int width;              // table entries of a request
@@ -130,7 +132,8 @@ int qllama_paged_append(const QPagedKV *c, const QPagedRows *r, void *stream);
 // request's tokens, NaN included, has no effect.  Products and sums in 32 bits: a
 // 16-bit or int8 row enters a product as it is, a query or a weight as two or three
 // 16-bit parts that together hold 22 (f16 cache) or 24 bits.  A cached infinity gives
-// NaN.  work: qllama_paged_attention_work bytes, 16-byte aligned.
+// NaN.  width * page_size has to be below 2^31 - 64.  work: qllama_paged_attention_work
+// bytes, 16-byte aligned.
 typedef struct {
   int n_req, n_heads, width;
   int64_t q_stride, o_stride, lse_stride;     // floats between requests; heads lie one behind another

@@ -776,8 +776,8 @@ extern "C" int qllama_paged_attention(const QPagedKV *c, const QPagedQuery *a, v
   if (!a->q || !a->o || !a->table || !a->lens) return qs::refuse(fn, "null q, o, table or lens");
   const int64_t qd = (int64_t)a->n_heads * c->head_dim;
   if (a->q_stride < qd || a->o_stride < qd || (a->lse && a->lse_stride < a->n_heads)) return qs::refuse(fn, "a row stride below the row's length");
-  if (a->width < 1 || a->table_stride < a->width || (int64_t)a->width * c->page_size > INT_MAX)
-    return qs::refuse(fn, "bad table width (width * page_size must fit in 31 bits) or stride");
+  if (a->width < 1 || a->table_stride < a->width || (int64_t)a->width * c->page_size > INT_MAX - 64)   // a step past it still fits
+    return qs::refuse(fn, "bad table width (width * page_size must be below 2^31 - 64) or stride");
   if ((int64_t)a->n_req * (((int64_t)a->width * c->page_size + 15) / 16) > INT_MAX)
     return qs::refuse(fn, "n_req * width * page_size is too large");
   if (!(a->scale >= 0.0f) || a->scale > 3.0e38f) return qs::refuse(fn, "scale must be finite and not negative");

@@ -124,7 +124,8 @@ REFUSED += [("rows", kw, w) for kw, w in [
 REFUSED += [("query", kw, w) for kw, w in [
     ({"n_req": -1}, "n_req"), ({"n_heads": 3}, "multiple"), ({"n_heads": 0}, "multiple"), ({"q": 0}, "null"), ({"o": 0}, "null"), ({"table": 0}, "null"),
     ({"lens": 0}, "null"), ({"q_stride": 255}, "stride"), ({"o_stride": 0}, "stride"), ({"lse": A, "lse_stride": 3}, "stride"), ({"width": 0}, "width"),
-    ({"table_stride": 4}, "width"), ({"width": 1 << 28, "table_stride": 1 << 28}, "31 bits"), ({"scale": -1.0}, "scale"), ({"scale": float("nan")}, "scale"),
+    ({"table_stride": 4}, "width"), ({"width": 1 << 28, "table_stride": 1 << 28}, "2^31 - 64"),
+    ({"width": (1 << 27) - 4, "table_stride": 1 << 27, "n_req": 1}, "2^31 - 64"), ({"scale": -1.0}, "scale"), ({"scale": float("nan")}, "scale"),
     ({"scale": float("inf")}, "scale"), ({"o": A}, "o must not"), ({"work": 0}, "work"), ({"work": A + 8}, "work"), ({"work_bytes": 100}, "work"),
     ({"q": A + 1}, "aligned")]]
 REFUSED += [("sample", kw, w) for kw, w in [
