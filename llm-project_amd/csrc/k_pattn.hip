@@ -145,8 +145,15 @@ __device__ inline void load_words(uint32_t (&d)[W], const char *p) {
 
 __device__ inline uint32_t hi16s(uint32_t b, uint32_t a) { return __builtin_amdgcn_perm(b, a, 0x07060302); }
 __device__ inline uint32_t lo16s(uint32_t b, uint32_t a) { return __builtin_amdgcn_perm(b, a, 0x05040100); }
-template <int B>
-__device__ inline float byte_f(uint32_t w) { return (float)(int)(int8_t)(w >> (8 * B)); }
+// 2^-9 times two int8 codes as f16: the codes plus 128, the bytes of y : x that SELECT
+// names, are subnormal numbers of 2^-24, and one packed multiply-add makes them 2^-9 and takes
+// the 128 off, exactly.  x and y have had the top bits of their bytes turned.
+constexpr int kCodeBits = 9;
+template <uint32_t SELECT>
+__device__ inline uint32_t codes(uint32_t y, uint32_t x) {
+  const h2 u = __builtin_bit_cast(h2, __builtin_amdgcn_perm(y, x, SELECT));
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(u, h2{32768.0f16, 32768.0f16}, h2{-0.25f16, -0.25f16}));
+}
 
 // Parts of a float operand of 8 values: sums of the parts are the values (bf16: 24
 // bits by cutting, f16: 22 by rounding to zero).
@@ -182,7 +189,7 @@ __device__ inline Parts2 cut2(const float (&x)[8]) {
 
 template <int T>
 __device__ inline f4 mfma16(u4 a, u4 b, f4 c) {
-  if constexpr (T == QLLAMA_KV_F16)
+  if constexpr (T != QLLAMA_KV_BF16)
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
   else
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
@@ -200,13 +207,14 @@ struct Cfg {
   static constexpr int PB0 = HDP * ES / 16, PB1 = PB0 < 16 ? PB0 : 16, PB = PB1 < 8 * ES ? PB1 : 8 * ES;
   static constexpr int PD = PB / ES, PIECES = HDP / (16 * PD), PW = PB / 4;
   static constexpr int DPL = HDP / 16;                         // dims of a value row in a lane
-  static constexpr int PARTS = T == QLLAMA_KV_F32 ? 1 : T == QLLAMA_KV_F16 ? 2 : 3;
+  static constexpr int PARTS = T == QLLAMA_KV_F32 ? 1 : T == QLLAMA_KV_BF16 ? 3 : 2;
+  static constexpr bool HALF = PARTS == 2;                     // f16 products
   // a query row in LDS: a part's values, and 64 bytes that spread rows over the banks
   static constexpr int QES = T == QLLAMA_KV_F32 ? 4 : 2;
   static constexpr int QROW = HDP * QES + 64;
   // 2^SHIFT times the weights: f16 parts then keep 22 bits down to 2^-18 of the largest
   // weight and the rest to 2^-40
-  static constexpr float SHIFT = T == QLLAMA_KV_F16 ? 15.0f : 0.0f;
+  static constexpr float SHIFT = HALF ? 15.0f : 0.0f;
 };
 
 template <int T, int HDP>
@@ -395,10 +403,10 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
           qmax = fmaxf(qmax, fabsf(qf[c][i]));
         }
       int e = 0;
-      if constexpr (T == QLLAMA_KV_F16) {           // into f16's range, by a power of two
+      if constexpr (C::HALF) {                      // into f16's range, by a power of two
         qmax = max_groups(qmax);
         e = qmax > 0.0f && qmax < __builtin_inff() ? ilogbf(qmax) - 13 : 0;
-        unscale = ldexpf(1.0f, e);
+        unscale = ldexpf(1.0f, T == QLLAMA_KV_I8 ? e + kCodeBits : e);
       }
       __builtin_amdgcn_wave_barrier();              // the last tile's reads come first
 #pragma unroll
@@ -406,7 +414,7 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
         char *to_lds = q_lds + row * C::QROW + (32 * c + 8 * g) * C::QES;
         if constexpr (T == QLLAMA_KV_F32) {
           if (n < rows) __builtin_memcpy(__builtin_assume_aligned(to_lds, 16), qf[c], sizeof qf[c]);
-        } else if constexpr (T == QLLAMA_KV_F16) {
+        } else if constexpr (C::HALF) {
 #pragma unroll
           for (int i = 0; i < 8; i++) qf[c][i] = ldexpf(qf[c][i], -e);
           const Parts2 x = cut2(qf[c]);
@@ -427,6 +435,8 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
     const char *q_mine = q_lds + row * C::QROW;
 
     float m = kNegInf, l = 0.0f;                    // of the lane's query head; l over the lane's keys
+    int v_exp = -126;                               // int8: the values' scales are below 2^v_exp
+    float v_unit = 0x1p126f;                        // 2^-v_exp
     f4 acc[DPL];
 #pragma unroll
     for (int c = 0; c < DPL; c++) acc[c] = f4{0, 0, 0, 0};
@@ -496,9 +506,9 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
               if constexpr (T == QLLAMA_KV_I8) {
 #pragma unroll
                 for (int w = 0; w < 2; w++) {
-                  const uint32_t b = k.w[i][x][2 * h + w];
-                  kk[2 * w] = hi16s(__float_as_uint(byte_f<1>(b)), __float_as_uint(byte_f<0>(b)));
-                  kk[2 * w + 1] = hi16s(__float_as_uint(byte_f<3>(b)), __float_as_uint(byte_f<2>(b)));
+                  const uint32_t b = k.w[i][x][2 * h + w] ^ 0x80808080u;
+                  kk[2 * w] = codes<0x0c010c00>(b, b);
+                  kk[2 * w + 1] = codes<0x0c030c02>(b, b);
                 }
               } else {
                 kk = u4{k.w[i][x][0], k.w[i][x][1], k.w[i][x][2], k.w[i][x][3]};
@@ -515,7 +525,7 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
 #pragma unroll
         for (int j = 0; j < 4; j++) {
           sc[i][j] = d[i][j];
-          if constexpr (T == QLLAMA_KV_F16) sc[i][j] *= unscale;
+          if constexpr (C::HALF) sc[i][j] *= unscale;
           if constexpr (T == QLLAMA_KV_I8) sc[i][j] *= ksc[i][j];
         }
       if (__any(absent)) {
@@ -547,6 +557,23 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
         for (int c = 0; c < DPL; c++) acc[c] *= f;
         m = top;
       }
+      if constexpr (T == QLLAMA_KV_I8) {            // weights times scales into f16's range, by a power of two
+        float most = 0.0f;
+#pragma unroll
+        for (int i = 0; i < SUB; i++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) most = fmaxf(most, vsc[i][j]);
+        most = max_groups(most);
+        if (__any(most * v_unit >= 1.0f)) {         // rare after the first step
+          const int e = (int)(__float_as_uint(most) >> 23) - 126;
+#pragma unroll
+          for (int c = 0; c < DPL; c++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[c][i] = ldexpf(acc[c][i], v_exp - e);
+          v_exp = e;
+          v_unit = ldexpf(1.0f, -e);
+        }
+      }
       const float ref = (m == kNegInf ? 0.0f : m) - C::SHIFT;
       float p[SUB][4];
 #pragma unroll
@@ -555,7 +582,7 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
         for (int j = 0; j < 4; j++) {
           p[i][j] = __builtin_amdgcn_exp2f(sc[i][j] - ref);
           l += p[i][j];
-          if constexpr (T == QLLAMA_KV_I8) p[i][j] *= vsc[i][j];
+          if constexpr (T == QLLAMA_KV_I8) p[i][j] *= vsc[i][j] * v_unit;
         }
 
       if constexpr (T == QLLAMA_KV_F32) {
@@ -567,12 +594,22 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
       } else {
         const float pf[8] = {p[0][0], p[0][1], p[0][2], p[0][3], p[SUB - 1][0], p[SUB - 1][1], p[SUB - 1][2], p[SUB - 1][3]};
         u4 pp[C::PARTS];
-        if constexpr (T == QLLAMA_KV_F16) {
+        if constexpr (C::HALF) {
           const Parts2 x = cut2(pf);
           pp[0] = x.p[0]; pp[1] = x.p[1];
         } else {
           const Parts3 x = cut3(pf);
           pp[0] = x.p[0]; pp[1] = x.p[1]; pp[2] = x.p[2];
+        }
+        if constexpr (T == QLLAMA_KV_I8) {
+#pragma unroll
+          for (int i = 0; i < SUB; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+              for (int x = 0; x < C::PIECES; x++)
+#pragma unroll
+                for (int w = 0; w < C::PW; w++) v.w[i][j][x][w] ^= 0x80808080u;
         }
 #pragma unroll
         for (int c = 0; c < DPL; c++) {
@@ -584,8 +621,9 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
               const uint32_t *x = v.w[i][2 * j][c / C::PD], *y = v.w[i][2 * j + 1][c / C::PD];
               constexpr int PD = C::PD;
               if constexpr (T == QLLAMA_KV_I8) {
-                const uint32_t xa = x[c % PD / 4] >> (8 * (c % 4)), ya = y[c % PD / 4] >> (8 * (c % 4));
-                vv[2 * i + j] = hi16s(__float_as_uint(byte_f<0>(ya)), __float_as_uint(byte_f<0>(xa)));
+                const uint32_t xa = x[c % PD / 4], ya = y[c % PD / 4];
+                vv[2 * i + j] = c % 4 == 0 ? codes<0x0c040c00>(ya, xa) : c % 4 == 1 ? codes<0x0c050c01>(ya, xa)
+                              : c % 4 == 2 ? codes<0x0c060c02>(ya, xa) : codes<0x0c070c03>(ya, xa);
               } else {
                 vv[2 * i + j] = c % 2 ? hi16s(y[c % PD / 2], x[c % PD / 2]) : lo16s(y[c % PD / 2], x[c % PD / 2]);
               }
@@ -614,7 +652,11 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
       for (int i = 0; i < 4; i++)
 #pragma unroll
         for (int c = 0; c < DPL; c += 4) {
-          const float x[4] = {acc[c][i] * by, acc[c + 1][i] * by, acc[c + 2][i] * by, acc[c + 3][i] * by};
+          float x[4] = {acc[c][i] * by, acc[c + 1][i] * by, acc[c + 2][i] * by, acc[c + 3][i] * by};
+          if constexpr (T == QLLAMA_KV_I8) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[j] = ldexpf(x[j], v_exp + kCodeBits);
+          }
           const int d = 16 * C::PD * (c / C::PD) + C::PD * (4 * g + i) + c % C::PD;
           if (d < a.hd) __builtin_memcpy(o + d, x, sizeof x);
         }
