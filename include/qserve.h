@@ -130,10 +130,11 @@ int qllama_paged_append(const QPagedKV *c, const QPagedRows *r, void *stream);
 // lens[r] <= 0 gives o = 0 and lse = -inf; lengths above width * page_size count as
 // that; tokens of a page outside the cache are left out.  What lies in slots behind a
 // request's tokens, NaN included, has no effect.  Products and sums in 32 bits: a
-// 16-bit or int8 row enters a product as it is, a query or a weight as two or three
-// 16-bit parts that together hold 22 (f16 cache) or 24 bits.  A cached infinity gives
-// NaN.  width * page_size has to be below 2^31 - 64.  work: qllama_paged_attention_work
-// bytes, 16-byte aligned.
+// 16-bit or int8 row enters a product as it is, a query or a weight (int8: times its
+// value's scale) as two or three 16-bit parts that together hold 22 (f16 and int8
+// caches; a weight at least 2^-37 of the largest) or 24 bits.  A cached infinity gives NaN.
+// width * page_size has to be below 2^31 - 64.  work: qllama_paged_attention_work bytes,
+// 16-byte aligned.
 typedef struct {
   int n_req, n_heads, width;
   int64_t q_stride, o_stride, lse_stride;     // floats between requests; heads lie one behind another

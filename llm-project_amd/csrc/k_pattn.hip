@@ -23,14 +23,17 @@
 // pieces of 8 keys are turned by byte permutes.
 //
 // What is under way carries the bandwidth: two waves a SIMD, a step's values and the next
-// step's keys in registers.  Loading the values a step ahead too took 82 us against 76
-// at the first row below, three waves a SIMD (with fewer registers) 110 against 84 at the
-// time, twice the blocks 92.
+// step's keys (int8: and scales, 138 -> 131 us at the third row below) in registers.  Loading
+// the values a step ahead too took 82 us against 76 at the first row, 138 against 131 at
+// the third; three waves a SIMD (with fewer registers) 110 against 84 at the time, twice
+// the blocks 92.
 //
 // Precision: float queries and weights meet 16-bit keys and values as parts that add up
-// to them (bf16: three parts of 8 bits, f16: two of 11), one MFMA a part; int8 codes
-// are exact in bf16.  fp32 caches use the fp32 MFMA.  At 8 TB/s the parts take a sixth
-// of the bf16 matrix rate.
+// to them (bf16: three parts of 8 bits, f16: two of 11), one MFMA a part.  int8 codes
+// become f16, with the values' scales in the weights, whose power of two follows the
+// largest product so far: three instructions for two codes, where bf16 takes five and a
+// third part (139 -> 132 us).  fp32 caches use the fp32 MFMA.  At 8 TB/s the parts take a
+// sixth of the bf16 matrix rate.
 //
 // Measured (both kernels, 32 query and 8 KV heads; a 1 GiB copy moves 5.1 TB/s):
 //   64 ragged requests of up to 2560 tokens, bf16, hd 128     73.7 us   4.8 TB/s
@@ -39,9 +42,8 @@
 //   24 requests of up to 768 tokens, f32, hd 64               17.1 us   2.1 TB/s
 //   1 request of 2060 tokens, bf16, hd 128                    12.5 us   0.7 TB/s
 // The short ones are two launches and a chain of dependent trips to memory (lengths,
-// table, keys, values, parts).  int8 rows take three times a 16-bit row's vector
-// instructions a byte: 34 thousand a SIMD at the third row, which with the MFMAs keep it
-// some 0.6 of the time.
+// table, keys, values, parts).  An int8 step has half a 16-bit one's bytes under way and
+// the same chain of waits.
 #include <hip/hip_runtime.h>
 
 #include "qserve_host.h"
@@ -148,7 +150,7 @@ __device__ inline uint32_t lo16s(uint32_t b, uint32_t a) { return __builtin_amdg
 // 2^-9 times two int8 codes as f16: the codes plus 128, the bytes of y : x that SELECT
 // names, are subnormal numbers of 2^-24, and one packed multiply-add makes them 2^-9 and takes
 // the 128 off, exactly.  x and y have had the top bits of their bytes turned.
-constexpr int kCodeBits = 9;
+constexpr int kCodeBits = 9, kRaise = 120;
 template <uint32_t SELECT>
 __device__ inline uint32_t codes(uint32_t y, uint32_t x) {
   const h2 u = __builtin_bit_cast(h2, __builtin_amdgcn_perm(y, x, SELECT));
@@ -214,11 +216,13 @@ struct Cfg {
   static constexpr int QROW = HDP * QES + 64;
   // 2^SHIFT times the weights: f16 parts then keep 22 bits down to 2^-18 of the largest
   // weight and the rest to 2^-40
-  static constexpr float SHIFT = HALF ? 15.0f : 0.0f;
+  static constexpr float SHIFT = T == QLLAMA_KV_F16 ? 15.0f : 0.0f;
 };
 
 template <int T, int HDP>
 struct KTile { uint32_t w[Cfg<T, HDP>::SUB][Cfg<T, HDP>::KL][4]; };
+template <int T>
+struct Scales { float k[T == QLLAMA_KV_I8 ? 2 : 1][4], v[T == QLLAMA_KV_I8 ? 2 : 1][4]; };
 template <int T, int HDP>
 struct VTile { uint32_t w[Cfg<T, HDP>::SUB][4][Cfg<T, HDP>::PIECES][Cfg<T, HDP>::PW]; };
 
@@ -388,7 +392,33 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
       }
     };
 
+    auto load_scales = [&](int s, Scales<T> &f) {
+      if constexpr (T == QLLAMA_KV_I8) {
+#pragma unroll
+        for (int i = 0; i < SUB; i++) {
+          int first = 0;
+          const int page = UNI ? lookup(s, i, 0, &first) : 0;
+          if (UNI && a.scs == 1) {                  // 4 keys' scales beside each other, on any 4-byte boundary
+            const long long at = (page < 0 ? 4 * g : page * a.scp + first + 4 * g) + kvh * a.sch;
+            __builtin_memcpy(f.k[i], a.ks + at, sizeof f.k[i]);
+            __builtin_memcpy(f.v[i], a.vs + at, sizeof f.v[i]);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              int place = first + 4 * g + j;
+              const int of = UNI ? page : lookup(s, i, 4 * g + j, &place);
+              const long long at = of < 0 ? 0 : of * a.scp + kvh * a.sch + place * a.scs;
+              f.k[i][j] = a.ks[at];
+              f.v[i][j] = a.vs[at];
+            }
+          }
+        }
+      }
+    };
+
     KTile<T, HDP> k0, k1;
+    Scales<T> f0, f1;
+    load_scales(from, f0);
     load_k(from, k0);
 
     // into LDS, scaled so that weights are powers of two
@@ -435,15 +465,16 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
     const char *q_mine = q_lds + row * C::QROW;
 
     float m = kNegInf, l = 0.0f;                    // of the lane's query head; l over the lane's keys
-    int v_exp = -126;                               // int8: the values' scales are below 2^v_exp
-    float v_unit = 0x1p126f;                        // 2^-v_exp
+    // int8: weights times scales are held times 2^raise, which keeps the largest so far below
+    // 2^15 and within a factor of 2^16 of it or so, whatever the scales are
+    int raise = kRaise;
+    float slack = 0.0f;                             // what a larger score has left over of a factor of 2
     f4 acc[DPL];
 #pragma unroll
     for (int c = 0; c < DPL; c++) acc[c] = f4{0, 0, 0, 0};
 
-    auto step = [&](int s, KTile<T, HDP> &k, KTile<T, HDP> &k_next) {
+    auto step = [&](int s, KTile<T, HDP> &k, KTile<T, HDP> &k_next, Scales<T> &f, Scales<T> &f_next) {
       VTile<T, HDP> v;
-      float ksc[SUB][4], vsc[SUB][4];
       bool out[SUB][4];                             // a key behind the last, or on no page
       bool absent = (s + 1) * STEP > len;
 #pragma unroll
@@ -461,24 +492,11 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
           out[i][j] = page[j] < 0 || s * STEP + 16 * i + 4 * g + j >= len;
           absent |= page[j] < 0;
         }
-        if constexpr (T == QLLAMA_KV_I8) {
-          if (UNI && a.scs == 1) {                  // 4 keys' scales beside each other, on any 4-byte boundary
-            const long long at = (page[0] < 0 ? 4 * g : page[0] * a.scp + place[0]) + kvh * a.sch;
-            __builtin_memcpy(ksc[i], a.ks + at, sizeof ksc[i]);
-            __builtin_memcpy(vsc[i], a.vs + at, sizeof vsc[i]);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-              const long long at = out[i][j] ? 0 : page[j] * a.scp + kvh * a.sch + place[j] * a.scs;
-              ksc[i][j] = a.ks[at];
-              vsc[i][j] = a.vs[at];
-            }
-          }
-        }
       }
       load_v(s, v);
       if (s + 1 < to) {
         advance(s + 1);
+        load_scales(s + 1, f_next);
         load_k(s + 1, k_next);
       }
 
@@ -526,7 +544,7 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
         for (int j = 0; j < 4; j++) {
           sc[i][j] = d[i][j];
           if constexpr (C::HALF) sc[i][j] *= unscale;
-          if constexpr (T == QLLAMA_KV_I8) sc[i][j] *= ksc[i][j];
+          if constexpr (T == QLLAMA_KV_I8) sc[i][j] *= f.k[i][j];
         }
       if (__any(absent)) {
 #pragma unroll
@@ -535,7 +553,7 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
           for (int j = 0; j < 4; j++) {
             if (out[i][j]) {                        // whatever the slot holds, NaN too, counts nothing
               sc[i][j] = kNegInf;
-              if constexpr (T == QLLAMA_KV_I8) vsc[i][j] = 0.0f;
+              if constexpr (T == QLLAMA_KV_I8) f.v[i][j] = 0.0f;
 #pragma unroll
               for (int x = 0; x < C::PIECES; x++)
 #pragma unroll
@@ -551,28 +569,19 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
         for (int j = 0; j < 4; j++) top = fmaxf(top, sc[i][j]);
       top = fmaxf(m, max_groups(top));
       if (__any(top > m)) {                         // rare after the first steps
-        const float f = m == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(m - top);
-        l *= f;
-#pragma unroll
-        for (int c = 0; c < DPL; c++) acc[c] *= f;
-        m = top;
-      }
-      if constexpr (T == QLLAMA_KV_I8) {            // weights times scales into f16's range, by a power of two
-        float most = 0.0f;
-#pragma unroll
-        for (int i = 0; i < SUB; i++)
-#pragma unroll
-          for (int j = 0; j < 4; j++) most = fmaxf(most, vsc[i][j]);
-        most = max_groups(most);
-        if (__any(most * v_unit >= 1.0f)) {         // rare after the first step
-          const int e = (int)(__float_as_uint(most) >> 23) - 126;
-#pragma unroll
-          for (int c = 0; c < DPL; c++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) acc[c][i] = ldexpf(acc[c][i], v_exp - e);
-          v_exp = e;
-          v_unit = ldexpf(1.0f, -e);
+        const float d = m == kNegInf ? kNegInf : m - top;
+        l *= __builtin_amdgcn_exp2f(d);
+        int up = 0;
+        if constexpr (T == QLLAMA_KV_I8) {          // what is held shrinks with the weights, by less than 2 in all
+          const float more = fminf(slack - d, 512.0f);
+          up = min((int)more, kRaise - raise);
+          raise += up;
+          slack = raise == kRaise ? 0.0f : more - up;
         }
+        const float by = __builtin_amdgcn_exp2f(d + up);
+#pragma unroll
+        for (int c = 0; c < DPL; c++) acc[c] *= by;
+        m = top;
       }
       const float ref = (m == kNegInf ? 0.0f : m) - C::SHIFT;
       float p[SUB][4];
@@ -582,8 +591,29 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
         for (int j = 0; j < 4; j++) {
           p[i][j] = __builtin_amdgcn_exp2f(sc[i][j] - ref);
           l += p[i][j];
-          if constexpr (T == QLLAMA_KV_I8) p[i][j] *= vsc[i][j] * v_unit;
+          if constexpr (T == QLLAMA_KV_I8) p[i][j] *= f.v[i][j];
         }
+      if constexpr (T == QLLAMA_KV_I8) {            // into f16's range
+        float most = 0.0f;
+#pragma unroll
+        for (int i = 0; i < SUB; i++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) most = fmaxf(most, p[i][j]);
+        most = max_groups(most);
+        const int room = 141 - (int)(__float_as_uint(most) >> 23);           // most < 2^(15 - room)
+        if (__any(room < raise)) {                  // rare after the first step
+          const int down = min(room - raise, 0);
+          raise += down;
+#pragma unroll
+          for (int c = 0; c < DPL; c++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[c][i] = ldexpf(acc[c][i], down);
+        }
+#pragma unroll
+        for (int i = 0; i < SUB; i++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) p[i][j] = ldexpf(p[i][j], raise);
+      }
 
       if constexpr (T == QLLAMA_KV_F32) {
 #pragma unroll
@@ -635,8 +665,8 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
     };
 
     for (int s = from; s < to; s += 2) {
-      step(s, k0, k1);
-      if (s + 1 < to) step(s + 1, k1, k0);
+      step(s, k0, k1, f0, f1);
+      if (s + 1 < to) step(s + 1, k1, k0, f1, f0);
     }
     l = sum_groups(l);
 
@@ -655,7 +685,7 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
           float x[4] = {acc[c][i] * by, acc[c + 1][i] * by, acc[c + 2][i] * by, acc[c + 3][i] * by};
           if constexpr (T == QLLAMA_KV_I8) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) x[j] = ldexpf(x[j], v_exp + kCodeBits);
+            for (int j = 0; j < 4; j++) x[j] = ldexpf(x[j], kCodeBits - raise);
           }
           const int d = 16 * C::PD * (c / C::PD) + C::PD * (4 * g + i) + c % C::PD;
           if (d < a.hd) __builtin_memcpy(o + d, x, sizeof x);

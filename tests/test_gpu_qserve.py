@@ -350,12 +350,17 @@ def test_append_int8_codes_of_nan(Q):
 # ---------------------------------------------------------------------------
 # Attention
 # ---------------------------------------------------------------------------
-def attend_ref(kv, q, table, lens, scale=None):
+def attend_ref(kv, q, table, lens, scale=None, uneven=False):
     """o, lse, and a bound of what 32-bit arithmetic may differ from them, all in 64 bits.
 
     A score is a sum of 3 hd products at most (three parts of a query), so it is off by (3 hd + 4) EPS sum |q k| scale;
     a weight by that of its score and of the maximum, the exponential's argument (2 EPS |score| each) and the exponential
-    (4 EPS); the sums over len tokens, in parts of three, by (3 len + 16) EPS of sum w |v|."""
+    (4 EPS); the sums over len tokens, in parts of three, by (3 len + 16) EPS of sum w |v|.
+
+    uneven (int8): a weight times its scale enters as two 16-bit floats of 11 bits, the largest such product between 2^14 and
+    2^15 (2^13 after a larger score has come, which halves it at most); the second float's last bit is 2^-24 or the product's
+    own 2^-22, so each product is off by 2^-24 / 2^13 = 2^-37 of the largest, and each of len tokens adds that times its code,
+    127 at most."""
     n, H, hd = q.shape
     KVH, page = kv.k.shape[1], kv.k.shape[2]
     G = H // KVH
@@ -383,6 +388,8 @@ def attend_ref(kv, q, table, lens, scale=None):
             dw = 2 * ds + 4 * EPS * s.abs().max() + 8 * EPS
             o[r, h], lse[r, h] = w @ v, z
             bound[r, h] = (2 * dw + (3 * len(t) + 16) * EPS) * (w @ v.abs())
+            if uneven:
+                bound[r, h] += len(t) * 127 * 2.0 ** -37 * (w * kv.v_scale.get().double()[p, h // G, t % page]).max()
             lse_bound[r, h] = dw + (len(t) + 16) * EPS + 4 * EPS * abs(z)
     return o, lse, bound, lse_bound
 
@@ -419,9 +426,9 @@ class Work:
     element_size = lambda self: 1  # noqa: E731
 
 
-def check(Q, kv, q, table, lens, **kw):
+def check(Q, kv, q, table, lens, uneven=False, **kw):
     o, lse = attend(Q, kv, q, table, lens, **kw)
-    wo, wl, bound, lb = attend_ref(kv, q, table, lens, kw.get("scale"))
+    wo, wl, bound, lb = attend_ref(kv, q, table, lens, kw.get("scale"), uneven)
     o, lse = o.double(), lse.double()
     assert bool(((o - wo).abs() <= bound).all()), ((o - wo).abs() - bound).max()
     empty = torch.isinf(wl)
@@ -523,6 +530,54 @@ def test_attention_leaves_out_what_is_no_token(Q, typ, page):
     assert bool(torch.isfinite(o).all()) and torch.equal(o, o2) and torch.equal(lse, lse2)
     assert bool((o[5] == 0).all()) and bool(torch.isinf(lse[5]).all())
     check(Q, kv, q, table, lens)
+
+
+@pytest.mark.parametrize("page", [16, 20])
+@pytest.mark.parametrize("order", ["up", "down", "mixed", "one", "zero", "unlikely"])
+def test_attention_int8_scales_of_every_size(Q, page, order):
+    """Scales of values that run over sixty powers of ten, in rising, falling and mixed order, a single enormous one, ones
+    of 0, and an enormous one whose weight is tiny."""
+    H, KVH, hd, n = 8, 2, 64, 90
+    pages = -(-n // page)
+    kv = make_cache(Q, "i8", pages, KVH, page, hd)
+    slots = torch.arange(pages * page)
+    e = {"up": slots * 0.6 - 27.0, "down": 27.0 - slots * 0.6, "mixed": (slots * 37 % 90) * 0.6 - 27.0, "one": torch.where(slots == 40, 20.0, -5.0),
+         "zero": slots * 0.0, "unlikely": torch.where(slots == 3, 18.0, 0.0)}[order].double()
+    scale = (10.0 ** e).float().reshape(pages, 1, page).expand(pages, KVH, page).contiguous()
+    if order == "zero":
+        scale[:, :, ::3] = 0.0
+    kv.v_scale.set(scale)
+    if order == "unlikely":                                   # the other keys' scores lie far above that one's
+        k = kv.k.get()
+        k[:] = torch.where(k >= 0, k.clamp(min=20), k.clamp(max=-20))
+        k[:, :, 1:] = k[:, :, :1]
+        k[0, :, 3] = -k[0, :, 3]
+        kv.k.set(k)
+        kv.k_scale.set(torch.full_like(scale, 0.05))
+    q = torch.randn((2, H, hd), generator=torch.Generator().manual_seed(4))
+    if order == "unlikely":
+        q = kv.k.get()[0, :, 0].float().repeat_interleave(H // KVH, 0).expand(2, H, hd) * 0.02 * torch.tensor([1.0, 2.0])[:, None, None]
+    table = torch.arange(pages, dtype=torch.int32).expand(2, pages).contiguous()
+    check(Q, kv, q.contiguous(), table, [n, n - 7], uneven=True)
+
+
+def test_attention_int8_scores_that_rise_slowly(Q):
+    """One enormous scale ahead of scores that rise by less than a factor of 2 a step of 32 keys, until its product is like
+    the others': as many equal requests as make every wave take all of a request's 45 steps."""
+    n, KVH, hd, page, steps = 1024, 2, 8, 32, 45
+    kv = make_cache(Q, "i8", steps, KVH, page, hd, gen=torch.Generator().manual_seed(9))
+    k, v = torch.zeros((steps, KVH, page, hd), dtype=torch.int8), kv.v.get()
+    k[..., 0] = 127
+    v[0, :, 0] = torch.tensor([127, 0, 0, 0, -127, 0, 0, 0], dtype=torch.int8)
+    rise = 0.9 * math.log(2.0) * torch.arange(steps)[:, None, None].expand(steps, KVH, page) / 127
+    scale = torch.ones((steps, KVH, page))
+    scale[0, :, 0] = 2.0 ** 40
+    kv.k.set(k), kv.v.set(v), kv.k_scale.set(rise.contiguous()), kv.v_scale.set(scale)
+    q = torch.ones((1, KVH, hd))
+    table = torch.arange(steps, dtype=torch.int32)[None]
+    o, lse = attend(Q, kv, q.expand(n, KVH, hd).contiguous(), table.expand(n, steps).contiguous(), [steps * page] * n, scale=1.0)
+    wo, wl, bound, lb = attend_ref(kv, q, table, [steps * page], 1.0, uneven=True)
+    assert bool(((o.double() - wo).abs() <= bound).all()) and bool(((lse.double() - wl).abs() <= lb).all())
 
 
 def test_attention_large_scores_and_nan(Q):
