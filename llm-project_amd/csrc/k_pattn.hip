@@ -284,10 +284,11 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
     r_begin += (long long)__builtin_amdgcn_readlane(upto, 63) * tiles;
   }
 
+  len = __builtin_amdgcn_readfirstlane(len);        // one for the wave from here on
   if (u < end) {
     const unsigned long long at = u - r_begin;
     steps = (len + STEP - 1) / STEP;
-    tile = at >> 32 ? (int)(at / (unsigned)steps) : (int)((unsigned)at / (unsigned)steps);
+    tile = __builtin_amdgcn_readfirstlane(at >> 32 ? (int)(at / (unsigned)steps) : (int)((unsigned)at / (unsigned)steps));
     from = (int)(at - (unsigned long long)tile * steps);
   }
   Window<UNI> win;
@@ -295,7 +296,7 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
 
   while (u < end) {
     if (tile == tiles) {                            // the next request that has tokens
-      do len = len_of(++r); while (len == 0);
+      do len = __builtin_amdgcn_readfirstlane(len_of(++r)); while (len == 0);
       steps = (len + STEP - 1) / STEP;
       tile = 0;
       win.first = -1;
@@ -319,11 +320,14 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
     if (fresh) win.settle(a, len);
 
     const char *kbase = a.k + kvh * a.hst, *vbase = a.v + kvh * a.hst;
-    int k_off[C::KL], v_off[C::PIECES];             // padded dims read dim 0: their products are dropped, or with 0
+    // a lane's place behind a row, UNI: behind the first row of 16; padded dims read dim 0: their
+    // products are dropped, or with 0
+    unsigned k_off[C::KL], v_off[C::PIECES];
 #pragma unroll
-    for (int x = 0; x < C::KL; x++) k_off[x] = 64 * x + 16 * g < a.hd * C::ES ? 64 * x + 16 * g : 0;
+    for (int x = 0; x < C::KL; x++) k_off[x] = (64 * x + 16 * g < a.hd * C::ES ? 64 * x + 16 * g : 0) + (UNI ? n * (int)a.sst : 0);
 #pragma unroll
-    for (int x = 0; x < C::PIECES; x++) v_off[x] = 16 * C::PD * x + C::PD * n < a.hd ? (16 * C::PD * x + C::PD * n) * C::ES : 0;
+    for (int x = 0; x < C::PIECES; x++)
+      v_off[x] = (16 * C::PD * x + C::PD * n < a.hd ? (16 * C::PD * x + C::PD * n) * C::ES : 0) + (UNI ? 4 * g * (int)a.sst : 0);
 
     // page and place of 16-key group i of step s (UNI), or of its key j
     auto lookup = [&](int s, int i, int j, int *place) -> int {
@@ -351,7 +355,6 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
         int page = lookup(s, i, UNI ? 0 : n, &place);
         if (page < 0) { page = 0; place = 0; }
         const char *p = kbase + page * a.pst + place * a.sst;
-        if constexpr (UNI) p += (unsigned)(n * (int)a.sst);
 #pragma unroll
         for (int x = 0; x < C::KL; x++) {
           if (T != QLLAMA_KV_I8 || a.hd % 16 == 0) {
@@ -359,7 +362,7 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
           } else {                                  // the row may end within the 16 bytes
             uint32_t lo[2], hi[2];
             load_words<STREAM>(lo, p + k_off[x]);
-            load_words<STREAM>(hi, p + (64 * x + 16 * g + 8 < a.hd ? k_off[x] + 8 : 0));
+            load_words<STREAM>(hi, p + (64 * x + 16 * g + 8 < a.hd ? k_off[x] + 8 : k_off[x]));
             k.w[i][x][0] = lo[0]; k.w[i][x][1] = lo[1]; k.w[i][x][2] = hi[0]; k.w[i][x][3] = hi[1];
           }
         }
@@ -379,7 +382,7 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
         for (int j = 0; j < 4; j++) {
           const char *pj = p;
           if constexpr (UNI) {
-            pj += (unsigned)((4 * g + j) * (int)a.sst);
+            pj += j * a.sst;
           } else {
             int place;
             int page = lookup(s, i, 4 * g + j, &place);
