@@ -12,7 +12,9 @@
 // weighted values in the workspace, and k_paged_join puts a tile's parts together.
 // Waves never meet: with four of them on a tile, meeting in LDS at its end, 512 requests
 // of up to 300 f16 tokens (8 KV heads of 128, pages of 16) took 167 us, with shares of
-// their own 134 (100 with all that follows here).
+// their own 134 (100 with all that follows here).  Only for short tables and not too many
+// tiles a block of 8 waves takes a tile, a wave a part of its steps, and they do meet: one
+// launch instead of two (launch() has the rule and its figures).
 //
 // A wave keeps its running maximum, sum and outputs in registers, its queries in LDS, and
 // takes a step of 16 or 32 keys at a time straight from the pages into registers.
@@ -41,7 +43,8 @@
 //   128 requests of up to 4100 tokens, int8, hd 128          132   us   4.3 TB/s
 //   24 requests of up to 768 tokens, f32, hd 64               17.1 us   2.1 TB/s
 //   1 request of 2060 tokens, bf16, hd 128                    12.5 us   0.7 TB/s
-// The short ones are two launches and a chain of dependent trips to memory (lengths,
+//   1 request of 200 tokens, f32, 6 + 2 heads of 48             7.2 us
+// The short ones are launches and a chain of dependent trips to memory (lengths,
 // table, keys, values, parts).  An int8 step has half a 16-bit one's bytes under way and
 // the same chain of waits.
 #include <hip/hip_runtime.h>
@@ -197,6 +200,9 @@ __device__ inline f4 mfma16(u4 a, u4 b, f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
 }
 
+// Waves that meet, as the registers allow.
+constexpr int meeting(int hdp) { return hdp > 128 ? 4 : 8; }
+
 // What a type and a padded head size fix.
 template <int T, int HDP>
 struct Cfg {
@@ -211,6 +217,7 @@ struct Cfg {
   static constexpr int DPL = HDP / 16;                         // dims of a value row in a lane
   static constexpr int PARTS = T == QLLAMA_KV_F32 ? 1 : T == QLLAMA_KV_BF16 ? 3 : 2;
   static constexpr bool HALF = PARTS == 2;                     // f16 products
+  static constexpr int MEETING = meeting(HDP);
   // a query row in LDS: a part's values, and 64 bytes that spread rows over the banks
   static constexpr int QES = T == QLLAMA_KV_F32 ? 4 : 2;
   static constexpr int QROW = HDP * QES + 64;
@@ -241,8 +248,9 @@ struct Window {
   __device__ inline void settle(const PaArgs &a, int len) { page = page_of(page, key(), len, a.n_pages); }
 };
 
-template <int T, int HDP, bool UNI, bool STREAM>
-__global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaArgs a) {
+// MEET: a block's waves share one tile, a request's where blockIdx says, and meet in LDS.
+template <int T, int HDP, bool UNI, bool STREAM, bool MEET>
+__global__ __launch_bounds__(MEET ? 64 * meeting(HDP) : kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaArgs a) {
   using C = Cfg<T, HDP>;
   constexpr int SUB = C::SUB, STEP = C::STEP, CH = HDP / 32, DPL = C::DPL;
   extern __shared__ __align__(16) char dyn[];       // a wave's queries: [part][row]
@@ -250,47 +258,59 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
   const int n = lane & 15, g = lane >> 4;           // key, query head or value piece; group of 16 lanes
   const int tiles = a.n_kv * a.tiles;
   char *q_lds = dyn + wave * (C::PARTS * a.rows * C::QROW);
+  float *parts = reinterpret_cast<float *>(dyn + C::MEETING * (C::PARTS * a.rows * C::QROW));     // of waves that meet
 
   // this wave's share of all steps; shares of one block lie far apart, so that few of
   // them are spread over the CUs
   const auto len_of = [&](int r) { return r < a.n_req ? clamp_len(a.lens[r], a.width, a.page_size) : 0; };
-  int len = len_of(lane);                           // of request `lane` of the 64 in hand, then of the one at work
-  int upto = wave_scan((len + STEP - 1) / STEP);    // steps of those up to it
-  long long units = (long long)__builtin_amdgcn_readlane(upto, 63) * tiles;
-  for (int r = 64; r < a.n_req; r += 64)
-    units += (long long)__builtin_amdgcn_readlane(wave_scan((len_of(r + lane) + STEP - 1) / STEP), 63) * tiles;
-  const long long share = share_of(units);
+  int len, r = 0, steps = 0, tile = 0, from = 0;    // a request, its steps, where in them this wave begins
+  long long u, end, share = 0;                      // units from u up to end are this wave's
   const int id = wave * kBlocks + blockIdx.x;
-  long long u = id * share;
-  const long long end = u + share < units ? u + share : units;
-  if (lane == 0) a.split[id] = make_int4(0, 0, 0, 0);
-  const long long begin = u;
-  int r = 0;                                        // the request it begins in, and that one's first unit
-  long long r_begin = 0;
-  int steps = 0, tile = 0, from = 0;                // of the request; in it; in that
-  for (; u < end; r += 64) {
-    if (r) {
-      len = len_of(r + lane);
-      upto = wave_scan((len + STEP - 1) / STEP);
-    }
-    const uint64_t past = __ballot(r_begin + (long long)upto * tiles > u);
-    if (past) {
-      const int at = __builtin_ctzll(past);
-      len = __builtin_amdgcn_readlane(len, at);
-      r_begin += (long long)(__builtin_amdgcn_readlane(upto, at) - (len + STEP - 1) / STEP) * tiles;
-      r += at;
-      break;
-    }
-    r_begin += (long long)__builtin_amdgcn_readlane(upto, 63) * tiles;
-  }
-
-  len = __builtin_amdgcn_readfirstlane(len);        // one for the wave from here on
-  if (u < end) {
-    const unsigned long long at = u - r_begin;
+  if constexpr (MEET) {
+    r = blockIdx.y;
+    tile = blockIdx.x;
+    len = __builtin_amdgcn_readfirstlane(len_of(r));
     steps = (len + STEP - 1) / STEP;
-    tile = __builtin_amdgcn_readfirstlane(at >> 32 ? (int)(at / (unsigned)steps) : (int)((unsigned)at / (unsigned)steps));
-    from = (int)(at - (unsigned long long)tile * steps);
+    const int each = (steps + C::MEETING - 1) / C::MEETING;
+    from = wave * each;
+    u = from;
+    end = from + each < steps ? from + each : steps;
+  } else {
+    len = len_of(lane);                               // of request `lane` of the 64 in hand, then of the one at work
+    int upto = wave_scan((len + STEP - 1) / STEP);    // steps of those up to it
+    long long units = (long long)__builtin_amdgcn_readlane(upto, 63) * tiles;
+    for (int r = 64; r < a.n_req; r += 64)
+      units += (long long)__builtin_amdgcn_readlane(wave_scan((len_of(r + lane) + STEP - 1) / STEP), 63) * tiles;
+    share = share_of(units);
+    u = id * share;
+    end = u + share < units ? u + share : units;
+    if (lane == 0) a.split[id] = make_int4(0, 0, 0, 0);
+    long long r_begin = 0;                            // the first unit of the request it begins in
+    for (; u < end; r += 64) {
+      if (r) {
+        len = len_of(r + lane);
+        upto = wave_scan((len + STEP - 1) / STEP);
+      }
+      const uint64_t past = __ballot(r_begin + (long long)upto * tiles > u);
+      if (past) {
+        const int at = __builtin_ctzll(past);
+        len = __builtin_amdgcn_readlane(len, at);
+        r_begin += (long long)(__builtin_amdgcn_readlane(upto, at) - (len + STEP - 1) / STEP) * tiles;
+        r += at;
+        break;
+      }
+      r_begin += (long long)__builtin_amdgcn_readlane(upto, 63) * tiles;
+    }
+
+    len = __builtin_amdgcn_readfirstlane(len);        // one for the wave from here on
+    if (u < end) {
+      const unsigned long long at = u - r_begin;
+      steps = (len + STEP - 1) / STEP;
+      tile = __builtin_amdgcn_readfirstlane(at >> 32 ? (int)(at / (unsigned)steps) : (int)((unsigned)at / (unsigned)steps));
+      from = (int)(at - (unsigned long long)tile * steps);
+    }
   }
+  const long long begin = u;
   Window<UNI> win;
   win.first = -1;
 
@@ -675,12 +695,7 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
 
     // lane (n, g) holds head n; acc[c][i] is dim c mod PD of the piece of lane 4 g + i
     const bool whole = from == 0 && to == steps;
-    float *o = a.part + ((long long)id * 2 + (u == begin ? 0 : 1)) * (a.rows * (a.hd + 2)) + row * (a.hd + 2), by = 1.0f;
-    if (whole) {
-      o = a.o + r * a.o_stride + (long long)(h0 + row) * a.hd;
-      by = l == 0.0f ? 0.0f : 1.0f / l;
-    }
-    if (n < rows) {
+    const auto put = [&](float *o, float by) {
 #pragma unroll
       for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -693,20 +708,49 @@ __global__ __launch_bounds__(kThreads, HDP > 128 ? 1 : 2) void k_paged_attn(PaAr
           const int d = 16 * C::PD * (c / C::PD) + C::PD * (4 * g + i) + c % C::PD;
           if (d < a.hd) __builtin_memcpy(o + d, x, sizeof x);
         }
-      if (g == 0) {
-        if (!whole) {
-          o[a.hd] = m;
-          o[a.hd + 1] = l;
-        } else if (a.lse) {
-          a.lse[r * a.lse_stride + h0 + row] = l == 0.0f ? kNegInf : (m - C::SHIFT + __builtin_amdgcn_logf(l)) * 0.69314718056f;
-        }
+    };
+    if (n < rows) {
+      if (whole) {
+        put(a.o + r * a.o_stride + (long long)(h0 + row) * a.hd, l == 0.0f ? 0.0f : 1.0f / l);
+        if (g == 0 && a.lse) a.lse[r * a.lse_stride + h0 + row] = l == 0.0f ? kNegInf : (m - C::SHIFT + __builtin_amdgcn_logf(l)) * 0.69314718056f;
+      } else if constexpr (MEET) {
+        float *o = parts + wave * (a.rows * (a.hd + 2)) + row * (a.hd + 2);
+        put(o, 1.0f);
+        if (g == 0) { o[a.hd] = m; o[a.hd + 1] = l; }
+      } else {
+        float *o = a.part + ((long long)id * 2 + (u == begin ? 0 : 1)) * (a.rows * (a.hd + 2)) + row * (a.hd + 2);
+        put(o, 1.0f);
+        if (g == 0) { o[a.hd] = m; o[a.hd + 1] = l; }
       }
     }
-    if (from == 0 && !whole && lane == 0)            // the tile goes on in the shares behind this one
+    if (!MEET && from == 0 && !whole && lane == 0)   // the tile goes on in the shares behind this one
       a.split[id] = make_int4(1 + (int)((steps - to + share - 1) / share), r, tile, u == begin ? 0 : 1);
     u += to - from;
     from = 0;
     tile++;
+  }
+
+  if constexpr (MEET) {
+    const int kvh = (int)blockIdx.x / a.tiles, part = (int)blockIdx.x - kvh * a.tiles;
+    const int h0 = kvh * a.G + part * 16, rows = a.G - part * 16 < 16 ? a.G - part * 16 : 16;
+    float *o = a.o + r * a.o_stride + (long long)h0 * a.hd, *lse = a.lse + r * a.lse_stride + h0;
+    const int each = (steps + C::MEETING - 1) / C::MEETING, n_parts = steps ? (steps + each - 1) / each : 0, one = a.hd + 2;
+    __syncthreads();
+    if (n_parts == 1) return;
+    for (int i = threadIdx.x; i < rows * a.hd; i += 64 * C::MEETING) {
+      const int row = i / a.hd, d = i - row * a.hd;
+      const float *p = parts + row * one;
+      float top = kNegInf, sum = 0.0f, x = 0.0f;
+      for (int j = 0; j < n_parts; j++) top = fmaxf(top, p[j * a.rows * one + a.hd]);
+      for (int j = 0; j < n_parts; j++) {
+        const float f = part_weight(p[j * a.rows * one + a.hd], top);
+        sum += p[j * a.rows * one + a.hd + 1] * f;
+        x += p[j * a.rows * one + d] * f;
+      }
+      o[i] = sum == 0.0f ? 0.0f : x * (1.0f / sum);
+      if (d == 0 && a.lse) lse[row] = sum == 0.0f ? kNegInf : (top - C::SHIFT + __builtin_amdgcn_logf(sum)) * 0.69314718056f;
+    }
+    return;
   }
 
   // a request without a token has no tile: its outputs are set here
@@ -804,20 +848,39 @@ int rows_of(const QPagedKV *c, int n_heads) {
 
 template <int T, int HDP>
 int launch(const char *fn, const PaArgs &a, hipStream_t stream) {
-  const size_t lds = (size_t)kWaves * Cfg<T, HDP>::PARTS * a.rows * Cfg<T, HDP>::QROW;
+  using C = Cfg<T, HDP>;
   const bool uni = a.page_size % 16 == 0, once = a.tiles == 1;
-  void (*f)(PaArgs) = uni ? once ? k_paged_attn<T, HDP, true, true> : k_paged_attn<T, HDP, true, false>
-                          : once ? k_paged_attn<T, HDP, false, true> : k_paged_attn<T, HDP, false, false>;
+  const long long tiles = (long long)a.n_req * a.n_kv * a.tiles, room = ((long long)a.width * a.page_size + C::STEP - 1) / C::STEP;
+  const size_t queries = (size_t)C::PARTS * a.rows * C::QROW, part = (size_t)a.rows * (a.hd + 2) * sizeof(float);
+  // Short tables: a block a tile, whose waves meet, and no second launch, where a wave takes
+  // few steps and the tiles few rounds of the chip.  Against shares, us: 32 bf16 requests of
+  // up to 120 tokens (hd 128, 8 KV heads) 7.2 / 11.8, 64 of 340 21.3 / 22.7, 128 of 120 22.8 / 20.3;
+  // one of 100 6.7 / 8.8, of 340 10.1 / 9.0 (idle CUs); 64 f32 ones of 340 (3 steps a wave) 32.7 /
+  // 30.8; hd 64, 24 f32 ones of 250 8.7 / 13.2, 64 bf16 ones of 340 11.0 / 17.1.
+  const long long each = (room + C::MEETING - 1) / C::MEETING;
+  const bool meet = each * HDP <= (tiles < 32 ? 128 : 256) && tiles <= 512 && C::MEETING * (queries + part) <= 64 * 1024;
+  void (*f)(PaArgs);
+  if (meet)
+    f = uni ? once ? k_paged_attn<T, HDP, true, true, true> : k_paged_attn<T, HDP, true, false, true>
+            : once ? k_paged_attn<T, HDP, false, true, true> : k_paged_attn<T, HDP, false, false, true>;
+  else
+    f = uni ? once ? k_paged_attn<T, HDP, true, true, false> : k_paged_attn<T, HDP, true, false, false>
+            : once ? k_paged_attn<T, HDP, false, true, false> : k_paged_attn<T, HDP, false, false, false>;
+  const size_t lds = meet ? C::MEETING * (queries + part) : kWaves * queries;
   if (lds > 64 * 1024 &&              // past what a launch may take unasked
       hipFuncSetAttribute(reinterpret_cast<const void *>(f), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) {
     (void)hipGetLastError();
     return qs::refuse(fn, "hipFuncSetAttribute failed");
   }
+  if (meet) {
+    QS_LAUNCH(fn, f, dim3(a.n_kv * a.tiles, a.n_req), dim3(64 * C::MEETING), lds, stream, a);
+    return 0;
+  }
   QS_LAUNCH(fn, f, dim3(kBlocks), dim3(kThreads), lds, stream, a);
   // shares that can hold a step, by the room of the tables
-  const long long most = (long long)a.n_req * a.n_kv * a.tiles * (((long long)a.width * a.page_size + Cfg<T, HDP>::STEP - 1) / Cfg<T, HDP>::STEP);
+  const long long most = tiles * room;
   const int shares = most / kMinShare + 1 < kShares ? (int)(most / kMinShare + 1) : kShares;
-  QS_LAUNCH(fn, k_paged_join, dim3(shares, a.rows), dim3(kJoinThreads), 0, stream, a, (float)Cfg<T, HDP>::SHIFT);
+  QS_LAUNCH(fn, k_paged_join, dim3(shares, a.rows), dim3(kJoinThreads), 0, stream, a, (float)C::SHIFT);
   return 0;
 }
 

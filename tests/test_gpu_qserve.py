@@ -426,14 +426,20 @@ class Work:
     element_size = lambda self: 1  # noqa: E731
 
 
+def widened(table, page):
+    """The table with room for 5000 tokens more, in which there are no pages: long tables are served otherwise than short ones."""
+    return torch.cat([table, torch.full((len(table), 5000 // page), 2 ** 31 - 1, dtype=torch.int32)], 1)
+
+
 def check(Q, kv, q, table, lens, uneven=False, **kw):
-    o, lse = attend(Q, kv, q, table, lens, **kw)
     wo, wl, bound, lb = attend_ref(kv, q, table, lens, kw.get("scale"), uneven)
-    o, lse = o.double(), lse.double()
-    assert bool(((o - wo).abs() <= bound).all()), ((o - wo).abs() - bound).max()
     empty = torch.isinf(wl)
-    assert torch.equal(torch.isinf(lse), empty) and bool((lse[empty] < 0).all()) and bool((o[empty] == 0).all())
-    assert bool(((lse - wl).abs()[~empty] <= lb[~empty]).all())
+    for t in (table, widened(table, kv.k.shape[2])):
+        o, lse = attend(Q, kv, q, t, lens, **kw)
+        o, lse = o.double(), lse.double()
+        assert bool(((o - wo).abs() <= bound).all()), ((o - wo).abs() - bound).max()
+        assert torch.equal(torch.isinf(lse), empty) and bool((lse[empty] < 0).all()) and bool((o[empty] == 0).all())
+        assert bool(((lse - wl).abs()[~empty] <= lb[~empty]).all())
 
 
 SHAPES = [(6, 2, 48), (32, 8, 64), (8, 2, 128), (4, 4, 128), (5, 1, 8), (20, 1, 72), (33, 1, 256), (16, 1, 160)]
@@ -523,12 +529,13 @@ def test_attention_leaves_out_what_is_no_token(Q, typ, page):
             kv.k.set(kv.k.host.masked_fill(empty, a))
             kv.v.set(kv.v.host.masked_fill(empty, b))
 
-    stale(float("nan"), float("inf"))
-    o, lse = attend(Q, kv, q, table, lens)
-    stale(0.0, 0.0)
-    o2, lse2 = attend(Q, kv, q, table, lens)
-    assert bool(torch.isfinite(o).all()) and torch.equal(o, o2) and torch.equal(lse, lse2)
-    assert bool((o[5] == 0).all()) and bool(torch.isinf(lse[5]).all())
+    for t in (table, widened(table, page)):
+        stale(float("nan"), float("inf"))
+        o, lse = attend(Q, kv, q, t, lens)
+        stale(0.0, 0.0)
+        o2, lse2 = attend(Q, kv, q, t, lens)
+        assert bool(torch.isfinite(o).all()) and torch.equal(o, o2) and torch.equal(lse, lse2)
+        assert bool((o[5] == 0).all()) and bool(torch.isinf(lse[5]).all())
     check(Q, kv, q, table, lens)
 
 
@@ -561,6 +568,21 @@ def test_attention_int8_scales_of_every_size(Q, page, order):
     check(Q, kv, q.contiguous(), table, [n, n - 7], uneven=True)
 
 
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16", "i8"])
+@pytest.mark.parametrize("H,KVH,hd", [(6, 2, 48), (8, 8, 64), (40, 2, 64), (32, 8, 128), (4, 1, 200)])
+@pytest.mark.parametrize("page,n", [(16, 1), (16, 20), (12, 20)])
+def test_attention_of_short_and_of_long_tables(Q, typ, H, KVH, hd, page, n):
+    """Lengths around those at which the waves of a block that takes a short request have one, two or more steps each."""
+    r = random.Random(hd + n)
+    lens = ([240] if n == 1 else [0, 1, 15, 16, 17, 31, 33, 127, 128, 129, 240, 255, 256, -1])
+    lens += [r.randint(0, 260) for _ in range(n - len(lens))]
+    g = torch.Generator().manual_seed(hd)
+    need = sum(-(-max(x, 0) // page) for x in lens)
+    kv = make_cache(Q, typ, need + 2, KVH, page, hd, "head", g)
+    q = torch.randn((n, H, hd), generator=g) * 2.0
+    check(Q, kv, q, pages_for(lens, page, -(-260 // page), need + 2, hd), lens)
+
+
 def test_attention_int8_scores_that_rise_slowly(Q):
     """One enormous scale ahead of scores that rise by less than a factor of 2 a step of 32 keys, until its product is like
     the others': as many equal requests as make every wave take all of a request's 45 steps."""
@@ -591,11 +613,13 @@ def test_attention_large_scores_and_nan(Q):
         lens = [60, 33]
         table = pages_for([60, 33], 16, 4, 8, 2)
         check(Q, kv, q, table, lens)
-        o, _ = attend(Q, kv, q, table, lens)
-        q[0, 1, 7] = float("nan")
-        o2, _ = attend(Q, kv, q, table, lens)
-        assert bool(o2[0, 1].isnan().all())
-        assert torch.equal(o2[0, [0, 2, 3]], o[0, [0, 2, 3]]) and torch.equal(o2[1], o[1])
+        spoilt = q.clone()
+        spoilt[0, 1, 7] = float("nan")
+        for t in (table, widened(table, 16)):
+            o, _ = attend(Q, kv, q, t, lens)
+            o2, _ = attend(Q, kv, spoilt, t, lens)
+            assert bool(o2[0, 1].isnan().all())
+            assert torch.equal(o2[0, [0, 2, 3]], o[0, [0, 2, 3]]) and torch.equal(o2[1], o[1])
 
 
 @pytest.mark.parametrize("typ", ["f32", "i8"])
