@@ -38,10 +38,10 @@
 // sixth of the bf16 matrix rate.
 //
 // Measured (both kernels, 32 query and 8 KV heads; a 1 GiB copy moves 5.1 TB/s):
-//   64 ragged requests of up to 2560 tokens, bf16, hd 128     73.7 us   4.8 TB/s
+//   64 ragged requests of up to 2560 tokens, bf16, hd 128     73   us   4.8 TB/s
 //   2 requests, up to 120000 tokens, f16, hd 128             134   us   5.5 TB/s
-//   128 requests of up to 4100 tokens, int8, hd 128          132   us   4.3 TB/s
-//   24 requests of up to 768 tokens, f32, hd 64               17.1 us   2.1 TB/s
+//   128 requests of up to 4100 tokens, int8, hd 128          130   us   4.4 TB/s
+//   24 requests of up to 768 tokens, f32, hd 64               17.0 us   2.1 TB/s
 //   1 request of 2060 tokens, bf16, hd 128                    12.5 us   0.7 TB/s
 //   1 request of 200 tokens, f32, 6 + 2 heads of 48             7.2 us
 // The short ones are launches and a chain of dependent trips to memory (lengths,
@@ -63,7 +63,7 @@ typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 constexpr int kThreads = 256, kWaves = 4;
 constexpr int kBlocks = 512;          // two blocks of four waves a CU
 constexpr int kShares = kBlocks * kWaves;
-constexpr int kMinShare = 1;          // steps a wave takes at least; one request of 200 tokens took 7.6 us, with 2 or 4 9.1
+constexpr int kMinShare = 1;          // steps a wave takes at least; one request of 2060 tokens took 12.5 us, with 2 or 4 13.3
 constexpr float kNegInf = -__builtin_inff();
 
 struct PaArgs {
@@ -764,8 +764,8 @@ __global__ __launch_bounds__(MEET ? 64 * meeting(HDP) : kThreads, HDP > 128 ? 1 
 
 // One block a share and row: where a tile begins in the share and goes on behind it, its
 // parts put together in the order of their keys, 8 (hd <= 128) or 4 side by side.  A
-// trip to the descriptor and one to the parts, with a launch in front: 3.8 us for two
-// tiles of 13 parts, 7.1 at 64 ragged requests (512 tiles of some 4 parts), 12.3 where
+// trip to the descriptor and one to the parts, with a launch in front: 5.2 us for eight
+// tiles of 67 parts, 7.3 at 64 ragged requests (512 tiles of some 4 parts), 12.3 where
 // 2048 shares make 16 tiles.
 constexpr int kJoinThreads = 256, kAhead = 4;
 __global__ __launch_bounds__(kJoinThreads) void k_paged_join(PaArgs a, float shift) {
