@@ -469,7 +469,7 @@ __device__ void list_tokens(const Row &row, Shared &s, int n_some, u64 lo, u64 h
     for (; in_range; in_range &= in_range - 1) {
       const int b = __builtin_ctz(in_range);
       const u64 k = token_key(pick_of(l, b), first(q0 + (b >> 2) * kPickThreads) + (b & 3));
-      if (k >= lo && k < hi) s.list[atomicAdd(&fill, 1u)] = k;
+      if (k >= lo && k < hi) s.list[min(atomicAdd(&fill, 1u), kList - 1u)] = k;    // never more, by the histogram
     }
   }
   __syncthreads();
@@ -553,7 +553,7 @@ __device__ Found locate(const Row &row, Shared &s, int &turn, int search, Goal g
     if (!inside) return {before, 0};
     if (t == 0) s.n_few = 0;
     __syncthreads();
-    in_list([&](u64 k, Place) { s.few[atomicAdd(&s.n_few, 1u)] = k; });
+    in_list([&](u64 k, Place) { s.few[min(atomicAdd(&s.n_few, 1u), 63u)] = k; });
     few = s.few;
   }
   turn ^= 1;
