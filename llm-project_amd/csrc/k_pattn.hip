@@ -12,9 +12,9 @@
 // weighted values in the workspace, and k_paged_join puts a tile's parts together.
 // Waves never meet: with four of them on a tile, meeting in LDS at its end, 512 requests
 // of up to 300 f16 tokens (8 KV heads of 128, pages of 16) took 167 us, with shares of
-// their own 134 (100 with all that follows here).  Only for short tables and not too many
-// tiles a block of 8 waves takes a tile, a wave a part of its steps, and they do meet: one
-// launch instead of two (launch() has the rule and its figures).
+// their own 134 (98 with what follows; 89 again with waves that meet, without a second launch).  Only for short tables a block takes
+// a tile, a wave a part of its steps, and they do meet: one launch instead of two (launch()
+// has the rule and its figures).
 //
 // A wave keeps its running maximum, sum and outputs in registers, its queries in LDS, and
 // takes a step of 16 or 32 keys at a time straight from the pages into registers.
@@ -200,7 +200,7 @@ __device__ inline f4 mfma16(u4 a, u4 b, f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
 }
 
-// Waves that meet, as the registers allow.
+// Waves that meet at most, as the registers allow.
 constexpr int meeting(int hdp) { return hdp > 128 ? 4 : 8; }
 
 // What a type and a padded head size fix.
@@ -258,7 +258,8 @@ __global__ __launch_bounds__(MEET ? 64 * meeting(HDP) : kThreads, HDP > 128 ? 1 
   const int n = lane & 15, g = lane >> 4;           // key, query head or value piece; group of 16 lanes
   const int tiles = a.n_kv * a.tiles;
   char *q_lds = dyn + wave * (C::PARTS * a.rows * C::QROW);
-  float *parts = reinterpret_cast<float *>(dyn + C::MEETING * (C::PARTS * a.rows * C::QROW));     // of waves that meet
+  const int waves = blockDim.x >> 6;
+  float *parts = reinterpret_cast<float *>(dyn + waves * (C::PARTS * a.rows * C::QROW));          // of waves that meet
 
   // this wave's share of all steps; shares of one block lie far apart, so that few of
   // them are spread over the CUs
@@ -271,7 +272,7 @@ __global__ __launch_bounds__(MEET ? 64 * meeting(HDP) : kThreads, HDP > 128 ? 1 
     tile = blockIdx.x;
     len = __builtin_amdgcn_readfirstlane(len_of(r));
     steps = (len + STEP - 1) / STEP;
-    const int each = (steps + C::MEETING - 1) / C::MEETING;
+    const int each = (steps + waves - 1) / waves;
     from = wave * each;
     u = from;
     end = from + each < steps ? from + each : steps;
@@ -734,10 +735,10 @@ __global__ __launch_bounds__(MEET ? 64 * meeting(HDP) : kThreads, HDP > 128 ? 1 
     const int kvh = (int)blockIdx.x / a.tiles, part = (int)blockIdx.x - kvh * a.tiles;
     const int h0 = kvh * a.G + part * 16, rows = a.G - part * 16 < 16 ? a.G - part * 16 : 16;
     float *o = a.o + r * a.o_stride + (long long)h0 * a.hd, *lse = a.lse + r * a.lse_stride + h0;
-    const int each = (steps + C::MEETING - 1) / C::MEETING, n_parts = steps ? (steps + each - 1) / each : 0, one = a.hd + 2;
+    const int each = (steps + waves - 1) / waves, n_parts = steps ? (steps + each - 1) / each : 0, one = a.hd + 2;
     __syncthreads();
     if (n_parts == 1) return;
-    for (int i = threadIdx.x; i < rows * a.hd; i += 64 * C::MEETING) {
+    for (int i = threadIdx.x; i < rows * a.hd; i += 64 * waves) {
       const int row = i / a.hd, d = i - row * a.hd;
       const float *p = parts + row * one;
       float top = kNegInf, sum = 0.0f, x = 0.0f;
@@ -852,13 +853,18 @@ int launch(const char *fn, const PaArgs &a, hipStream_t stream) {
   const bool uni = a.page_size % 16 == 0, once = a.tiles == 1;
   const long long tiles = (long long)a.n_req * a.n_kv * a.tiles, room = ((long long)a.width * a.page_size + C::STEP - 1) / C::STEP;
   const size_t queries = (size_t)C::PARTS * a.rows * C::QROW, part = (size_t)a.rows * (a.hd + 2) * sizeof(float);
-  // Short tables: a block a tile, whose waves meet, and no second launch, where a wave takes
-  // few steps and the tiles few rounds of the chip.  Against shares, us: 32 bf16 requests of
-  // up to 120 tokens (hd 128, 8 KV heads) 7.2 / 11.8, 64 of 340 21.3 / 22.7, 128 of 120 22.8 / 20.3;
-  // one of 100 6.7 / 8.8, of 340 10.1 / 9.0 (idle CUs); 64 f32 ones of 340 (3 steps a wave) 32.7 /
-  // 30.8; hd 64, 24 f32 ones of 250 8.7 / 13.2, 64 bf16 ones of 340 11.0 / 17.1.
-  const long long each = (room + C::MEETING - 1) / C::MEETING;
-  const bool meet = each * HDP <= (tiles < 32 ? 128 : 256) && tiles <= 512 && C::MEETING * (queries + part) <= 64 * 1024;
+  // Short tables: a block a tile, whose waves meet, and no second launch: 8 waves while a CU
+  // has one tile at most, else 4, with a limit on the steps that a wave takes.  Against shares, us
+  // (8 KV heads, hd 128 if not said, lengths up to the number): bf16, 32 requests of 120 7.2 / 11.7, 64
+  // of 340 17.8 / 22.7 (8 waves 21.3), 64 of 900 34.1 / 35.7, 128 of 340 29.3 / 34.4, 512 of 900 201 / 213;
+  // 64 int8 ones of 340 15.9 / 21.7; hd 64, 24 f32 ones of 250 8.7 / 13.2, 128 of 450 30.6 / 35.3, 64 bf16 ones
+  // of 1900 (16 steps) 36.1 / 34.5.  One request leaves CUs idle: of 100 6.7 / 8.8, of 340 10.1 / 9.0.
+  // Among thousands of tiles whose waves have a step at most, or of int8, shares are better:
+  // 256 of 60 24.1 / 18.6, 512 int8 ones of 300 82 / 77.
+  const int waves = tiles > 256 ? 4 : C::MEETING;
+  const long long each = (room + waves - 1) / waves;
+  const bool few = tiles > 256 ? each <= 8 && each * HDP <= 1024 && (tiles <= 1024 || (each > 1 && T != QLLAMA_KV_I8)) : each * HDP <= (tiles < 32 ? 128 : 256);
+  const bool meet = few && a.n_req <= 65535 && waves * (queries + part) <= 64 * 1024;
   void (*f)(PaArgs);
   if (meet)
     f = uni ? once ? k_paged_attn<T, HDP, true, true, true> : k_paged_attn<T, HDP, true, false, true>
@@ -866,14 +872,14 @@ int launch(const char *fn, const PaArgs &a, hipStream_t stream) {
   else
     f = uni ? once ? k_paged_attn<T, HDP, true, true, false> : k_paged_attn<T, HDP, true, false, false>
             : once ? k_paged_attn<T, HDP, false, true, false> : k_paged_attn<T, HDP, false, false, false>;
-  const size_t lds = meet ? C::MEETING * (queries + part) : kWaves * queries;
+  const size_t lds = meet ? waves * (queries + part) : kWaves * queries;
   if (lds > 64 * 1024 &&              // past what a launch may take unasked
       hipFuncSetAttribute(reinterpret_cast<const void *>(f), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) != hipSuccess) {
     (void)hipGetLastError();
     return qs::refuse(fn, "hipFuncSetAttribute failed");
   }
   if (meet) {
-    QS_LAUNCH(fn, f, dim3(a.n_kv * a.tiles, a.n_req), dim3(64 * C::MEETING), lds, stream, a);
+    QS_LAUNCH(fn, f, dim3(a.n_kv * a.tiles, a.n_req), dim3(64 * waves), lds, stream, a);
     return 0;
   }
   QS_LAUNCH(fn, f, dim3(kBlocks), dim3(kThreads), lds, stream, a);

@@ -570,7 +570,7 @@ def test_attention_int8_scales_of_every_size(Q, page, order):
 
 @pytest.mark.parametrize("typ", ["f32", "f16", "bf16", "i8"])
 @pytest.mark.parametrize("H,KVH,hd", [(6, 2, 48), (8, 8, 64), (40, 2, 64), (32, 8, 128), (4, 1, 200)])
-@pytest.mark.parametrize("page,n", [(16, 1), (16, 20), (12, 20)])
+@pytest.mark.parametrize("page,n", [(16, 1), (16, 20), (12, 20), (16, 40)])
 def test_attention_of_short_and_of_long_tables(Q, typ, H, KVH, hd, page, n):
     """Lengths around those at which the waves of a block that takes a short request have one, two or more steps each."""
     r = random.Random(hd + n)
