@@ -14,8 +14,10 @@
 // returns without waiting, allocates nothing, keeps nothing between calls and may be
 // captured into a HIP graph.  The buffers' device need not be the current one; the
 // stream has to be on it.  Calls return 0, or print "Error: ..." and return nonzero
-// before anything is enqueued; none aborts.  Calls that overlap need workspaces of
-// their own.  What lies in device memory (lengths, tables, slots, settings) cannot be
+// before anything is enqueued (but for a launch that the runtime itself refuses: a
+// call's first kernel may have run by then, and its outputs are not to be used); none
+// aborts.  An error that an earlier HIP call has left behind is not looked at and stays.
+// Calls that overlap need workspaces of their own.  What lies in device memory (lengths, tables, slots, settings) cannot be
 // refused by the host: each call states what it does with values out of range, and
 // none of them makes it read or write outside its buffers.  Float sums are held in 32
 // bits or more and in a fixed order: equal inputs give equal bits.

@@ -9,8 +9,6 @@
 #include <cstdint>
 #include <cstdio>
 
-#include "qhip.h"
-#include "qhip_internal.h"
 #include "qserve.h"
 
 namespace qs {
@@ -75,13 +73,25 @@ inline const char *bad_cache(const QPagedKV *c) {
   return nullptr;
 }
 
+template <typename P>
+struct Same { using type = P; };         // a kernel's parameters follow from the kernel alone
+template <typename... P>
+inline hipError_t launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t shmem, hipStream_t stream, typename Same<P>::type... args) {
+  void *at[] = {&args...};
+  const hipError_t e = hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, at, shmem, stream);
+  if (e != hipSuccess) (void)hipGetLastError();      // told by the call's own return
+  return e;
+}
+
 }  // namespace qs
 
-// Launch on the caller's stream; on an error the enclosing entry point refuses.
-#define QS_LAUNCH(fn, kernel, grid, block, shmem, stream, ...)              \
-  do {                                                                      \
-    hipLaunchKernelGGL(kernel, grid, block, shmem, stream, __VA_ARGS__);    \
-    if (qh::check_launch(#kernel)) return qs::refuse(fn, qhip_last_error()); \
+// Launch on the caller's stream; on an error the enclosing entry point refuses.  The
+// launch's own result counts: the thread's last error may be that of an earlier call of
+// the caller's, and is left for the caller to find.
+#define QS_LAUNCH(fn, kernel, grid, block, shmem, stream, ...)                       \
+  do {                                                                               \
+    const hipError_t qs_e_ = qs::launch(kernel, grid, block, shmem, stream, __VA_ARGS__); \
+    if (qs_e_ != hipSuccess) return qs::refuse(fn, hipGetErrorString(qs_e_));        \
   } while (0)
 
 #endif
