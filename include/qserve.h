@@ -37,9 +37,9 @@ extern "C" {
 #define QLLAMA_KV_F32  0   // as LlamaKV holds it
 #define QLLAMA_KV_F16  1   // rounded to nearest even
 #define QLLAMA_KV_BF16 2   // rounded to nearest even
-#define QLLAMA_KV_I8   3   // int8 codes with a float scale per (slot, KV head): scale = max|x| * (1/127) (1 for a row of
-                           // zeros), code = x * (1/scale) rounded to nearest even, as quant.c:10-27 up to the last
-                           // bit of the scale
+#define QLLAMA_KV_I8   3   // int8 codes with a float scale per (slot, KV head), of either sign; the append's scale =
+                           // max|x| * (1/127) (1 for a row of zeros), code = x * (1/scale) rounded to nearest even, as
+                           // quant.c:10-27 up to the last bit of the scale
 
 // A view of memory the caller owns: n_pages pages of page_size slots.  Element d of
 // KV head h in slot s of page p is k[p * page_stride + h * head_stride + s *

@@ -489,7 +489,7 @@ __global__ __launch_bounds__(MEET ? 64 * meeting(HDP) : kThreads, HDP > 128 ? 1 
     const char *q_mine = q_lds + row * C::QROW;
 
     float m = kNegInf, l = 0.0f;                    // of the lane's query head; l over the lane's keys
-    // int8: weights times scales are held times 2^raise, which keeps the largest so far below
+    // int8: weights times scales are held times 2^raise, which keeps the largest magnitude so far below
     // 2^15 and within a factor of 2^16 of it or so, whatever the scales are
     int raise = kRaise;
     float slack = 0.0f;                             // what a larger score has left over of a factor of 2
@@ -622,7 +622,7 @@ __global__ __launch_bounds__(MEET ? 64 * meeting(HDP) : kThreads, HDP > 128 ? 1 
 #pragma unroll
         for (int i = 0; i < SUB; i++)
 #pragma unroll
-          for (int j = 0; j < 4; j++) most = fmaxf(most, p[i][j]);
+          for (int j = 0; j < 4; j++) most = fmaxf(most, fabsf(p[i][j]));      // a scale may be negative
         most = max_groups(most);
         const int room = 141 - (int)(__float_as_uint(most) >> 23);           // most < 2^(15 - room)
         if (__any(room < raise)) {                  // rare after the first step

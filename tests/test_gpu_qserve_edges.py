@@ -47,3 +47,30 @@ def attend_two_launches(Q):
     g = torch.Generator().manual_seed(2)
     kv = make_cache(Q, "f16", 130, 2, 16, 64, gen=g)
     return attend(Q, kv, torch.randn((1, 4, 64), generator=g), pages_for([2000], 16, 125, 130, 1), [2000])
+
+
+@pytest.mark.parametrize("page", [16, 20])
+@pytest.mark.parametrize("order", ["all", "mixed", "one", "up", "down"])
+def test_attention_int8_negative_scales(Q, page, order):
+    """A scale is the caller's number, of either sign: all of them negative, signs in turn, one enormous negative one among
+    small positive ones, and negative ones that run over sixty powers of ten.  The bound is the one of positive scales of
+    these sizes."""
+    H, KVH, hd, n = 8, 2, 64, 90
+    pages = -(-n // page)
+    kv = make_cache(Q, "i8", pages, KVH, page, hd, gen=torch.Generator().manual_seed(page))
+    slots = torch.arange(pages * page)
+    e = {"up": slots * 0.6 - 27.0, "down": 27.0 - slots * 0.6, "one": torch.where(slots == 40, 20.0, -5.0)}.get(order, slots * 0.0 - 1.5).double()
+    sign = {"mixed": 1.0 - 2.0 * (slots % 3 != 0), "one": torch.where(slots == 40, -1.0, 1.0)}.get(order, -torch.ones(len(slots)))
+    size = (10.0 ** e).float()
+    shape = lambda x: x.float().reshape(pages, 1, page).expand(pages, KVH, page).contiguous()  # noqa: E731
+    kv.v_scale.set(shape(size * sign))
+    kv.k_scale.set(kv.k_scale.get() * shape(sign))
+    sizes = Q.PagedKV(kv.k, kv.v, kv.k_scale, Dev(shape(size)))
+    q = torch.randn((2, H, hd), generator=torch.Generator().manual_seed(4))
+    table, lens = torch.arange(pages, dtype=torch.int32).expand(2, pages).contiguous(), [n, n - 7]
+    wo, wl, _, lb = attend_ref(kv, q, table, lens)
+    bound = attend_ref(sizes, q, table, lens, uneven=True)[2]
+    for t in (table, widened(table, page)):
+        o, lse = attend(Q, kv, q, t, lens)
+        assert bool(((o.double() - wo).abs() <= bound).all()), ((o.double() - wo).abs() - bound).max()
+        assert bool(((lse.double() - wl).abs() <= lb).all())
