@@ -756,9 +756,11 @@ def paged_append(cache, k, v, slots, q=None, q_out=None, positions=None, cos=Non
         qp, qs = _rows(q, "q", "float32", shape)
         op, os_ = _rows(q_out, "q_out", "float32", shape)
     if cos is not None:
-        n_pos = cos.shape[0]
         if sin is None or positions is None:
             raise ValueError("a rotation needs cos, sin and positions")
+        n_pos = cos.shape[0]
+        if cos.shape != (n_pos, hd // 2) or sin.shape != cos.shape:
+            raise ValueError(f"cos and sin must have the shape (positions, head_dim / 2), not {tuple(cos.shape)} and {tuple(sin.shape)}")
     sp, pp, bp = _flat("int32", (slots, "slots", rows), (positions, "positions", rows), (bad, "bad", 1))
     cp, np_ = _flat("float32", (cos, "cos", n_pos * hd // 2), (sin, "sin", n_pos * hd // 2))
     a = PAGED_ROWS.pack(rows, heads, qp, kp, vp, op, qs, ks, vs, os_, sp, pp, cp, np_, n_pos, bp)
