@@ -689,6 +689,9 @@ def _stream(stream):
 def _work(t):
     if not t.is_cuda:
         raise ValueError("work is not on the GPU")
+    contiguous = getattr(t, "is_contiguous", None)
+    if contiguous is not None and not contiguous():       # its number of elements would not be its memory's
+        raise ValueError("work is not contiguous")
     return t.data_ptr(), t.numel() * t.element_size()
 
 

@@ -39,3 +39,15 @@ def test_tables_of_another_shape_are_refused(cos, sin):
     i = on_gpu(3, dtype=torch.int32)
     with pytest.raises(ValueError, match="positions, head_dim / 2"):
         Q.paged_append(paged_kv(), on_gpu(3, 2, 64), on_gpu(3, 2, 64), i, positions=i, cos=on_gpu(*cos), sin=on_gpu(*sin), stream=0)
+
+
+@pytest.mark.parametrize("call", ["attention", "sample"])
+def test_a_workspace_that_is_larger_than_its_memory_is_refused(call):
+    """An expanded tensor has more elements than bytes behind it."""
+    work = OnGpu(torch.zeros(1, dtype=torch.uint8).expand(1 << 28))
+    i = on_gpu(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="work is not contiguous"):
+        if call == "sample":
+            Q.sample_rows(on_gpu(2, 100), on_gpu(2), i, work, stream=0)
+        else:
+            Q.paged_attention(paged_kv(), on_gpu(2, 4, 64), on_gpu(2, 3, dtype=torch.int32), i, on_gpu(2, 4, 64), work, stream=0)
