@@ -128,7 +128,7 @@ int qllama_paged_append(const QPagedKV *c, const QPagedRows *r, void *stream);
 // For every request r and query head h (of KV head h / (n_heads / n_kv)), over the
 // cached tokens j < lens[r]: o = sum_j w_j v_j, w = softmax_j(scale * q . k_j), and lse
 // = ln sum_j e^(scale * q . k_j) (lse may be NULL).  Token j lies in slot j mod
-// page_size of page table[r][j / page_size].  scale 0 stands for 1 / sqrt(head_dim).
+// page_size of page table[r][j / page_size].  scale 0 stands for 1 / sqrt(head_dim); up to 2.35e38.
 // lens[r] <= 0 gives o = 0 and lse = -inf; lengths above width * page_size count as
 // that; tokens of a page outside the cache are left out.  What lies in slots behind a
 // request's tokens, NaN included, has no effect.  Products and sums in 32 bits: a

@@ -924,7 +924,8 @@ extern "C" int qllama_paged_attention(const QPagedKV *c, const QPagedQuery *a, v
     return qs::refuse(fn, "bad table width (width * page_size must be below 2^31 - 64) or stride");
   if ((int64_t)a->n_req * (((int64_t)a->width * c->page_size + 15) / 16) > INT_MAX)
     return qs::refuse(fn, "n_req * width * page_size is too large");
-  if (!(a->scale >= 0.0f) || a->scale > 3.0e38f) return qs::refuse(fn, "scale must be finite and not negative");
+  if (!(a->scale >= 0.0f) || a->scale > 2.35e38f)      // times log2 e within a float's range
+    return qs::refuse(fn, "scale must be 0 .. 2.35e38");
   if (a->q == a->o) return qs::refuse(fn, "o must not be q");
   if (qs::misaligned(a->q, 4) || qs::misaligned(a->o, 4) || qs::misaligned(a->lse, 4) || qs::misaligned(a->table, 4) || qs::misaligned(a->lens, 4))
     return qs::refuse(fn, "a buffer is not aligned to its elements");

@@ -2,7 +2,7 @@
 import pytest
 
 import qlib
-from test_qserve import A
+from test_qserve import A, CALLS
 
 torch = pytest.importorskip("torch")
 Q = qlib.load()
@@ -51,3 +51,13 @@ def test_a_workspace_that_is_larger_than_its_memory_is_refused(call):
             Q.sample_rows(on_gpu(2, 100), on_gpu(2), i, work, stream=0)
         else:
             Q.paged_attention(paged_kv(), on_gpu(2, 4, 64), on_gpu(2, 3, dtype=torch.int32), i, on_gpu(2, 4, 64), work, stream=0)
+
+
+@pytest.mark.skipif(qlib.gpu_available(), reason="the calls that are not refused would run")
+def test_scales_up_to_the_last_one_whose_base_two_form_is_finite(capfd):
+    """Scores are formed in base two: a scale times log2 e above a float's range would make a score of 0 a NaN."""
+    for scale in (2.4e38, 2.9e38, 3e38):
+        assert CALLS["query"]({"scale": scale}) != 0
+        assert "scale must" in capfd.readouterr().err
+    assert CALLS["query"]({"scale": 2.3e38}) != 0
+    assert "no GPU" in capfd.readouterr().err
