@@ -221,9 +221,10 @@ struct Cfg {
   // a query row in LDS: a part's values, and 64 bytes that spread rows over the banks
   static constexpr int QES = T == QLLAMA_KV_F32 ? 4 : 2;
   static constexpr int QROW = HDP * QES + 64;
-  // 2^SHIFT times the weights: f16 parts then keep 22 bits down to 2^-18 of the largest
-  // weight and the rest to 2^-40
-  static constexpr float SHIFT = T == QLLAMA_KV_F16 ? 15.0f : 0.0f;
+  // what weights are held times in the products: f16 parts then keep 22 bits down to 2^-18
+  // of the largest weight and the rest to 2^-40.  Not in the exponent, where a 15 beside a
+  // small score takes 2^-21 of the weight and of lse.
+  static constexpr float RAISED = T == QLLAMA_KV_F16 ? 32768.0f : 1.0f;
 };
 
 template <int T, int HDP>
@@ -607,7 +608,7 @@ __global__ __launch_bounds__(MEET ? 64 * meeting(HDP) : kThreads, HDP > 128 ? 1 
         for (int c = 0; c < DPL; c++) acc[c] *= by;
         m = top;
       }
-      const float ref = (m == kNegInf ? 0.0f : m) - C::SHIFT;
+      const float ref = m == kNegInf ? 0.0f : m;
       float p[SUB][4];
 #pragma unroll
       for (int i = 0; i < SUB; i++)
@@ -616,6 +617,7 @@ __global__ __launch_bounds__(MEET ? 64 * meeting(HDP) : kThreads, HDP > 128 ? 1 
           p[i][j] = __builtin_amdgcn_exp2f(sc[i][j] - ref);
           l += p[i][j];
           if constexpr (T == QLLAMA_KV_I8) p[i][j] *= f.v[i][j];
+          else p[i][j] *= C::RAISED;
         }
       if constexpr (T == QLLAMA_KV_I8) {            // into f16's range
         float most = 0.0f;
@@ -697,6 +699,7 @@ __global__ __launch_bounds__(MEET ? 64 * meeting(HDP) : kThreads, HDP > 128 ? 1 
     // lane (n, g) holds head n; acc[c][i] is dim c mod PD of the piece of lane 4 g + i
     const bool whole = from == 0 && to == steps;
     const auto put = [&](float *o, float by) {
+      by *= 1.0f / C::RAISED;
 #pragma unroll
       for (int i = 0; i < 4; i++)
 #pragma unroll
@@ -713,7 +716,7 @@ __global__ __launch_bounds__(MEET ? 64 * meeting(HDP) : kThreads, HDP > 128 ? 1 
     if (n < rows) {
       if (whole) {
         put(a.o + r * a.o_stride + (long long)(h0 + row) * a.hd, l == 0.0f ? 0.0f : 1.0f / l);
-        if (g == 0 && a.lse) a.lse[r * a.lse_stride + h0 + row] = l == 0.0f ? kNegInf : (m - C::SHIFT + __builtin_amdgcn_logf(l)) * 0.69314718056f;
+        if (g == 0 && a.lse) a.lse[r * a.lse_stride + h0 + row] = l == 0.0f ? kNegInf : (m + __builtin_amdgcn_logf(l)) * 0.69314718056f;
       } else if constexpr (MEET) {
         float *o = parts + wave * (a.rows * (a.hd + 2)) + row * (a.hd + 2);
         put(o, 1.0f);
@@ -749,7 +752,7 @@ __global__ __launch_bounds__(MEET ? 64 * meeting(HDP) : kThreads, HDP > 128 ? 1 
         x += p[j * a.rows * one + d] * f;
       }
       o[i] = sum == 0.0f ? 0.0f : x * (1.0f / sum);
-      if (d == 0 && a.lse) lse[row] = sum == 0.0f ? kNegInf : (top - C::SHIFT + __builtin_amdgcn_logf(sum)) * 0.69314718056f;
+      if (d == 0 && a.lse) lse[row] = sum == 0.0f ? kNegInf : (top + __builtin_amdgcn_logf(sum)) * 0.69314718056f;
     }
     return;
   }
@@ -769,7 +772,7 @@ __global__ __launch_bounds__(MEET ? 64 * meeting(HDP) : kThreads, HDP > 128 ? 1 
 // tiles of 67 parts, 7.3 at 64 ragged requests (512 tiles of some 4 parts), 12.3 where
 // 2048 shares make 16 tiles.
 constexpr int kJoinThreads = 256, kAhead = 4;
-__global__ __launch_bounds__(kJoinThreads) void k_paged_join(PaArgs a, float shift) {
+__global__ __launch_bounds__(kJoinThreads) void k_paged_join(PaArgs a) {
   __shared__ float weight[kShares], lds[kJoinThreads / 32][256], red[2][kJoinThreads / 64];
   const int4 s = a.split[blockIdx.x];
   const int parts = s.x, r = s.y, tile = s.z, row = blockIdx.y;
@@ -839,7 +842,7 @@ __global__ __launch_bounds__(kJoinThreads) void k_paged_join(PaArgs a, float shi
     for (int j = 0; j < groups; j++) x += lds[j][i];
     a.o[r * a.o_stride + (long long)h * a.hd + i] = x * by;
   }
-  if (threadIdx.x == 0 && a.lse) a.lse[r * a.lse_stride + h] = sum == 0.0f ? kNegInf : (top - shift + __builtin_amdgcn_logf(sum)) * 0.69314718056f;
+  if (threadIdx.x == 0 && a.lse) a.lse[r * a.lse_stride + h] = sum == 0.0f ? kNegInf : (top + __builtin_amdgcn_logf(sum)) * 0.69314718056f;
 }
 
 int rows_of(const QPagedKV *c, int n_heads) {
@@ -886,7 +889,7 @@ int launch(const char *fn, const PaArgs &a, hipStream_t stream) {
   // shares that can hold a step, by the room of the tables
   const long long most = tiles * room;
   const int shares = most / kMinShare + 1 < kShares ? (int)(most / kMinShare + 1) : kShares;
-  QS_LAUNCH(fn, k_paged_join, dim3(shares, a.rows), dim3(kJoinThreads), 0, stream, a, (float)C::SHIFT);
+  QS_LAUNCH(fn, k_paged_join, dim3(shares, a.rows), dim3(kJoinThreads), 0, stream, a);
   return 0;
 }
 

@@ -74,3 +74,25 @@ def test_attention_int8_negative_scales(Q, page, order):
         o, lse = attend(Q, kv, q, t, lens)
         assert bool(((o.double() - wo).abs() <= bound).all()), ((o.double() - wo).abs() - bound).max()
         assert bool(((lse.double() - wl).abs() <= lb).all())
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16", "i8"])
+def test_attention_lse_of_small_scores(Q, typ):
+    """One token whose score is small: its log-sum-exp is the score.  q and k are powers of two, so that the score is exact but
+    for its way through base two: log2 e as a float (EPS), that in two 16-bit floats (2 EPS: off by 2^-23), and back (the
+    constant and the product, 2 EPS).  The logarithm of a sum of one weight is 0."""
+    H, KVH, hd = 4, 2, 64
+    kv = make_cache(Q, typ, 2, KVH, 16, hd)
+    kv.k.set(torch.zeros_like(kv.k.host))
+    k = kv.k.host.clone()
+    k[:, :, 0, 3] = 1
+    kv.k.set(k)
+    if typ == "i8":
+        kv.k_scale.set(torch.ones_like(kv.k_scale.host))
+    q = torch.zeros((6, H, hd))
+    score = torch.tensor([2.0 ** -3, 2.0 ** -6, -2.0 ** -6, 2.0 ** -9, 2.0 ** -12, -2.0 ** -15])
+    q[:, :, 3] = score[:, None]
+    table = torch.zeros((6, 1), dtype=torch.int32)
+    for t in (table, widened(table, 16)):
+        _, lse = attend(Q, kv, q, t, [1] * 6, scale=1.0)
+        assert bool(((lse.double() - score.double()[:, None]).abs() <= 5 * EPS * score.abs().double()[:, None]).all()), lse
