@@ -133,7 +133,7 @@ int qllama_paged_append(const QPagedKV *c, const QPagedRows *r, void *stream);
 // that; tokens of a page outside the cache are left out.  What lies in slots behind a
 // request's tokens, NaN included, has no effect.  Products and sums in 32 bits: a
 // 16-bit or int8 row enters a product as it is, a query or a weight (int8: times its
-// value's scale) as two or three 16-bit parts that together hold 22 (f16 and int8
+// value's scale) as two or three 16-bit parts that together hold 23 (f16 and int8
 // caches; a weight at least 2^-37 of the largest) or 24 bits.  A cached infinity gives NaN.
 // width * page_size has to be below 2^31 - 64.  work: qllama_paged_attention_work bytes,
 // 16-byte aligned.

@@ -53,6 +53,7 @@
 
 namespace {
 
+typedef float f2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
@@ -160,8 +161,9 @@ __device__ inline uint32_t codes(uint32_t y, uint32_t x) {
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(u, h2{32768.0f16, 32768.0f16}, h2{-0.25f16, -0.25f16}));
 }
 
-// Parts of a float operand of 8 values: sums of the parts are the values (bf16: 24
-// bits by cutting, f16: 22 by rounding to zero).
+// Parts of a float operand of 8 values: sums of the parts are the values (bf16: all 24
+// bits by cutting; f16: to nearest twice, off by 2^-23 at most and without a bias, where
+// cutting twice takes up to 3 x 2^-23).
 struct Parts3 { u4 p[3]; };
 __device__ inline Parts3 cut3(const float (&x)[8]) {
   Parts3 r;
@@ -184,8 +186,8 @@ __device__ inline Parts2 cut2(const float (&x)[8]) {
   Parts2 r;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
-    const h2 hi = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(x[2 * i], x[2 * i + 1]));
-    const h2 lo = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(x[2 * i] - (float)hi.x, x[2 * i + 1] - (float)hi.y));
+    const h2 hi = __builtin_convertvector(f2{x[2 * i], x[2 * i + 1]}, h2);
+    const h2 lo = __builtin_convertvector(f2{x[2 * i] - (float)hi.x, x[2 * i + 1] - (float)hi.y}, h2);
     r.p[0][i] = __builtin_bit_cast(uint32_t, hi);
     r.p[1][i] = __builtin_bit_cast(uint32_t, lo);
   }
@@ -221,7 +223,7 @@ struct Cfg {
   // a query row in LDS: a part's values, and 64 bytes that spread rows over the banks
   static constexpr int QES = T == QLLAMA_KV_F32 ? 4 : 2;
   static constexpr int QROW = HDP * QES + 64;
-  // what weights are held times in the products: f16 parts then keep 22 bits down to 2^-18
+  // what weights are held times in the products: f16 parts then keep 23 bits down to 2^-17
   // of the largest weight and the rest to 2^-40.  Not in the exponent, where a 15 beside a
   // small score takes 2^-21 of the weight and of lse.
   static constexpr float RAISED = T == QLLAMA_KV_F16 ? 32768.0f : 1.0f;

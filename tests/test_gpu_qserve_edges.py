@@ -96,3 +96,25 @@ def test_attention_lse_of_small_scores(Q, typ):
     for t in (table, widened(table, 16)):
         _, lse = attend(Q, kv, q, t, [1] * 6, scale=1.0)
         assert bool(((lse.double() - score.double()[:, None]).abs() <= 5 * EPS * score.abs().double()[:, None]).all()), lse
+
+
+def test_attention_int8_keeps_a_scale_to_23_bits(Q):
+    """One token: the output is its code times its scale.  The scale enters the product as two 16-bit floats, each rounded to
+    nearest: the first is off by half a step of 11 bits, 2^-11 of the scale's power of two, the second by half a step of 11
+    bits of that, 2^-23; the products' sum is rounded once (2^-23 if that is cut off).  Scales whose last bits make two floats
+    that are cut off differ by 3 x 2^-23 are among them."""
+    KVH, hd, n = 2, 64, 64
+    g = torch.Generator().manual_seed(3)
+    kv = make_cache(Q, "i8", n, KVH, 16, hd, gen=g)
+    r = np.random.default_rng(1)
+    m = r.integers(0, 1 << 23, (n, KVH)).astype(np.uint32)
+    m[:8] = (1 << 12) * np.arange(1, 9)[:, None] + 3
+    m[8:16] = 0x7fffff
+    scale = torch.zeros((n, KVH, 16))
+    scale[:, :, 0] = torch.from_numpy((m + np.uint32(0x3f800000)).view(np.float32).copy()) * torch.tensor([0.5, 0.03125] * (n // 2))[:, None]
+    kv.v_scale.set(scale)
+    table = torch.arange(n, dtype=torch.int32)[:, None].contiguous()
+    want = (kv.v.get()[:, :, 0].double() * scale[:, :, 0, None].double())
+    for t in (table, widened(table, 16)):
+        o, _ = attend(Q, kv, torch.randn((n, KVH, hd), generator=g), t, [1] * n)
+        assert bool(((o.double() - want).abs() <= 2.0 ** -22 * want.abs()).all()), ((o.double() - want).abs() / want.abs().clamp(min=1e-30)).max()
