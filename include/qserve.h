@@ -169,8 +169,9 @@ int qllama_test_page_of(const int32_t *table, int width, int page_size, int n_pa
 // counts as the nearest inside, NaN as 0; a NaN setting is no limit.  Logits of -inf
 // and NaN are masked: never kept; a row with nothing else gives token -1, kept 0 and
 // prob 0.  Logits of +inf share the row between them.
-// Sums and comparisons in 64 bits (each e to 2^-39 of the largest), so a token differs
-// from sample_token's only where that one's float rounding decides.
+// Sums and comparisons in 64 bits (each e to 2^-37 + 2^-52 |l_0| / temperature of the
+// largest), so a token differs from sample_token's only where that one's float rounding
+// decides.
 // prob: the token's probability among the kept ones; kept: n.  Both may be NULL.  The
 // settings' arrays may be NULL: temperature 1, no limit.  work: qllama_sample_rows_work
 // bytes, 16-byte aligned.
@@ -188,6 +189,9 @@ typedef struct {
 } QSampleRows;
 int qllama_sample_rows(const QSampleRows *s, void *stream);
 size_t qllama_sample_rows_work(int rows, int vocab);
+// The weight e of a token among its row's sums, in units of which the largest logit has 2^43
+// to 1.045 times that (host arithmetic, as the kernels').  For tests.
+unsigned long long qllama_test_sample_weight(float logit, float top, float temperature);
 
 #ifdef __cplusplus
 }

@@ -65,11 +65,11 @@ __device__ inline u64 smallest_key(float l) { return token_key(l, 0xfffff); }   
 // series (the seventh is 2^-6 at most), and 2^52 whose addition rounds
 struct Series {
   double a[6];
-  __device__ inline Series() {
+  __host__ __device__ inline Series() {
     constexpr double x = 0.69314718055994530942 / kGrid, s = (double)(1ull << kFractionBits);
     a[0] = s * x; a[1] = a[0] * x / 2; a[2] = a[1] * x / 3; a[3] = a[2] * x / 4; a[4] = a[3] * x / 5; a[5] = a[4] * x / 6;
   }
-  __device__ inline u64 operator()(double f) const {
+  __host__ __device__ inline u64 operator()(double f) const {
     double s = a[5];
 #pragma unroll
     for (int i = 4; i >= 0; i--) s = fma(s, f, a[i]);
@@ -80,16 +80,16 @@ struct Series {
 // A token below `top`: its cell's distance from top's (kBins: past the last) and f.  per: 16
 // log2(e) / T.  Tokens equal to top share its cell whatever it is, infinity too.
 struct Place { int bin; double f; };
-__device__ inline Place place_of(float l, float top, double cell_top, double per) {
+__host__ __device__ inline Place place_of(float l, float top, double cell_top, double per) {
   const double u = (double)l * per, cell = floor(u), d = cell_top - cell;
   if (l == top && !(u - cell >= 0.0)) return {0, 0.0};
   return {d < kBins ? (int)d : kBins, u - cell};
 }
-__device__ inline double cell_of(float l, double per) { return floor((double)l * per); }
+__host__ __device__ inline double cell_of(float l, double per) { return floor((double)l * per); }
 
 // 2^(5 - bin / 16): a histogram's 2^-38 as units of 2^-43, and the cell's weight.  The
 // sixteenths by the exponential's series (0.65^16 / 16! is 5e-17).
-__device__ inline double scale_of(int bin) {
+__host__ __device__ inline double scale_of(int bin) {
   const double x = (bin & 15) * (-0.69314718055994530942 / kGrid);
   double s = 1.0 / 1307674368000.0;
   s = fma(s, x, 1.0 / 87178291200.0);
@@ -111,12 +111,14 @@ __device__ inline double scale_of(int bin) {
 }
 // n tokens of a cell, x of whose fractions: their weight in units.  In bin 0 exact, so
 // equal largest logits weigh alike, alone and together; elsewhere rounded.
-__device__ inline u64 units(int bin, double scale, u64 n, u64 x) {
+__host__ __device__ inline u64 units(int bin, double scale, u64 n, u64 x) {
   const u64 raw = (n << kFractionBits) + x;
   return bin == 0 ? raw << (kUnitBits - kFractionBits) : (u64)((double)raw * scale + 0.5);
 }
 // A token's weight unrounded, in units
 __device__ inline double weight(Place p) { return exp2(kUnitBits + (p.f - p.bin) * (1.0 / kGrid)); }
+
+__host__ __device__ inline double per_of(float temperature) { return kGrid * kLog2e / (double)temperature; }
 
 // What one row asks for.
 struct Ask {
@@ -125,7 +127,7 @@ struct Ask {
 };
 __device__ inline Ask ask_of(const QSampleRows &a, int r) {
   const float T = a.temperature ? a.temperature[r] : 1.0f;
-  return {kGrid * kLog2e / (double)T, !(T > 0.0f)};
+  return {per_of(T), !(T > 0.0f)};
 }
 
 struct Mass { u64 w; uint32_t n; };
@@ -707,6 +709,12 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(QSampleRows a, int
 extern "C" size_t qllama_sample_rows_work(int rows, int vocab) {
   if (rows < 0 || rows > 65535 || vocab < 1 || vocab > (1 << 20)) return 0;
   return 16 + (size_t)rows * ((vocab + kSlice - 1) / kSlice) * (kBins * sizeof(u64) + sizeof(Slice) + kSliceGroups * sizeof(float));
+}
+
+extern "C" unsigned long long qllama_test_sample_weight(float logit, float top, float temperature) {
+  const double per = per_of(temperature);
+  const Place p = place_of(logit, top, cell_of(top, per), per);
+  return p.bin < kBins ? units(p.bin, scale_of(p.bin), 1, Series()(p.f)) : 0;
 }
 
 extern "C" int qllama_sample_rows(const QSampleRows *s, void *stream) {

@@ -1,4 +1,8 @@
 """Calls of the serving operators' Python mirror and C ABI that must be refused before any device work, without a GPU."""
+import ctypes as C
+import decimal
+
+import numpy as np
 import pytest
 
 import qlib
@@ -61,3 +65,27 @@ def test_scales_up_to_the_last_one_whose_base_two_form_is_finite(capfd):
         assert "scale must" in capfd.readouterr().err
     assert CALLS["query"]({"scale": 2.3e38}) != 0
     assert "no GPU" in capfd.readouterr().err
+
+
+@pytest.mark.parametrize("top", [0.0, 0.7, 20.0, -20.0, 333.25, 1e6, -1e6, 1e9, 2.0 ** 40])
+@pytest.mark.parametrize("temperature", [0.001, 0.7, 1.0, 3.0, 64.0, 1e6])
+def test_weights_of_sampled_tokens(top, temperature):
+    """e of a token against 60 digits: off by 2^-37 + 2^-52 |top| / temperature of the largest at most, as documented.
+
+    The first part: both tokens' fractions of a cell are rounded to 2^-38 (2^-39 each), their series ends behind 2^-44, and
+    each is rounded to 2^-43; 2 (2^-39 + 2^-43) in all.  The second: the grid's place of a logit, 16 log2(e) l / T, is a product
+    rounded to 2^-53 of itself, and an error of it counts ln 2 / 16 times; for the top and a token near it 2 x 2^-53 |top| / T, and a
+    token far from it weighs little.  The factor's own rounding counts (l_0 - l) / T 2^-52 e^-((l_0 - l) / T) < 2^-53."""
+    t = np.float32(temperature)
+    rng, l0 = np.random.default_rng(int(temperature * 1000)), np.float32(top)
+    x = np.float32(np.float64(l0) - float(t) * np.concatenate([rng.random(150) * 3.0, rng.random(150) * 30.0]))
+    f = Q.lib().qllama_test_sample_weight
+    f.argtypes, f.restype = [C.c_float] * 3, C.c_ulonglong
+    whole = f(l0, l0, t)
+    assert 2 ** 43 <= whole < 1.045 * 2 ** 43
+    with decimal.localcontext(decimal.Context(prec=60)):
+        bound = decimal.Decimal(2) ** -37 + decimal.Decimal(2) ** -52 * abs(decimal.Decimal(float(l0))) / decimal.Decimal(float(t))
+        for l in x:
+            e = ((decimal.Decimal(float(l)) - decimal.Decimal(float(l0))) / decimal.Decimal(float(t))).exp()
+            off = abs(decimal.Decimal(f(l, l0, t)) / whole - e)
+            assert off <= bound, (l, off / bound)
