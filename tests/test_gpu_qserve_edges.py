@@ -118,3 +118,16 @@ def test_attention_int8_keeps_a_scale_to_23_bits(Q):
     for t in (table, widened(table, 16)):
         o, _ = attend(Q, kv, torch.randn((n, KVH, hd), generator=g), t, [1] * n)
         assert bool(((o.double() - want).abs() <= 2.0 ** -22 * want.abs()).all()), ((o.double() - want).abs() / want.abs().clamp(min=1e-30)).max()
+
+
+@pytest.mark.parametrize("typ", ["f32", "f16", "bf16", "i8"])
+def test_attention_equal_requests_give_equal_bits(Q, typ):
+    """Short tables: a block takes a tile, so equal requests are equal work, and give equal bits."""
+    g = torch.Generator().manual_seed(14)
+    kv = make_cache(Q, typ, 12, 2, 32, 128, "head", g)
+    table = torch.tensor([[0, 1, 2, 3], [0, 1, 4, 5], [0, 1, 2, 3], [7, 7, 7, 7]], dtype=torch.int32)
+    q = torch.randn((4, 4, 128), generator=g)
+    q[2] = q[0]
+    o, lse = attend(Q, kv, q, table, [128, 100, 128, 97])
+    assert torch.equal(o[0], o[2]) and torch.equal(lse[0], lse[2])
+    assert not torch.equal(o[0], o[1])
