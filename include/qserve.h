@@ -7,9 +7,12 @@
 // need and names each new row's slot and position; qllama_paged_append rotates the
 // rows' queries and keys and stores keys and values in their slots;
 // qllama_paged_attention lets the newest token of every request attend to its pages;
-// qllama_sample_rows draws a token from every row of logits.
+// qllama_sample_rows draws a token from every row of logits.  The model's products between
+// them may be qmatmul_device_noalloc's: that one always enqueues on qllama_stream(), with
+// which no other stream is ordered, so that such a step runs on that stream as a whole or
+// orders its own with it by events.
 //
-// All pointers are DEVICE memory unless stated otherwise.  Every call enqueues on the
+// All pointers are DEVICE memory, of one device in a call, unless stated otherwise.  Every call enqueues on the
 // hipStream_t it is given (0 is HIP's default stream, qllama_stream() the library's),
 // returns without waiting, allocates nothing, keeps nothing between calls and may be
 // captured into a HIP graph.  The buffers' device need not be the current one; the

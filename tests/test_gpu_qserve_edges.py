@@ -131,3 +131,110 @@ def test_attention_equal_requests_give_equal_bits(Q, typ):
     o, lse = attend(Q, kv, q, table, [128, 100, 128, 97])
     assert torch.equal(o[0], o[2]) and torch.equal(lse[0], lse[2])
     assert not torch.equal(o[0], o[1])
+
+
+def test_a_step_with_the_models_products_between(Q):
+    """The step as a model's layer makes it, with nothing waited for: rows of q, k and v from an int8 product, plan, append,
+    attention, the output's product, logits, sampling.  The products run on the library's stream, so the calls do too."""
+    L = Q.lib()
+    L.qmatmul_device_noalloc.argtypes = [C.c_void_p, C.c_int, C.POINTER(Q.QTensor), C.c_void_p]
+    H, KVH, hd, n, D, V = 8, 2, 64, 5, 256, 500
+    r = np.random.default_rng(8)
+    weights = [(r.standard_normal(s) * 0.05).astype(np.float32) for s in ((D, (H + 2 * KVH) * hd), (H * hd, D), (D, V))]
+    W = [Q.QWeight(w) for w in weights]
+    x = r.standard_normal((n, D)).astype(np.float32)
+    s = Server(Q, rows=n, seed=2)
+    dx, dy = Dev(torch.from_numpy(x)), Dev(torch.zeros((n, D)))
+
+    def product(a, w, out):
+        assert L.qmatmul_device_noalloc(a.data_ptr(), n, C.byref(w.t), out.data_ptr()) == 0
+
+    try:
+        for step in range(6):
+            s.feed(step, [1] * n)
+            assert L.qllama_device_sync() == 0
+            product(dx, W[0], s.qkv)
+            s.store()
+            s.answer(s.q)
+            product(s.o, W[1], dy)
+            product(dy, W[2], s.logits)
+            s.sample()
+            assert L.qllama_sync() == 0
+            # each product on the values that the call before it left, through the host entry point
+            assert np.array_equal(s.qkv.get().numpy().reshape(n, -1), Q.qmatmul(x, W[0]))
+            y = Q.qmatmul(s.o.get().numpy().reshape(n, -1), W[1])
+            assert np.array_equal(dy.get().numpy(), y) and np.array_equal(s.logits.get().numpy(), Q.qmatmul(y, W[2]))
+            lens = s.lens.get().tolist()
+            assert lens == [step + 1] * n and s.slots.get().min() >= 0
+            wo, _, bound, _ = attend_ref(s.kv, s.q.get(), s.table.get(), lens)
+            assert bool(((s.o.get().double() - wo).abs() <= bound).all())
+            token, u = s.token.get().tolist(), s.u.get().tolist()
+            for i in range(n):
+                want = sample_ref(s.logits.host.numpy()[i], float(np.float32(0.9)), 50, float(np.float32(0.9)), float(np.float32(0.01)), u[i])
+                assert token[i] == want[0]
+            s.next()
+    finally:
+        for w in W:
+            w.close()
+
+
+PRODUCTS_CHILD = """
+import ctypes as C, sys
+import numpy as np, torch
+sys.path.insert(0, "tests")
+import qlib
+Q = qlib.load()
+L = Q.lib()
+L.qmatmul_device_noalloc.argtypes = [C.c_void_p, C.c_int, C.POINTER(Q.QTensor), C.c_void_p]
+n, D, H, KVH, hd, page = 7, 256, 8, 2, 64, 16
+r = np.random.default_rng(3)
+W = [Q.QWeight((r.standard_normal(s) * 0.05).astype(np.float32)) for s in ((D, (H + 2 * KVH) * hd), (H * hd, D))]
+product = lambda a, w, out: L.qmatmul_device_noalloc(a.data_ptr(), n, C.byref(w.t), out.data_ptr())
+stream = torch.cuda.ExternalStream(L.qllama_stream())
+stream.wait_stream(torch.cuda.current_stream())
+with torch.cuda.stream(stream):
+    s = torch.cuda.current_stream().cuda_stream
+    i32 = lambda *d: torch.zeros(d, dtype=torch.int32, device="cuda")
+    kv = Q.PagedKV(*(torch.zeros((9, KVH, page, hd), dtype=torch.bfloat16, device="cuda") for _ in range(2)))
+    table, ring, state, cached, added = i32(n, 2), torch.arange(9, dtype=torch.int32, device="cuda"), i32(2), i32(n), i32(n) + 1
+    state[1] = 9
+    lens, status, starts, state_out, slots, positions, requests = i32(n), i32(n), i32(n + 1), i32(2), i32(n), i32(n), i32(n)
+    cos, sin = torch.ones((32, hd // 2), device="cuda"), torch.zeros((32, hd // 2), device="cuda")
+    work = torch.empty(Q.paged_attention_work(kv, n, H), dtype=torch.uint8, device="cuda")
+    seen = []
+    for step in range(4):                    # nothing is waited for: torch's work, the products and the calls follow each other
+        x = torch.full((n, D), 0.001 * (step + 1), device="cuda") * torch.arange(D, device="cuda")
+        qkv, o, y = torch.empty((n, H + 2 * KVH, hd), device="cuda"), torch.empty((n, H, hd), device="cuda"), torch.empty((n, D), device="cuda")
+        assert product(x, W[0], qkv) == 0
+        Q.paged_plan(cached, added, table, ring, state, page, lens, status, starts, state_out, slots, positions, requests, stream=s)
+        q, k, v = qkv.split([H, KVH, KVH], 1)
+        Q.paged_append(kv, k, v, slots, q=q, q_out=q, positions=positions, cos=cos, sin=sin, stream=s)
+        Q.paged_attention(kv, q, table, lens, o, work, stream=s)
+        assert product(o, W[1], y) == 0
+        cached, state = lens.clone(), state_out.clone()
+        seen.append((x, qkv, o, y * 1.0))
+stream.synchronize()
+values = []
+for x, qkv, o, y in seen:
+    x, qkv, o, y = (t.cpu().numpy() for t in (x, qkv, o, y))
+    assert np.array_equal(qkv.reshape(n, -1), Q.qmatmul(x, W[0])) and np.array_equal(y, Q.qmatmul(o.reshape(n, -1), W[1]))
+    values.append(torch.from_numpy(qkv).bfloat16().double().numpy()[:, H + KVH:])
+    k = torch.from_numpy(np.stack([t[1].cpu().numpy() for t in seen[:len(values)]])).bfloat16().double()[:, :, H:H + KVH]
+    for h in range(H):                       # the rotation is none here; a weight is off by 200 EPS sum |q k| / 8 = 5e-5 at most
+        w = torch.softmax(torch.from_numpy(qkv).double()[None, :, h].mul(k[:, :, h // 4]).sum(-1) / 8.0, 0)
+        want = (w[..., None] * torch.from_numpy(np.stack(values))[:, :, h // 4]).sum(0)
+        assert (torch.from_numpy(o).double()[:, h] - want).abs().max() <= 1e-4 * max(1.0, want.abs().max().item())
+print("steps", len(seen))
+"""
+
+
+def in_torch(code):
+    """What a process prints that has loaded torch's HIP runtime first."""
+    done = subprocess.run([sys.executable, "-u", "-c", code], cwd=qlib.ROOT, capture_output=True, text=True, timeout=100)
+    assert done.returncode == 0, done.stdout + done.stderr[-2000:]
+    return done.stdout
+
+
+def test_torch_tensors_and_products_on_the_librarys_stream():
+    """A step as documented: torch's work, the products and the calls all on the library's stream, none waited for."""
+    assert "steps 4" in in_torch(PRODUCTS_CHILD)
