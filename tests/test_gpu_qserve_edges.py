@@ -238,3 +238,36 @@ def in_torch(code):
 def test_torch_tensors_and_products_on_the_librarys_stream():
     """A step as documented: torch's work, the products and the calls all on the library's stream, none waited for."""
     assert "steps 4" in in_torch(PRODUCTS_CHILD)
+
+
+TORCH_CHILD = """
+import random, sys
+import torch
+sys.path.insert(0, "perf")
+import operators as P
+rng = random.Random(5)
+cases = [c for c in P.listed() if c["name"] in ("plan_step", "append_step", "attend_tiny", "attend_one", "sample_few")]
+cases += [dict(kind="append", shape="1b", type="i8", page=20, rows=33, mix=4),
+          dict(kind="attend", shape="1b", type="i8", page=20, requests=9, most=300, mix=5),
+          dict(kind="sample", rows=20, vocab=5001, settings="mixed", mix=6)]
+for c in cases:
+    out = []
+    for P.own in (False, True):
+        o = P.run(P.prepare(c, 3))
+        torch.cuda.synchronize()
+        out.append({k: v.cpu() for k, v in o.items()})
+    for k, want in out[0].items():
+        got = out[1][k]
+        if want.dtype.is_floating_point:
+            torch.testing.assert_close(got.float(), want.float(), rtol=2e-5, atol=2e-5)
+        else:
+            assert torch.equal(got, want), (c, k)
+    print("same", c.get("name", c["kind"]), flush=True)
+print("all", len(cases))
+"""
+
+
+def test_torch_tensors_on_the_gpu():
+    """The Python mirror on torch's own GPU tensors, on torch's stream, in a process that has loaded torch's HIP runtime first:
+    whole outputs against elementary torch operations."""
+    assert "all 8" in in_torch(TORCH_CHILD)
