@@ -12,7 +12,7 @@ import pytest
 
 import qlib
 from test_gpu_qserve import (EPS, HIP, Buffer, Dev, Server, Work, attend, attend_ref, dev_i32, i32, make_cache, one_step, pages_for,  # noqa: F401
-                             sample_ref, widened, Q)
+                             sample_ref, sample_run, widened, Q)
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -271,3 +271,91 @@ def test_torch_tensors_on_the_gpu():
     """The Python mirror on torch's own GPU tensors, on torch's stream, in a process that has loaded torch's HIP runtime first:
     whole outputs against elementary torch operations."""
     assert "all 8" in in_torch(TORCH_CHILD)
+
+# ---------------------------------------------------------------------------
+# The documented limits
+# ---------------------------------------------------------------------------
+def attend_dense(kv, q, table, lens):
+    """attend_ref for many short requests at once: tables of few pages inside the cache, one KV head a query head."""
+    page, hd = kv.k.shape[2], q.shape[2]
+    n, room = len(lens), table.shape[1] * page
+    rows = lambda x: x.get().double()[table.long()].transpose(1, 2).reshape(n, -1, room, hd)  # noqa: E731
+    k, v, q = rows(kv.k), rows(kv.v), q.double()[:, :, None]
+    scale, there = 1.0 / math.sqrt(hd), (torch.arange(room) < torch.tensor(lens)[:, None])[:, None]
+    s = ((k * q).sum(-1) * scale).masked_fill(~there, -math.inf)
+    z = torch.logsumexp(s, 2, keepdim=True)
+    w = torch.where(there, torch.exp(s - z), 0.0)
+    size = torch.where(there, ((3 * hd + 4) * EPS * (k * q).abs().sum(-1)) * scale + 2 * EPS * s.abs(), 0.0).amax(2, keepdim=True)
+    dw = 2 * size + 4 * EPS * torch.where(there, s.abs(), 0.0).amax(2, keepdim=True) + 8 * EPS
+    tokens = torch.tensor(lens).double()[:, None]
+    wide = lambda x: (x[..., None] * v).sum(2)  # noqa: E731
+    bound = (2 * dw + (3 * tokens[..., None] + 16) * EPS) * (w[..., None] * v.abs()).sum(2)
+    return wide(w), z[..., 0], bound, dw[..., 0] + (tokens + 16) * EPS + 4 * EPS * z[..., 0].abs()
+
+
+@pytest.mark.parametrize("typ", ["f32", "i8"])
+def test_attention_of_seventy_thousand_requests(Q, typ):
+    """More requests than a grid's second dimension takes."""
+    n, page, hd, pages = 70000, 16, 8, 500
+    g = torch.Generator().manual_seed(1)
+    kv = make_cache(Q, typ, pages, 1, page, hd, "head", g)
+    if typ == "i8":
+        values = kv.k.get().double() * kv.k_scale.get().double()[..., None], kv.v.get().double() * kv.v_scale.get().double()[..., None]
+    else:
+        values = kv.k.get().double(), kv.v.get().double()
+    q = torch.randn((n, 1, hd), generator=g)
+    table = torch.randint(0, pages, (n, 2), generator=g, dtype=torch.int32)
+    lens = torch.randint(1, 33, (n,), generator=g).tolist()
+    o, lse = attend(Q, kv, q, table, lens)
+
+    class Held:
+        k, v = (type("T", (), {"shape": x.shape, "get": lambda self, x=x: x})() for x in values)
+
+    wo, wl, bound, lb = attend_dense(Held, q, table, lens)
+    if typ == "i8":                                        # 2^-37 of the largest product a token, times its code
+        bound = bound + torch.tensor(lens)[:, None, None] * 127 * 2.0 ** -37 * 0.035
+    assert bool(((o.double() - wo).abs() <= bound).all()) and bool(((lse.double() - wl).abs() <= lb).all())
+
+
+@pytest.mark.parametrize("H,KVH", [(65535, 1), (65535, 65535), (65534, 32767)])
+def test_attention_of_the_most_heads(Q, H, KVH):
+    page, hd, lens = 16, 8, [20]
+    g = torch.Generator().manual_seed(2)
+    kv = make_cache(Q, "bf16", 2, KVH, page, hd, "head", g)
+    q = torch.randn((1, H, hd), generator=g)
+    o, lse = attend(Q, kv, q, torch.tensor([[1, 0]], dtype=torch.int32), lens)
+
+    class Held:
+        k, v = (type("T", (), {"shape": x.shape, "get": lambda self, x=x: x.get().repeat_interleave(H // KVH, 1)})() for x in (kv.k, kv.v))
+
+    wo, wl, bound, lb = attend_dense(Held, q, torch.tensor([[1, 0]]), lens)
+    assert bool(((o.double() - wo).abs() <= bound).all()) and bool(((lse.double() - wl).abs() <= lb).all())
+
+
+def test_append_of_the_most_rows(Q):
+    """2^23 rows, in a random order of their slots."""
+    rows, page, hd = 1 << 23, 64, 8
+    g = torch.Generator().manual_seed(3)
+    kv = Q.PagedKV(*(Dev(torch.zeros((rows // page, 1, page, hd), dtype=torch.bfloat16)) for _ in range(2)))
+    k = torch.randn((rows, 1, hd), generator=g)
+    slots = torch.randperm(rows, generator=g).to(torch.int32)
+    dk = Dev(k)
+    Q.paged_append(kv, dk, dk, Dev(slots))
+    want = torch.zeros((rows, hd), dtype=torch.bfloat16)
+    want[slots.long()] = k[:, 0].bfloat16()
+    for x in (kv.k, kv.v):
+        assert torch.equal(x.get().view(rows, hd), want)
+
+
+def test_sample_rows_of_the_most_rows(Q):
+    """65535 rows of 7 tokens, every setting in turn."""
+    n, V = 65535, 7
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn((n, V), generator=g) * 2.0
+    u = torch.rand(n, generator=g).tolist()
+    t, k, p, m = ([y[i % len(y)] for i in range(n)] for y in ([0.8, 1.0, 0.0], [0, 3, 5, 0, 1], [1.0, 0.9, 0.5, 0.97], [0.0, 0.05, 0.0, 0.0, 0.3, 0.0, 0.0]))
+    token, kept, prob = sample_run(Q, x, u, t, k, p, m)
+    f = lambda y: float(np.float32(y))  # noqa: E731
+    for i in list(range(0, n, 61)) + [n - 2, n - 1]:
+        want = sample_ref(x[i].numpy(), f(t[i]), k[i], f(p[i]), f(m[i]), u[i])
+        assert (token[i], kept[i]) == want[:2] and abs(prob[i] - want[2]) <= 2.0 ** -20 * want[2], i
