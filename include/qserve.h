@@ -22,8 +22,9 @@
 // aborts.  An error that an earlier HIP call has left behind is not looked at and stays.
 // Calls that overlap need workspaces of their own.  What lies in device memory (lengths, tables, slots, settings) cannot be
 // refused by the host: each call states what it does with values out of range, and
-// none of them makes it read or write outside its buffers.  Float sums are held in 32
-// bits or more and in a fixed order: equal inputs give equal bits.
+// none of them makes it read or write outside its buffers, as long as nothing else
+// writes them while the call runs.  Float sums are held in 32 bits or more and in a
+// fixed order: equal inputs give equal bits.
 #ifndef QSERVE_H
 #define QSERVE_H
 
@@ -71,10 +72,10 @@ typedef struct {
 //   * The pages of ended requests are put at the ring's back, request by request, for
 //     later calls (this one does not take them); lens[r] = 0; the table row is left.
 //     What does not fit in the ring any more is dropped.
-//   * Requests are admitted in order: r is refused when the pages it needs together
-//     with those that r and every request before it asked for exceed the free ones
-//     (status 3), or the rows do (max_rows, status 4); a request that needs no page is
-//     not held up by missing pages.  cached + added > width * page_size: status 1.
+//   * Requests are admitted in order: r is refused when the pages that r and all requests
+//     before it ask for, refused ones among them, exceed the free ones (status 3), or
+//     their rows exceed max_rows (status 4); a request that needs no page is not held up
+//     by missing pages.  cached + added > width * page_size: status 1.
 //     Refused requests keep lens[r] = cached and add nothing.  cached < 0 or above
 //     width * page_size: status 2, lens[r] = 0, nothing else.
 //   * Admitted rows lie one behind another: starts[r] is the first of request r,
@@ -137,7 +138,8 @@ int qllama_paged_append(const QPagedKV *c, const QPagedRows *r, void *stream);
 // request's tokens, NaN included, has no effect.  Products and sums in 32 bits: a
 // 16-bit or int8 row enters a product as it is, a query or a weight (int8: times its
 // value's scale) as two or three 16-bit parts that together hold 23 (f16 and int8
-// caches; a weight at least 2^-37 of the largest) or 24 bits.  A cached infinity gives NaN.
+// caches, where a weight is held to 2^-37 of the largest at least) or 24 bits.  A cached
+// infinity gives NaN.
 // width * page_size has to be below 2^31 - 64.  work: qllama_paged_attention_work bytes,
 // 16-byte aligned.
 typedef struct {

@@ -65,7 +65,8 @@ __device__ inline int plan_place(int x, int y, int R) {
 // count) and returned to those behind, table entries below a request's first new one
 // are read and those from it on written.  A chain of latencies, not bytes: 6.7 us at 250
 // requests of a token each (two blocks: lengths, three scans, table and ring behind a
-// search), 5.4 at 48 requests with 16384 rows (65 blocks; 0.2 MB).
+// search), 5.4 at 48 requests with 16384 rows (65 blocks; 0.2 MB); 13 us at 1000 requests and
+// 63 at 8192, whose 32 passes every block makes.
 __global__ __launch_bounds__(kPlanThreads) void k_paged_plan(QPagedPlan p) {
   extern __shared__ int lds[];
   int *row0 = lds, *take0 = lds + p.n_req + 1, *give0 = take0 + p.n_req + 1;
@@ -207,7 +208,8 @@ __device__ inline int code(float x) {
 // the keys', then the values'.  Memory bound: 4 (2 H + 2 KVH) hd bytes of a row and its
 // cache bytes.  int8: the lanes of a head agree on its largest magnitude.  4001 rows of
 // 32 + 2 x 8 heads of 128 into an f16 cache: 37.5 us, 4.9 TB/s (a 1 GiB copy: 5.1); 64
-// rows 3.1 us, a launch and one trip to memory.
+// rows 3.0 us, a launch and one trip to memory.  Other caches: 42.2 us f32 (4.7 TB/s), 38.1 bf16,
+// 39.1 int8 (4.5 TB/s; 64 rows 3.4).
 template <int T, bool VEC>
 __global__ __launch_bounds__(kAppThreads) void k_paged_append(AppArgs a) {
   const int row = blockIdx.x;

@@ -40,7 +40,9 @@
 // Measured (both kernels, 32 query and 8 KV heads; a 1 GiB copy moves 5.1 TB/s):
 //   64 ragged requests of up to 2560 tokens, bf16, hd 128     73   us   4.8 TB/s
 //   2 requests, up to 120000 tokens, f16, hd 128             134   us   5.5 TB/s
-//   128 requests of up to 4100 tokens, int8, hd 128          130   us   4.4 TB/s
+//   128 requests of up to 4100 tokens, int8, hd 128          126   us   4.5 TB/s
+//   64 ragged requests of up to 2560 tokens, f32, hd 128     125   us   5.6 TB/s
+//   the same, hd 64                                           68   us   5.1 TB/s
 //   24 requests of up to 768 tokens, f32, hd 64               17.0 us   2.1 TB/s
 //   1 request of 2060 tokens, bf16, hd 128                    12.5 us   0.7 TB/s
 //   1 request of 200 tokens, f32, 6 + 2 heads of 48             7.2 us
@@ -134,9 +136,10 @@ __device__ inline float sum_groups(float x) {
   return x + __shfl_xor(x, 32);
 }
 
-// W words of a row; STREAM: read once (one tile of query heads a KV head), so past the
-// caches' retention: 84 -> 77 us at 64 ragged bf16 requests, together with whole 64-byte
-// runs a load; more tiles of a KV head find the rows in L2
+// W words of a row; STREAM: read once by its request (one tile of query heads a KV head), so
+// past the caches' retention: 84 -> 77 us at 64 ragged bf16 requests, together with whole
+// 64-byte runs a load; more tiles of a KV head find the rows in L2.  Pages that requests
+// share are read so too: 64 requests on one request's pages take 72 us, on their own 73
 template <bool STREAM, int W>
 __device__ inline void load_words(uint32_t (&d)[W], const char *p) {
   typedef uint32_t vec __attribute__((ext_vector_type(W), aligned(W > 2 ? 8 : 4)));
@@ -865,7 +868,8 @@ int launch(const char *fn, const PaArgs &a, hipStream_t stream) {
   // 64 int8 ones of 340 15.9 / 21.7; hd 64, 24 f32 ones of 250 8.7 / 13.2, 128 of 450 30.6 / 35.3, 64 bf16 ones
   // of 1900 (16 steps) 36.1 / 34.5.  One request leaves CUs idle: of 100 6.7 / 8.8, of 340 10.1 / 9.0.
   // Among thousands of tiles whose waves have a step at most, or of int8, shares are better:
-  // 256 of 60 24.1 / 18.6, 512 int8 ones of 300 82 / 77.
+  // 256 of 60 24.1 / 18.6, 512 int8 ones of 300 82 / 77.  The rule knows the tables' width, not the
+  // lengths in device memory: 32 requests of 120 behind tables of 2560 take 12.6, 64 of 340 22.6.
   const int waves = tiles > 256 ? 4 : C::MEETING;
   const long long each = (room + waves - 1) / waves;
   const bool few = tiles > 256 ? each <= 8 && each * HDP <= 1024 && (tiles <= 1024 || (each > 1 && T != QLLAMA_KV_I8)) : each * HDP <= (tiles < 32 ? 128 : 256);

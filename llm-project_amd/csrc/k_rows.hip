@@ -185,8 +185,8 @@ __device__ inline float wave_max4(const float (&x)[4]) {
 }
 
 // A slice of kSlice tokens in registers: the only reading of most of a row.  Near the
-// memory's rate for many rows: 192 rows of 128256 tokens 27.4 us, 98 MB read and 19 MB
-// of histograms written, beside 16 tokens' arithmetic and atomics a thread; 4 rows
+// memory's rate for many rows: 192 rows of 128256 tokens 27.4 us, 98 MB read and 16 MB
+// of histograms written (greedy rows leave none), beside 16 tokens' arithmetic and atomics a thread; 4 rows
 // 5.3 us.
 __global__ __launch_bounds__(kSliceThreads) void k_sample_slices(QSampleRows a, Slice *slices, u64 *hist, float *groups) {
   __shared__ u64 h[kBins], bests[kSliceThreads / 64];
@@ -609,7 +609,9 @@ __device__ inline void write_first(const QSampleRows &a, int r, u64 best) {
 // steps, each a barrier or a trip to memory behind the one before: 10.8 us for 4 rows
 // with top-k 40 and top-p 0.95.  Of 192 rows with settings of their own (35 us) a few keep
 // thousands of tokens and end in cells that every group may hold some of: their CU reads
-// most of the row again, at some 16 bytes a cycle, which takes 15 us.
+// most of the row again, at some 16 bytes a cycle, which takes 15 us.  (768 threads with four
+// loads of 16 bytes each under way, and 1.5 us a trip, come to as much: whether the CU or
+// what is under way sets that rate has not been told apart.)
 __device__ void pick(const QSampleRows &a, int r, const Row &row, Shared &s, const Limits &limits, uint32_t n, u64 x, uint32_t all_n) {
   const int t = threadIdx.x;
   int turn = 0;
