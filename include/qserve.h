@@ -12,19 +12,20 @@
 // which no other stream is ordered, so that such a step runs on that stream as a whole or
 // orders its own with it by events.
 //
-// All pointers are DEVICE memory, of one device in a call, unless stated otherwise.  Every call enqueues on the
-// hipStream_t it is given (0 is HIP's default stream, qllama_stream() the library's),
-// returns without waiting, allocates nothing, keeps nothing between calls and may be
-// captured into a HIP graph.  The buffers' device need not be the current one; the
-// stream has to be on it.  Calls return 0, or print "Error: ..." and return nonzero
-// before anything is enqueued (but for a launch that the runtime itself refuses: a
-// call's first kernel may have run by then, and its outputs are not to be used); none
-// aborts.  An error that an earlier HIP call has left behind is not looked at and stays.
-// Calls that overlap need workspaces of their own.  What lies in device memory (lengths, tables, slots, settings) cannot be
-// refused by the host: each call states what it does with values out of range, and
-// none of them makes it read or write outside its buffers, as long as nothing else
-// writes them while the call runs.  Float sums are held in 32 bits or more and in a
-// fixed order: equal inputs give equal bits.
+// All pointers are DEVICE memory, of one device in a call, unless stated
+// otherwise.  Every call enqueues on the hipStream_t it is given (0 is HIP's default
+// stream, qllama_stream() the library's), returns without waiting, allocates nothing,
+// keeps nothing between calls and may be captured into a HIP graph.  The buffers'
+// device need not be the current one; the stream has to be on it.  Calls return 0, or
+// print "Error: ..." and return nonzero before anything is enqueued (but for a launch
+// that the runtime itself refuses: a call's first kernel may have run by then, and its
+// outputs are not to be used); none aborts.  An error that an earlier HIP call has
+// left behind is not looked at, and stays unless the call is refused.  Calls that
+// overlap need workspaces of their own.  What lies in device memory (lengths, tables,
+// slots, settings) cannot be refused by the host: each call states what it does with
+// values out of range, and none of them makes it read or write outside its buffers, as
+// long as nothing else writes them while the call runs.  Float sums are held in 32
+// bits or more and in a fixed order: equal inputs give equal bits.
 #ifndef QSERVE_H
 #define QSERVE_H
 
@@ -132,14 +133,14 @@ int qllama_paged_append(const QPagedKV *c, const QPagedRows *r, void *stream);
 // For every request r and query head h (of KV head h / (n_heads / n_kv)), over the
 // cached tokens j < lens[r]: o = sum_j w_j v_j, w = softmax_j(scale * q . k_j), and lse
 // = ln sum_j e^(scale * q . k_j) (lse may be NULL).  Token j lies in slot j mod
-// page_size of page table[r][j / page_size].  scale 0 stands for 1 / sqrt(head_dim); up to 2.35e38.
-// lens[r] <= 0 gives o = 0 and lse = -inf; lengths above width * page_size count as
-// that; tokens of a page outside the cache are left out.  What lies in slots behind a
-// request's tokens, NaN included, has no effect.  Products and sums in 32 bits: a
-// 16-bit or int8 row enters a product as it is, a query or a weight (int8: times its
-// value's scale) as two or three 16-bit parts that together hold 23 (f16 and int8
-// caches, where a weight is held to 2^-37 of the largest at least) or 24 bits.  A cached
-// infinity gives NaN.
+// page_size of page table[r][j / page_size].  scale 0 stands for 1 / sqrt(head_dim);
+// up to 2.35e38.  lens[r] <= 0 gives o = 0 and lse = -inf; lengths above width *
+// page_size count as that; tokens of a page outside the cache are left out.  What lies
+// in slots behind a request's tokens, NaN included, has no effect.  Products and sums
+// in 32 bits: a 16-bit or int8 row enters a product as it is, a query or a weight
+// (int8: times its value's scale) as two or three 16-bit parts that together hold 23
+// (f16 and int8 caches, where a weight is held to 2^-37 of the largest at least) or 24
+// bits.  A cached infinity gives NaN.
 // width * page_size has to be below 2^31 - 64.  work: qllama_paged_attention_work bytes,
 // 16-byte aligned.
 typedef struct {
