@@ -199,6 +199,189 @@ size_t qllama_sample_rows_work(int rows, int vocab);
 // to 1.045 times that (host arithmetic, as the kernels').  For tests.
 unsigned long long qllama_test_sample_weight(float logit, float top, float temperature);
 
+// ---------------------------------------------------------------------------
+// Several new tokens a request: drafted trees
+// ---------------------------------------------------------------------------
+// A step that verifies drafted tokens gives every request a forest of new rows.  Row j of
+// request r is row i = starts[r] + j of the step, and token lens[r] - m + j of the
+// request's pages, where m = starts[r + 1] - starts[r] is the number of its new rows and
+// lens[r] its tokens with them (starts, lens, slots as qllama_paged_plan leaves them).
+// In order: qllama_paged_plan, qllama_tree_plan, qllama_paged_append,
+// qllama_tree_attention, (qllama_logit_rules,) qllama_sample_rows for every row,
+// qllama_tree_accept, qllama_paged_move in every layer's cache, and qllama_paged_fork with
+// keep = the accepted lengths, which gives the pages of rejected rows back.
+//
+// parents[r][j] is the row (0 .. j - 1, of the same request) that row j follows; any other
+// value means none: the row follows the request's earlier tokens.  Rows behind the first
+// `nodes` of a request have none.  starts outside 0 .. max_rows count as the nearest
+// inside; rows that no request has are left as they were.
+
+// positions[i] = lens[r] - m + depth of the row (0 for a row that follows none); bit b of
+// mask[i] (bit b mod 64 of its word b / 64) is set for b = j and every row above j.  Rows
+// behind the first 64 * words of a request get mask 0 and the position lens[r] - m + j.
+typedef struct {
+  int n_req;                // 0 .. 8192
+  int nodes;                // rows of a request that parents has room for: 1 .. 1024
+  int max_rows;             // rows of positions and mask
+  int words;                // 64-bit words of a row of mask: 1 .. 4
+  int64_t parent_stride;    // entries between two requests' parents, >= nodes
+  const int32_t *starts, *lens, *parents;    // n_req + 1, n_req, n_req x nodes
+  int32_t *positions;                        // max_rows
+  uint64_t *mask;                            // max_rows x words
+} QTreePlan;
+int qllama_tree_plan(const QTreePlan *p, void *stream);
+
+// What the chosen tokens confirm.  Row 0 of a request is accepted (its token was certain);
+// then, as long as there is one, the first row c whose parent is the row accepted last and
+// whose token tokens[c] is the one that was chosen behind that row (chosen[] >= 0).
+// accepted[r] rows in all, lens_out[r] = lens[r] - m + accepted[r], last[r] = what was
+// chosen behind the last of them (-1 if the request has no rows).  path[starts[r] + k] is
+// the k-th accepted row of the step, -1 behind them; where it is not row k of its request,
+// src and dst are the slots that its keys and values have to be moved between (dst: that
+// of row k), else -1: groups of qllama_paged_move, with starts as they are.  Rows that no
+// request has are left as they were.
+typedef struct {
+  int n_req, nodes, max_rows;                // as QTreePlan's
+  int64_t parent_stride;
+  const int32_t *starts, *lens, *parents;    // n_req + 1, n_req, n_req x nodes
+  const int32_t *tokens, *chosen, *slots;    // max_rows
+  int32_t *accepted, *last, *lens_out;       // n_req
+  int32_t *path, *src, *dst;                 // max_rows
+} QTreeAccept;
+int qllama_tree_accept(const QTreeAccept *p, void *stream);
+
+// qllama_paged_attention for all new rows: row i = starts[r] + j attends to the tokens t <
+// lens[r] - m of its request and to those new rows b < m whose bit is set in mask[i]; mask
+// NULL: to b = 0 .. j (the next piece of a prompt).  Bits behind a row's words count as 0.
+// A row that attends to nothing gives o = 0 and lse = -inf.  A masked token has no effect,
+// whatever its slot holds.  Lengths, pages, scale, padding and precision are those of
+// qllama_paged_attention, except that int8 rows also meet queries and weights held to 24
+// bits.  `nodes` is the number of rows of a request that the call is laid out for (0: rows
+// / n_req); any number of rows is right, other ones are slower.  Rows that no request has
+// are left as they were.  starts outside 0 .. rows count as the nearest inside; a row that
+// two requests name gets either result.  work: qllama_tree_attention_work bytes, 16-byte aligned.
+typedef struct {
+  int rows;                 // of q, o, lse and mask
+  int n_req, n_heads, width, words, nodes;
+  int64_t q_stride, o_stride, lse_stride;     // floats between rows; heads lie one behind another
+  int64_t table_stride;
+  const float *q;
+  float *o, *lse;
+  const uint64_t *mask;     // rows x words; NULL: words 0
+  const int32_t *starts, *table, *lens;
+  float scale;
+  void *work;
+  size_t work_bytes;
+} QTreeQuery;
+int qllama_tree_attention(const QPagedKV *c, const QTreeQuery *a, void *stream);
+size_t qllama_tree_attention_work(const QPagedKV *c, int rows, int n_req, int n_heads, int nodes);
+
+// ---------------------------------------------------------------------------
+// Pages that several requests hold
+// ---------------------------------------------------------------------------
+// New request i continues old request from[i] (0 .. n_old - 1; any other value: it is
+// empty) with its first min(keep[i], lens[from[i]]) tokens (keep NULL: all; below 0: none).
+// Old requests that nothing continues end.  extra[p] counts who holds page p beyond one: 0
+// for pages as qllama_paged_plan gives them and for free ones; holders that are no row of
+// the call (a kept beginning of prompts) count too and keep what they have.
+//   * Pages are held by every new request that continues over them.  A page that new
+//     request i would write to next (its last one, unless full) and that others hold as
+//     well is copied: i gets a free page for it, and src[i], dst[i] (slots) and count[i] (tokens)
+//     say what to copy (-1, -1, 0: nothing), for qllama_paged_move without starts.  Of the
+//     new requests that hold such a page, the one with the most of its tokens (the first
+//     of these) keeps it without a copy, if no one outside the call holds it.
+//   * Free pages are taken from the ring's front, request by request.  Request i is refused
+//     (status 3, lens_out 0, nothing held) when the copies that it and all requests before
+//     it ask for, refused ones among them, exceed the free pages at the start.
+//   * Pages that no one holds any more are put at the ring's back, in the order of the old
+//     rows (a page that several held: where the first of them has it), for later calls.
+//     What does not fit in the ring any more is dropped.
+//   * lens_out[i] is the number of tokens, the first ceil(lens_out / page_size) entries of
+//     table_out[i] the pages; entries behind them are left.  extra_out and state_out follow.
+//     state outside the ring counts as in qllama_paged_plan; lens outside 0 .. width *
+//     page_size as the nearest inside; a table entry outside 0 .. n_pages - 1 is no page:
+//     it is carried over as -1, and not copied.
+// extra_out may be extra; no other output may be one of the inputs.  work:
+// qllama_paged_fork_work bytes, 16-byte aligned.
+typedef struct {
+  int n_old, n_new;         // 0 .. 8192
+  int width;                // table entries of a request, old and new
+  int page_size, n_pages;   // n_pages * page_size fits in 31 bits
+  int ring_size;            // up to 2^30
+  int64_t table_stride, table_out_stride;     // >= width
+  const int32_t *lens, *table;                // n_old, n_old x width
+  const int32_t *from, *keep;                 // n_new
+  const int32_t *extra, *state;               // n_pages, 2
+  int32_t *ring;                              // ring_size, changes in place
+  int32_t *table_out, *lens_out, *status;     // n_new x width, n_new, n_new
+  int32_t *extra_out, *state_out;             // n_pages, 2
+  int32_t *src, *dst, *count;                 // n_new
+  void *work;
+  size_t work_bytes;
+} QPagedFork;
+int qllama_paged_fork(const QPagedFork *p, void *stream);
+size_t qllama_paged_fork_work(int n_old, int n_new, int n_pages);
+
+// Keys and values (and scales) of slot src[i] into slot dst[i], in n_caches caches at once
+// (one a layer; alike in type, sizes and strides).  Without starts the moves are
+// independent: count[i] slots from src[i] into as many from dst[i] (count NULL: 1), and no
+// slot that one move writes may be read or written by another.  With starts, moves
+// starts[g] .. starts[g + 1] - 1 happen one after another, and so a slot may be moved on
+// into another's old place; groups are independent, and count has to be NULL.  Moves with
+// a negative slot, or no count, do nothing; those that leave the cache do nothing either
+// and increase *bad (if not NULL) by their number.  starts outside 0 .. n_moves count as
+// the nearest inside.
+typedef struct {
+  int n_moves;              // 0 .. 2^23
+  int n_groups;             // 0 .. 2^23; with starts
+  const int32_t *src, *dst, *count;           // n_moves
+  const int32_t *starts;                      // n_groups + 1
+  int32_t *bad;
+} QPagedMoves;
+int qllama_paged_move(const QPagedKV *caches, int n_caches, const QPagedMoves *m, void *stream);
+
+// ---------------------------------------------------------------------------
+// Rules on logits
+// ---------------------------------------------------------------------------
+// For every row i of request r = requests[i] (NULL: r = i) and every token t:
+//   x = logits[i][t];  if t is known, x = x > 0 ? x / repetition[r] : x * repetition[r];
+//   x -= frequency[r] * n + (n > 0 ? presence[r] : 0);  x += the bias of t;
+//   out[i][t] = x, or -inf where the row's mask does not allow t
+// evaluated in 64 bits and rounded once.  n is how often t was generated, t is known if it
+// was generated or stands in the prompt: tokens[r] holds n_tokens[r] tokens, the first
+// n_prompt[r] (NULL: 0) of them the prompt.  With mask (a tree's, as QTreePlan's), the
+// tokens drafted[starts[r] + b] of the bits b of mask[i] were generated too: list those of
+// earlier steps alone in tokens.  bias_tokens[r] names n_bias tokens with a bias each; one
+// that it names twice gets the first.  allowed_rows[i] names the row's mask, of n_masks:
+// bit t mod 32 of word t / 32 is set for an allowed token; other numbers: no mask.
+// Tokens outside 0 .. vocab - 1 are none; lengths outside 0 .. capacity count as the
+// nearest inside.  A NaN setting, and a repetition that is not above 0, is none.  A row
+// whose request lies outside 0 .. n_req - 1 is not written.  out may be logits (with the
+// same stride), else they must not overlap.
+typedef struct {
+  int rows, vocab, n_req;                     // rows up to 65535, vocab 1 .. 1048576
+  int64_t stride, out_stride;                 // floats between rows, >= vocab
+  const float *logits;
+  float *out;
+  const int32_t *requests;                    // rows
+  int capacity;                               // entries of a row of tokens: 0 .. 2^28
+  int64_t token_stride;
+  const int32_t *tokens, *n_tokens, *n_prompt;            // NULL: no history
+  const float *repetition, *presence, *frequency;         // n_req; NULL: none
+  int words;                                  // of a row of mask, 1 .. 4
+  const int32_t *starts, *drafted;            // n_req + 1, rows
+  const uint64_t *mask;                       // rows x words; NULL: none, and no starts, drafted
+  int n_bias;                                 // 0 .. 4096
+  int64_t bias_stride;
+  const int32_t *bias_tokens;                 // n_req x n_bias
+  const float *bias;
+  int n_masks;
+  int64_t allowed_stride;                     // words between masks, >= ceil(vocab / 32)
+  const uint32_t *allowed;                    // NULL: none
+  const int32_t *allowed_rows;                // rows
+} QLogitRules;
+int qllama_logit_rules(const QLogitRules *p, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -83,6 +83,12 @@ PAGED_PLAN = struct.Struct("@iiiiiqPPPPPPPPPPPP")
 PAGED_ROWS = struct.Struct("@iiPPPPqqqqPPPPiP")
 PAGED_QUERY = struct.Struct("@iiiqqqqPPPPPfPN")
 SAMPLE_ROWS = struct.Struct("@iiqPPPPPPPPPPN")
+TREE_PLAN = struct.Struct("@iiiiqPPPPP")
+TREE_ACCEPT = struct.Struct("@iiiqPPPPPPPPPPPP")
+TREE_QUERY = struct.Struct("@iiiiiiqqqqPPPPPPPfPN")
+PAGED_FORK = struct.Struct("@iiiiiiqqPPPPPPPPPPPPPPPPN")
+PAGED_MOVES = struct.Struct("@iiPPPPP")
+LOGIT_RULES = struct.Struct("@iiiqqPPPiqPPPPPPiPPPiqPPiqPP")
 
 
 class Rng(C.Structure):
@@ -187,6 +193,14 @@ def lib():
         L.qllama_paged_attention_work.restype = C.c_size_t
         L.qllama_sample_rows.argtypes = [C.c_char_p, C.c_void_p]
         L.qllama_sample_rows_work.argtypes = [C.c_int, C.c_int]
+        for name in ("qllama_tree_plan", "qllama_tree_accept", "qllama_paged_fork", "qllama_logit_rules"):
+            getattr(L, name).argtypes = [C.c_char_p, C.c_void_p]
+        L.qllama_tree_attention.argtypes = [P(QPagedKV), C.c_char_p, C.c_void_p]
+        L.qllama_tree_attention_work.argtypes = [P(QPagedKV)] + [C.c_int] * 4
+        L.qllama_paged_move.argtypes = [P(QPagedKV), C.c_int, C.c_char_p, C.c_void_p]
+        L.qllama_paged_fork_work.argtypes = [C.c_int] * 3
+        for name in ("qllama_tree_attention_work", "qllama_paged_fork_work"):
+            getattr(L, name).restype = C.c_size_t
         L.qllama_sample_rows_work.restype = C.c_size_t
         _lib = L
     return _lib
@@ -811,3 +825,149 @@ def sample_rows(logits, u, token, work, temperature=None, top_k=None, top_p=None
     kp, ip, np_ = _flat("int32", (top_k, "top_k", n), (token, "token", n), (kept, "kept", n))
     a = SAMPLE_ROWS.pack(n, V, ls, lp, up, tp, kp, pp, mp, ip, np_, op, *_work(work))
     _done((_lib or lib()).qllama_sample_rows(a, _stream(stream)), "qllama_sample_rows")
+
+
+# ---- qserve.h: drafted trees, pages that requests share, rules on logits -----------------
+def tree_plan(starts, lens, parents, positions, mask, stream=None):
+    """qllama_tree_plan: position and ancestors (mask (rows, words) int64, bit b of a row: new row b of its request) of every
+    new row, from parents (requests, nodes) int32; starts and lens are paged_plan's."""
+    n, nodes = parents.shape
+    rows, words = mask.shape
+    pp, ps = _rows(parents, "parents", "int32", parents.shape)
+    at = _flat("int32", (starts, "starts", n + 1), (lens, "lens", n), (positions, "positions", rows))
+    a = TREE_PLAN.pack(n, nodes, rows, words, ps, at[0], at[1], pp, at[2], _flat("int64", (mask, "mask", rows * words))[0])
+    _done((_lib or lib()).qllama_tree_plan(a, _stream(stream)), "qllama_tree_plan")
+
+
+def tree_accept(starts, lens, parents, tokens, chosen, slots, accepted, last, lens_out, path, src, dst, stream=None):
+    """qllama_tree_accept: how many new rows of every request the chosen tokens confirm, what was chosen behind the last of
+    them, the requests' new lengths, the accepted rows and the moves that put them one behind another.  int32 tensors; the
+    arguments after slots are outputs."""
+    n, nodes = parents.shape
+    rows = path.numel()
+    pp, ps = _rows(parents, "parents", "int32", parents.shape)
+    at = _flat("int32", (starts, "starts", n + 1), (lens, "lens", n), (tokens, "tokens", rows), (chosen, "chosen", rows), (slots, "slots", rows),
+               (accepted, "accepted", n), (last, "last", n), (lens_out, "lens_out", n), (path, "path", rows), (src, "src", rows), (dst, "dst", rows))
+    a = TREE_ACCEPT.pack(n, nodes, rows, ps, at[0], at[1], pp, *at[2:])
+    _done((_lib or lib()).qllama_tree_accept(a, _stream(stream)), "qllama_tree_accept")
+
+
+def tree_attention_work(cache, rows, n_req, n_heads, nodes=0):
+    """Bytes of workspace of tree_attention (calls that overlap need one each)."""
+    n = lib().qllama_tree_attention_work(cache.ref, rows, n_req, n_heads, nodes)
+    if n == 0:
+        raise ValueError("no such attention over this cache")
+    return n
+
+
+def tree_attention(cache, q, starts, table, lens, o, work, mask=None, lse=None, scale=0.0, nodes=0, stream=None):
+    """qllama_tree_attention: o (rows, heads, head_dim) and lse (rows, heads) of the new rows starts[r] .. starts[r + 1] - 1 of
+    every request over its pages table (requests, width): over the tokens before them, and those of the new rows whose bits
+    mask (rows, words) int64 has set (None: every row over those up to it)."""
+    rows, heads, hd = shape = q.shape
+    n = lens.numel()
+    tn, width = table.shape
+    if tn < n or hd != cache.head_dim:
+        raise ValueError("q, table and the cache do not fit together")
+    qp, qs = _rows(q, "q", "float32", shape)
+    op, os_ = _rows(o, "o", "float32", shape)
+    tp, ts = _rows(table, "table", "int32", table.shape)
+    lp, ls = (0, 0) if lse is None else _rows(lse, "lse", "float32", shape[:2])
+    mp = words = 0
+    if mask is not None:
+        words = mask.shape[1]
+        mp = _flat("int64", (mask, "mask", rows * words))[0]
+    sp, np_ = _flat("int32", (starts, "starts", n + 1), (lens, "lens", n))
+    a = TREE_QUERY.pack(rows, n, heads, width, words, nodes, qs, os_, ls, ts, qp, op, lp, mp, sp, tp, np_, scale, *_work(work))
+    _done((_lib or lib()).qllama_tree_attention(cache.ref, a, _stream(stream)), "qllama_tree_attention")
+
+
+def paged_fork_work(n_old, n_new, n_pages):
+    """Bytes of workspace of paged_fork (calls that overlap need one each)."""
+    n = lib().qllama_paged_fork_work(n_old, n_new, n_pages)
+    if n == 0:
+        raise ValueError("no such requests or pages")
+    return n
+
+
+def paged_fork(lens, table, source, extra, ring, state, page_size, table_out, lens_out, status, extra_out, state_out, src, dst, count,
+               work, keep=None, stream=None):
+    """qllama_paged_fork: new request i continues old request source[i] (its first keep[i] tokens) over the same pages, extra
+    being how many hold a page beyond the first; src, dst and count are the copies to make with paged_move.  int32 tensors;
+    ring changes in place, the arguments after page_size are outputs."""
+    n, m, pages = lens.numel(), source.numel(), extra.numel()
+    tn, width = table.shape
+    if tn < n or table_out.shape[0] < m or table_out.shape[1] != width:
+        raise ValueError("table and table_out must have a row for every request, and one width")
+    tp, ts = _rows(table, "table", "int32", table.shape)
+    op, os_ = _rows(table_out, "table_out", "int32", table_out.shape)
+    at = _flat("int32", (lens, "lens", n), (source, "source", m), (keep, "keep", m), (extra, "extra", pages), (state, "state", 2), (ring, "ring", 1),
+               (lens_out, "lens_out", m), (status, "status", m), (extra_out, "extra_out", pages), (state_out, "state_out", 2), (src, "src", m),
+               (dst, "dst", m), (count, "count", m))
+    a = PAGED_FORK.pack(n, m, width, page_size, pages, ring.numel(), ts, os_, at[0], tp, *at[1:6], op, *at[6:], *_work(work))
+    _done((_lib or lib()).qllama_paged_fork(a, _stream(stream)), "qllama_paged_fork")
+
+
+class PagedCaches:
+    """Several layers' caches, alike in type, sizes and strides, for paged_move.  Keeps them."""
+
+    def __init__(self, caches):
+        self.caches = list(caches)
+        self.array = (QPagedKV * max(1, len(self.caches)))(*[c.c for c in self.caches])
+
+
+def paged_move(caches, src, dst, starts=None, count=None, bad=None, stream=None):
+    """qllama_paged_move: slots src of every cache (PagedCaches, or a PagedKV) to slots dst; count consecutive ones each, or (with
+    starts) one after another in groups."""
+    if isinstance(caches, PagedKV):
+        caches = PagedCaches([caches])
+    n = src.numel()
+    sp, dp, cp, bp, gp = _flat("int32", (src, "src", n), (dst, "dst", n), (count, "count", n), (bad, "bad", 1), (starts, "starts", 1))
+    a = PAGED_MOVES.pack(n, 0 if starts is None else starts.numel() - 1, sp, dp, cp, gp, bp)
+    _done((_lib or lib()).qllama_paged_move(caches.array, len(caches.caches), a, _stream(stream)), "qllama_paged_move")
+
+
+def logit_rules(logits, out, requests=None, tokens=None, n_tokens=None, n_prompt=None, repetition=None, presence=None, frequency=None,
+                starts=None, drafted=None, mask=None, bias_tokens=None, bias=None, allowed=None, allowed_rows=None, stream=None):
+    """qllama_logit_rules: out (rows, vocab; may be logits) = logits with penalties for the tokens (requests, capacity) that
+    a row's request has used and for the drafted ones above the row (mask (rows, words) int64), biases (requests, n_bias), and
+    -inf where the mask allowed[allowed_rows] (masks, words) int32 has no bit set.  requests: the request of every row (None:
+    its own number)."""
+    rows, V = logits.shape
+    lp, ls = _rows(logits, "logits", "float32", logits.shape)
+    op, os_ = _rows(out, "out", "float32", logits.shape)
+    n = rows
+    for t in (n_tokens, repetition, presence, frequency, bias):
+        if t is not None:
+            n = t.shape[0]
+            break
+    cap = ts = tp = words = nb = bs = btp = bp = nm = ms = mp = 0
+    if tokens is not None:
+        if n_tokens is None:
+            raise ValueError("tokens need n_tokens")
+        cap = tokens.shape[1]
+        tp, ts = _rows(tokens, "tokens", "int32", (n, cap))
+    if mask is not None:
+        if starts is None or drafted is None:
+            raise ValueError("a mask needs starts and drafted")
+        words = mask.shape[1]
+    if bias is not None:
+        nb = bias.shape[1]
+        bp, bs = _rows(bias, "bias", "float32", (n, nb))
+        btp, s = _rows(bias_tokens, "bias_tokens", "int32", (n, nb))
+        if s != bs:
+            raise ValueError("bias and bias_tokens must have alike strides")
+    if allowed is not None:
+        if allowed_rows is None:
+            raise ValueError("allowed needs allowed_rows")
+        nm = allowed.shape[0]
+        mp, ms = _rows(allowed, "allowed", "int32", allowed.shape)
+        if allowed.shape[1] * 32 < V:
+            raise ValueError("allowed must have a bit for every token")
+    at = _flat("int32", (requests, "requests", rows), (n_tokens if tokens is not None else None, "n_tokens", n), (n_prompt, "n_prompt", n),
+               (starts if mask is not None else None, "starts", n + 1), (drafted if mask is not None else None, "drafted", rows),
+               (allowed_rows if allowed is not None else None, "allowed_rows", rows))
+    st = _flat("float32", (repetition, "repetition", n), (presence, "presence", n), (frequency, "frequency", n))
+    a = LOGIT_RULES.pack(rows, V, n, ls, os_, lp, op, at[0], cap, ts, tp, at[1], at[2], *st, words, at[3], at[4],
+                         _flat("int64", (mask, "mask", rows * words))[0], nb, bs, btp, bp, nm, ms, mp, at[5])
+    _done((_lib or lib()).qllama_logit_rules(a, _stream(stream)), "qllama_logit_rules")
