@@ -51,23 +51,17 @@
 // the same chain of waits.
 #include <hip/hip_runtime.h>
 
+#include "qdev_paged.h"
 #include "qserve_host.h"
 
 namespace {
 
-typedef float f2 __attribute__((ext_vector_type(2)));
-typedef float f4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+using namespace qpaged;
 
 constexpr int kThreads = 256, kWaves = 4;
 constexpr int kBlocks = 512;          // two blocks of four waves a CU
 constexpr int kShares = kBlocks * kWaves;
 constexpr int kMinShare = 1;          // steps a wave takes at least; one request of 2060 tokens took 12.5 us, with 2 or 4 13.3
-constexpr float kNegInf = -__builtin_inff();
 
 struct PaArgs {
   const char *k, *v;
@@ -83,23 +77,6 @@ struct PaArgs {
   int n_req, n_heads, n_kv, G, tiles, rows, hd, n_pages, page_size, width;
   float qscale;                       // scale * log2(e)
 };
-
-__host__ __device__ inline int clamp_len(int len, int width, int page_size) {
-  const int most = width * page_size;   // fits: checked by the host
-  return len < 0 ? 0 : len > most ? most : len;
-}
-
-// Where a token lies: its table entry (of the last token for one behind it, so that the
-// entry can always be read; len > 0) and its place there; then the entry's page, -1 for
-// no page of the cache or no token.
-__host__ __device__ inline int entry_of(long long key, int len, int page_size, int *place) {
-  const int k = key < len ? (int)key : len - 1, e = k / page_size;
-  *place = k - e * page_size;
-  return e;
-}
-__host__ __device__ inline int page_of(int entry, long long key, int len, int n_pages) {
-  return key < len && entry >= 0 && entry < n_pages ? entry : -1;
-}
 
 // Inclusive sums over a wave: within rows of 16 lanes, then from row to row.
 template <int CTRL, int ROWS>
@@ -119,23 +96,6 @@ __device__ inline long long share_of(long long units) {
   return s < kMinShare ? kMinShare : s;
 }
 
-// What a part with maximum m counts against the maximum of all.  A part without one holds
-// zeros, or the NaN of its scores, which has to stay.
-__device__ inline float part_weight(float m, float top) { return m == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(m - top); }
-
-// max of a lane's value with those of lanes l ^ 16, l ^ 32 and l ^ 48
-__device__ inline float max_groups(float x) {
-  const uint32_t u = __float_as_uint(x);
-  u2 r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-  const uint32_t y = __float_as_uint(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)));
-  r = __builtin_amdgcn_permlane16_swap(y, y, false, false);
-  return fmaxf(__uint_as_float(r.x), __uint_as_float(r.y));
-}
-__device__ inline float sum_groups(float x) {
-  x += __shfl_xor(x, 16);
-  return x + __shfl_xor(x, 32);
-}
-
 // W words of a row; STREAM: read once by its request (one tile of query heads a KV head), so
 // past the caches' retention: 84 -> 77 us at 64 ragged bf16 requests, together with whole
 // 64-byte runs a load; more tiles of a KV head find the rows in L2.  Pages that requests
@@ -152,8 +112,6 @@ __device__ inline void load_words(uint32_t (&d)[W], const char *p) {
   }
 }
 
-__device__ inline uint32_t hi16s(uint32_t b, uint32_t a) { return __builtin_amdgcn_perm(b, a, 0x07060302); }
-__device__ inline uint32_t lo16s(uint32_t b, uint32_t a) { return __builtin_amdgcn_perm(b, a, 0x05040100); }
 // 2^-9 times two int8 codes as f16: the codes plus 128, the bytes of y : x that SELECT
 // names, are subnormal numbers of 2^-24, and one packed multiply-add makes them 2^-9 and takes
 // the 128 off, exactly.  x and y have had the top bits of their bytes turned.
@@ -162,47 +120,6 @@ template <uint32_t SELECT>
 __device__ inline uint32_t codes(uint32_t y, uint32_t x) {
   const h2 u = __builtin_bit_cast(h2, __builtin_amdgcn_perm(y, x, SELECT));
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(u, h2{32768.0f16, 32768.0f16}, h2{-0.25f16, -0.25f16}));
-}
-
-// Parts of a float operand of 8 values: sums of the parts are the values (bf16: all 24
-// bits by cutting; f16: to nearest twice, off by 2^-23 at most and without a bias, where
-// cutting twice takes up to 3 x 2^-23).
-struct Parts3 { u4 p[3]; };
-__device__ inline Parts3 cut3(const float (&x)[8]) {
-  Parts3 r;
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    float a = x[2 * i], b = x[2 * i + 1];
-#pragma unroll
-    for (int k = 0; k < 3; k++) {
-      r.p[k][i] = hi16s(__float_as_uint(b), __float_as_uint(a));
-      if (k < 2) {
-        a -= __uint_as_float(__float_as_uint(a) & 0xffff0000u);
-        b -= __uint_as_float(__float_as_uint(b) & 0xffff0000u);
-      }
-    }
-  }
-  return r;
-}
-struct Parts2 { u4 p[2]; };
-__device__ inline Parts2 cut2(const float (&x)[8]) {
-  Parts2 r;
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const h2 hi = __builtin_convertvector(f2{x[2 * i], x[2 * i + 1]}, h2);
-    const h2 lo = __builtin_convertvector(f2{x[2 * i] - (float)hi.x, x[2 * i + 1] - (float)hi.y}, h2);
-    r.p[0][i] = __builtin_bit_cast(uint32_t, hi);
-    r.p[1][i] = __builtin_bit_cast(uint32_t, lo);
-  }
-  return r;
-}
-
-template <int T>
-__device__ inline f4 mfma16(u4 a, u4 b, f4 c) {
-  if constexpr (T != QLLAMA_KV_BF16)
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
 }
 
 // Waves that meet at most, as the registers allow.
