@@ -14,7 +14,10 @@ int pick(const QPagedKV *c, int rows, int n_req, int n_heads, int nodes) {
   if (nodes == 0) nodes = n_req ? (rows + n_req - 1) / n_req : 1;
   const int64_t cols = (int64_t)nodes * (n_heads / c->n_kv);
   if (c->head_dim > 128) return cols <= 64 ? 2 : 3;
-  return cols <= 16 ? 0 : cols <= 32 ? 1 : cols <= 64 ? 2 : 3;
+  if (cols <= 64) return cols <= 16 ? 0 : cols <= 32 ? 1 : 2;
+  // 128 columns a tile unless 64 leave fewer of them empty, by a sixth of all
+  const int64_t wide = (cols + 127) / 128 * 128, narrow = (cols + 63) / 64 * 64;
+  return 7 * narrow < 6 * wide ? 2 : 3;
 }
 
 }  // namespace
@@ -22,7 +25,7 @@ int pick(const QPagedKV *c, int rows, int n_req, int n_heads, int nodes) {
 extern "C" size_t qllama_tree_attention_work(const QPagedKV *c, int rows, int n_req, int n_heads, int nodes) {
   if (qs::bad_cache(c) || rows < 0 || n_req < 0 || n_heads < 1 || n_heads > 65535 || n_heads % c->n_kv || nodes < 0) return 0;
   const int hdp = c->head_dim <= 64 ? 64 : c->head_dim <= 128 ? 128 : 256, cols = 16 << pick(c, rows, n_req, n_heads, nodes);
-  return qtree::kShares * (sizeof(int4) + (size_t)2 * cols * (hdp + 2) * sizeof(float));
+  return qtree::kShares * sizeof(int4) + (size_t)(qtree::kShares * 16 / cols) * 2 * cols * (hdp + 2) * sizeof(float);
 }
 
 extern "C" int qllama_tree_attention(const QPagedKV *c, const QTreeQuery *a, void *stream) {
@@ -38,6 +41,7 @@ extern "C" int qllama_tree_attention(const QPagedKV *c, const QTreeQuery *a, voi
   if (a->width < 1 || a->table_stride < a->width || (int64_t)a->width * c->page_size > INT_MAX - 1024)   // a step past it still fits
     return qs::refuse(fn, "bad table width (width * page_size must be below 2^31 - 1024) or stride");
   if ((int64_t)a->rows * a->n_heads > INT_MAX) return qs::refuse(fn, "rows * n_heads must fit in 31 bits");
+  if (((double)a->rows * a->n_heads + c->n_kv) * a->n_req * ((double)a->width * c->page_size + 512) > 4e18) return qs::refuse(fn, "n_req * rows * width * page_size is too large");
   if (!(a->scale >= 0.0f) || a->scale > 2.35e38f)      // times log2 e within a float's range
     return qs::refuse(fn, "scale must be 0 .. 2.35e38");
   if (a->q == a->o) return qs::refuse(fn, "o must not be q");
@@ -60,6 +64,7 @@ extern "C" int qllama_tree_attention(const QPagedKV *c, const QTreeQuery *a, voi
   p.q_stride = a->q_stride; p.o_stride = a->o_stride; p.lse_stride = a->lse_stride; p.table_stride = a->table_stride;
   p.rows = a->rows; p.n_req = a->n_req; p.n_kv = c->n_kv; p.G = a->n_heads / c->n_kv; p.hd = c->head_dim;
   p.n_pages = c->n_pages; p.page_size = c->page_size; p.width = a->width; p.words = a->words;
+  p.wide = ((c->head_dim * es) | p.pst | p.hst | p.sst) % 16 == 0;
   p.qscale = (a->scale > 0.0f ? a->scale : 1.0f / __builtin_sqrtf((float)c->head_dim)) * 1.44269504089f;
   const int tile = pick(c, a->rows, a->n_req, a->n_heads, a->nodes);
   switch (c->type) {

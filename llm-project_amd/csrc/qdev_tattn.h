@@ -28,7 +28,7 @@
 
 namespace qtree {
 
-constexpr int kShares = 512;          // two blocks a CU; of eight waves, one
+constexpr int kShares = 2048;         // eight waves a CU; a share takes as many as lie side by side
 
 struct TaArgs {
   const char *k, *v;
@@ -43,6 +43,7 @@ struct TaArgs {
   long long scp, sch, scs;            // floats
   long long q_stride, o_stride, lse_stride, table_stride;
   int rows, n_req, n_kv, G, hd, n_pages, page_size, width, words;
+  int wide;                           // rows and strides are multiples of 16 bytes
   float qscale;                       // scale * log2(e)
 };
 
@@ -61,34 +62,38 @@ using namespace qpaged;
 using namespace qtree;
 
 
-// What a type, a padded head size, 16-column groups of a wave and waves side by side fix.
-template <int T, int HDP, int NC_, int CG_>
+// What a type, a padded head size, the waves side by side and the parts of a step's keys fix.
+template <int T, int HDP, int CG_, int KP_>
 struct Cfg {
-  static constexpr int NC = NC_, CG = CG_, WAVES = CG == 8 ? 8 : 4, THREADS = 64 * WAVES, KP = WAVES / CG, COLS = 16 * NC * CG;
-  static constexpr int SHARES = kShares * 4 / WAVES;
-  static constexpr int OVER = CG >= 4 ? 4 : 2;                          // steps that a tile's beginning and end take the time of
+  static constexpr int CG = CG_, KP = KP_, THREADS = 64 * CG * KP, COLS = 16 * CG;
+  static constexpr int SHARES = kShares / CG;
   static constexpr bool F32 = T == QLLAMA_KV_F32, HALF = T == QLLAMA_KV_F16;
   static constexpr int ES = F32 ? 4 : T == QLLAMA_KV_I8 ? 1 : 2;        // of an element in the cache
   static constexpr int LES = F32 ? 4 : 2;                               // in LDS (int8: bf16, which holds the codes)
   static constexpr int LT = T == QLLAMA_KV_I8 ? QLLAMA_KV_BF16 : T;     // the products' type
-  static constexpr int SUB = F32 ? 1 : 2, KS = 16 * SUB, STEP = KS * KP;      // keys of a wave's step and of a block's
+  static constexpr int SUB = F32 ? 1 : 2, KEYS = 16 * SUB;              // keys that a wave takes at a time
+  // times that it does between two barriers, as far as registers and LDS allow
+  static constexpr int TIMES = CG >= 4 && HDP <= 128 ? 2 : 1, KS = KEYS * TIMES, STEP = KS * KP;
+  static constexpr int OVER = 128 / STEP < 1 ? 1 : 128 / STEP;          // steps that a tile's beginning and end take the time of
   static constexpr int ROWB = HDP * LES, CH = ROWB / 16, SWZ = (CH < 16 ? CH : 16) - 1, EPC = 16 / LES;
   static constexpr int PARTB = 2 * KS * ROWB;                           // a part's keys, then values
   static constexpr int NBUF = CG == 1 ? 1 : 2;                          // a wave alone with its part needs no second buffer
-  static constexpr int TP = 64 * CG, U = 2 * KS * CH / TP;              // threads that stage a part, 16-byte units of each
+  // threads that stage a part, and units of each: 16 bytes of the cache, CPU chunks of 16 bytes in LDS
+  static constexpr int CPU = T == QLLAMA_KV_I8 ? 2 : 1, TP = 64 * CG, U = 2 * KS * CH / CPU / TP;
   static constexpr int DPL = HDP / 16, QC = F32 ? HDP / 16 : HDP / 32;
   static constexpr int PARTS = F32 ? 1 : HALF ? 2 : 3;
-  // a value row in LDS: piece x of lane (n, g) takes dims 16 PD x + PD n .. of key 4 g + j
-  static constexpr int PB = 4 * LES, PD = PB / LES, PIECES = HDP / (16 * PD), PW = PB / 4;
   // weights are held times this in f16 products: two parts then keep 23 bits down to 2^-17 of the largest and the rest to 2^-40
   static constexpr float RAISED = HALF ? 32768.0f : 1.0f;
-  // LDS: staged parts (and what waves hand over at a tile's end), places of the keys, scales, absent keys
-  static constexpr int HANDB = (KP / 2) * CG * NC * (DPL * 1024 + 512);
+  // LDS: staged parts (and what waves hand over at a tile's end), places of the keys, absent keys, scales
+  static constexpr int HANDB = (KP / 2) * CG * (DPL * 1024 + 512);
   static constexpr int STAGEB = NBUF * KP * PARTB > HANDB ? NBUF * KP * PARTB : HANDB;
-  static constexpr int OFFB = 4 * KP * KS * 8, SCALEB = T == QLLAMA_KV_I8 ? 2 * 2 * KP * KS * 4 : 0;
-  static constexpr int LDSB = STAGEB + OFFB + SCALEB + 4 * KP * 4;
-  static constexpr int PARTF = CG * NC * (DPL * 256 + 32);              // floats of a tile's part in the workspace
+  static constexpr int OFFB = 4 * KP * KS * 8, GONEB = 4 * KP * 8, SCALEB = T == QLLAMA_KV_I8 ? 2 * 2 * KP * KS * 4 : 0;
+  static constexpr int LDSB = STAGEB + OFFB + GONEB + SCALEB;
+  static constexpr int PARTF = CG * (DPL * 256 + 32);                   // floats of a tile's part in the workspace
 };
+
+typedef short s4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s4 s4_lds;
 
 // Rows of request r, and the first of them.
 __device__ inline int rows_of(const TaArgs &a, int r, int *first) {
@@ -136,31 +141,31 @@ __device__ inline bool odd_value(uint32_t x) {
 
 // The dim of a head whose output is element c of an accumulator's row `lane` of 16.
 template <typename C>
-__device__ inline int dim_of(int c, int lane) { return 16 * C::PD * (c / C::PD) + C::PD * lane + c % C::PD; }
+__device__ inline int dim_of(int c, int lane) { return C::F32 ? 64 * (c / 4) + 4 * lane + c % 4 : 16 * c + lane; }
 
-// A column's outputs from what a lane holds: dims c mod PD of the piece of lane 4 g + i.
+// A column's outputs from what a lane holds: rows 4 g .. of every accumulator.
 template <typename C>
 __device__ inline void put(float *o, const f4 (&acc)[C::DPL], int g, int hd, float by) {
   by *= 1.0f / C::RAISED;
 #pragma unroll
-  for (int i = 0; i < 4; i++)
-#pragma unroll
-    for (int c = 0; c < C::DPL; c += 4) {
-      const float x[4] = {acc[c][i] * by, acc[c + 1][i] * by, acc[c + 2][i] * by, acc[c + 3][i] * by};
-      const int d = dim_of<C>(c, 4 * g + i);
-      if (d < hd) __builtin_memcpy(o + d, x, sizeof x);
-    }
+  for (int i = 0; i < C::DPL; i++) {
+    const int k = i % 4, c = i - k;                   // f32: dims beside each other lie in four accumulators
+    const float x[4] = {(C::F32 ? acc[c][k] : acc[i][0]) * by, (C::F32 ? acc[c + 1][k] : acc[i][1]) * by,
+                        (C::F32 ? acc[c + 2][k] : acc[i][2]) * by, (C::F32 ? acc[c + 3][k] : acc[i][3]) * by};
+    const int d = C::F32 ? dim_of<C>(c, 4 * g + k) : dim_of<C>(i, 4 * g);
+    if (d < hd) __builtin_memcpy(o + d, x, sizeof x);
+  }
 }
 
 // WHOLE: a block takes whole tiles of request blockIdx.y.
-template <int T, int HDP, int NC, int CG, bool WHOLE>
-__global__ __launch_bounds__((Cfg<T, HDP, NC, CG>::THREADS), 2) void k_tree_attn(TaArgs a) {
-  using C = Cfg<T, HDP, NC, CG>;
-  constexpr int SUB = C::SUB, KS = C::KS, STEP = C::STEP, DPL = C::DPL, U = C::U, CH = C::CH, KP = C::KP;
+template <int T, int HDP, int CG, int KP, bool WHOLE>
+__global__ __launch_bounds__((Cfg<T, HDP, CG, KP>::THREADS), 2) void k_tree_attn(TaArgs a) {
+  using C = Cfg<T, HDP, CG, KP>;
+  constexpr int SUB = C::SUB, KS = C::KS, STEP = C::STEP, DPL = C::DPL, U = C::U, CH = C::CH;
   extern __shared__ __align__(16) char lds[];
   long long *offs = reinterpret_cast<long long *>(lds + C::STAGEB);                 // [4][KP][KS]: where a key lies, -1 for nowhere
-  float *scales = reinterpret_cast<float *>(lds + C::STAGEB + C::OFFB);             // [2][k, v][KP][KS]
-  uint32_t *gone = reinterpret_cast<uint32_t *>(lds + C::STAGEB + C::OFFB + C::SCALEB);       // [4][KP]: bits of keys that are nowhere
+  uint64_t *gone = reinterpret_cast<uint64_t *>(lds + C::STAGEB + C::OFFB);         // [4][KP]: bits of keys that are nowhere
+  float *scales = reinterpret_cast<float *>(lds + C::STAGEB + C::OFFB + C::GONEB);  // [2][k, v][KP][KS]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
   const int part = wave / CG, cg = wave % CG, tp = cg * 64 + lane;                  // tp: among the threads that stage the part
@@ -185,14 +190,15 @@ __global__ __launch_bounds__((Cfg<T, HDP, NC, CG>::THREADS), 2) void k_tree_attn
     steps = (len + STEP - 1) / STEP;
   };
 
-  long long u = 0, end = 0, share = 0, tile = 0;
+  long long u = 0, end = 0, share = 0;  // units from u up to end are this block's
+  int tile = 0;                         // fits: the host has checked rows * n_heads
   int at = 0;                           // units of the tile that shares before this one take
   if constexpr (WHOLE) {
     r = blockIdx.y;
     request(r);
     tile = blockIdx.x;
     u = tile;
-    end = (long long)ct * a.n_kv;
+    end = ct * a.n_kv;
   } else {
     const auto units_of = [&](int x) -> long long {
       if (x >= a.n_req) return 0;
@@ -200,12 +206,11 @@ __global__ __launch_bounds__((Cfg<T, HDP, NC, CG>::THREADS), 2) void k_tree_attn
       const int rows = rows_of(a, x, &i0), tokens = clamp_len(a.lens[x], a.width, a.page_size);
       return tokens ? (long long)((rows * a.G + C::COLS - 1) / C::COLS) * a.n_kv * ((tokens + STEP - 1) / STEP + C::OVER) : 0;
     };
-    long long upto = scan64(units_of(lane)), units = __shfl(upto, 63);
-    for (int x = 64; x < a.n_req; x += 64) units += __shfl(scan64(units_of(x + lane)), 63);
-    units = uniform(units);
-    share = (units + C::SHARES - 1) / C::SHARES;
+    long long upto = scan64(units_of(lane)), units = uniform(__shfl(upto, 63));            // of requests up to the lane's, 64 at a time
+    for (int x = 64; x < a.n_req; x += 64) units += uniform(__shfl(scan64(units_of(x + lane)), 63));
+    share = max((units + C::SHARES - 1) / C::SHARES, 2LL);
     u = blockIdx.x * share;
-    end = u + share < units ? u + share : units;
+    end = min(u + share, units);
     if (threadIdx.x == 0) a.split[blockIdx.x] = make_int4(0, 0, 0, 0);
     long long before = 0;               // units before the request
     for (; u < end; r += 64) {
@@ -221,8 +226,8 @@ __global__ __launch_bounds__((Cfg<T, HDP, NC, CG>::THREADS), 2) void k_tree_attn
     }
     if (u < end) {
       request(r);
-      tile = (u - before) / (steps + C::OVER);
-      at = (int)(u - before - tile * (steps + C::OVER));
+      tile = (int)((u - before) / (steps + C::OVER));
+      at = (int)(u - before - (long long)tile * (steps + C::OVER));
     }
   }
   const long long begin = u;
@@ -230,7 +235,7 @@ __global__ __launch_bounds__((Cfg<T, HDP, NC, CG>::THREADS), 2) void k_tree_attn
 
   while (u < end) {
     if constexpr (!WHOLE) {
-      if (tile == (long long)ct * a.n_kv) {           // the next request that has rows and tokens
+      if (tile == ct * a.n_kv) {           // the next request that has rows and tokens
         do request(++r); while (ct == 0 || steps == 0);
         tile = 0;
       }
@@ -239,7 +244,7 @@ __global__ __launch_bounds__((Cfg<T, HDP, NC, CG>::THREADS), 2) void k_tree_attn
     const int take = WHOLE ? 1 : (int)min(end - u, (long long)(steps + C::OVER - at));
     const int from = WHOLE ? 0 : max(at - C::OVER, 0), to = WHOLE ? steps : max(at + take - C::OVER, 0);
     if (!WHOLE && to == from) break;                  // the share ends before the tile's first step
-    const int kvh = (int)(tile / ct), c0 = (int)(tile - (long long)kvh * ct) * C::COLS;        // its first column
+    const int kvh = tile / ct, c0 = (tile - kvh * ct) * C::COLS;        // its first column
     const int cols = min(C::COLS, m * a.G - c0);
     const int ctx = max(len - m, 0);
     const int *table = a.table + r * a.table_stride;
@@ -251,402 +256,377 @@ __global__ __launch_bounds__((Cfg<T, HDP, NC, CG>::THREADS), 2) void k_tree_attn
       last = (int)min((long long)to, (keys + STEP - 1) / STEP);
     }
 
-    // ---- finding and staging keys and values
-    int entry = 0, place = 0, key = 0;                // of the lane's key in the step that is looked for next
-    if (looks) {
-      key = from * STEP + part * KS + (lane & (KS - 1));
-      entry = key / a.page_size;
-      place = key - entry * a.page_size;
-    }
+    // ---- finding and staging keys and values: in step s those of s + 1 are under way, the places of s + 2 are settled
+    // and the table entries of s + 3 asked for
+    // (every wave asks, so that nothing waits where the paths of the one that writes and the others meet)
+    int key = from * STEP + part * KS + lane % KS, entry = key / a.page_size, place = key - entry * a.page_size;       // asked for next
     const int last_entry = len > 0 ? (len - 1) / a.page_size : 0;
-    const auto look = [&](int ahead) -> int {         // the table entry of the step that is settled next, or the one behind it
-      const int e = ahead ? entry + step_e + (place + step_p >= a.page_size) : entry;
-      return len > 0 ? table[min(e, last_entry)] : -1;
-    };
-    int page1 = 0, place1 = 0, page1_a = 0, place1_a = 0;       // where the scales of the lane's key lie, of the step settled last and the first
-    const auto settle = [&](int s, int page) {
-      const bool there = key < len && page >= 0 && page < a.n_pages;
-      if (lane < KS) offs[((s & 3) * KP + part) * KS + lane] = there ? page * a.pst + place * a.sst : -1;
-      const uint64_t no = __ballot(!there);
-      if (lane == 0) gone[(s & 3) * KP + part] = (uint32_t)no & (KS == 32 ? ~0u : 0xffffu);
-      page1 = there ? page : 0;
-      place1 = there ? place : 0;
+    int page_at = 0, key_at = 0, place_at = 0;        // asked for: a table entry, its key and the key's place
+    const auto ask = [&] {
+      page_at = table[min(entry, last_entry)];        // there is a token
+      key_at = key;
+      place_at = place;
       key += STEP;
       entry += step_e;
       place += step_p;
       if (place >= a.page_size) { place -= a.page_size; entry++; }
     };
+    const auto settle = [&](int s) -> long long {     // where the lane's scales lie
+      const bool there = key_at < len && page_at >= 0 && page_at < a.n_pages;
+      const long long off = there ? page_at * a.pst + place_at * a.sst : -1;
+      const uint64_t no = __ballot(!there);
+      if (looks) {
+        if (lane < KS) offs[((s & 3) * KP + part) * KS + lane] = off;
+        if (lane == 0) gone[(s & 3) * KP + part] = no;
+      }
+      return T == QLLAMA_KV_I8 ? (there ? page_at : 0) * a.scp + kvh * a.sch + (there ? place_at : 0) * a.scs : 0;
+    };
     u4 staged[U];
     uint32_t dead = 0;                                // units of no key, or of no dim
-    float ks1 = 0.0f, vs1 = 0.0f;
-    const auto issue = [&](int s, int scale_page, int scale_place) {
+    constexpr int UNITS = KS * CH / C::CPU, PER = CH / C::CPU;                 // of a part's keys, of a row
+    const auto issue = [&](int s) {
       dead = 0;
 #pragma unroll
       for (int x = 0; x < U; x++) {
-        const int unit = tp + x * C::TP, is_v = unit >= KS * CH, at = is_v ? unit - KS * CH : unit;
-        const int row = at / CH, d = (at % CH) * C::EPC;
+        const int unit = tp + x * C::TP, is_v = unit >= UNITS, at = is_v ? unit - UNITS : unit;
+        const int row = at / PER, d = (at % PER) * C::EPC * C::CPU;
         const long long off = offs[((s & 3) * KP + part) * KS + row];
         const bool no = off < 0 || d >= a.hd;
         const char *p = (is_v ? vbase : kbase) + (no ? 0 : off + d * C::ES);
         if (no) dead |= 1u << x;
         if constexpr (T == QLLAMA_KV_I8) {
-          const u2 w = *reinterpret_cast<const u2 *>(p);
-          staged[x][0] = w.x;
-          staged[x][1] = w.y;
+          const bool half = no || d + 8 >= a.hd;      // the row may end within the 16 codes
+          if (half) dead |= 0x10000u << x;
+          if (a.wide) {
+            staged[x] = *reinterpret_cast<const u4 *>(p);
+          } else {
+            const u2 lo = *reinterpret_cast<const u2 *>(p), hi = *reinterpret_cast<const u2 *>(half ? p : p + 8);
+            staged[x] = u4{lo.x, lo.y, hi.x, hi.y};
+          }
         } else {
           staged[x] = *reinterpret_cast<const u4 *>(p);
         }
       }
-      if constexpr (T == QLLAMA_KV_I8) {
-        if (looks) {
-          const long long at = scale_page * a.scp + kvh * a.sch + scale_place * a.scs;
-          ks1 = a.ks[at];
-          vs1 = a.vs[at];
-        }
-      }
     };
+    uint32_t odd = 0;                                 // whether a new token's value was not finite
     const auto write = [&](int s) {
+      const bool fresh = s * STEP + (part + 1) * KS > ctx;        // new tokens among the part's keys
       char *to_lds = lds + (C::NBUF == 1 ? part : (s & 1) * KP + part) * C::PARTB;
 #pragma unroll
       for (int x = 0; x < U; x++) {
-        const int unit = tp + x * C::TP, is_v = unit >= KS * CH, at = is_v ? unit - KS * CH : unit;
-        const int row = at / CH, chunk = at % CH;
-        u4 w = staged[x];
+        const int unit = tp + x * C::TP, is_v = unit >= UNITS, at = is_v ? unit - UNITS : unit;
+        const int row = at / PER, chunk = at % PER * C::CPU;
+        char *to = to_lds + is_v * KS * C::ROWB + row * C::ROWB;
         if constexpr (T == QLLAMA_KV_I8) {            // bf16 holds a code
-          const uint32_t b[2] = {w[0], w[1]};
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const int b0 = (int)(b[i / 2] << (24 - 16 * (i % 2))) >> 24, b1 = (int)(b[i / 2] << (16 - 16 * (i % 2))) >> 24;
-            w[i] = hi16s(__float_as_uint((float)b1), __float_as_uint((float)b0));
+          for (int h = 0; h < 2; h++) {
+            u4 w;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const uint32_t b = staged[x][2 * h + i / 2] >> (16 * (i % 2));
+              w[i] = hi16s(__float_as_uint((float)(signed char)(b >> 8)), __float_as_uint((float)(signed char)b));
+            }
+            if (dead >> (x + 16 * h) & 1) w = u4{0, 0, 0, 0};
+            *reinterpret_cast<u4 *>(to + (((chunk + h) ^ (row & C::SWZ)) << 4)) = w;
           }
-        }
-        if (dead >> x & 1) w = u4{0, 0, 0, 0};
-        *reinterpret_cast<u4 *>(to_lds + is_v * KS * C::ROWB + row * C::ROWB + ((chunk ^ (row & C::SWZ)) << 4)) = w;
-      }
-      if constexpr (T == QLLAMA_KV_I8) {
-        if (looks && lane < KS) {
-          float *to = scales + ((s & 1) * 2 * KP + part) * KS + lane;
-          to[0] = ks1;
-          to[KP * KS] = vs1;
+        } else {
+          u4 w = staged[x];
+          if (dead >> x & 1) w = u4{0, 0, 0, 0};
+          if (fresh && is_v) {                        // what is not finite must not reach the columns that do not see it
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const uint32_t all = w[i];
+              if constexpr (C::F32) {
+                w[i] = odd_value<T>(all) ? 0 : all;
+              } else {
+                w[i] = (odd_value<T>(all & 0xffffu) ? 0 : all & 0xffffu) | (odd_value<T>(all >> 16) ? 0 : all & 0xffff0000u);
+              }
+              odd |= w[i] ^ all;
+            }
+          }
+          *reinterpret_cast<u4 *>(to + ((chunk ^ (row & C::SWZ)) << 4)) = w;
         }
       }
     };
+    const auto write_scales = [&](int s, float k, float v) {
+      if (looks && lane < KS) {
+        float *to = scales + ((s & 1) * 2 * KP + part) * KS + lane;
+        to[0] = k;
+        to[KP * KS] = v;
+      }
+    };
 
-    // both table entries, then the queries, then the first keys and values are under way; the queries are cut meanwhile
-    const bool any = from < last, live = cg * 16 * NC < cols;
-    const auto col_of = [&](int x) -> int { return c0 + min(cg * 16 * NC + 16 * x + n, cols - 1); };         // columns past the last repeat it
-    const auto row_of = [&](int x) -> int { return col_of(x) / a.G; };
-    const auto head_of = [&](int x) -> int { return kvh * a.G + col_of(x) % a.G; };
-    int page_a = -1, page_b = -1;
-    if (any && looks) {
-      page_a = look(0);
-      page_b = look(1);
-    }
+    // table entries, then the queries, then the first keys and values are under way; the queries are cut meanwhile
+    const bool any = from < last, live = cg * 16 < cols;
+    const int col = c0 + min(cg * 16 + n, cols - 1);  // the lane's column; those past the last repeat it
+    const int row = first + col / a.G, head = kvh * a.G + col % a.G;
     constexpr int QE = C::F32 ? 4 : 8;
-    float f[NC][C::QC][QE];
+    float f[C::QC][QE];
+    long long scale_at = 0, scale_next = 0;           // of the steps that are settled
+    {
+      int pages[2], keys[2], places[2];
+      if (any) {
 #pragma unroll
-    for (int x = 0; x < NC; x++) {
-      const float *q = a.q + (first + row_of(x)) * a.q_stride + (long long)head_of(x) * a.hd;
+        for (int i = 0; i < 2; i++) {
+          ask();
+          pages[i] = page_at; keys[i] = key_at; places[i] = place_at;
+        }
+        ask();
+      }
+      const float *q = a.q + row * a.q_stride + (long long)head * a.hd;
 #pragma unroll
       for (int c = 0; c < C::QC; c++) {
         const int d = 4 * QE * c + QE * g;
-        __builtin_memcpy(f[x][c], q + (d < a.hd ? d : 0), sizeof f[x][c]);       // 4-byte aligned
+        __builtin_memcpy(f[c], q + (d < a.hd ? d : 0), sizeof f[c]);             // 4-byte aligned
+      }
+      if (any) {
+        const int p2 = page_at, k2 = key_at, x2 = place_at;
+        page_at = pages[0]; key_at = keys[0]; place_at = places[0];
+        scale_at = settle(from);
+        page_at = pages[1]; key_at = keys[1]; place_at = places[1];
+        scale_next = settle(from + 1);
+        page_at = p2; key_at = k2; place_at = x2;
       }
     }
-    if (any && looks) {
-      settle(from, page_a);
-      page1_a = page1; place1_a = place1;
-      settle(from + 1, page_b);
-    }
     sync();
-    if (any) issue(from, page1_a, place1_a);
+    float ks1 = 0.0f, vs1 = 0.0f;
+    if (any) {
+      issue(from);
+      if constexpr (T == QLLAMA_KV_I8) {
+        ks1 = a.ks[scale_at];
+        vs1 = a.vs[scale_at];
+      }
+    }
 
     // the wave's queries, as parts of 16 bits
-    u4 qp[NC][C::QC][C::PARTS];
-    float unscale[NC];
+    u4 qp[C::QC][C::PARTS];
+    float unscale = 1.0f, most = 0.0f;
 #pragma unroll
-    for (int x = 0; x < NC; x++) {
-      unscale[x] = 1.0f;
-      float most = 0.0f;
+    for (int c = 0; c < C::QC; c++)
+#pragma unroll
+      for (int e = 0; e < QE; e++) {
+        f[c][e] = 4 * QE * c + QE * g < a.hd ? f[c][e] * a.qscale : 0.0f;
+        most = fmaxf(most, fabsf(f[c][e]));
+      }
+    if constexpr (C::HALF) {                          // into f16's range, by a power of two
+      most = max_groups(most);
+      const int e = most > 0.0f && most < __builtin_inff() ? ilogbf(most) - 13 : 0;
+      unscale = ldexpf(1.0f, e);
 #pragma unroll
       for (int c = 0; c < C::QC; c++)
 #pragma unroll
-        for (int e = 0; e < QE; e++) {
-          f[x][c][e] = 4 * QE * c + QE * g < a.hd ? f[x][c][e] * a.qscale : 0.0f;
-          most = fmaxf(most, fabsf(f[x][c][e]));
-        }
-      if constexpr (C::HALF) {                        // into f16's range, by a power of two
-        most = max_groups(most);
-        const int e = most > 0.0f && most < __builtin_inff() ? ilogbf(most) - 13 : 0;
-        unscale[x] = ldexpf(1.0f, e);
+        for (int i = 0; i < QE; i++) f[c][i] = ldexpf(f[c][i], -e);
+    }
 #pragma unroll
-        for (int c = 0; c < C::QC; c++)
+    for (int c = 0; c < C::QC; c++) {
+      if constexpr (C::F32) {
 #pragma unroll
-          for (int i = 0; i < QE; i++) f[x][c][i] = ldexpf(f[x][c][i], -e);
-      }
+        for (int e = 0; e < QE; e++) qp[c][0][e] = __float_as_uint(f[c][e]);
+      } else if constexpr (C::HALF) {
+        const Parts2 y = cut2(f[c]);
 #pragma unroll
-      for (int c = 0; c < C::QC; c++) {
-        if constexpr (C::F32) {
+        for (int p = 0; p < C::PARTS; p++) qp[c][p] = y.p[p];
+      } else {
+        const Parts3 y = cut3(f[c]);
 #pragma unroll
-          for (int e = 0; e < QE; e++) qp[x][c][0][e] = __float_as_uint(f[x][c][e]);
-        } else if constexpr (C::HALF) {
-          const Parts2 y = cut2(f[x][c]);
-#pragma unroll
-          for (int p = 0; p < C::PARTS; p++) qp[x][c][p] = y.p[p];
-        } else {
-          const Parts3 y = cut3(f[x][c]);
-#pragma unroll
-          for (int p = 0; p < C::PARTS; p++) qp[x][c][p] = y.p[p];
-        }
+        for (int p = 0; p < C::PARTS; p++) qp[c][p] = y.p[p];
       }
     }
 
-    float top[NC], sum[NC];                           // of the lane's columns; sum over the lane's keys
-    f4 acc[NC][DPL];
+    float top = kNegInf, sum = 0.0f;                  // of the lane's column; sum over the lane's keys
+    f4 acc[DPL];
 #pragma unroll
-    for (int x = 0; x < NC; x++) {
-      top[x] = kNegInf;
-      sum[x] = 0.0f;
-#pragma unroll
-      for (int c = 0; c < DPL; c++) acc[x][c] = f4{0, 0, 0, 0};
-    }
+    for (int c = 0; c < DPL; c++) acc[c] = f4{0, 0, 0, 0};
 
-    bool odd = false;                                 // a new token's value was not finite
-    const auto compute = [&](int s) {
-      const char *kl = lds + (C::NBUF == 1 ? part : (s & 1) * KP + part) * C::PARTB, *vl = kl + KS * C::ROWB;
-      const int key0 = s * STEP + part * KS;
-      f4 d[NC][SUB];
+    // keys KEYS t .. of step s's part
+    const auto compute = [&](int s, int t) {
+      const char *kl = lds + (C::NBUF == 1 ? part : (s & 1) * KP + part) * C::PARTB + t * C::KEYS * C::ROWB, *vl = kl + KS * C::ROWB;
+      const int key0 = s * STEP + part * KS + t * C::KEYS;
+      u4 kf[C::QC][SUB];
 #pragma unroll
-      for (int x = 0; x < NC; x++)
+      for (int c = 0; c < C::QC; c++)
 #pragma unroll
-        for (int i = 0; i < SUB; i++) d[x][i] = f4{0, 0, 0, 0};
+        for (int i = 0; i < SUB; i++) kf[c][i] = *reinterpret_cast<const u4 *>(kl + (16 * i + n) * C::ROWB + (((4 * c + g) ^ (n & C::SWZ)) << 4));
+      __builtin_amdgcn_sched_barrier(0);              // all under way before the first product
+      f4 d[SUB];
+#pragma unroll
+      for (int i = 0; i < SUB; i++) d[i] = f4{0, 0, 0, 0};
 #pragma unroll
       for (int c = 0; c < C::QC; c++)
 #pragma unroll
         for (int i = 0; i < SUB; i++) {
-          const u4 kk = *reinterpret_cast<const u4 *>(kl + (16 * i + n) * C::ROWB + (((4 * c + g) ^ (n & C::SWZ)) << 4));
+          if constexpr (C::F32) {
 #pragma unroll
-          for (int x = 0; x < NC; x++) {
-            if constexpr (C::F32) {
+            for (int e = 0; e < 4; e++)
+              d[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[c][i][e]), __uint_as_float(qp[c][0][e]), d[i], 0, 0, 0);
+          } else {
 #pragma unroll
-              for (int e = 0; e < 4; e++)
-                d[x][i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kk[e]), __uint_as_float(qp[x][c][0][e]), d[x][i], 0, 0, 0);
-            } else {
-#pragma unroll
-              for (int p = 0; p < C::PARTS; p++) d[x][i] = mfma16<C::LT>(kk, qp[x][c][p], d[x][i]);
-            }
+            for (int p = 0; p < C::PARTS; p++) d[i] = mfma16<C::LT>(kf[c][i], qp[c][p], d[i]);
           }
         }
 
-      f4 fk[SUB], fv[SUB];
+      f4 fv[SUB];
       if constexpr (T == QLLAMA_KV_I8) {
-        const float *f = scales + ((s & 1) * 2 * KP + part) * KS;
+        const float *f = scales + ((s & 1) * 2 * KP + part) * KS + t * C::KEYS;
 #pragma unroll
         for (int i = 0; i < SUB; i++) {
-          fk[i] = *reinterpret_cast<const f4 *>(f + 16 * i + 4 * g);
+          d[i] *= *reinterpret_cast<const f4 *>(f + 16 * i + 4 * g);
           fv[i] = *reinterpret_cast<const f4 *>(f + KP * KS + 16 * i + 4 * g);
         }
       }
+      if constexpr (C::HALF) {
 #pragma unroll
-      for (int x = 0; x < NC; x++)
-#pragma unroll
-        for (int i = 0; i < SUB; i++) {
-          if constexpr (C::HALF) d[x][i] *= unscale[x];
-          if constexpr (T == QLLAMA_KV_I8) d[x][i] *= fk[i];
-        }
-
-      const uint32_t none = __builtin_amdgcn_readfirstlane(gone[(s & 3) * KP + part]);
-      const bool masked = none != 0 || key0 + KS > ctx;          // one for the wave
-      uint32_t seen[NC];
-      if (masked) {
-#pragma unroll
-        for (int x = 0; x < NC; x++) {
-          seen[x] = seen_of(a, first + row_of(x), row_of(x), key0 - ctx) & ~none;
-#pragma unroll
-          for (int i = 0; i < SUB; i++)
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-              if (!(seen[x] >> (16 * i + 4 * g + j) & 1)) d[x][i][j] = kNegInf;
-        }
+        for (int i = 0; i < SUB; i++) d[i] *= unscale;
       }
-
-      float up[NC];
-      bool more = false;
-#pragma unroll
-      for (int x = 0; x < NC; x++) {
-        up[x] = d[x][0][0];
+      const uint32_t none = __builtin_amdgcn_readfirstlane((uint32_t)(gone[(s & 3) * KP + part] >> (t * C::KEYS)) & (C::KEYS == 32 ? ~0u : 0xffffu));
+      if (none != 0 || key0 + C::KEYS > ctx) {        // one for the wave
+        const uint32_t seen = seen_of(a, row, row - first, key0 - ctx) & ~none;
 #pragma unroll
         for (int i = 0; i < SUB; i++)
 #pragma unroll
-          for (int j = 0; j < 4; j++) up[x] = fmaxf(up[x], d[x][i][j]);
-        up[x] = fmaxf(top[x], max_groups(up[x]));
-        more |= up[x] > top[x];
-      }
-      if (__any(more)) {                              // rare after the first steps
-#pragma unroll
-        for (int x = 0; x < NC; x++) {
-          const float by = top[x] == kNegInf ? 0.0f : __builtin_amdgcn_exp2f(top[x] - up[x]);
-          sum[x] *= top[x] == kNegInf ? 1.0f : by;    // a sum without a maximum is 0, or the NaN of its scores
-#pragma unroll
-          for (int c = 0; c < DPL; c++) acc[x][c] *= top[x] == kNegInf ? 1.0f : by;
-          top[x] = up[x];
-        }
-      }
-      u4 pp[NC][C::PARTS];
-      float p32[NC][4];
-#pragma unroll
-      for (int x = 0; x < NC; x++) {
-        const float ref = top[x] == kNegInf ? 0.0f : top[x];
-        float p[8];
-#pragma unroll
-        for (int i = 0; i < SUB; i++)
-#pragma unroll
-          for (int j = 0; j < 4; j++) {
-            float w = __builtin_amdgcn_exp2f(d[x][i][j] - ref);
-            sum[x] += w;
-            if constexpr (T == QLLAMA_KV_I8) {
-              w *= fv[i][j];
-              if (masked && !(seen[x] >> (16 * i + 4 * g + j) & 1)) w = 0.0f;        // whatever the scale is
+          for (int j = 0; j < 4; j++)
+            if (!(seen >> (16 * i + 4 * g + j) & 1)) {
+              d[i][j] = kNegInf;
+              if constexpr (T == QLLAMA_KV_I8) fv[i][j] = 0.0f;          // whatever the scale is
             }
-            if constexpr (C::F32) p32[x][j] = w;
-            else p[4 * i + j] = w * C::RAISED;
-          }
-        if constexpr (C::HALF) {
-          const Parts2 y = cut2(p);
+      }
+      float up = d[0][0];
 #pragma unroll
-          for (int k = 0; k < C::PARTS; k++) pp[x][k] = y.p[k];
-        } else if constexpr (!C::F32) {
-          const Parts3 y = cut3(p);
+      for (int i = 0; i < SUB; i++)
 #pragma unroll
-          for (int k = 0; k < C::PARTS; k++) pp[x][k] = y.p[k];
+        for (int j = 0; j < 4; j++) up = fmaxf(up, d[i][j]);
+      up = fmaxf(top, max_groups(up));
+      if (__any(up > top)) {                          // rare after the first steps
+        const float by = top == kNegInf ? 1.0f : __builtin_amdgcn_exp2f(top - up);     // without a maximum all is 0, or the NaN of its scores
+        sum *= by;
+#pragma unroll
+        for (int c = 0; c < DPL; c++) acc[c] *= by;
+        top = up;
+      }
+      const float ref = top == kNegInf ? 0.0f : top;
+      u4 pp[C::PARTS];
+      float p[4 * SUB];
+#pragma unroll
+      for (int i = 0; i < SUB; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          float w = __builtin_amdgcn_exp2f(d[i][j] - ref);
+          sum += w;
+          if constexpr (T == QLLAMA_KV_I8) w *= fv[i][j];
+          p[4 * i + j] = C::HALF ? w * C::RAISED : w;
         }
+      if constexpr (C::HALF) {
+        const Parts2 y = cut2(p);
+#pragma unroll
+        for (int k = 0; k < C::PARTS; k++) pp[k] = y.p[k];
+      } else if constexpr (!C::F32) {
+        const Parts3 y = cut3(p);
+#pragma unroll
+        for (int k = 0; k < C::PARTS; k++) pp[k] = y.p[k];
       }
 
-      const bool fresh = T != QLLAMA_KV_I8 && key0 + KS > ctx && key0 < len;        // new tokens among the keys
+      if constexpr (C::F32) {
 #pragma unroll
-      for (int y = 0; y < C::PIECES; y++) {
-        uint32_t v[SUB][4][C::PW];
-#pragma unroll
-        for (int i = 0; i < SUB; i++)
+        for (int y = 0; y < DPL / 4; y++)             // dims 64 y + 4 n .. of the lane's 4 keys
 #pragma unroll
           for (int j = 0; j < 4; j++) {
-            const int byte = C::PB * (16 * y + n), row = 16 * i + 4 * g + j;
-            __builtin_memcpy(v[i][j], __builtin_assume_aligned(vl + row * C::ROWB + (((byte >> 4) ^ ((4 * g + j) & C::SWZ)) << 4) + (byte & 15), C::PB), C::PB);
+            const f4 v = *reinterpret_cast<const f4 *>(vl + (4 * g + j) * C::ROWB + (((16 * y + n) ^ ((4 * g + j) & C::SWZ)) << 4));
+#pragma unroll
+            for (int c = 0; c < 4; c++) acc[4 * y + c] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[c], p[j], acc[4 * y + c], 0, 0, 0);
           }
-        if (fresh) {                                  // what is not finite must not reach the columns that do not see it
+      } else {
+        // a transposing read: lane n of a group names row n / 4 and 4 dims of it, and gets dim n of the group's 4 keys
+        const int row = 4 * g + n / 4;
+        const char *at = vl + row * C::ROWB + n % 2 * 8;
+        const int turn = (n % 4 / 2) ^ (row & C::SWZ);
 #pragma unroll
-          for (int i = 0; i < SUB; i++)
+        for (int c = 0; c < DPL; c++) {
+          u4 vv;                                      // dim 16 c + n, 8 keys
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-#pragma unroll
-              for (int w = 0; w < C::PW; w++) {
-                uint32_t &x = v[i][j][w];
-                if constexpr (C::F32) {
-                  if (odd_value<T>(x)) { x = 0; odd = true; }
-                } else {
-                  if (odd_value<T>(x & 0xffffu)) { x &= 0xffff0000u; odd = true; }
-                  if (odd_value<T>(x >> 16)) { x &= 0xffffu; odd = true; }
-                }
-              }
-        }
-#pragma unroll
-        for (int c = 0; c < C::PD; c++) {
-          const int at = y * C::PD + c;
-          if constexpr (C::F32) {
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-#pragma unroll
-              for (int x = 0; x < NC; x++)
-                acc[x][at] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[0][j][c]), p32[x][j], acc[x][at], 0, 0, 0);
-          } else {
-            u4 vv;                                    // dim c of the lane's piece, 8 keys
-#pragma unroll
-            for (int i = 0; i < SUB; i++)
-#pragma unroll
-              for (int j = 0; j < 2; j++) {
-                const uint32_t lo = v[i][2 * j][c / 2], hi = v[i][2 * j + 1][c / 2];
-                vv[2 * i + j] = c % 2 ? hi16s(hi, lo) : lo16s(hi, lo);
-              }
-#pragma unroll
-            for (int x = 0; x < NC; x++)
-#pragma unroll
-              for (int k = 0; k < C::PARTS; k++) acc[x][at] = mfma16<C::LT>(vv, pp[x][k], acc[x][at]);
+          for (int i = 0; i < SUB; i++) {
+            const u2 y = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4_lds *)(at + 16 * i * C::ROWB + (((2 * c) ^ turn) << 4))));
+            vv[2 * i] = y.x;
+            vv[2 * i + 1] = y.y;
           }
+#pragma unroll
+          for (int k = 0; k < C::PARTS; k++) acc[c] = mfma16<C::LT>(vv, pp[k], acc[c]);
         }
       }
     };
 
-    if (any) write(from);
+    if (any) {
+      write(from);
+      if constexpr (T == QLLAMA_KV_I8) {
+        write_scales(from, ks1, vs1);
+      }
+    }
     sync();
     for (int s = from; s < last; s++) {
-      int page = 0;
       if (s + 1 < last) {
-        issue(s + 1, page1, place1);
-        if (looks) page = look(0);                    // of step s + 2
+        // before the loads below: what this waits for is older than they
+        if constexpr (T == QLLAMA_KV_I8) { ks1 = a.ks[scale_next]; vs1 = a.vs[scale_next]; }
+        scale_next = settle(s + 2);
+        ask();
+        issue(s + 1);
       }
-      if (live) compute(s);
+      if (live) {
+#pragma unroll
+        for (int t = 0; t < C::TIMES; t++) compute(s, t);
+      }
       if (s + 1 < last) {
-        if (looks) settle(s + 2, page);
         write(s + 1);
+        if constexpr (T == QLLAMA_KV_I8) {
+          write_scales(s + 1, ks1, vs1);
+        }
       }
       sync();
     }
 
     // ---- values of new tokens that are not finite: NaN where they are seen
-    if (live && __any(odd)) {
+    bool found = false;
+    if constexpr (T != QLLAMA_KV_I8) found = CG == 1 ? __any(odd != 0) : __syncthreads_or(odd != 0);
+    if (live && found) {
 #pragma unroll 1
       for (int s = from; s < last; s++) {
         const int key0 = s * STEP + part * KS;
 #pragma unroll 1
         for (int k = max(key0, ctx); k < min(key0 + KS, len); k++) {
           const int page = table[k / a.page_size];
-          if (page < 0 || page >= a.n_pages) continue;
+          if (page < 0 || page >= a.n_pages || !(seen_of(a, row, row - first, k - ctx) & 1)) continue;
           const char *v = vbase + page * a.pst + k % a.page_size * a.sst;
 #pragma unroll
-          for (int x = 0; x < NC; x++) {
-            const int i = row_of(x);
-            if (!(seen_of(a, first + i, i, k - ctx) & 1)) continue;
+          for (int j = 0; j < 4; j++)
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-#pragma unroll
-              for (int c = 0; c < DPL; c++) {
-                const int d = dim_of<C>(c, 4 * g + j);
-                if (d < a.hd && odd_value<T>(C::F32 ? reinterpret_cast<const uint32_t *>(v)[d] : reinterpret_cast<const unsigned short *>(v)[d]))
-                  acc[x][c][j] = __builtin_nanf("");
-              }
-          }
+            for (int c = 0; c < DPL; c++) {
+              const int d = dim_of<C>(c, 4 * g + j);
+              if (d < a.hd && odd_value<T>(C::F32 ? reinterpret_cast<const uint32_t *>(v)[d] : reinterpret_cast<const unsigned short *>(v)[d]))
+                acc[c][j] = __builtin_nanf("");
+            }
         }
       }
     }
 
     // ---- parts of the keys meet, two by two; the first part's waves hold the tile then
-#pragma unroll
-    for (int x = 0; x < NC; x++) sum[x] = sum_groups(sum[x]);
+    sum = sum_groups(sum);
     if constexpr (KP > 1) {
       if constexpr (CG == 1) __syncthreads();
 #pragma unroll
       for (int half = KP / 2; half; half /= 2) {
         if (part >= half && part < 2 * half && live) {
-          char *at = lds + ((part - half) * CG + cg) * (NC * (DPL * 1024 + 512));
+          char *at = lds + ((part - half) * CG + cg) * (DPL * 1024 + 512);
 #pragma unroll
-          for (int x = 0; x < NC; x++) {
-#pragma unroll
-            for (int c = 0; c < DPL; c++) *reinterpret_cast<f4 *>(at + ((x * DPL + c) * 64 + lane) * 16) = acc[x][c];
-            *reinterpret_cast<f2 *>(at + NC * DPL * 1024 + (x * 64 + lane) * 8) = f2{top[x], sum[x]};
-          }
+          for (int c = 0; c < DPL; c++) *reinterpret_cast<f4 *>(at + (c * 64 + lane) * 16) = acc[c];
+          *reinterpret_cast<f2 *>(at + DPL * 1024 + lane * 8) = f2{top, sum};
         }
         __syncthreads();
         if (part < half && live) {
-          const char *at = lds + (part * CG + cg) * (NC * (DPL * 1024 + 512));
+          const char *at = lds + (part * CG + cg) * (DPL * 1024 + 512);
+          const f2 other = *reinterpret_cast<const f2 *>(at + DPL * 1024 + lane * 8);
+          const float up = fmaxf(top, other.x), mine = part_weight(top, up), its = part_weight(other.x, up);
+          sum = sum * mine + other.y * its;
+          top = up;
 #pragma unroll
-          for (int x = 0; x < NC; x++) {
-            const f2 other = *reinterpret_cast<const f2 *>(at + NC * DPL * 1024 + (x * 64 + lane) * 8);
-            const float up = fmaxf(top[x], other.x), mine = part_weight(top[x], up), its = part_weight(other.x, up);
-            sum[x] = sum[x] * mine + other.y * its;
-            top[x] = up;
-#pragma unroll
-            for (int c = 0; c < DPL; c++) acc[x][c] = acc[x][c] * mine + *reinterpret_cast<const f4 *>(at + ((x * DPL + c) * 64 + lane) * 16) * its;
-          }
+          for (int c = 0; c < DPL; c++) acc[c] = acc[c] * mine + *reinterpret_cast<const f4 *>(at + (c * 64 + lane) * 16) * its;
         }
         __syncthreads();
       }
@@ -654,32 +634,28 @@ __global__ __launch_bounds__((Cfg<T, HDP, NC, CG>::THREADS), 2) void k_tree_attn
 
     const bool whole = from == 0 && to == steps;
     if (part == 0 && live) {
+      if (WHOLE || whole) {
+        if (cg * 16 + n < cols) {
+          put<C>(a.o + row * a.o_stride + (long long)head * a.hd, acc, g, a.hd, sum == 0.0f ? 0.0f : 1.0f / sum);
+          if (g == 0 && a.lse) a.lse[row * a.lse_stride + head] = sum == 0.0f ? kNegInf : (top + __builtin_amdgcn_logf(sum)) * 0.69314718056f;
+        }
+      } else {
+        float *o = a.part + ((long long)blockIdx.x * 2 + (u == begin ? 0 : 1)) * C::PARTF;
 #pragma unroll
-      for (int x = 0; x < NC; x++) {
-        if (WHOLE || whole) {
-          if (cg * 16 * NC + 16 * x + n < cols) {
-            const long long i = first + row_of(x);
-            put<C>(a.o + i * a.o_stride + (long long)head_of(x) * a.hd, acc[x], g, a.hd, sum[x] == 0.0f ? 0.0f : 1.0f / sum[x]);
-            if (g == 0 && a.lse) a.lse[i * a.lse_stride + head_of(x)] = sum[x] == 0.0f ? kNegInf : (top[x] + __builtin_amdgcn_logf(sum[x])) * 0.69314718056f;
-          }
-        } else {
-          float *o = a.part + ((long long)blockIdx.x * 2 + (u == begin ? 0 : 1)) * C::PARTF;
-#pragma unroll
-          for (int c = 0; c < DPL; c++) *reinterpret_cast<f4 *>(o + (((cg * NC + x) * DPL + c) * 64 + lane) * 4) = acc[x][c];
-          if (g == 0) {
-            o += CG * NC * DPL * 256 + (cg * NC + x) * 32 + n;
-            o[0] = top[x];
-            o[16] = sum[x];
-          }
+        for (int c = 0; c < DPL; c++) *reinterpret_cast<f4 *>(o + ((cg * DPL + c) * 64 + lane) * 4) = acc[c];
+        if (g == 0) {
+          o += CG * DPL * 256 + cg * 32 + n;
+          o[0] = top;
+          o[16] = sum;
         }
       }
     }
     if constexpr (WHOLE) {
       u += gridDim.x;
-      tile = u;
+      tile = (int)u;
     } else {
       if (from == 0 && !whole && threadIdx.x == 0)    // the tile goes on in the shares behind this one
-        a.split[blockIdx.x] = make_int4(1 + (int)((steps - to + share - 1) / share), r, (int)tile, u == begin ? 0 : 1);
+        a.split[blockIdx.x] = make_int4(1 + (int)((steps - to + share - 1) / share), r, tile, u == begin ? 0 : 1);
       u += take;
       at = 0;
       tile++;
@@ -705,9 +681,9 @@ __global__ __launch_bounds__((Cfg<T, HDP, NC, CG>::THREADS), 2) void k_tree_attn
 // parts are put together: a wave every fourth part in the order of their keys, then the
 // four waves'.  Outputs leave through LDS in whole rows (in 4-byte pieces straight from the
 // lanes that hold them the join took 40 us of 99, 32 requests with trees of up to 16 rows).
-template <int T, int HDP, int NC, int CG>
+template <int T, int HDP, int CG>
 __global__ __launch_bounds__(256) void k_tree_join(TaArgs a) {
-  using C = Cfg<T, HDP, NC, CG>;
+  using C = Cfg<T, HDP, CG, 1>;
   constexpr int DPL = C::DPL, ROW = HDP + 4;
   __shared__ __align__(16) float hand[2][DPL * 256 + 128];
   const int4 s = a.split[blockIdx.x];
@@ -718,12 +694,12 @@ __global__ __launch_bounds__(256) void k_tree_join(TaArgs a) {
   const int kvh = s.z / ct, c0 = (s.z - kvh * ct) * C::COLS + block * 16, cols = min(16, m * a.G - c0);
   if (cols <= 0) return;
   const int lane = threadIdx.x & 63, n = lane & 15, g = lane >> 4, w = threadIdx.x >> 6;
-  const int stat = CG * NC * DPL * 256 + block * 32 + n;
+  const int stat = CG * DPL * 256 + block * 32 + n;
   float top = kNegInf, sum = 0.0f;
   f4 acc[DPL];
 #pragma unroll
   for (int c = 0; c < DPL; c++) acc[c] = f4{0, 0, 0, 0};
-#pragma unroll 2
+#pragma unroll 4
   for (int i = w; i < parts; i += 4) {
     // the first part may follow another tile's in its share
     const float *p = a.part + (2LL * (blockIdx.x + i) + (i ? 0 : s.w)) * C::PARTF;
@@ -775,39 +751,42 @@ __global__ __launch_bounds__(256) void k_tree_join(TaArgs a) {
   }
 }
 
-template <int T, int HDP, int NC, int CG>
+template <int T, int HDP, int CG>
 int launch(const char *fn, const TaArgs &a, hipStream_t stream) {
-  using C = Cfg<T, HDP, NC, CG>;
-  static_assert(C::LDSB <= 160 * 1024, "LDS");
-  const long long room = ((long long)a.width * a.page_size + C::STEP - 1) / C::STEP;
-  const bool whole = room <= 4 && a.n_req <= 65535;
-  void (*f)(TaArgs) = whole ? k_tree_attn<T, HDP, NC, CG, true> : k_tree_attn<T, HDP, NC, CG, false>;
-  if (C::LDSB > 64 * 1024 &&          // past what a launch may take unasked
-      hipFuncSetAttribute(reinterpret_cast<const void *>(f), hipFuncAttributeMaxDynamicSharedMemorySize, C::LDSB) != hipSuccess) {
+  constexpr int KP = CG >= 4 ? 1 : 4 / CG;            // parts of a step's keys where a block takes whole tiles
+  using W = Cfg<T, HDP, CG, KP>;
+  using C = Cfg<T, HDP, CG, 1>;
+  static_assert(W::LDSB <= 160 * 1024 && C::LDSB <= 160 * 1024, "LDS");
+  const long long room = ((long long)a.width * a.page_size + W::STEP - 1) / W::STEP;
+  const long long tiles = ((long long)a.rows * a.G / W::COLS + a.n_req) * a.n_kv;
+  const bool whole = room <= (tiles >= 256 ? 16 : tiles >= 128 ? 8 : 4) && a.n_req <= 65535;
+  void (*f)(TaArgs) = whole ? k_tree_attn<T, HDP, CG, KP, true> : k_tree_attn<T, HDP, CG, 1, false>;
+  const int lds = whole ? W::LDSB : C::LDSB;
+  if (lds > 64 * 1024 &&              // past what a launch may take unasked
+      hipFuncSetAttribute(reinterpret_cast<const void *>(f), hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
     (void)hipGetLastError();
     return qs::refuse(fn, "hipFuncSetAttribute failed");
   }
   if (whole) {
-    const long long each = ((long long)a.rows * a.G / a.n_req + C::COLS - 1) / C::COLS;       // column tiles of a request, about
+    const long long each = ((long long)a.rows * a.G / a.n_req + W::COLS - 1) / W::COLS;       // column tiles of a request, about
     const long long x = each < 1 ? a.n_kv : each * a.n_kv;
-    QS_LAUNCH(fn, f, dim3((unsigned)(x < 65535 ? x : 65535), a.n_req), dim3(C::THREADS), C::LDSB, stream, a);
+    QS_LAUNCH(fn, f, dim3((unsigned)(x < 65535 ? x : 65535), a.n_req), dim3(W::THREADS), lds, stream, a);
     return 0;
   }
-  QS_LAUNCH(fn, f, dim3(C::SHARES), dim3(C::THREADS), C::LDSB, stream, a);
-  QS_LAUNCH(fn, (k_tree_join<T, HDP, NC, CG>), dim3(C::SHARES, CG * NC), dim3(256), 0, stream, a);
+  QS_LAUNCH(fn, f, dim3(C::SHARES), dim3(C::THREADS), lds, stream, a);
+  QS_LAUNCH(fn, (k_tree_join<T, HDP, CG>), dim3(C::SHARES, CG), dim3(256), 0, stream, a);
   return 0;
 }
 
 template <int T, int HDP>
 int launch_tile(const char *fn, const TaArgs &a, int tile, hipStream_t stream) {
-  if constexpr (HDP == 256) return tile == 2 ? launch<T, HDP, 1, 4>(fn, a, stream) : launch<T, HDP, 1, 8>(fn, a, stream);
+  if constexpr (HDP == 256) return tile == 2 ? launch<T, HDP, 4>(fn, a, stream) : launch<T, HDP, 8>(fn, a, stream);
   else {
     switch (tile) {
-      case 0: return launch<T, HDP, 1, 1>(fn, a, stream);
-      case 1: return launch<T, HDP, 1, 2>(fn, a, stream);
-      case 2: return launch<T, HDP, 1, 4>(fn, a, stream);
-      case 3: return launch<T, HDP, 1, 8>(fn, a, stream);
-      default: return launch<T, HDP, 2, 8>(fn, a, stream);
+      case 0: return launch<T, HDP, 1>(fn, a, stream);
+      case 1: return launch<T, HDP, 2>(fn, a, stream);
+      case 2: return launch<T, HDP, 4>(fn, a, stream);
+      default: return launch<T, HDP, 8>(fn, a, stream);
     }
   }
 }
