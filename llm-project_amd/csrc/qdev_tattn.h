@@ -589,8 +589,9 @@ __global__ __launch_bounds__((Cfg<T, HDP, CG, KP>::THREADS), 2) void k_tree_attn
 #pragma unroll 1
       for (int s = from; s < last; s++) {
         const int key0 = s * STEP + part * KS;
+        if (key0 + KS <= ctx) continue;               // its values were taken as they are
 #pragma unroll 1
-        for (int k = max(key0, ctx); k < min(key0 + KS, len); k++) {
+        for (int k = key0; k < min(key0 + KS, len); k++) {
           const int page = table[k / a.page_size];
           if (page < 0 || page >= a.n_pages || !(seen_of(a, row, row - first, k - ctx) & 1)) continue;
           const char *v = vbase + page * a.pst + k % a.page_size * a.sst;
