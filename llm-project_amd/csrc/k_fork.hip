@@ -12,11 +12,13 @@ namespace {
 // ---------------------------------------------------------------------------
 constexpr int kForkThreads = 256, kForkPlanThreads = 1024;
 
+constexpr int kNoPage = -1, kNoCopy = -2, kRefused = -3;          // the ring names no page, none is needed, none is left
+
 struct ForkArgs {
   QPagedFork p;
   unsigned long long *best, *first;      // of a page: the new holder with most of it, the first old one
   int *holders;                          // of a page, as far as they are counted
-  int *got;                              // of a new request: the page for its copy, -1 for none, -2: refused
+  int *got;                              // of a new request: the page for its copy, or one of those below
   int *freed;                            // of an old request: pages that it is the first to give back
   int *taken;                            // pages taken from the ring
 };
@@ -120,8 +122,8 @@ __global__ __launch_bounds__(kForkPlanThreads) void k_fork_copies(ForkArgs a) {
     taken = min(asked, count);
     if (i < p.n_new) {
       const int got = in ? p.ring[ring_place(head, place, p.ring_size)] : -1;
-      a.got[i] = refused ? -2 : in ? got : -1;
       const bool there = in && got >= 0 && got < p.n_pages;
+      a.got[i] = refused ? kRefused : there ? got : in ? kNoPage : kNoCopy;
       p.lens_out[i] = refused ? 0 : tokens;
       p.status[i] = refused ? 3 : 0;
       p.src[i] = there ? page * p.page_size : -1;
@@ -136,12 +138,12 @@ __global__ __launch_bounds__(kForkPlanThreads) void k_fork_copies(ForkArgs a) {
 __global__ __launch_bounds__(kForkThreads) void k_fork_hold(ForkArgs a) {
   const QPagedFork &p = a.p;
   const int i = blockIdx.x, got = a.got[i];
-  if (got == -2) return;
+  if (got == kRefused) return;
   int tokens;
   const int r = fork_source(p, i, &tokens), want = fork_pages(p, tokens);
   for (int e = threadIdx.x; e < want; e += kForkThreads) {
     int page = fork_page(p, r, e);
-    if (got >= 0 && e == want - 1) page = got < p.n_pages ? got : -1;
+    if (got != kNoCopy && e == want - 1) page = got;
     else if (page >= 0) atomicAdd(a.holders + page, 1);
     p.table_out[i * p.table_out_stride + e] = page;
   }
