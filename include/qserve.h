@@ -325,7 +325,7 @@ size_t qllama_paged_fork_work(int n_old, int n_new, int n_pages);
 // Keys and values (and scales) of slot src[i] into slot dst[i], in n_caches caches at once
 // (one a layer; alike in type, sizes and strides).  Without starts the moves are
 // independent: count[i] slots from src[i] into as many from dst[i] (count NULL: 1), and no
-// slot that one move writes may be read or written by another.  With starts, moves
+// slot that a move writes may be read by any or written by another.  With starts, moves
 // starts[g] .. starts[g + 1] - 1 happen one after another, and so a slot may be moved on
 // into another's old place; groups are independent, and count has to be NULL.  Moves with
 // a negative slot, or no count, do nothing; those that leave the cache do nothing either

@@ -11,6 +11,7 @@ namespace {
 // Fork
 // ---------------------------------------------------------------------------
 constexpr int kForkThreads = 256, kForkPlanThreads = 1024;
+constexpr int kForkOne = 64;             // requests that one block takes
 
 constexpr int kNoPage = -1, kNoCopy = -2, kRefused = -3;          // the ring names no page, none is needed, none is left
 
@@ -48,55 +49,66 @@ __device__ inline unsigned long long fork_id(const QPagedFork &p, int r, int e) 
 // What new request i holds of a page, above what others hold: more of its tokens, then a smaller i.
 __device__ inline unsigned long long fork_rank(int covered, int i) { return (unsigned long long)covered << 32 | (0xffffffffu - (unsigned)i); }
 
-// A block a row of old requests from here on, or of new ones behind them.  First the pages
-// in hand are cleared and extra is copied, ...
-__global__ __launch_bounds__(kForkThreads) void k_fork_clear(ForkArgs a) {
+// The steps of a fork, each over all entries of the requests' tables.  Where there are few
+// requests one block takes all steps, a wave a request at a time; else every step is a launch,
+// with a block a request.  Two requests of up to 700 tokens continued by four each: 8 us in one
+// block, 14 in six launches, whose enqueueing takes the host 15 us more; 512 requests (256 old
+// and new, 40 pages each): 110 us in one block, 20 in launches, latencies all.
+// Of what a step hands to the next: in the L2, also within one launch.
+template <typename T>
+__device__ inline T load(const T *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+template <typename T>
+__device__ inline void store(T *p, T x) { __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+struct Span { int row, rows, entry, entries; };       // first request and entry, and steps between them
+
+// The pages in hand are cleared, ...
+__device__ inline void fork_clear(const ForkArgs &a, Span s) {
   const QPagedFork &p = a.p;
-  const int r = blockIdx.x;
-  if (r < p.n_old) {
+  for (int r = s.row; r < p.n_old; r += s.rows) {
     const int have = fork_pages(p, fork_len(p, r));
-    for (int e = threadIdx.x; e < have; e += kForkThreads) {
+    for (int e = s.entry; e < have; e += s.entries) {
       const int page = fork_page(p, r, e);
       if (page < 0) continue;
-      a.holders[page] = p.extra[page] + 1;
-      a.best[page] = 0;
-      a.first[page] = 0;
+      store(a.holders + page, p.extra[page] + 1);
+      store(a.best + page, 0ull);
+      store(a.first + page, 0ull);
     }
   }
-  if (p.extra_out != p.extra)
-    for (int i = blockIdx.x * kForkThreads + threadIdx.x; i < p.n_pages; i += gridDim.x * kForkThreads) p.extra_out[i] = p.extra[i];
 }
 
 // ... then the old holders are taken off, which leaves those outside the call, and new ones ranked, ...
-__global__ __launch_bounds__(kForkThreads) void k_fork_rank(ForkArgs a) {
+__device__ inline void fork_rank_all(const ForkArgs &a, Span s) {
   const QPagedFork &p = a.p;
-  if ((int)blockIdx.x < p.n_old) {
-    const int r = blockIdx.x, have = fork_pages(p, fork_len(p, r));
-    for (int e = threadIdx.x; e < have; e += kForkThreads) {
-      const int page = fork_page(p, r, e);
-      if (page < 0) continue;
-      atomicSub(a.holders + page, 1);
-      atomicMax(a.first + page, fork_id(p, r, e));
+  for (int x = s.row; x < p.n_old + p.n_new; x += s.rows) {
+    if (x < p.n_old) {
+      const int have = fork_pages(p, fork_len(p, x));
+      for (int e = s.entry; e < have; e += s.entries) {
+        const int page = fork_page(p, x, e);
+        if (page < 0) continue;
+        atomicSub(a.holders + page, 1);
+        atomicMax(a.first + page, fork_id(p, x, e));
+      }
+    } else {
+      const int i = x - p.n_old;
+      int tokens;
+      const int r = fork_source(p, i, &tokens), want = fork_pages(p, tokens);
+      for (int e = s.entry; e < want; e += s.entries) {
+        const int page = fork_page(p, r, e);
+        if (page >= 0) atomicMax(a.best + page, fork_rank(min(p.page_size, tokens - e * p.page_size), i));
+      }
     }
-    return;
-  }
-  const int i = blockIdx.x - p.n_old;
-  int tokens;
-  const int r = fork_source(p, i, &tokens), want = fork_pages(p, tokens);
-  for (int e = threadIdx.x; e < want; e += kForkThreads) {
-    const int page = fork_page(p, r, e);
-    if (page >= 0) atomicMax(a.best + page, fork_rank(min(p.page_size, tokens - e * p.page_size), i));
   }
 }
 
-// ... copies decided and their pages taken, request by request, ...
-__global__ __launch_bounds__(kForkPlanThreads) void k_fork_copies(ForkArgs a) {
+// ... copies decided and their pages taken, request by request, by one block; all threads return the pages taken, ...
+__device__ int fork_copies(const ForkArgs &a) {
   const QPagedFork &p = a.p;
-  __shared__ int wave_sums[2][kForkPlanThreads / 64];
+  __shared__ int wave_sums[kForkPlanThreads / 64];
   const int t = threadIdx.x, lane = t & 63, w = t >> 6;
   int head, count;
   fork_ring(p, &head, &count);
-  int asked = 0, taken = 0;              // of the requests before this pass
+  int asked = 0;                         // by the requests before this pass
   for (int i0 = 0; i0 < p.n_new; i0 += kForkPlanThreads) {
     const int i = i0 + t;
     int tokens = 0, r = -1, page = -1, part = 0;
@@ -105,25 +117,22 @@ __global__ __launch_bounds__(kForkPlanThreads) void k_fork_copies(ForkArgs a) {
       part = tokens % p.page_size;
       if (part) page = fork_page(p, r, tokens / p.page_size);
     }
-    const bool copies = page >= 0 && (a.holders[page] > 0 || a.best[page] != fork_rank(part, i));
+    const bool copies = page >= 0 && (load(a.holders + page) > 0 || load(a.best + page) != fork_rank(part, i));
     const uint64_t wanting = __ballot(copies);
-    const uint64_t before = (1ull << lane) - 1;
     __syncthreads();                     // the sums of the pass before have been read
-    if (lane == 0) wave_sums[0][w] = __popcll(wanting);
+    if (lane == 0) wave_sums[w] = __popcll(wanting);
     __syncthreads();
-    int upto = asked + __popcll(wanting & before) + copies;
+    // requests are admitted up to a border, so a request's place among the free pages is that among all that ask
+    int place = asked + __popcll(wanting & ((1ull << lane) - 1));
     for (int j = 0; j < kForkPlanThreads / 64; j++) {
-      if (j < w) upto += wave_sums[0][j];
-      asked += wave_sums[0][j];
+      if (j < w) place += wave_sums[j];
+      asked += wave_sums[j];
     }
-    const bool refused = copies && upto > count, in = copies && !refused;
-    // requests are admitted up to a border, so a request's place is that among all that ask
-    const int place = upto - 1;
-    taken = min(asked, count);
+    const bool refused = copies && place >= count, in = copies && !refused;
     if (i < p.n_new) {
       const int got = in ? p.ring[ring_place(head, place, p.ring_size)] : -1;
       const bool there = in && got >= 0 && got < p.n_pages;
-      a.got[i] = refused ? kRefused : there ? got : in ? kNoPage : kNoCopy;
+      store(a.got + i, refused ? kRefused : there ? got : in ? kNoPage : kNoCopy);
       p.lens_out[i] = refused ? 0 : tokens;
       p.status[i] = refused ? 3 : 0;
       p.src[i] = there ? page * p.page_size : -1;
@@ -131,28 +140,109 @@ __global__ __launch_bounds__(kForkPlanThreads) void k_fork_copies(ForkArgs a) {
       p.count[i] = there ? part : 0;
     }
   }
-  if (t == 0) *a.taken = taken;
+  return min(asked, count);
 }
 
 // ... what every new request holds written down, ...
-__global__ __launch_bounds__(kForkThreads) void k_fork_hold(ForkArgs a) {
+__device__ inline void fork_hold(const ForkArgs &a, Span s) {
   const QPagedFork &p = a.p;
-  const int i = blockIdx.x, got = a.got[i];
-  if (got == kRefused) return;
-  int tokens;
-  const int r = fork_source(p, i, &tokens), want = fork_pages(p, tokens);
-  for (int e = threadIdx.x; e < want; e += kForkThreads) {
-    int page = fork_page(p, r, e);
-    if (got != kNoCopy && e == want - 1) page = got;
-    else if (page >= 0) atomicAdd(a.holders + page, 1);
-    p.table_out[i * p.table_out_stride + e] = page;
+  for (int i = s.row; i < p.n_new; i += s.rows) {
+    const int got = load(a.got + i);
+    if (got == kRefused) continue;
+    int tokens;
+    const int r = fork_source(p, i, &tokens), want = fork_pages(p, tokens);
+    for (int e = s.entry; e < want; e += s.entries) {
+      int page = fork_page(p, r, e);
+      if (got != kNoCopy && e == want - 1) page = got;
+      else if (page >= 0) atomicAdd(a.holders + page, 1);
+      p.table_out[i * p.table_out_stride + e] = page;
+    }
   }
 }
 
 // Whether old request r is the one to give back the page of its entry e.
-__device__ inline bool fork_gone(const ForkArgs &a, int r, int e, int page) { return page >= 0 && a.holders[page] <= 0 && a.first[page] == fork_id(a.p, r, e); }
+__device__ inline bool fork_gone(const ForkArgs &a, int r, int e, int page) { return page >= 0 && load(a.holders + page) <= 0 && load(a.first + page) == fork_id(a.p, r, e); }
 
-// ... pages that no one holds any more counted, ...
+// ... and pages that no one holds any more counted and put at the ring's back, row by row.
+// The state behind the call: `taken` pages from the front, `all` to the back, as far as there is room.
+__device__ inline void fork_state(const QPagedFork &p, int head, int count, int taken, long long all) {
+  const int room = p.ring_size - count;
+  p.state_out[0] = ring_place(head, taken, p.ring_size);
+  p.state_out[1] = count - taken + (int)(all < room ? all : room);
+}
+
+__device__ inline void fork_between() {
+  __builtin_amdgcn_s_waitcnt(0);         // what this wave has written is in the L2, from where the counts below are read
+  __syncthreads();
+}
+// All steps by one block.  (With fences of the whole device between them it took 32 us.)
+__global__ __launch_bounds__(kForkPlanThreads) void k_fork_one(ForkArgs a) {
+  const QPagedFork &p = a.p;
+  __shared__ int sums[kForkPlanThreads / 64], before[kForkPlanThreads];
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+  const Span all = {w, kForkPlanThreads / 64, lane, 64};
+  if (p.extra_out != p.extra)
+    for (int i = t; i < p.n_pages; i += kForkPlanThreads) p.extra_out[i] = p.extra[i];
+  fork_clear(a, all);
+  fork_between();
+  fork_rank_all(a, all);
+  fork_between();
+  const int taken = fork_copies(a);
+  fork_between();
+  fork_hold(a, all);
+  fork_between();
+  for (int r = w; r < p.n_old; r += kForkPlanThreads / 64) {
+    const int have = fork_pages(p, fork_len(p, r));
+    int n = 0;
+    for (int e0 = 0; e0 < have; e0 += 64) {
+      const int page = e0 + lane < have ? fork_page(p, r, e0 + lane) : -1;
+      if (page >= 0) p.extra_out[page] = max(load(a.holders + page) - 1, 0);
+      n += __popcll(__ballot(fork_gone(a, r, e0 + lane, page)));
+    }
+    if (lane == 0) before[r] = n;
+  }
+  __syncthreads();
+  const int mine = t < p.n_old ? before[t] : 0;
+  int upto = mine;
+  for (int d = 1; d < 64; d <<= 1) {
+    const int x = __shfl_up(upto, d);
+    if (lane >= d) upto += x;
+  }
+  if (lane == 63) sums[w] = upto;
+  __syncthreads();
+  for (int j = 0; j < w; j++) upto += sums[j];
+  before[t] = upto - mine;
+  int head, count;
+  fork_ring(p, &head, &count);
+  const int room = p.ring_size - count;
+  if (t == kForkPlanThreads - 1) fork_state(p, head, count, taken, upto);
+  __syncthreads();
+  for (int r = w; r < p.n_old; r += kForkPlanThreads / 64) {
+    const int have = fork_pages(p, fork_len(p, r));
+    int at = before[r];
+    for (int e0 = 0; e0 < have; e0 += 64) {
+      const int page = e0 + lane < have ? fork_page(p, r, e0 + lane) : -1;
+      const bool gone = fork_gone(a, r, e0 + lane, page);
+      const uint64_t which = __ballot(gone);
+      const int place = at + __popcll(which & ((1ull << lane) - 1));
+      if (gone && place < room) p.ring[ring_place(ring_place(head, count, p.ring_size), place, p.ring_size)] = page;
+      at += __popcll(which);
+    }
+  }
+}
+
+__device__ inline Span fork_block() { return {(int)blockIdx.x, (int)gridDim.x, (int)threadIdx.x, kForkThreads}; }
+__global__ __launch_bounds__(kForkThreads) void k_fork_clear(ForkArgs a) {
+  fork_clear(a, fork_block());
+  if (a.p.extra_out != a.p.extra)
+    for (int i = blockIdx.x * kForkThreads + threadIdx.x; i < a.p.n_pages; i += gridDim.x * kForkThreads) a.p.extra_out[i] = a.p.extra[i];
+}
+__global__ __launch_bounds__(kForkThreads) void k_fork_rank(ForkArgs a) { fork_rank_all(a, fork_block()); }
+__global__ __launch_bounds__(kForkPlanThreads) void k_fork_copies(ForkArgs a) {
+  const int taken = fork_copies(a);
+  if (threadIdx.x == 0) *a.taken = taken;
+}
+__global__ __launch_bounds__(kForkThreads) void k_fork_hold(ForkArgs a) { fork_hold(a, fork_block()); }
 __global__ __launch_bounds__(kForkThreads) void k_fork_count(ForkArgs a) {
   const QPagedFork &p = a.p;
   const int r = blockIdx.x, have = fork_pages(p, fork_len(p, r));
@@ -160,13 +250,11 @@ __global__ __launch_bounds__(kForkThreads) void k_fork_count(ForkArgs a) {
   for (int e0 = 0; e0 < have; e0 += kForkThreads) {
     const int e = e0 + threadIdx.x;
     const int page = e < have ? fork_page(p, r, e) : -1;
-    if (page >= 0) p.extra_out[page] = max(a.holders[page] - 1, 0);
+    if (page >= 0) p.extra_out[page] = max(load(a.holders + page) - 1, 0);
     n += __syncthreads_count(fork_gone(a, r, e, page));
   }
   if (threadIdx.x == 0) a.freed[r] = n;
 }
-
-// ... and put at the ring's back, row by row.
 __global__ __launch_bounds__(kForkThreads) void k_fork_free(ForkArgs a) {
   const QPagedFork &p = a.p;
   __shared__ int sums[kForkThreads / 64];
@@ -183,13 +271,7 @@ __global__ __launch_bounds__(kForkThreads) void k_fork_free(ForkArgs a) {
     for (int j = 0; j < kForkThreads / 64; j++) at += sums[j];
   }
   const int room = p.ring_size - count;
-  if (t == 0 && r + 1 >= p.n_old) {
-    const long long all = at + (p.n_old ? a.freed[r] : 0);
-    const int taken = *a.taken;
-    p.state_out[0] = ring_place(head, taken, p.ring_size);
-    p.state_out[1] = count - taken + (int)(all < room ? all : room);
-  }
-  if (p.n_old == 0) return;
+  if (t == 0 && r + 1 == p.n_old) fork_state(p, head, count, *a.taken, at + a.freed[r]);
   const int have = fork_pages(p, fork_len(p, r));
   for (int e0 = 0; e0 < have; e0 += kForkThreads) {
     const int e = e0 + t;
@@ -247,7 +329,10 @@ __device__ inline long long move_scale_at(const MoveArgs &a, int slot, int head)
 }
 
 // Independent moves: a block a move and cache (and share of its slots), a thread a unit of
-// 16 bytes of one slot's row of one head.
+// 16 bytes of one slot's row of one head.  256 moves of 7 slots on average in 16 caches (8 heads of
+// 64 bf16) take 18 us: 36 MB read and written in pieces of 128 bytes to 2 KB, 2 TB/s, 9 us at a
+// copy's rate.  A wave a head, four heads under way at a time, took 24, a block for four caches
+// with their loads under way together 30.
 template <int U>
 __global__ __launch_bounds__(kMoveThreads) void k_move(MoveArgs a) {
   using T = typename Unit<U>::type;
@@ -259,8 +344,9 @@ __global__ __launch_bounds__(kMoveThreads) void k_move(MoveArgs a) {
   const auto &c = a.c[blockIdx.y];
   const int per_slot = a.units + a.scales;
   const long long all = (long long)n * per_slot;
+  const bool small = all <= INT_MAX;       // a division of 32 bits
   for (long long u = blockIdx.z * kMoveThreads + threadIdx.x; u < all; u += gridDim.z * kMoveThreads) {
-    const int s = (int)(u / per_slot);
+    const int s = small ? (int)u / per_slot : (int)(u / per_slot);
     int x = (int)(u - (long long)s * per_slot);
     if (x < a.units) {
       char *base = x < a.units / 2 ? c.k : c.v;
@@ -374,14 +460,17 @@ extern "C" int qllama_paged_fork(const QPagedFork *p, void *stream) {
   a.freed = a.got + p->n_new;
   a.taken = a.freed + p->n_old;
   const hipStream_t s = (hipStream_t)stream;
-  const int copy = p->extra_out == p->extra ? 0 : (p->n_pages + kForkThreads - 1) / kForkThreads;
-  const int clear = copy > 256 ? 256 : copy;
-  if (p->n_old || clear) QS_LAUNCH(fn, k_fork_clear, dim3(p->n_old > clear ? p->n_old : clear), dim3(kForkThreads), 0, s, a);
-  if (p->n_old + p->n_new) QS_LAUNCH(fn, k_fork_rank, dim3(p->n_old + p->n_new), dim3(kForkThreads), 0, s, a);
+  if (p->n_old == 0 || (p->n_old + p->n_new <= kForkOne && p->n_pages <= 16384)) {
+    QS_LAUNCH(fn, k_fork_one, dim3(1), dim3(kForkPlanThreads), 0, s, a);
+    return 0;
+  }
+  const int copy = p->extra_out == p->extra ? 0 : (p->n_pages + kForkThreads - 1) / kForkThreads, clear = copy > 256 ? 256 : copy;
+  QS_LAUNCH(fn, k_fork_clear, dim3(p->n_old > clear ? p->n_old : clear), dim3(kForkThreads), 0, s, a);
+  QS_LAUNCH(fn, k_fork_rank, dim3(p->n_old + p->n_new), dim3(kForkThreads), 0, s, a);
   QS_LAUNCH(fn, k_fork_copies, dim3(1), dim3(kForkPlanThreads), 0, s, a);
   if (p->n_new) QS_LAUNCH(fn, k_fork_hold, dim3(p->n_new), dim3(kForkThreads), 0, s, a);
-  if (p->n_old) QS_LAUNCH(fn, k_fork_count, dim3(p->n_old), dim3(kForkThreads), 0, s, a);
-  QS_LAUNCH(fn, k_fork_free, dim3(p->n_old ? p->n_old : 1), dim3(kForkThreads), 0, s, a);
+  QS_LAUNCH(fn, k_fork_count, dim3(p->n_old), dim3(kForkThreads), 0, s, a);
+  QS_LAUNCH(fn, k_fork_free, dim3(p->n_old), dim3(kForkThreads), 0, s, a);
   return 0;
 }
 
@@ -429,7 +518,7 @@ extern "C" int qllama_paged_move(const QPagedKV *caches, int n_caches, const QPa
     } else {
       // few moves: their slots over several blocks
       const long long blocks = (long long)m->n_moves * n;
-      const dim3 grid(m->n_moves, n, blocks >= 1024 ? 1 : blocks >= 128 ? 4 : 16);
+      const dim3 grid(m->n_moves, n, !m->count || blocks >= 1024 ? 1 : blocks >= 128 ? 4 : 16);
       QS_LAUNCH(fn, (wide ? k_move<16> : k_move<8>), grid, dim3(kMoveThreads), 0, (hipStream_t)stream, a);
     }
   }

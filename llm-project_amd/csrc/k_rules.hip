@@ -13,7 +13,7 @@
 
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 512, kAhead = 8;
 constexpr uint32_t kBiased = 1u << 30, kCount = kBiased - 1, kPrompt = 1u << 31;
 
 __device__ inline float setting(const float *p, int r, float none) {
@@ -64,11 +64,17 @@ __global__ __launch_bounds__(kThreads) void k_rules(QLogitRules p) {
       if (p.tokens) {
         const int *tokens = p.tokens + r * p.token_stride;
         const int len = min(max(p.n_tokens[r], 0), p.capacity), prompt = p.n_prompt ? min(max(p.n_prompt[r], 0), len) : 0;
-        for (int j = t; j < len; j += kThreads) {
-          const unsigned at = (unsigned)tokens[j] - (unsigned)lo;
-          if (at < (unsigned)n && tokens[j] >= 0) {
-            if (j < prompt) atomicOr(used + at, kPrompt);
-            else atomicAdd(used + at, 1u);
+        for (int j0 = t; j0 < len; j0 += kAhead * kThreads) {          // several loads under way at a time
+          int token[kAhead];
+#pragma unroll
+          for (int k = 0; k < kAhead; k++) token[k] = j0 + k * kThreads < len ? tokens[j0 + k * kThreads] : -1;
+#pragma unroll
+          for (int k = 0; k < kAhead; k++) {
+            const unsigned at = (unsigned)token[k] - (unsigned)lo;
+            if (at < (unsigned)n && token[k] >= 0) {
+              if (j0 + k * kThreads < prompt) atomicOr(used + at, kPrompt);
+              else atomicAdd(used + at, 1u);
+            }
           }
         }
       }
@@ -165,9 +171,9 @@ extern "C" int qllama_logit_rules(const QLogitRules *p, void *stream) {
   qs::OnDevice on(p->logits, (hipStream_t)stream);
   if (on.why) return qs::refuse(fn, on.why);
   const bool vec = !qs::misaligned(p->logits, 16) && !qs::misaligned(p->out, 16) && p->stride % 4 == 0 && p->out_stride % 4 == 0;
-  // slices of 2048 to 16384 tokens: the largest that leave the chip two blocks a CU
+  // slices of 2048 to 8192 tokens: the largest that leave the chip two blocks a CU.  192 rows of 128256: slices of 4096 53
+  // us, 8192 47, 16384 (whose counters take 64 KB of LDS: two blocks a CU, not four) 57
   const long long tokens = (long long)p->rows * p->vocab;
-  if (tokens >= 512LL * 16384) return launch<8>(fn, *p, vec, (hipStream_t)stream);
   if (tokens >= 512LL * 8192) return launch<4>(fn, *p, vec, (hipStream_t)stream);
   if (tokens >= 512LL * 4096) return launch<2>(fn, *p, vec, (hipStream_t)stream);
   return launch<1>(fn, *p, vec, (hipStream_t)stream);
