@@ -67,19 +67,23 @@ template <int T, int HDP, int CG_, int KP_>
 struct Cfg {
   static constexpr int CG = CG_, KP = KP_, THREADS = 64 * CG * KP, COLS = 16 * CG;
   static constexpr int SHARES = kShares / CG;
-  static constexpr bool F32 = T == QLLAMA_KV_F32, HALF = T == QLLAMA_KV_F16;
-  static constexpr int ES = F32 ? 4 : T == QLLAMA_KV_I8 ? 1 : 2;        // of an element in the cache
-  static constexpr int LES = F32 ? 4 : 2;                               // in LDS (int8: bf16, which holds the codes)
-  static constexpr int LT = T == QLLAMA_KV_I8 ? QLLAMA_KV_BF16 : T;     // the products' type
+  // f32 rows: as they are, or (many columns) in three bf16 parts, which the matrix cores take 16 times as fast: the six
+  // products of parts that count make it 2.7 times.  Dropped ones are below 2^-22 of a product
+  static constexpr bool SPLIT = T == QLLAMA_KV_F32 && (HDP == 64 ? CG >= 4 : HDP == 128 && CG == 8), F32 = T == QLLAMA_KV_F32 && !SPLIT;
+  static constexpr bool HALF = T == QLLAMA_KV_F16;
+  static constexpr int PLANES = SPLIT ? 3 : 1;
+  static constexpr int ES = T == QLLAMA_KV_F32 ? 4 : T == QLLAMA_KV_I8 ? 1 : 2;         // of an element in the cache
+  static constexpr int LES = F32 ? 4 : 2;                               // in LDS, of a part (int8: bf16, which holds the codes)
+  static constexpr int LT = T == QLLAMA_KV_I8 || SPLIT ? QLLAMA_KV_BF16 : T;            // the products' type
   static constexpr int SUB = F32 ? 1 : 2, KEYS = 16 * SUB;              // keys that a wave takes at a time
   // times that it does between two barriers, as far as registers and LDS allow
-  static constexpr int TIMES = CG >= 4 && HDP <= 128 ? 2 : 1, KS = KEYS * TIMES, STEP = KS * KP;
+  static constexpr int TIMES = SPLIT ? (HDP == 64 && CG == 8 ? 2 : 1) : CG >= 4 && HDP <= 128 ? 2 : 1, KS = KEYS * TIMES, STEP = KS * KP;
   static constexpr int OVER = 128 / STEP < 1 ? 1 : 128 / STEP;          // steps that a tile's beginning and end take the time of
   static constexpr int ROWB = HDP * LES, CH = ROWB / 16, SWZ = (CH < 16 ? CH : 16) - 1, EPC = 16 / LES;
-  static constexpr int PARTB = 2 * KS * ROWB;                           // a part's keys, then values
+  static constexpr int PLANEB = KS * ROWB, SIDEB = PLANES * PLANEB, PARTB = 2 * SIDEB;  // a part's keys, then values
   static constexpr int NBUF = CG == 1 ? 1 : 2;                          // a wave alone with its part needs no second buffer
-  // threads that stage a part, and units of each: 16 bytes of the cache, CPU chunks of 16 bytes in LDS
-  static constexpr int CPU = T == QLLAMA_KV_I8 ? 2 : 1, TP = 64 * CG, U = 2 * KS * CH / CPU / TP;
+  // threads that stage a part, and units of each: 16 bytes of the cache (split: 32), CPU chunks of 16 bytes in LDS (split: one a part)
+  static constexpr int LOADS = SPLIT ? 2 : 1, CPU = T == QLLAMA_KV_I8 ? 2 : 1, TP = 64 * CG, U = 2 * KS * CH / CPU / TP;
   static constexpr int DPL = HDP / 16, QC = F32 ? HDP / 16 : HDP / 32;
   static constexpr int PARTS = F32 ? 1 : HALF ? 2 : 3;
   // weights are held times this in f16 products: two parts then keep 23 bits down to 2^-17 of the largest and the rest to 2^-40
@@ -137,6 +141,24 @@ template <int T>
 __device__ inline bool odd_value(uint32_t x) {
   constexpr uint32_t E = T == QLLAMA_KV_F32 ? 0x7f800000u : T == QLLAMA_KV_F16 ? 0x7c00u : 0x7f80u;
   return (x & E) == E;
+}
+
+// 8 floats as sums of three bf16 numbers: the first cut (a float's range fits), the others rounded to nearest, off by 2^-25.
+typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+__device__ inline Parts3 split3(u4 x, u4 y) {
+  Parts3 r;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const uint32_t lo = i < 2 ? x[2 * i] : y[2 * i - 4], hi = i < 2 ? x[2 * i + 1] : y[2 * i - 3];
+    r.p[0][i] = hi16s(hi, lo);
+    float a = __uint_as_float(lo) - __uint_as_float(lo & 0xffff0000u), b = __uint_as_float(hi) - __uint_as_float(hi & 0xffff0000u);
+    const uint32_t mid = __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{a, b}, bf2));
+    a -= __uint_as_float(mid << 16);
+    b -= __uint_as_float(mid & 0xffff0000u);
+    r.p[1][i] = mid;
+    r.p[2][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{a, b}, bf2));
+  }
+  return r;
 }
 
 // The dim of a head whose output is element c of an accumulator's row `lane` of 16.
@@ -281,7 +303,7 @@ __global__ __launch_bounds__((Cfg<T, HDP, CG, KP>::THREADS), 2) void k_tree_attn
       }
       return T == QLLAMA_KV_I8 ? (there ? page_at : 0) * a.scp + kvh * a.sch + (there ? place_at : 0) * a.scs : 0;
     };
-    u4 staged[U];
+    u4 staged[U * C::LOADS];
     uint32_t dead = 0;                                // units of no key, or of no dim
     constexpr int UNITS = KS * CH / C::CPU, PER = CH / C::CPU;                 // of a part's keys, of a row
     const auto issue = [&](int s) {
@@ -304,7 +326,8 @@ __global__ __launch_bounds__((Cfg<T, HDP, CG, KP>::THREADS), 2) void k_tree_attn
             staged[x] = u4{lo.x, lo.y, hi.x, hi.y};
           }
         } else {
-          staged[x] = *reinterpret_cast<const u4 *>(p);
+#pragma unroll
+          for (int i = 0; i < C::LOADS; i++) staged[x * C::LOADS + i] = reinterpret_cast<const u4 *>(p)[i];
         }
       }
     };
@@ -316,7 +339,7 @@ __global__ __launch_bounds__((Cfg<T, HDP, CG, KP>::THREADS), 2) void k_tree_attn
       for (int x = 0; x < U; x++) {
         const int unit = tp + x * C::TP, is_v = unit >= UNITS, at = is_v ? unit - UNITS : unit;
         const int row = at / PER, chunk = at % PER * C::CPU;
-        char *to = to_lds + is_v * KS * C::ROWB + row * C::ROWB;
+        char *to = to_lds + is_v * C::SIDEB + row * C::ROWB;
         if constexpr (T == QLLAMA_KV_I8) {            // bf16 holds a code
 #pragma unroll
           for (int h = 0; h < 2; h++) {
@@ -330,21 +353,32 @@ __global__ __launch_bounds__((Cfg<T, HDP, CG, KP>::THREADS), 2) void k_tree_attn
             *reinterpret_cast<u4 *>(to + (((chunk + h) ^ (row & C::SWZ)) << 4)) = w;
           }
         } else {
-          u4 w = staged[x];
-          if (dead >> x & 1) w = u4{0, 0, 0, 0};
-          if (fresh && is_v) {                        // what is not finite must not reach the columns that do not see it
+          u4 w[C::LOADS];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-              const uint32_t all = w[i];
-              if constexpr (C::F32) {
-                w[i] = odd_value<T>(all) ? 0 : all;
-              } else {
-                w[i] = (odd_value<T>(all & 0xffffu) ? 0 : all & 0xffffu) | (odd_value<T>(all >> 16) ? 0 : all & 0xffff0000u);
+          for (int k = 0; k < C::LOADS; k++) {
+            w[k] = staged[x * C::LOADS + k];
+            if (dead >> x & 1) w[k] = u4{0, 0, 0, 0};
+            if (fresh && is_v) {                      // what is not finite must not reach the columns that do not see it
+#pragma unroll
+              for (int i = 0; i < 4; i++) {
+                const uint32_t all = w[k][i];
+                if constexpr (C::ES == 4) {
+                  w[k][i] = odd_value<T>(all) ? 0 : all;
+                } else {
+                  w[k][i] = (odd_value<T>(all & 0xffffu) ? 0 : all & 0xffffu) | (odd_value<T>(all >> 16) ? 0 : all & 0xffff0000u);
+                }
+                odd |= w[k][i] ^ all;
               }
-              odd |= w[i] ^ all;
             }
           }
-          *reinterpret_cast<u4 *>(to + ((chunk ^ (row & C::SWZ)) << 4)) = w;
+          to += (chunk ^ (row & C::SWZ)) << 4;
+          if constexpr (C::SPLIT) {
+            const Parts3 y = split3(w[0], w[1]);
+#pragma unroll
+            for (int k = 0; k < 3; k++) *reinterpret_cast<u4 *>(to + k * C::PLANEB) = y.p[k];
+          } else {
+            *reinterpret_cast<u4 *>(to) = w[0];
+          }
         }
       }
     };
@@ -440,30 +474,34 @@ __global__ __launch_bounds__((Cfg<T, HDP, CG, KP>::THREADS), 2) void k_tree_attn
 
     // keys KEYS t .. of step s's part
     const auto compute = [&](int s, int t) {
-      const char *kl = lds + (C::NBUF == 1 ? part : (s & 1) * KP + part) * C::PARTB + t * C::KEYS * C::ROWB, *vl = kl + KS * C::ROWB;
+      const char *kl = lds + (C::NBUF == 1 ? part : (s & 1) * KP + part) * C::PARTB + t * C::KEYS * C::ROWB, *vl = kl + C::SIDEB;
       const int key0 = s * STEP + part * KS + t * C::KEYS;
-      u4 kf[C::QC][SUB];
-#pragma unroll
-      for (int c = 0; c < C::QC; c++)
-#pragma unroll
-        for (int i = 0; i < SUB; i++) kf[c][i] = *reinterpret_cast<const u4 *>(kl + (16 * i + n) * C::ROWB + (((4 * c + g) ^ (n & C::SWZ)) << 4));
-      __builtin_amdgcn_sched_barrier(0);              // all under way before the first product
       f4 d[SUB];
 #pragma unroll
       for (int i = 0; i < SUB; i++) d[i] = f4{0, 0, 0, 0};
 #pragma unroll
-      for (int c = 0; c < C::QC; c++)
+      for (int y = 0; y < C::PLANES; y++) {
+        u4 kf[C::QC][SUB];
 #pragma unroll
-        for (int i = 0; i < SUB; i++) {
-          if constexpr (C::F32) {
+        for (int c = 0; c < C::QC; c++)
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-              d[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[c][i][e]), __uint_as_float(qp[c][0][e]), d[i], 0, 0, 0);
-          } else {
+          for (int i = 0; i < SUB; i++)
+            kf[c][i] = *reinterpret_cast<const u4 *>(kl + y * C::PLANEB + (16 * i + n) * C::ROWB + (((4 * c + g) ^ (n & C::SWZ)) << 4));
+        __builtin_amdgcn_sched_barrier(0);            // all under way before the first product
 #pragma unroll
-            for (int p = 0; p < C::PARTS; p++) d[i] = mfma16<C::LT>(kf[c][i], qp[c][p], d[i]);
+        for (int c = 0; c < C::QC; c++)
+#pragma unroll
+          for (int i = 0; i < SUB; i++) {
+            if constexpr (C::F32) {
+#pragma unroll
+              for (int e = 0; e < 4; e++)
+                d[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[c][i][e]), __uint_as_float(qp[c][0][e]), d[i], 0, 0, 0);
+            } else {
+#pragma unroll
+              for (int p = 0; p < C::PARTS - y; p++) d[i] = mfma16<C::LT>(kf[c][i], qp[c][p], d[i]);
+            }
           }
-        }
+      }
 
       f4 fv[SUB];
       if constexpr (T == QLLAMA_KV_I8) {
@@ -540,17 +578,20 @@ __global__ __launch_bounds__((Cfg<T, HDP, CG, KP>::THREADS), 2) void k_tree_attn
         const char *at = vl + row * C::ROWB + n % 2 * 8;
         const int turn = (n % 4 / 2) ^ (row & C::SWZ);
 #pragma unroll
-        for (int c = 0; c < DPL; c++) {
-          u4 vv;                                      // dim 16 c + n, 8 keys
+        for (int c = 0; c < DPL; c++)
 #pragma unroll
-          for (int i = 0; i < SUB; i++) {
-            const u2 y = __builtin_bit_cast(u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4_lds *)(at + 16 * i * C::ROWB + (((2 * c) ^ turn) << 4))));
-            vv[2 * i] = y.x;
-            vv[2 * i + 1] = y.y;
+          for (int z = 0; z < C::PLANES; z++) {
+            u4 vv;                                    // dim 16 c + n, 8 keys
+#pragma unroll
+            for (int i = 0; i < SUB; i++) {
+              const u2 y = __builtin_bit_cast(
+                  u2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4_lds *)(at + z * C::PLANEB + 16 * i * C::ROWB + (((2 * c) ^ turn) << 4))));
+              vv[2 * i] = y.x;
+              vv[2 * i + 1] = y.y;
+            }
+#pragma unroll
+            for (int k = 0; k < C::PARTS - z; k++) acc[c] = mfma16<C::LT>(vv, pp[k], acc[c]);
           }
-#pragma unroll
-          for (int k = 0; k < C::PARTS; k++) acc[c] = mfma16<C::LT>(vv, pp[k], acc[c]);
-        }
       }
     };
 
@@ -600,7 +641,7 @@ __global__ __launch_bounds__((Cfg<T, HDP, CG, KP>::THREADS), 2) void k_tree_attn
 #pragma unroll
             for (int c = 0; c < DPL; c++) {
               const int d = dim_of<C>(c, 4 * g + j);
-              if (d < a.hd && odd_value<T>(C::F32 ? reinterpret_cast<const uint32_t *>(v)[d] : reinterpret_cast<const unsigned short *>(v)[d]))
+              if (d < a.hd && odd_value<T>(C::ES == 4 ? reinterpret_cast<const uint32_t *>(v)[d] : reinterpret_cast<const unsigned short *>(v)[d]))
                 acc[c][j] = __builtin_nanf("");
             }
         }
