@@ -78,11 +78,13 @@ struct Cfg {
   static constexpr int SUB = F32 ? 1 : 2, KEYS = 16 * SUB;              // keys that a wave takes at a time
   // times that it does between two barriers, as far as registers and LDS allow
   static constexpr int TIMES = SPLIT ? (HDP == 64 && CG == 8 ? 2 : 1) : CG >= 4 && HDP <= 128 ? 2 : 1, KS = KEYS * TIMES, STEP = KS * KP;
-  static constexpr int OVER = 128 / STEP < 1 ? 1 : 128 / STEP;          // steps that a tile's beginning and end take the time of
+// steps that a tile's beginning and end take the time of
+  static constexpr int OVERKEYS = CG == 8 ? 256 : CG == 4 && HDP > 64 ? 128 : 64, OVER = OVERKEYS / STEP < 1 ? 1 : OVERKEYS / STEP;
   static constexpr int ROWB = HDP * LES, CH = ROWB / 16, SWZ = (CH < 16 ? CH : 16) - 1, EPC = 16 / LES;
   static constexpr int PLANEB = KS * ROWB, SIDEB = PLANES * PLANEB, PARTB = 2 * SIDEB;  // a part's keys, then values
   static constexpr int NBUF = CG == 1 ? 1 : 2;                          // a wave alone with its part needs no second buffer
   // threads that stage a part, and units of each: 16 bytes of the cache (split: 32), CPU chunks of 16 bytes in LDS (split: one a part)
+  static constexpr bool ONCE = CG <= 2;                                 // a tile has all of a request's columns, or nearly: past the caches' retention
   static constexpr int LOADS = SPLIT ? 2 : 1, CPU = T == QLLAMA_KV_I8 ? 2 : 1, TP = 64 * CG, U = 2 * KS * CH / CPU / TP;
   static constexpr int DPL = HDP / 16, QC = F32 ? HDP / 16 : HDP / 32;
   static constexpr int PARTS = F32 ? 1 : HALF ? 2 : 3;
@@ -320,14 +322,17 @@ __global__ __launch_bounds__((Cfg<T, HDP, CG, KP>::THREADS), 2) void k_tree_attn
           const bool half = no || d + 8 >= a.hd;      // the row may end within the 16 codes
           if (half) dead |= 0x10000u << x;
           if (a.wide) {
-            staged[x] = *reinterpret_cast<const u4 *>(p);
+            staged[x] = C::ONCE ? __builtin_nontemporal_load(reinterpret_cast<const u4 *>(p)) : *reinterpret_cast<const u4 *>(p);
           } else {
             const u2 lo = *reinterpret_cast<const u2 *>(p), hi = *reinterpret_cast<const u2 *>(half ? p : p + 8);
             staged[x] = u4{lo.x, lo.y, hi.x, hi.y};
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < C::LOADS; i++) staged[x * C::LOADS + i] = reinterpret_cast<const u4 *>(p)[i];
+          for (int i = 0; i < C::LOADS; i++) {
+            const u4 *q = reinterpret_cast<const u4 *>(p) + i;
+            staged[x * C::LOADS + i] = C::ONCE ? __builtin_nontemporal_load(q) : *q;
+          }
         }
       }
     };
