@@ -7,7 +7,11 @@
 // need and names each new row's slot and position; qllama_paged_append rotates the
 // rows' queries and keys and stores keys and values in their slots;
 // qllama_paged_attention lets the newest token of every request attend to its pages;
-// qllama_sample_rows draws a token from every row of logits.  The model's products between
+// qllama_sample_rows draws a token from every row of logits.  A step that verifies drafted
+// tokens adds qllama_tree_plan, qllama_tree_attention in place of the attention above, and
+// qllama_tree_accept (below); qllama_logit_rules applies penalties, biases and masks before
+// tokens are drawn, and qllama_paged_fork and qllama_paged_move continue requests over pages
+// that they share.  The model's products between
 // them may be qmatmul_device_noalloc's: that one always enqueues on qllama_stream(), with
 // which no other stream is ordered, so that such a step runs on that stream as a whole or
 // orders its own with it by events.
@@ -254,10 +258,14 @@ int qllama_tree_accept(const QTreeAccept *p, void *stream);
 // lens[r] - m of its request and to those new rows b < m whose bit is set in mask[i]; mask
 // NULL: to b = 0 .. j (the next piece of a prompt).  Bits behind a row's words count as 0.
 // A row that attends to nothing gives o = 0 and lse = -inf.  A masked token has no effect,
-// whatever its slot holds.  Lengths, pages, scale, padding and precision are those of
+// whatever its slot holds; an infinity or NaN among the values that a row attends to leaves
+// that dim of its output infinite or NaN.  Lengths, pages, scale, padding and precision are those of
 // qllama_paged_attention, except that int8 rows also meet queries and weights held to 24
-// bits.  `nodes` is the number of rows of a request that the call is laid out for (0: rows
-// / n_req); any number of rows is right, other ones are slower.  Rows that no request has
+// bits, and that f32 rows, where a tile has 64 columns or more (rows times query heads of a
+// KV head), may enter the products as three 16-bit parts each: what is dropped is below 2^-22
+// of a product.  width * page_size and rows * n_heads have to be below 2^31 - 1024.  `nodes` is the number of rows of a request that the call is laid out for (0: rows
+// / n_req), the same that qllama_tree_attention_work is asked for; any number of rows is
+// right, other ones are slower.  Rows that no request has
 // are left as they were.  starts outside 0 .. rows count as the nearest inside; a row that
 // two requests name gets either result.  work: qllama_tree_attention_work bytes, 16-byte aligned.
 typedef struct {

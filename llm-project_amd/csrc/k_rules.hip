@@ -6,7 +6,9 @@
 // in registers while the row's history is counted into LDS, a counter a token of the slice
 // (every block of a row reads the whole history, 4 bytes a token out of L2), then every
 // thread looks at its tokens' counters and the mask's bits.  The few tokens that a rule
-// touches are evaluated in 64 bits.
+// touches are evaluated in 64 bits.  192 rows of 128256 with histories of up to 8000 tokens,
+// biases and masks: 44 us, 4.6 TB/s (a 1 GiB copy: 5.1); 9 rows each of 40 trees, 32000
+// tokens: 21.6 us, 3.7 TB/s; 4 rows 5.1 us, a launch and three trips to memory.
 #include <hip/hip_runtime.h>
 
 #include "qserve_host.h"

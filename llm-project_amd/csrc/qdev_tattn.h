@@ -5,19 +5,45 @@
 // (llama.c:554-576) serves one token.
 //
 // The columns of a (request, KV head) are its rows times the query heads that share the KV
-// head; a tile is up to COLS of them, and takes every key and value of the request
-// through LDS once.  Eight waves: CG groups of columns, and KP = 8 / CG parts of a step's
-// keys, so that few columns leave every wave a part of the keys to itself, and many share
-// what was staged.  S^T = K q^T on the matrix cores puts a column in a lane's column and 4
-// keys of each 16 in its rows; the same lane's weights are then the operand of
-// O^T += V^T P^T, whose contraction slots are matched to the keys that the lane holds, so
-// weights never move between lanes.
+// head; a tile is 16 CG of them, and takes every key and value of the request once: CG waves
+// side by side, 16 columns each, share what they stage in LDS.  S^T = K q^T on the matrix
+// cores puts a column in a lane's column and 4 keys of each 16 in its rows; the same lane's
+// weights are then the operand of O^T += V^T P^T, whose contraction slots are matched to the
+// keys that the lane holds, so weights never move between lanes; values come out of LDS by
+// transposing reads.
 //
-// The work of a call is the key steps of all tiles, laid one behind another; every block
-// takes an equal share of them, whatever the lengths are, without the host knowing one.  A
-// share that ends inside a tile leaves its maxima, sums and weighted values in the
-// workspace, and k_tree_join puts a tile's parts together.  Where the tables are short a
-// block takes whole tiles, and there is no second launch.
+// The work of a call is the key steps of all tiles, laid one behind another, and for each tile
+// some steps more for its beginning and end; every group of CG waves takes an equal share,
+// whatever the lengths are, without the host knowing one.  A share that ends inside a tile
+// leaves its maxima, sums and weighted values in the workspace, and k_tree_join puts a tile's
+// parts together.  Where the tables are short a block takes whole tiles, its waves also parts
+// of the keys that meet at the end, and there is no second launch (launch() has the rule).
+//
+// Precision as in k_pattn.hip: float queries and weights meet 16-bit keys and values as three
+// (bf16, int8 codes) or two (f16) 16-bit parts; f32 rows go through the fp32 MFMA, or,
+// where a tile has many columns, as three parts themselves.
+//
+// What bounds it: up to 32 columns memory (every byte takes part in 8 multiply-adds a
+// 4 rows of 4 heads); from 64 on the matrix products of the parts and the softmax beside them:
+// of a step's 6700 cycles (64 keys, 128 bf16 columns, heads of 128) 4500 are products and
+// weights, 1500 of them on the matrix cores' own count for each of a SIMD's two waves, the
+// rest is staging, places and the barrier.  Measured (both kernels; 32 query and 8 KV heads
+// of 128 if not said; a 1 GiB copy moves 5.1 TB/s, a large bf16 product 1190 TFLOP/s):
+//   64 ragged requests of up to 2560 tokens, bf16, 4 rows      84-89 us   4.5 TB/s
+//   the same, 8 rows                                           88-91 us   4.3 TB/s
+//   32 of them, up to 16 rows                                  72 us      3.0 TB/s
+//   32 of them, up to 32 rows                                  89 us      2.0 TB/s, 570 TFLOP/s in parts
+//   32 of them, up to 64 rows                                  162 us     700 TFLOP/s in parts
+//   2 requests of up to 60000 tokens, f16, 48 rows             120-130 us 2.7 TB/s, 400 TFLOP/s in parts
+//   64 requests of up to 4100 tokens, int8, 7 rows             101-114 us 2.6 TB/s
+//   6 requests of up to 2048 tokens, f32, heads of 64, 200 rows in a chain  106-113 us  680 TFLOP/s in parts
+//   1 request of 2060 tokens, bf16, 8 rows                     22 us
+// Measured and not kept: 32 columns a wave (queries and sums of both spill: 225 us against 144 at
+// 32 rows); eight waves a tile whatever its columns, four of them on other keys (82 against
+// 72); scores a step ahead of the weights, so that products run beside the exponentials (107
+// against 102 at 8 rows, 192 against 201 at 64, before other steps); a raised priority while
+// products run (95 against 89 at 32 rows); blocks of one XCD on shares beside each other (132
+// against 127 for the two long requests).
 #ifndef QDEV_TATTN_H
 #define QDEV_TATTN_H
 
@@ -232,7 +258,7 @@ __global__ __launch_bounds__((Cfg<T, HDP, CG, KP>::THREADS), 2) void k_tree_attn
     };
     long long upto = scan64(units_of(lane)), units = uniform(__shfl(upto, 63));            // of requests up to the lane's, 64 at a time
     for (int x = 64; x < a.n_req; x += 64) units += uniform(__shfl(scan64(units_of(x + lane)), 63));
-    share = max((units + C::SHARES - 1) / C::SHARES, 2LL);
+    share = max((units + C::SHARES - 1) / C::SHARES, 2LL);      // one request of 2060 tokens: 27 us with 1, 22.5 with 2
     u = blockIdx.x * share;
     end = min(u + share, units);
     if (threadIdx.x == 0) a.split[blockIdx.x] = make_int4(0, 0, 0, 0);
@@ -806,6 +832,10 @@ int launch(const char *fn, const TaArgs &a, hipStream_t stream) {
   static_assert(W::LDSB <= 160 * 1024 && C::LDSB <= 160 * 1024, "LDS");
   const long long room = ((long long)a.width * a.page_size + W::STEP - 1) / W::STEP;
   const long long tiles = ((long long)a.rows * a.G / W::COLS + a.n_req) * a.n_kv;
+  // Whole tiles where their steps are few, more where there are tiles for all CUs.  Against shares, us (8 KV heads, hd 128):
+  // 16 bf16 requests of up to 300 tokens and 8 rows 16.6 / 21.3, 32 of 500 and 16 rows 30.7 / 34.9, 2 int8 ones of 100 and
+  // 10 rows 10.8 / 14.3; few tiles of more steps the other way: 4 of 450 and 16 rows 27.6 / 19.2, one f32 request of 200
+  // tokens, 2 KV heads of 48, 13.8 / 12.2
   const bool whole = room <= (tiles >= 256 ? 16 : tiles >= 128 ? 8 : 4) && a.n_req <= 65535;
   void (*f)(TaArgs) = whole ? k_tree_attn<T, HDP, CG, KP, true> : k_tree_attn<T, HDP, CG, 1, false>;
   const int lds = whole ? W::LDSB : C::LDSB;

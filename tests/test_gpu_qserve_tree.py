@@ -4,7 +4,7 @@ import math
 import random
 
 import pytest
-from test_gpu_qserve import EPS, Buffer, Dev, Q, Work, dev_i32, i32, make_cache, pages_for, same, widened  # noqa: F401
+from test_gpu_qserve import EPS, Buffer, Dev, Graph, Q, Work, dev_i32, i32, make_cache, pages_for, same, widened  # noqa: F401
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -338,3 +338,20 @@ def test_equal_inputs_give_equal_bits(Q):  # noqa: F811
     for _ in range(3):
         again = attend(Q, kv, q, starts, widened(table, 16), lens, mask)
         assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
+@pytest.mark.parametrize("typ,H,KVH,hd,nodes", [("bf16", 16, 1, 256, 8), ("f32", 16, 2, 128, 12), ("i8", 4, 4, 128, 9)])
+def test_in_a_graph(Q, typ, H, KVH, hd, nodes):  # noqa: F811
+    """The largest tiles in LDS (set as the launch's own size), and both launches of a split call, under capture."""
+    kv, q, starts, table, lens, seen, mask = case(typ, H, KVH, hd, 16, "head", [2000, 77, 300], [nodes, 2, nodes], 1, 4, Q, "tree")
+    for t in (table, table[1:2, :5].contiguous()):
+        n, s = len(t), starts if len(t) == 3 else [0, 2]
+        x, m, L = (q, mask, lens) if n == 3 else (q[nodes:nodes + 2].contiguous(), mask[nodes:nodes + 2].contiguous(), lens[1:2])
+        want = attend(Q, kv, x, s, t, L, m, nodes, spare=0)
+        dq, dm, dt, dn, ds, o, lse = Dev(x), Dev(m), Dev(t), dev_i32(L), dev_i32(s), Dev(torch.zeros_like(x)), Dev(torch.zeros(x.shape[:2]))
+        work = Work(Buffer(Q.tree_attention_work(kv, len(x), n, H, nodes)))
+        graph = Graph(lambda stream: Q.tree_attention(kv, dq, ds, dt, dn, o, work, mask=dm, lse=lse, nodes=nodes, stream=stream))
+        for _ in range(3):
+            o.set(torch.zeros_like(x))
+            graph.replay()
+            assert same(o, want[0]) and same(lse, want[1])

@@ -105,7 +105,7 @@ REFUSED += [("query", kw, w) for kw, w in [
     ({"mask": 0}, "words"), ({"mask": A + 4}, "aligned"), ({"q_stride": 255}, "stride"), ({"o_stride": 0}, "stride"), ({"lse": A, "lse_stride": 3}, "stride"),
     ({"width": 0}, "width"), ({"table_stride": 4}, "width"), ({"width": (1 << 27) - 60, "table_stride": 1 << 27}, "2^31 - 1024"), ({"scale": -1.0}, "scale"),
     ({"scale": float("nan")}, "scale"), ({"scale": float("inf")}, "scale"), ({"o": A}, "o must not"), ({"work": 0}, "work"), ({"work": A + 8}, "work"),
-    ({"work_bytes": 100}, "work"), ({"q": A + 1}, "aligned"), ({"rows": 1 << 23, "n_heads": 256, "q_stride": 1 << 20, "o_stride": 1 << 20}, "31 bits"),
+    ({"work_bytes": 100}, "work"), ({"q": A + 1}, "aligned"), ({"rows": 1 << 23, "n_heads": 256, "q_stride": 1 << 20, "o_stride": 1 << 20}, "2^31 - 1024"),
     ({"n_req": 1 << 30, "rows": 1 << 22, "n_heads": 256, "q_stride": 1 << 20, "o_stride": 1 << 20, "width": 1 << 26, "table_stride": 1 << 26}, "too large")]]
 REFUSED += [("fork", kw, w) for kw, w in [
     ({"n_old": -1}, "n_old"), ({"n_new": 8193}, "n_old"), ({"width": 0}, "width"), ({"page_size": 0}, "page size"),
