@@ -53,7 +53,7 @@ __device__ inline unsigned long long fork_rank(int covered, int i) { return (uns
 // requests one block takes all steps, a wave a request at a time; else every step is a launch,
 // with a block a request.  Two requests of up to 700 tokens continued by four each: 8 us in one
 // block, 14 in six launches, whose enqueueing takes the host 15 us more; 512 requests (256 old
-// and new, 40 pages each): 110 us in one block, 20 in launches, latencies all.
+// and new, 40 pages each): more than 100 us in one block, 20 in launches, latencies all.
 // Of what a step hands to the next: in the L2, also within one launch.
 template <typename T>
 __device__ inline T load(const T *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }

@@ -23,8 +23,8 @@
 // (bf16, int8 codes) or two (f16) 16-bit parts; f32 rows go through the fp32 MFMA, or,
 // where a tile has many columns, as three parts themselves.
 //
-// What bounds it: up to 32 columns memory (every byte takes part in 8 multiply-adds a
-// 4 rows of 4 heads); from 64 on the matrix products of the parts and the softmax beside them:
+// What bounds it: up to 32 columns memory (int8: the codes' conversion too); from 64 on the
+// matrix products of the parts and the softmax beside them:
 // of a step's 6700 cycles (64 keys, 128 bf16 columns, heads of 128) 4500 are products and
 // weights, 1500 of them on the matrix cores' own count for each of a SIMD's two waves, the
 // rest is staging, places and the barrier.  Measured (both kernels; 32 query and 8 KV heads
@@ -39,9 +39,10 @@
 //   6 requests of up to 2048 tokens, f32, heads of 64, 200 rows in a chain  106-113 us  680 TFLOP/s in parts
 //   1 request of 2060 tokens, bf16, 8 rows                     22 us
 // Measured and not kept: 32 columns a wave (queries and sums of both spill: 225 us against 144 at
-// 32 rows); eight waves a tile whatever its columns, four of them on other keys (82 against
-// 72); scores a step ahead of the weights, so that products run beside the exponentials (107
-// against 102 at 8 rows, 192 against 201 at 64, before other steps); a raised priority while
+// 32 rows); blocks of eight waves whatever the columns, on other parts of a step's keys, that
+// begin and end tiles together (113 against 99 at 16 rows); scores a step ahead of the weights,
+// so that products run beside the exponentials (107 against 102 at 8 rows, 192 against 201 at
+// 64; with registers that the queries need); a raised priority while
 // products run (95 against 89 at 32 rows); blocks of one XCD on shares beside each other (132
 // against 127 for the two long requests).
 #ifndef QDEV_TATTN_H
