@@ -863,7 +863,8 @@ int launch_tile(const char *fn, const TaArgs &a, int tile, hipStream_t stream) {
     switch (tile) {
       case 0: return launch<T, HDP, 1>(fn, a, stream);
       case 1: return launch<T, HDP, 2>(fn, a, stream);
-      case 2: return launch<T, HDP, 4>(fn, a, stream);
+      case 2:
+        if constexpr (T != QLLAMA_KV_F32 || HDP != 128) return launch<T, HDP, 4>(fn, a, stream);       // never asked for
       default: return launch<T, HDP, 8>(fn, a, stream);
     }
   }
