@@ -88,7 +88,6 @@ namespace {
 using namespace qpaged;
 using namespace qtree;
 
-
 // What a type, a padded head size, the waves side by side and the parts of a step's keys fix.
 template <int T, int HDP, int CG_, int KP_>
 struct Cfg {
@@ -105,13 +104,13 @@ struct Cfg {
   static constexpr int SUB = F32 ? 1 : 2, KEYS = 16 * SUB;              // keys that a wave takes at a time
   // times that it does between two barriers, as far as registers and LDS allow
   static constexpr int TIMES = SPLIT ? (HDP == 64 && CG == 8 ? 2 : 1) : CG >= 4 && HDP <= 128 ? 2 : 1, KS = KEYS * TIMES, STEP = KS * KP;
-// steps that a tile's beginning and end take the time of
+  // keys, and steps, whose time a tile's beginning and end take
   static constexpr int OVERKEYS = CG == 8 ? 256 : CG == 4 && HDP > 64 ? 128 : 64, OVER = OVERKEYS / STEP < 1 ? 1 : OVERKEYS / STEP;
   static constexpr int ROWB = HDP * LES, CH = ROWB / 16, SWZ = (CH < 16 ? CH : 16) - 1, EPC = 16 / LES;
   static constexpr int PLANEB = KS * ROWB, SIDEB = PLANES * PLANEB, PARTB = 2 * SIDEB;  // a part's keys, then values
   static constexpr int NBUF = CG == 1 ? 1 : 2;                          // a wave alone with its part needs no second buffer
+  static constexpr bool ONCE = CG <= 2;                                 // a tile has a request's columns, all or nearly: loads past the caches' retention
   // threads that stage a part, and units of each: 16 bytes of the cache (split: 32), CPU chunks of 16 bytes in LDS (split: one a part)
-  static constexpr bool ONCE = CG <= 2;                                 // a tile has all of a request's columns, or nearly: past the caches' retention
   static constexpr int LOADS = SPLIT ? 2 : 1, CPU = T == QLLAMA_KV_I8 ? 2 : 1, TP = 64 * CG, U = 2 * KS * CH / CPU / TP;
   static constexpr int DPL = HDP / 16, QC = F32 ? HDP / 16 : HDP / 32;
   static constexpr int PARTS = F32 ? 1 : HALF ? 2 : 3;
