@@ -932,15 +932,21 @@ def logit_rules(logits, out, requests=None, tokens=None, n_tokens=None, n_prompt
     """qllama_logit_rules: out (rows, vocab; may be logits) = logits with penalties for the tokens (requests, capacity) that
     a row's request has used and for the drafted ones above the row (mask (rows, words) int64), biases (requests, n_bias), and
     -inf where the mask allowed[allowed_rows] (masks, words) int32 has no bit set.  requests: the request of every row (None:
-    its own number)."""
+    its own number); there are as many requests as rows of the settings, and where none is given (masks alone) every number
+    but a negative one is a request."""
     rows, V = logits.shape
     lp, ls = _rows(logits, "logits", "float32", logits.shape)
     op, os_ = _rows(out, "out", "float32", logits.shape)
-    n = rows
+    if bias is not None and bias_tokens is None:
+        raise ValueError("bias needs bias_tokens")
+    n = rows if requests is None else 2 ** 31 - 1         # nothing is looked up by request
     for t in (n_tokens, repetition, presence, frequency, bias):
         if t is not None:
             n = t.shape[0]
             break
+    else:
+        if mask is not None and starts is not None:
+            n = starts.numel() - 1
     cap = ts = tp = words = nb = bs = btp = bp = nm = ms = mp = 0
     if tokens is not None:
         if n_tokens is None:

@@ -153,3 +153,29 @@ def test_lengths_out_of_range(Q):  # noqa: F811
     Q.logit_rules(Dev(torch.ones(3, 6)), out, tokens=tokens, n_tokens=dev_i32([2 ** 31 - 1, -5, 2]), n_prompt=dev_i32([-1, 3, 9]),
                   presence=Dev(torch.tensor([1.0, 1.0, 1.0])), repetition=Dev(torch.tensor([1.0, 2.0, 2.0])))
     assert out.get().tolist() == [[1, 0, 0, 0, 1, 1], [1] * 6, [1, 1, 1, 1, 0.5, 1]]
+
+
+def test_masks_of_requests_beyond_the_rows(Q):  # noqa: F811
+    """Without settings nothing is looked up by request, and any number but a negative one names a row that takes part: a grammar
+    alone, one active request of many; a drafted tree's rows with no penalties."""
+    x = torch.randn(3, 70)
+    words = torch.tensor([[5, 0, 1], [-1, -1, -1]], dtype=torch.int32)
+    want = torch.full((3, 70), -INF)
+    want[0, [0, 2, 64]] = x[0, [0, 2, 64]]
+    want[1] = x[1]
+    for req in ([3, 900, 2 ** 31 - 2], [3, 3, -1]):
+        want[2] = x[2] if req[2] < 0 else torch.where(want[0] > -INF, x[2], -INF)
+        same_row = Dev(x.clone())
+        Q.logit_rules(same_row, same_row, requests=dev_i32(req), allowed=Dev(words), allowed_rows=dev_i32([0, 1, 0]))
+        assert torch.equal(same_row.get(), want)
+        out = Dev(torch.full((3, 70), 7.0))
+        Q.logit_rules(Dev(x), out, requests=dev_i32(req), allowed=Dev(words), allowed_rows=dev_i32([0, 1, 0]))
+        if req[2] < 0:
+            want[2] = 7.0
+        assert torch.equal(out.get(), want)
+    out = Dev(torch.full((3, 70), 7.0))
+    Q.logit_rules(Dev(x), out, requests=dev_i32([0, 0, 0]), starts=dev_i32([0, 3]), drafted=dev_i32([1, 2, 3]), mask=Dev(torch.ones((3, 1), dtype=torch.int64)),
+                  allowed=Dev(words), allowed_rows=dev_i32([0, 1, 1]))
+    want[0], want[2] = torch.full((70,), -INF), x[2]
+    want[0, [0, 2, 64]] = x[0, [0, 2, 64]]
+    assert torch.equal(out.get(), want)

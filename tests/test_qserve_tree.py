@@ -172,3 +172,50 @@ def test_python_mirror_refuses_what_does_not_fit():
         Q.logit_rules(f, f, stream=0)
     with pytest.raises(ValueError, match="no such requests"):
         Q.paged_fork_work(1, 1, 0)
+
+
+class Tensor:
+    """A host tensor that passes for one on the GPU: the mirror only reads its address, type, shape and strides."""
+    is_cuda = True
+
+    def __init__(self, t):
+        self.t = t
+
+    def __getattr__(self, name):
+        return getattr(self.t, name)
+
+
+class Calls:
+    """In the library's place: keeps the structures that it is handed."""
+
+    def __getattr__(self, name):
+        return lambda a, stream: self.__dict__.__setitem__("got", a) or 0
+
+
+def packed(monkeypatch, kind, call):
+    monkeypatch.setattr(Q, "_lib", Calls())
+    call()
+    _, fmt, fields = FIELDS[kind]
+    return dict(zip(fields.split(), fmt.unpack(Q._lib.__dict__["got"])))
+
+
+def test_logit_rules_counts_requests_where_something_is_looked_up_by_them(monkeypatch):
+    """The number of requests is that of the settings' rows; without any, all numbers but negative ones are requests."""
+    torch = pytest.importorskip("torch")
+    i = lambda *s: Tensor(torch.zeros(s, dtype=torch.int32))  # noqa: E731
+    f = lambda *s: Tensor(torch.zeros(s))  # noqa: E731
+    x, masks, tree = f(2, 40), dict(allowed=i(1, 2), allowed_rows=i(2)), dict(mask=Tensor(torch.zeros((2, 1), dtype=torch.int64)), drafted=i(2))
+    n_req = lambda **kw: packed(monkeypatch, "rules", lambda: Q.logit_rules(x, x, stream=0, **kw))["n_req"]  # noqa: E731
+    assert n_req(**masks) == 2
+    assert n_req(requests=i(2), **masks) == 2 ** 31 - 1
+    assert n_req(requests=i(2)) == 2 ** 31 - 1
+    assert n_req(requests=i(2), starts=i(6), **tree, **masks) == 5
+    assert n_req(requests=i(2), starts=i(2), **tree) == 1
+    assert n_req(requests=i(2), tokens=i(5, 3), n_tokens=i(5)) == 5
+    for name, t in (("repetition", f(7)), ("presence", f(7)), ("frequency", f(7))):
+        assert n_req(requests=i(2), **{name: t}, **masks) == 7
+    assert n_req(requests=i(2), bias=f(4, 2), bias_tokens=i(4, 2)) == 4
+    with pytest.raises(ValueError, match="frequency has 3 elements"):
+        n_req(requests=i(2), presence=f(4), frequency=f(3))
+    with pytest.raises(ValueError, match="bias_tokens"):
+        n_req(bias=f(2, 2))
