@@ -21,7 +21,7 @@
 //
 // Precision as in k_pattn.hip: float queries and weights meet 16-bit keys and values as three
 // (bf16, int8 codes) or two (f16) 16-bit parts; f32 rows go through the fp32 MFMA, or,
-// where a tile has many columns, as three parts themselves.
+// where a tile has many columns, as three parts themselves, as close as 32-bit products.
 //
 // What bounds it: up to 32 columns memory (int8: the codes' conversion too); from 64 on the
 // matrix products of the parts and the softmax beside them:
@@ -93,8 +93,10 @@ template <int T, int HDP, int CG_, int KP_>
 struct Cfg {
   static constexpr int CG = CG_, KP = KP_, THREADS = 64 * CG * KP, COLS = 16 * CG;
   static constexpr int SHARES = kShares / CG;
-  // f32 rows: as they are, or (many columns) in three bf16 parts, which the matrix cores take 16 times as fast: the six
-  // products of parts that count make it 2.7 times.  Dropped ones are below 2^-22 of a product
+  // f32 rows: as they are, or (many columns) in three bf16 parts, queries and weights too, which the matrix cores take 16 times
+  // as fast: the six products of parts that count make it 2.7 times.  Dropped ones, of a second with a third part or two
+  // thirds, add up to 2^-24 of a product, what rounding it to 32 bits takes (with cut queries and weights it was 2^-21.6, always
+  // toward 0)
   static constexpr bool SPLIT = T == QLLAMA_KV_F32 && (HDP == 64 ? CG >= 4 : HDP == 128 && CG == 8), F32 = T == QLLAMA_KV_F32 && !SPLIT;
   static constexpr bool HALF = T == QLLAMA_KV_F16;
   static constexpr int PLANES = SPLIT ? 3 : 1;
@@ -171,24 +173,28 @@ __device__ inline bool odd_value(uint32_t x) {
   return (x & E) == E;
 }
 
-// 8 floats as sums of three bf16 numbers: the first cut (a float's range fits), the others rounded to nearest, off by 2^-25.
+// 8 floats as sums of three bf16 numbers, each rounded to nearest: exact, the second at most 2^-8 and the third 2^-17 of the
+// first.  ANY: the first has to be kept within bf16's range, which ends 2^-9 below a float's.
 typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
-__device__ inline Parts3 split3(u4 x, u4 y) {
+template <bool ANY>
+__device__ inline Parts3 round3(const float (&x)[8]) {
   Parts3 r;
+  constexpr float most = 0x1.fep127f;
 #pragma unroll
   for (int i = 0; i < 4; i++) {
-    const uint32_t lo = i < 2 ? x[2 * i] : y[2 * i - 4], hi = i < 2 ? x[2 * i + 1] : y[2 * i - 3];
-    r.p[0][i] = hi16s(hi, lo);
-    float a = __uint_as_float(lo) - __uint_as_float(lo & 0xffff0000u), b = __uint_as_float(hi) - __uint_as_float(hi & 0xffff0000u);
-    const uint32_t mid = __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{a, b}, bf2));
-    a -= __uint_as_float(mid << 16);
-    b -= __uint_as_float(mid & 0xffff0000u);
-    r.p[1][i] = mid;
-    r.p[2][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{a, b}, bf2));
+    float a = x[2 * i], b = x[2 * i + 1];
+#pragma unroll
+    for (int k = 0; k < 3; k++) {
+      const f2 y = !ANY || k ? f2{a, b} : f2{__builtin_amdgcn_fmed3f(a, -most, most), __builtin_amdgcn_fmed3f(b, -most, most)};
+      r.p[k][i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(y, bf2));
+      if (k < 2) {
+        a -= __uint_as_float(r.p[k][i] << 16);
+        b -= __uint_as_float(r.p[k][i] & 0xffff0000u);
+      }
+    }
   }
   return r;
 }
-
 // The dim of a head whose output is element c of an accumulator's row `lane` of 16.
 template <typename C>
 __device__ inline int dim_of(int c, int lane) { return C::F32 ? 64 * (c / 4) + 4 * lane + c % 4 : 16 * c + lane; }
@@ -404,7 +410,10 @@ __global__ __launch_bounds__((Cfg<T, HDP, CG, KP>::THREADS), 2) void k_tree_attn
           }
           to += (chunk ^ (row & C::SWZ)) << 4;
           if constexpr (C::SPLIT) {
-            const Parts3 y = split3(w[0], w[1]);
+            float f[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) f[i] = __uint_as_float(w[i / 4][i % 4]);
+            const Parts3 y = round3<true>(f);
 #pragma unroll
             for (int k = 0; k < 3; k++) *reinterpret_cast<u4 *>(to + k * C::PLANEB) = y.p[k];
           } else {
@@ -492,7 +501,7 @@ __global__ __launch_bounds__((Cfg<T, HDP, CG, KP>::THREADS), 2) void k_tree_attn
 #pragma unroll
         for (int p = 0; p < C::PARTS; p++) qp[c][p] = y.p[p];
       } else {
-        const Parts3 y = cut3(f[c]);
+        const Parts3 y = C::SPLIT ? round3<true>(f[c]) : cut3(f[c]);
 #pragma unroll
         for (int p = 0; p < C::PARTS; p++) qp[c][p] = y.p[p];
       }
@@ -589,7 +598,7 @@ __global__ __launch_bounds__((Cfg<T, HDP, CG, KP>::THREADS), 2) void k_tree_attn
 #pragma unroll
         for (int k = 0; k < C::PARTS; k++) pp[k] = y.p[k];
       } else if constexpr (!C::F32) {
-        const Parts3 y = cut3(p);
+        const Parts3 y = C::SPLIT ? round3<false>(p) : cut3(p);
 #pragma unroll
         for (int k = 0; k < C::PARTS; k++) pp[k] = y.p[k];
       }

@@ -355,3 +355,66 @@ def test_in_a_graph(Q, typ, H, KVH, hd, nodes):  # noqa: F811
             o.set(torch.zeros_like(x))
             graph.replay()
             assert same(o, want[0]) and same(lse, want[1])
+
+
+# ---------------------------------------------------------------------------
+# f32 rows in 16-bit parts (64 heads: from 33 columns of a tile on)
+# ---------------------------------------------------------------------------
+LN2 = float(torch.tensor(0.69314718056))             # what a sum of exponents of 2 is multiplied by, as a 32-bit number
+UNIT = 0.6931471824645996                             # scale: times log2 e, in 32 bits, it is 1
+
+
+def alone(Q, k, q, hd, nodes):  # noqa: F811
+    """Scores of single products: row i of a request attends to itself alone, and key and queries of a row have one dim that is
+    not 0 (its own).  k (requests, rows), q (requests, rows, heads); what comes back is each lse."""
+    n, m, H = q.shape
+    page = 16
+    per = -(-m // page)
+    kv = Q.PagedKV(*(Dev(torch.zeros((n * per, 1, page, hd))) for _ in range(2)))
+    keys, rows, queries = torch.zeros((n, per * page, hd)), torch.arange(m), torch.zeros((n, m, H, hd))
+    keys[:, rows, rows % hd] = k
+    queries[:, rows, :, rows % hd] = q.transpose(0, 1)
+    kv.k.set(keys.view(n * per, 1, page, hd))
+    table = torch.arange(n * per, dtype=torch.int32).view(n, per)
+    mask = torch.tensor([signed(1 << j) for j in range(m)], dtype=torch.int64)[:, None].repeat(n, 1)
+    _, lse = attend(Q, kv, queries.view(n * m, H, hd), [m * i for i in range(n + 1)], table, [m] * n, mask, nodes=nodes, scale=UNIT)
+    return lse.view(n, m, H).double()
+
+
+@pytest.mark.parametrize("hd,nodes", [(64, 64), (64, 5), (128, 64), (64, 1), (128, 1)])
+def test_f32_products_are_as_close_as_32_bits(Q, hd, nodes):  # noqa: F811
+    """Keys and queries whose low halves are worst for parts that are cut (0xff7f and 0xffff: cut queries lose 5.6 x 2^-24 of
+    every product, toward 0).  Parts to nearest leave out 2^-24 of a product at most.  The roundings beside them (five sums, the
+    product with ln 2: 2^-24 each) go either way: over 4096 products of random signs and exponents their mean stays below
+    4 x 6 x 2^-24 / 64 < 2^-25.  Of a single one: 2^-24 and six roundings.  The same in tiles that take f32 products."""
+    g = torch.Generator().manual_seed(hd + nodes)
+
+    def numbers(shape, low):
+        bits = (torch.randint(0, 2, shape, generator=g) << 31) | (torch.randint(120, 134, shape, generator=g) << 23) | (torch.randint(0, 8, shape, generator=g) << 16) | low
+        return bits.to(torch.int64).where(bits < 2 ** 31, bits - 2 ** 32).to(torch.int32).view(torch.float32)
+
+    k, q = numbers((8, 64), 0xff7f), numbers((8, 64, 8), 0xffff)
+    want = k.double()[..., None] * q.double() * LN2
+    off = alone(Q, k, q, hd, nodes) / want - 1
+    assert float(off.abs().max()) <= 7 * EPS, off.abs().max() / EPS
+    assert abs(float(off.mean())) <= 2 * EPS, off.mean() / EPS
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_f32_weights_are_as_close_as_32_bits(Q, hd):  # noqa: F811
+    """All values of a request are alike, so that o = v whatever the weights are.  Weights that are cut make every product 2^-25.5
+    smaller on average, and o with them; what is rounded to nearest goes either way: some ten roundings of 2^-24 / sqrt(3) on
+    average, over 8 x hd different values (each with hundreds of weights) a mean below 4 x 10 ^ 0.5 x 2^-24 / (3 x 512) ^ 0.5 < 2^-25
+    even if all weights of a value agreed, and 2^-27 as they do not (tens of different ones)."""
+    g = torch.Generator().manual_seed(hd)
+    n, m, H, ctx, page = 8, 64, 8, 48, 16
+    per = (ctx + m) // page
+    kv = Q.PagedKV(*(Dev(torch.zeros((n * per, 1, page, hd))) for _ in range(2)))
+    v = torch.randn((n, 1, hd), generator=g).repeat(1, per * page, 1)
+    kv.k.set(torch.randn((n * per, 1, page, hd), generator=g))
+    kv.v.set(v.reshape(n * per, 1, page, hd))
+    q = torch.randn((n * m, H, hd), generator=g)
+    table = torch.arange(n * per, dtype=torch.int32).view(n, per)
+    o, _ = attend(Q, kv, q, [m * i for i in range(n + 1)], table, [ctx + m] * n, None, nodes=m)
+    off = o.double().view(n, m * H, hd) / v[:, :1].double() - 1
+    assert abs(float(off.mean())) <= EPS / 8, off.mean() / EPS
