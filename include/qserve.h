@@ -259,7 +259,9 @@ int qllama_tree_accept(const QTreeAccept *p, void *stream);
 // NULL: to b = 0 .. j (the next piece of a prompt).  Bits behind a row's words count as 0.
 // A row that attends to nothing gives o = 0 and lse = -inf.  A masked token has no effect,
 // whatever its slot holds; an infinity or NaN among the values that a row attends to leaves
-// that dim of its output infinite or NaN.  Lengths, pages, scale, padding and precision are
+// that dim of its output infinite or NaN.  A score of -inf, of an infinite f32 key, is a
+// weight of 0, one of +inf or NaN makes the row's outputs NaN; an infinite key in 16 bits
+// may make them NaN either way.  Lengths, pages, scale, padding and precision are
 // those of qllama_paged_attention, except that int8 rows also meet queries and weights held
 // to 24 bits, and that f32 rows, where a tile has 64 columns or more (rows times query heads
 // of a KV head), may enter the products, as queries and weights do, as three 16-bit parts

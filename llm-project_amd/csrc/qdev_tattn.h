@@ -568,6 +568,35 @@ __global__ __launch_bounds__((Cfg<T, HDP, CG, KP>::THREADS), 2) void k_tree_attn
               if constexpr (T == QLLAMA_KV_I8) fv[i][j] = 0.0f;          // whatever the scale is
             }
       }
+      if constexpr (C::SPLIT) {
+        // parts of an infinity, or of products that leave a float's range, make a score NaN that may be an infinity: such scores
+        // one by one, for a column that is not NaN anyway
+        float all = 0.0f;
+#pragma unroll
+        for (int i = 0; i < SUB; i++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) all += d[i][j];
+        if (__any(all != all && sum == sum)) {
+          const float *q = a.q + row * a.q_stride + (long long)head * a.hd;
+#pragma unroll
+          for (int i = 0; i < SUB; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+              if (d[i][j] == d[i][j] || sum != sum) continue;          // a score that is left is a key's
+              const float *k = reinterpret_cast<const float *>(kbase + offs[((s & 3) * KP + part) * KS + t * C::KEYS + 16 * i + 4 * g + j]);
+              float x = 0.0f;
+#pragma unroll 1
+              for (int e = 0; e < a.hd; e += 8) {
+                float y[8], z[8];
+                __builtin_memcpy(y, q + e, sizeof y);
+                __builtin_memcpy(z, k + e, sizeof z);
+#pragma unroll
+                for (int l = 0; l < 8; l++) x = fmaf(y[l] * a.qscale, z[l], x);
+              }
+              d[i][j] = x;
+            }
+        }
+      }
       float up = d[0][0];
 #pragma unroll
       for (int i = 0; i < SUB; i++)

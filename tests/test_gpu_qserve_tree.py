@@ -418,3 +418,33 @@ def test_f32_weights_are_as_close_as_32_bits(Q, hd):  # noqa: F811
     o, _ = attend(Q, kv, q, [m * i for i in range(n + 1)], table, [ctx + m] * n, None, nodes=m)
     off = o.double().view(n, m * H, hd) / v[:, :1].double() - 1
     assert abs(float(off.mean())) <= EPS / 8, off.mean() / EPS
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("nodes", [1, 11, 40])
+def test_an_infinite_f32_key(Q, hd, nodes):  # noqa: F811
+    """A score of -inf is a weight of 0, in every tile: rows whose queries turn an infinite key to that have the outputs that they
+    have without the token, the others none that is a number.  Both for an earlier token and for a new one."""
+    ctx, m = 70, 40
+    kv, q, starts, table, lens, _, _ = case("f32", 8, 2, hd, 1, "head", [ctx + m], [m], 1, 3, Q)
+    r = random.Random(hd)
+    seen = above(forest(r, m))
+    mask = torch.tensor([[signed(sum(1 << b for b in s))] for s in seen], dtype=torch.int64)
+    q[:, :, 3] = q[:, :, 3].abs() + 0.125
+    q[1::2, :, 3] *= -1.0
+    for t in (7, ctx + 2):
+        keep = kv.k.get()
+        x = keep.clone()
+        x[int(table[0, t]), :, 0, 3] = -math.inf
+        without = table.clone()
+        without[0, t] = -1
+        wo, wl, bound, lb = attend_ref(kv, q, starts, without, lens, seen)
+        kv.k.set(x)
+        for tab in (table, widened(table, 1)):
+            o, lse = (y.double() for y in attend(Q, kv, q, starts, tab, lens, mask, nodes))
+            for i in range(m):
+                if i % 2 and (t < ctx or t - ctx in seen[i]):
+                    assert not bool(torch.isfinite(o[i]).any()), i
+                else:
+                    assert bool(((o - wo)[i].abs() <= bound[i]).all()) and bool(((lse - wl)[i].abs() <= lb[i]).all()), i
+        kv.k.set(keep)
