@@ -261,17 +261,17 @@ int qllama_tree_accept(const QTreeAccept *p, void *stream);
 // whatever its slot holds; an infinity or NaN among the values that a row attends to leaves
 // that dim of its output infinite or NaN.  A score of -inf, of an infinite f32 key, is a
 // weight of 0, one of +inf or NaN makes the row's outputs NaN; an infinite key in 16 bits
-// may make them NaN either way.  Lengths, pages, scale, padding and precision are
-// those of qllama_paged_attention, except that int8 rows also meet queries and weights held
-// to 24 bits, and that f32 rows, where a tile has 64 columns or more (rows times query heads
-// of a KV head), may enter the products, as queries and weights do, as three 16-bit parts
-// that are exact; what is left out of a product of parts is below 1.001 x 2^-24 of it, as
-// rounding it to 32 bits leaves out.  width * page_size and rows * n_heads have to be below
-// 2^31 - 1024.  `nodes` is the number of rows of a request that the call is laid out for (0:
-// rows / n_req), the same that qllama_tree_attention_work is asked for; any number of rows
-// is right, other ones are slower.  Rows that no request has are left as they were.  starts
-// outside 0 .. rows count as the nearest inside; a row that two requests name gets either
-// result.  work: qllama_tree_attention_work bytes, 16-byte aligned.
+// may make them NaN either way.  Lengths, pages, scale, padding and precision are those of
+// qllama_paged_attention, except that int8 rows also meet queries and weights held to 24
+// bits, and that f32 rows of up to 128 dims, where `nodes` times the query heads of a KV
+// head is above 32, enter the products, as queries and weights do, as three 16-bit parts
+// that together are exact: what is left out of a product is below 1.001 x 2^-24 of it, as
+// much as rounding it to 32 bits leaves out.  width * page_size and rows * n_heads have to
+// be below 2^31 - 1024.  `nodes` is the number of rows of a request that the call is laid
+// out for (0: rows / n_req), the same that qllama_tree_attention_work is asked for; any
+// number of rows is right, other ones are slower.  Rows that no request has are left as they
+// were.  starts outside 0 .. rows count as the nearest inside; a row that two requests name
+// gets either result.  work: qllama_tree_attention_work bytes, 16-byte aligned.
 typedef struct {
   int rows;                 // of q, o, lse and mask
   int n_req, n_heads, width, words, nodes;

@@ -14,8 +14,9 @@ int pick(const QPagedKV *c, int rows, int n_req, int n_heads, int nodes) {
   if (nodes == 0) nodes = n_req ? (rows + n_req - 1) / n_req : 1;
   const int64_t cols = (int64_t)nodes * (n_heads / c->n_kv);
   if (c->head_dim > 128) return cols <= 64 ? 2 : 3;
-  // f32 rows of more than 64 dims go as 16-bit parts in 128 columns only (LDS): 8 requests with 45 rows 118 -> 99 us, 32 with
-  // 16, whose 64 columns fill half of it, 142 -> 138
+  // f32 rows of 65 to 128 dims have room for 16-bit parts (LDS) in tiles of 128 columns only, which pay from 33 on, half empty:
+  // against f32 products in 64 columns, 8 requests with 45 rows of 4 heads 118 -> 99 us, 64 ragged ones with 16 269 -> 256, 8
+  // with 12 60 -> 56, 2 of up to 20000 tokens with 16 125 -> 113; 32 ragged ones with 10 or 16 the same (149, 140)
   if (c->type == QLLAMA_KV_F32 && c->head_dim > 64 && cols > 32) return 3;
   if (cols <= 64) return cols <= 16 ? 0 : cols <= 32 ? 1 : 2;
   // 128 columns a tile unless 64 leave fewer of them empty, by a sixth of all

@@ -21,7 +21,8 @@
 //
 // Precision as in k_pattn.hip: float queries and weights meet 16-bit keys and values as three
 // (bf16, int8 codes) or two (f16) 16-bit parts; f32 rows go through the fp32 MFMA, or,
-// where a tile has many columns, as three parts themselves, as close as 32-bit products.
+// from 33 columns on with heads of up to 128, as three parts themselves, as close as 32-bit
+// products.
 //
 // What bounds it: up to 32 columns memory (int8: the codes' conversion too); from 64 on the
 // matrix products of the parts and the softmax beside them:
@@ -901,7 +902,7 @@ int launch_tile(const char *fn, const TaArgs &a, int tile, hipStream_t stream) {
       case 0: return launch<T, HDP, 1>(fn, a, stream);
       case 1: return launch<T, HDP, 2>(fn, a, stream);
       case 2:
-        if constexpr (T != QLLAMA_KV_F32 || HDP != 128) return launch<T, HDP, 4>(fn, a, stream);       // never asked for
+        if constexpr (T != QLLAMA_KV_F32 || HDP != 128) return launch<T, HDP, 4>(fn, a, stream);       // f32: pick() takes 128 columns
       default: return launch<T, HDP, 8>(fn, a, stream);
     }
   }

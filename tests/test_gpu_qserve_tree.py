@@ -358,7 +358,7 @@ def test_in_a_graph(Q, typ, H, KVH, hd, nodes):  # noqa: F811
 
 
 # ---------------------------------------------------------------------------
-# f32 rows in 16-bit parts (64 heads: from 33 columns of a tile on)
+# f32 rows in 16-bit parts (heads of up to 128, from 33 columns on)
 # ---------------------------------------------------------------------------
 LN2 = float(torch.tensor(0.69314718056))             # what a sum of exponents of 2 is multiplied by, as a 32-bit number
 UNIT = 0.6931471824645996                             # scale: times log2 e, in 32 bits, it is 1
@@ -399,6 +399,15 @@ def test_f32_products_are_as_close_as_32_bits(Q, hd, nodes):  # noqa: F811
     assert float(off.abs().max()) <= 7 * EPS, off.abs().max() / EPS
     assert abs(float(off.mean())) <= 2 * EPS, off.mean() / EPS
 
+
+@pytest.mark.parametrize("hd,nodes", [(64, 1), (64, 4), (72, 4), (128, 1), (128, 4), (160, 8), (256, 64)])
+def test_f32_products_of_few_columns_are_rounded_once(Q, hd, nodes):  # noqa: F811
+    """Up to 32 columns (8 a row here), and with heads of more than 128, f32 rows are not taken apart: a product has one rounding,
+    its product with ln 2 another."""
+    g = torch.Generator().manual_seed(hd + nodes)
+    k, q = torch.randn((8, 64), generator=g), torch.randn((8, 64, 8), generator=g)
+    off = alone(Q, k, q, hd, nodes) / (k.double()[..., None] * q.double() * LN2) - 1
+    assert float(off.abs().max()) <= 2 * EPS * (1 + EPS), off.abs().max() / EPS
 
 @pytest.mark.parametrize("hd", [64, 128])
 def test_f32_weights_are_as_close_as_32_bits(Q, hd):  # noqa: F811
