@@ -223,6 +223,8 @@ unsigned long long qllama_test_sample_weight(float logit, float top, float tempe
 // positions[i] = lens[r] - m + depth of the row (0 for a row that follows none); bit b of
 // mask[i] (bit b mod 64 of its word b / 64) is set for b = j and every row above j.  Rows
 // behind the first 64 * words of a request get mask 0 and the position lens[r] - m + j.
+// Such rows attend to nothing new, not even to themselves, so that trees need words >=
+// ceil(nodes / 64), and have 256 rows at most.
 typedef struct {
   int n_req;                // 0 .. 8192
   int nodes;                // rows of a request that parents has room for: 1 .. 1024
@@ -243,7 +245,11 @@ int qllama_tree_plan(const QTreePlan *p, void *stream);
 // the k-th accepted row of the step, -1 behind them; where it is not row k of its request,
 // src and dst are the slots that its keys and values have to be moved between (dst: that
 // of row k), else -1: groups of qllama_paged_move, with starts as they are.  Rows that no
-// request has are left as they were.
+// request has are left as they were.  Rows behind the first `nodes` follow none and are not
+// accepted: where the rows attended with a mask, nodes has to be 64 * words at most (the
+// stride as it is), as what was chosen behind the other rows is no one's choice.  Every
+// request of a call is verified: rows that are certain (a piece of a prompt) go without
+// this call, in a step of their own, or have their next row's token in chosen.
 typedef struct {
   int n_req, nodes, max_rows;                // as QTreePlan's
   int64_t parent_stride;

@@ -830,7 +830,8 @@ def sample_rows(logits, u, token, work, temperature=None, top_k=None, top_p=None
 # ---- qserve.h: drafted trees, pages that requests share, rules on logits -----------------
 def tree_plan(starts, lens, parents, positions, mask, stream=None):
     """qllama_tree_plan: position and ancestors (mask (rows, words) int64, bit b of a row: new row b of its request) of every
-    new row, from parents (requests, nodes) int32; starts and lens are paged_plan's."""
+    new row, from parents (requests, nodes) int32; starts and lens are paged_plan's.  words: ceil(nodes / 64), up to 4; rows
+    behind the first 64 * words get mask 0 (tree_accept leaves them out when it is given the mask)."""
     n, nodes = parents.shape
     rows, words = mask.shape
     pp, ps = _rows(parents, "parents", "int32", parents.shape)
@@ -839,13 +840,16 @@ def tree_plan(starts, lens, parents, positions, mask, stream=None):
     _done((_lib or lib()).qllama_tree_plan(a, _stream(stream)), "qllama_tree_plan")
 
 
-def tree_accept(starts, lens, parents, tokens, chosen, slots, accepted, last, lens_out, path, src, dst, stream=None):
+def tree_accept(starts, lens, parents, tokens, chosen, slots, accepted, last, lens_out, path, src, dst, stream=None, mask=None):
     """qllama_tree_accept: how many new rows of every request the chosen tokens confirm, what was chosen behind the last of
     them, the requests' new lengths, the accepted rows and the moves that put them one behind another.  int32 tensors; the
-    arguments after slots are outputs."""
+    arguments after slots are outputs.  mask: what the rows attended with; rows behind its 64 * words, which have attended to
+    nothing new, are not accepted (None: a chain without a mask, or one that has room for all)."""
     n, nodes = parents.shape
     rows = path.numel()
     pp, ps = _rows(parents, "parents", "int32", parents.shape)
+    if mask is not None:
+        nodes = min(nodes, 64 * mask.shape[1])
     at = _flat("int32", (starts, "starts", n + 1), (lens, "lens", n), (tokens, "tokens", rows), (chosen, "chosen", rows), (slots, "slots", rows),
                (accepted, "accepted", n), (last, "last", n), (lens_out, "lens_out", n), (path, "path", rows), (src, "src", rows), (dst, "dst", rows))
     a = TREE_ACCEPT.pack(n, nodes, rows, ps, at[0], at[1], pp, *at[2:])

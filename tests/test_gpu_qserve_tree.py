@@ -457,3 +457,17 @@ def test_an_infinite_f32_key(Q, hd, nodes):  # noqa: F811
                 else:
                     assert bool(((o - wo)[i].abs() <= bound[i]).all()) and bool(((lse - wl)[i].abs() <= lb[i]).all()), i
         kv.k.set(keep)
+
+
+def test_no_row_behind_the_mask_is_accepted(Q):  # noqa: F811
+    """A chain of 100 drafted rows whose tokens all fit, with a mask of one word: rows 64 .. 99 have mask 0 and are left out."""
+    m = 100
+    par, starts, lens = Dev(torch.arange(-1, m - 1, dtype=torch.int32).view(1, m)), dev_i32([0, m]), dev_i32([300])
+    for words, want in ((1, 64), (2, 100)):
+        pos, mask = i32(m), Dev(torch.zeros((m, words), dtype=torch.int64))
+        Q.tree_plan(starts, lens, par, pos, mask)
+        assert (mask.get() != 0).any(1).sum().item() == want
+        out, rows = [i32(1), i32(1), i32(1)], [i32(m), i32(m), i32(m)]
+        Q.tree_accept(starts, lens, par, dev_i32([5] * m), dev_i32([5] * m), dev_i32(list(range(m))), *out, *rows, mask=mask)
+        assert [x.get().item() for x in out] == [want, 5, 200 + want]
+        assert rows[0].get().tolist() == list(range(want)) + [-1] * (m - want) and rows[1].get().tolist() == [-1] * m

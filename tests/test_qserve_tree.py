@@ -219,3 +219,12 @@ def test_logit_rules_counts_requests_where_something_is_looked_up_by_them(monkey
         n_req(requests=i(2), presence=f(4), frequency=f(3))
     with pytest.raises(ValueError, match="bias_tokens"):
         n_req(bias=f(2, 2))
+
+
+def test_tree_accept_leaves_out_rows_that_the_mask_has_no_bit_for(monkeypatch):
+    torch = pytest.importorskip("torch")
+    i = lambda *s: Tensor(torch.zeros(s, dtype=torch.int32))  # noqa: E731
+    args = (i(3), i(2), i(2, 100), *(i(200) for _ in range(3)), *(i(2) for _ in range(3)), *(i(200) for _ in range(3)))
+    call = lambda *m: packed(monkeypatch, "tree_accept", lambda: Q.tree_accept(*args, stream=0, **(dict(mask=Tensor(torch.zeros((200, m[0]), dtype=torch.int64))) if m else {})))  # noqa: E731
+    for got, nodes in ((call(), 100), (call(1), 64), (call(2), 100), (call(4), 100)):
+        assert got["nodes"] == nodes and got["parent_stride"] == 100
