@@ -273,7 +273,7 @@ int qllama_tree_accept(const QTreeAccept *p, void *stream);
 // head is above 32, enter the products, as queries and weights do, as three 16-bit parts
 // that together are exact: what is left out of a product is below 1.001 x 2^-24 of it, as
 // much as rounding it to 32 bits leaves out.  width * page_size and rows * n_heads have to
-// be below 2^31 - 1024.  `nodes` is the number of rows of a request that the call is laid
+// be below 2^31 - 1024, n_req below 2^31 - 4096.  `nodes` is the number of rows of a request that the call is laid
 // out for (0: rows / n_req), the same that qllama_tree_attention_work is asked for; any
 // number of rows is right, other ones are slower.  Rows that no request has are left as they
 // were.  starts outside 0 .. rows count as the nearest inside; a row that two requests name

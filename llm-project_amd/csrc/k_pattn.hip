@@ -848,7 +848,7 @@ extern "C" int qllama_paged_attention(const QPagedKV *c, const QPagedQuery *a, v
   if (a->q_stride < qd || a->o_stride < qd || (a->lse && a->lse_stride < a->n_heads)) return qs::refuse(fn, "a row stride below the row's length");
   if (a->width < 1 || a->table_stride < a->width || (int64_t)a->width * c->page_size > INT_MAX - 64)   // a step past it still fits
     return qs::refuse(fn, "bad table width (width * page_size must be below 2^31 - 64) or stride");
-  if ((int64_t)a->n_req * (((int64_t)a->width * c->page_size + 15) / 16) > INT_MAX)
+  if ((int64_t)a->n_req * (((int64_t)a->width * c->page_size + 15) / 16) > INT_MAX - 4096)      // a step of the loops over requests past it still fits
     return qs::refuse(fn, "n_req * width * page_size is too large");
   if (!(a->scale >= 0.0f) || a->scale > 2.35e38f)      // times log2 e within a float's range
     return qs::refuse(fn, "scale must be 0 .. 2.35e38");

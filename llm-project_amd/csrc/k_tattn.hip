@@ -45,6 +45,7 @@ extern "C" int qllama_tree_attention(const QPagedKV *c, const QTreeQuery *a, voi
   if (a->width < 1 || a->table_stride < a->width || (int64_t)a->width * c->page_size > INT_MAX - 1024)   // a step past it still fits
     return qs::refuse(fn, "bad table width (width * page_size must be below 2^31 - 1024) or stride");
   if ((int64_t)a->rows * a->n_heads > INT_MAX - 1024) return qs::refuse(fn, "rows * n_heads must be below 2^31 - 1024");
+  if (a->n_req > INT_MAX - 4096) return qs::refuse(fn, "n_req is too large (2^31 - 4096 and more)");      // a step of the loops over requests past it still fits
   if (((double)a->rows * a->n_heads + c->n_kv) * a->n_req * ((double)a->width * c->page_size + 512) > 4e18) return qs::refuse(fn, "n_req * rows * width * page_size is too large");
   if (!(a->scale >= 0.0f) || a->scale > 2.35e38f)      // times log2 e within a float's range
     return qs::refuse(fn, "scale must be 0 .. 2.35e38");

@@ -228,3 +228,13 @@ def test_tree_accept_leaves_out_rows_that_the_mask_has_no_bit_for(monkeypatch):
     call = lambda *m: packed(monkeypatch, "tree_accept", lambda: Q.tree_accept(*args, stream=0, **(dict(mask=Tensor(torch.zeros((200, m[0]), dtype=torch.int64))) if m else {})))  # noqa: E731
     for got, nodes in ((call(), 100), (call(1), 64), (call(2), 100), (call(4), 100)):
         assert got["nodes"] == nodes and got["parent_stride"] == 100
+
+
+@pytest.mark.parametrize("n_req", [2 ** 31 - 1, 2 ** 31 - 4096])
+def test_loops_over_requests_stay_in_32_bits(n_req, capfd):
+    """As many requests as a step of 64 or 2048 past them would leave 32 bits: both attentions refuse them."""
+    assert CALLS["query"]({"n_req": n_req, "rows": 1, "n_heads": 2, "width": 1, "table_stride": 1}) != 0
+    assert "n_req" in capfd.readouterr().err
+    c = cache(page_size=1, page_stride=2 * 64, head_stride=64)
+    assert L.qllama_paged_attention(C.byref(c), Q.PAGED_QUERY.pack(n_req, 2, 1, 128, 128, 2, 1, A, B, 0, A, A, 0.0, A, 1 << 40), None) != 0
+    assert "too large" in capfd.readouterr().err
