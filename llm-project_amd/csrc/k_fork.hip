@@ -11,7 +11,7 @@ namespace {
 // Fork
 // ---------------------------------------------------------------------------
 constexpr int kForkThreads = 256, kForkPlanThreads = 1024;
-constexpr int kForkOne = 64;             // requests that one block takes
+constexpr int kForkOne = 64, kForkOneWidth = 256;        // requests, and table entries of each, that one block takes
 
 constexpr int kNoPage = -1, kNoCopy = -2, kRefused = -3;          // the ring names no page, none is needed, none is left
 
@@ -50,10 +50,13 @@ __device__ inline unsigned long long fork_id(const QPagedFork &p, int r, int e) 
 __device__ inline unsigned long long fork_rank(int covered, int i) { return (unsigned long long)covered << 32 | (0xffffffffu - (unsigned)i); }
 
 // The steps of a fork, each over all entries of the requests' tables.  Where there are few
-// requests one block takes all steps, a wave a request at a time; else every step is a launch,
-// with a block a request.  Two requests of up to 700 tokens continued by four each: 8 us in one
-// block, 14 in six launches, whose enqueueing takes the host 15 us more; 512 requests (256 old
-// and new, 40 pages each): more than 100 us in one block, 20 in launches, latencies all.
+// requests with short tables one block takes all steps, a wave a request at a time; else every
+// step is a launch, with a block a request.  One block against six launches, whose enqueueing
+// takes the host 15 us more: 2 old and 2 new requests 8 us against 14 with 16 or 64 pages each,
+// 14 against 14 with 256, 36 against 22 with 1024; 16 and 16 10 against 15, 20 against 16, 55
+// against 23; 32 and 32 17 against 17, 32 against 17, and with 512 55 against 19; 256 and 256 of
+// 40 more than 100 against 20.  How many pages a request has the host does not know, only how
+// many its table has room for.
 // Of what a step hands to the next: in the L2, also within one launch.
 template <typename T>
 __device__ inline T load(const T *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
@@ -460,11 +463,15 @@ extern "C" int qllama_paged_fork(const QPagedFork *p, void *stream) {
   a.freed = a.got + p->n_new;
   a.taken = a.freed + p->n_old;
   const hipStream_t s = (hipStream_t)stream;
-  if (p->n_old == 0 || (p->n_old + p->n_new <= kForkOne && p->n_pages <= 16384)) {
+  const int copy = p->extra_out == p->extra ? 0 : (p->n_pages + kForkThreads - 1) / kForkThreads, clear = copy > 256 ? 256 : copy;
+  if (p->n_old == 0 && copy > 64) {      // more counts than one block should copy
+    QS_LAUNCH(fn, k_fork_clear, dim3(clear), dim3(kForkThreads), 0, s, a);
+    a.p.extra = a.p.extra_out;
+  }
+  if (p->n_old == 0 || (p->n_old + p->n_new <= kForkOne && p->width <= kForkOneWidth && p->n_pages <= 16384)) {
     QS_LAUNCH(fn, k_fork_one, dim3(1), dim3(kForkPlanThreads), 0, s, a);
     return 0;
   }
-  const int copy = p->extra_out == p->extra ? 0 : (p->n_pages + kForkThreads - 1) / kForkThreads, clear = copy > 256 ? 256 : copy;
   QS_LAUNCH(fn, k_fork_clear, dim3(p->n_old > clear ? p->n_old : clear), dim3(kForkThreads), 0, s, a);
   QS_LAUNCH(fn, k_fork_rank, dim3(p->n_old + p->n_new), dim3(kForkThreads), 0, s, a);
   QS_LAUNCH(fn, k_fork_copies, dim3(1), dim3(kForkPlanThreads), 0, s, a);

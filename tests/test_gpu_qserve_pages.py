@@ -270,3 +270,26 @@ def test_moves_out_of_range(Q):  # noqa: F811
     Q.paged_move(kv, dev_i32([1]), dev_i32([2]), starts=dev_i32([1, 0, -4]))           # falling: no moves
     Q.paged_move(kv, i32(0), i32(0))
     assert all(torch.equal(x, y) for x, y in zip(held(kv), before))
+
+
+@pytest.mark.parametrize("width", [256, 257, 1100])
+@pytest.mark.parametrize("new", [3, 70])
+def test_fork_of_long_tables(Q, width, new):  # noqa: F811
+    """Tables on both sides of what one block takes, full or nearly, with a shared beginning."""
+    pool = Pool(5 * width + 80, 2, width)
+    r = pool.r
+    lens = [2 * width - 1, 2 * width - 2, 2 * width - 3, 5]
+    table = [pool.request(lens[0], width)]
+    for t in lens[1:]:
+        table.append(pool.request(t, width, table[0], min(t // 2, width - 9)))
+    ring, state = pool.ring(len(pool.extra), 3)
+    source = [r.choice([0, 0, 1, 2, 3, -1]) for _ in range(new)]
+    check_fork(Q, lens, table, source, [r.randint(0, 2 * width) for _ in range(new)], pool.extra, ring, state, 2, width)
+
+
+def test_fork_of_nothing_over_many_pages(Q):  # noqa: F811
+    """No old request, and more counts to carry over than one block copies."""
+    extra = [(7 * i) % 5 for i in range(100_003)]
+    for in_place in (False, True):
+        got = check_fork(Q, [], [], [0, -1, 3], None, extra, [4, 5, 6], [1, 2], 16, 3, in_place=in_place)
+        assert got["lens"] == [0, 0, 0] and got["extra"] == extra
