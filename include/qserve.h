@@ -308,9 +308,11 @@ size_t qllama_tree_attention_work(const QPagedKV *c, int rows, int n_req, int n_
 //     say what to copy (-1, -1, 0: nothing), for qllama_paged_move without starts.  Of the
 //     new requests that hold such a page, the one with the most of its tokens (the first
 //     of these) keeps it without a copy, if no one outside the call holds it.
-//   * Free pages are taken from the ring's front, request by request.  Request i is refused
-//     (status 3, lens_out 0, nothing held) when the copies that it and all requests before
-//     it ask for, refused ones among them, exceed the free pages at the start.
+//   * Free pages are taken from the ring's front, request by request.  A request that needs a
+//     copy is refused (status 3, lens_out 0, nothing held) when the copies that it and all
+//     requests before it ask for, refused ones among them, exceed the free pages at the
+//     start; one that needs none is never refused.  A page number of the ring outside 0 ..
+//     n_pages - 1 is no page: the request that it falls to has -1 there, and nothing to copy.
 //   * Pages that no one holds any more are put at the ring's back, in the order of the old
 //     rows (a page that several held: where the first of them has it), for later calls.
 //     What does not fit in the ring any more is dropped.
@@ -319,6 +321,12 @@ size_t qllama_tree_attention_work(const QPagedKV *c, int rows, int n_req, int n_
 //     state outside the ring counts as in qllama_paged_plan; lens outside 0 .. width *
 //     page_size as the nearest inside; a table entry outside 0 .. n_pages - 1 is no page:
 //     it is carried over as -1, and not copied.
+//   * What a refused request continued ends with the call, like every old request that
+//     nothing continues, though it was only to be cut back into a page that others hold.  The
+//     old requests are not lost: of the ring only places behind the count at the start change,
+//     so that lens, table, extra (where extra_out is another), state and the ring are valid
+//     as before the call, which can be made again from them with other requests, as long as
+//     its results have not been used.
 // extra_out may be extra; no other output may be one of the inputs.  work:
 // qllama_paged_fork_work bytes, 16-byte aligned.
 typedef struct {

@@ -293,3 +293,54 @@ def test_fork_of_nothing_over_many_pages(Q):  # noqa: F811
     for in_place in (False, True):
         got = check_fork(Q, [], [], [0, -1, 3], None, extra, [4, 5, 6], [1, 2], 16, 3, in_place=in_place)
         assert got["lens"] == [0, 0, 0] and got["extra"] == extra
+
+
+@pytest.mark.parametrize("old,new,page,most", [(4, 9, 8, 60), (40, 70, 4, 50), (3, 20, 16, 5000)])
+def test_fork_without_free_pages(Q, old, new, page, most):  # noqa: F811
+    """Nothing is copied or taken; who would need a copy is refused, the others keep their source's pages, and what is written next
+    lies on a page of one request alone."""
+    width = -(-most // page) + 1
+    pool = Pool(old * width, page, old)
+    r = pool.r
+    lens = [r.randint(page, most) for _ in range(old)]
+    table = [pool.request(lens[0], width)]
+    for t in lens[1:]:
+        table.append(pool.request(t, width, table[0], r.randint(0, min(t, lens[0]) // page)))
+    source, keep = [r.randrange(old) for _ in range(new)], [r.randint(0, 2 * most) for _ in range(new)]
+    tokens = [min(keep[i], lens[s]) for i, s in enumerate(source)]
+    ring, state = pool.ring(len(pool.extra), 2)
+    got = fork_run(Q, lens, table, source, keep, pool.extra, ring, [state[0], 0], page, width)
+    assert got["src"] == [-1] * new and got["dst"] == [-1] * new and got["count"] == [0] * new and got["state"][0] == state[0]
+    assert got["status"].count(3) > 0 and got["status"].count(0) > 0 and set(got["status"]) == {0, 3}
+    held = {}
+    for i, (s, t, status, n) in enumerate(zip(source, tokens, got["status"], got["lens"])):
+        assert n == (0 if status else t)
+        for e in range(-(-n // page)):
+            assert got["table"][i][e] == table[s][e]
+            held[table[s][e]] = held.get(table[s][e], 0) + 1
+        if status:
+            assert t % page, "a request that writes to no page that it holds needs no copy"
+    assert all(held[table[s][n // page]] == 1 for s, n in zip(source, got["lens"]) if n % page)
+    assert all(got["extra"][p] == n - 1 for p, n in held.items())
+
+
+@pytest.mark.parametrize("new", [9, 70])
+def test_a_fork_that_was_refused_is_made_again(Q, new):  # noqa: F811
+    """From the same lengths, table, counts and state, and the ring as the refused call has left it."""
+    page, width, old = 8, 12, 6
+    pool = Pool(old * width, page, new)
+    r = pool.r
+    lens = [r.randint(18, 90) for _ in range(old)]
+    table = [pool.request(t, width) for t in lens]
+    ring, state = pool.ring(len(pool.extra) + 5, 4)
+    state = [state[0], 3]
+    source, keep = [i % 3 for i in range(new)], [r.choice([3, 10, 17]) for _ in range(new)]
+    got = check_fork(Q, lens, table, source, keep, pool.extra, ring, state, page, width)
+    assert 3 in got["status"] and got["ring"] != ring
+    fewer = [i if i < old else -1 for i in range(new)]
+    again = check_fork(Q, lens, table, fewer, None, pool.extra, got["ring"], state, page, width)
+    assert again["lens"] == lens + [0] * (new - old) and again["status"] == [0] * new and again["state"] == state
+    assert [row[:-(-t // page)] for row, t in zip(again["table"], lens)] == [row[:-(-t // page)] for row, t in zip(table, lens)]
+    one = check_fork(Q, lens, table, [0, 0, 1, 1, 2, 2], [17] * 6, pool.extra, got["ring"], state, page, width)
+    assert one["status"] == [0] * 6 and one["dst"].count(-1) == 3
+    assert sorted(d // page for d in one["dst"] if d >= 0) == sorted(pool.free[:3])
