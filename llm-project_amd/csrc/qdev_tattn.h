@@ -521,7 +521,7 @@ __global__ __launch_bounds__((Cfg<T, HDP, CG, KP>::THREADS), 2) void k_tree_attn
 #pragma unroll
       for (int i = 0; i < SUB; i++) d[i] = f4{0, 0, 0, 0};
 #pragma unroll
-      for (int y = 0; y < C::PLANES; y++) {
+      for (int y = C::PLANES - 1; y >= 0; y--) {      // the smallest products first: their sums round to less
         u4 kf[C::QC][SUB];
 #pragma unroll
         for (int c = 0; c < C::QC; c++)
@@ -539,7 +539,7 @@ __global__ __launch_bounds__((Cfg<T, HDP, CG, KP>::THREADS), 2) void k_tree_attn
                 d[i] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kf[c][i][e]), __uint_as_float(qp[c][0][e]), d[i], 0, 0, 0);
             } else {
 #pragma unroll
-              for (int p = 0; p < C::PARTS - y; p++) d[i] = mfma16<C::LT>(kf[c][i], qp[c][p], d[i]);
+              for (int p = 0; p < C::PARTS - y; p++) d[i] = mfma16<C::LT>(kf[c][i], qp[c][C::SPLIT ? C::PARTS - 1 - y - p : p], d[i]);
             }
           }
       }

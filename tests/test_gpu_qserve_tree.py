@@ -409,6 +409,15 @@ def test_f32_products_of_few_columns_are_rounded_once(Q, hd, nodes):  # noqa: F8
     off = alone(Q, k, q, hd, nodes) / (k.double()[..., None] * q.double() * LN2) - 1
     assert float(off.abs().max()) <= 2 * EPS * (1 + EPS), off.abs().max() / EPS
 
+@pytest.mark.parametrize("hd,nodes", [(64, 5), (64, 64), (72, 8), (128, 5), (128, 64)])
+def test_f32_products_of_parts_add_up_from_the_smallest(Q, hd, nodes):  # noqa: F811
+    """A product of parts leaves out 1.001 x 2^-24; its small products sum up to 2^-6.9 of it, so that five roundings of them
+    take 0.05 x 2^-24; the largest product, added last, takes one of 2^-24, and ln 2 another.  (From the largest on: six.)"""
+    g = torch.Generator().manual_seed(hd + nodes)
+    k, q = torch.randn((8, 64), generator=g), torch.randn((8, 64, 8), generator=g)
+    off = alone(Q, k, q, hd, nodes) / (k.double()[..., None] * q.double() * LN2) - 1
+    assert float(off.abs().max()) <= 3.06 * EPS, off.abs().max() / EPS
+
 @pytest.mark.parametrize("hd", [64, 128])
 def test_f32_weights_are_as_close_as_32_bits(Q, hd):  # noqa: F811
     """All values of a request are alike, so that o = v whatever the weights are.  Weights that are cut make every product 2^-25.5
