@@ -35,9 +35,10 @@
 //   32 of them, up to 16 rows                                  72 us      3.0 TB/s
 //   32 of them, up to 32 rows                                  89 us      2.0 TB/s, 570 TFLOP/s in parts
 //   32 of them, up to 64 rows                                  162 us     700 TFLOP/s in parts
-//   2 requests of up to 60000 tokens, f16, 48 rows             120-130 us 2.7 TB/s, 400 TFLOP/s in parts
+//   2 requests of up to 60000 tokens, f16, 48 rows             117-127 us 2.8 TB/s, 410 TFLOP/s in parts
 //   64 requests of up to 4100 tokens, int8, 7 rows             101-114 us 2.6 TB/s
-//   6 requests of up to 2048 tokens, f32, heads of 64, 200 rows in a chain  106-113 us  680 TFLOP/s in parts
+//   6 requests of up to 2048 tokens, f32, heads of 64, 200 rows in a chain  114-125 us  630 TFLOP/s in parts
+//   the same, heads of 128, bf16 117 us, f16 106, int8 119      640, 480, 630 TFLOP/s in parts
 //   1 request of 2060 tokens, bf16, 8 rows                     22 us
 // Measured and not kept: 32 columns a wave (queries and sums of both spill: 225 us against 144 at
 // 32 rows); blocks of eight waves whatever the columns, on other parts of a step's keys, that
