@@ -559,8 +559,9 @@ __global__ __launch_bounds__((Cfg<T, HDP, CG, KP>::THREADS), 2) void k_tree_attn
         for (int i = 0; i < SUB; i++) d[i] *= unscale;
       }
       const uint32_t none = __builtin_amdgcn_readfirstlane((uint32_t)(gone[(s & 3) * KP + part] >> (t * C::KEYS)) & (C::KEYS == 32 ? ~0u : 0xffffu));
+      uint32_t seen = ~0u;
       if (none != 0 || key0 + C::KEYS > ctx) {        // one for the wave
-        const uint32_t seen = seen_of(a, row, row - first, key0 - ctx) & ~none;
+        seen = seen_of(a, row, row - first, key0 - ctx) & ~none;
 #pragma unroll
         for (int i = 0; i < SUB; i++)
 #pragma unroll
@@ -571,20 +572,20 @@ __global__ __launch_bounds__((Cfg<T, HDP, CG, KP>::THREADS), 2) void k_tree_attn
             }
       }
       if constexpr (C::SPLIT) {
-        // parts of an infinity, or of products that leave a float's range, make a score NaN that may be an infinity: such scores
-        // one by one, for a column that is not NaN anyway
+        // parts of an infinity, or whose products leave a float's range, give a NaN or an infinity for what may be none: such
+        // scores one by one, for a column that is not NaN already
         float all = 0.0f;
 #pragma unroll
         for (int i = 0; i < SUB; i++)
 #pragma unroll
           for (int j = 0; j < 4; j++) all += d[i][j];
-        if (__any(all != all && sum == sum)) {
+        if (__any(all - all != 0.0f && sum == sum)) {
           const float *q = a.q + row * a.q_stride + (long long)head * a.hd;
 #pragma unroll
           for (int i = 0; i < SUB; i++)
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-              if (d[i][j] == d[i][j] || sum != sum) continue;          // a score that is left is a key's
+              if (d[i][j] - d[i][j] == 0.0f || sum != sum || !(seen >> (16 * i + 4 * g + j) & 1)) continue;
               const float *k = reinterpret_cast<const float *>(kbase + offs[((s & 3) * KP + part) * KS + t * C::KEYS + 16 * i + 4 * g + j]);
               float x = 0.0f;
 #pragma unroll 1

@@ -438,6 +438,16 @@ def test_f32_weights_are_as_close_as_32_bits(Q, hd):  # noqa: F811
     assert abs(float(off.mean())) <= EPS / 8, off.mean() / EPS
 
 
+@pytest.mark.parametrize("hd,nodes", [(64, 1), (64, 64), (128, 64), (64, 5)])
+def test_f32_products_at_the_end_of_the_range(Q, hd, nodes):  # noqa: F811
+    """1.998 x 1.7e38 is a 32-bit number, 2 x 2^127, which the first parts are rounded to, is not; likewise the largest number
+    times 1.  The scores of either sign come out, with the roundings of any other product (one more of each sum)."""
+    most = float(torch.finfo(torch.float32).max)
+    k = torch.tensor([1.7e38, -1.7e38, most, -most, 1.0, 2.0 ** 127, 3.3e38, -3e38]).repeat(8)[None]
+    q = torch.tensor([1.998, 1.998, 1.0, 1.0, 1.7e38, 1.99, 1.03, 1.1]).repeat(8)[None, :, None].repeat(1, 1, 8)
+    off = alone(Q, k, q, hd, nodes) / (k.double()[..., None] * q.double() * LN2) - 1
+    assert float(off.abs().max()) <= 7 * EPS
+
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("nodes", [1, 11, 40])
 def test_an_infinite_f32_key(Q, hd, nodes):  # noqa: F811
