@@ -490,3 +490,21 @@ def test_no_row_behind_the_mask_is_accepted(Q):  # noqa: F811
         Q.tree_accept(starts, lens, par, dev_i32([5] * m), dev_i32([5] * m), dev_i32(list(range(m))), *out, *rows, mask=mask)
         assert [x.get().item() for x in out] == [want, 5, 200 + want]
         assert rows[0].get().tolist() == list(range(want)) + [-1] * (m - want) and rows[1].get().tolist() == [-1] * m
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_f32_values_in_parts_that_are_not_finite(Q, hd, bad):  # noqa: F811
+    """Of an earlier token, alone in its step and beside new ones: no row has a number at that dim, and the others stay."""
+    kv, q, starts, table, lens, seen, mask = case("f32", 4, 2, hd, 16, "head", [700], [40], 1, 3, Q, "tree")
+    clean, _ = attend(Q, kv, q, starts, widened(table, 16), lens, mask)
+    for at in (20, 657):
+        keep = kv.v.get()
+        x = keep.clone()
+        x[int(table[0, at // 16]), 1, at % 16, 5] = bad
+        kv.v.set(x)
+        o, lse = attend(Q, kv, q, starts, widened(table, 16), lens, mask)
+        kv.v.set(keep)
+        assert not bool(torch.isfinite(o[:, 2:, 5]).any()) and bool(torch.isfinite(lse).all())
+        o[:, 2:, 5] = clean[:, 2:, 5]
+        assert torch.equal(o, clean)
