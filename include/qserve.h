@@ -247,9 +247,9 @@ int qllama_tree_plan(const QTreePlan *p, void *stream);
 // of row k), else -1: groups of qllama_paged_move, with starts as they are.  Rows that no
 // request has are left as they were.  Rows behind the first `nodes` follow none and are not
 // accepted: where the rows attended with a mask, nodes has to be 64 * words at most (the
-// stride as it is), as what was chosen behind the other rows is no one's choice.  Every
-// request of a call is verified: rows that are certain (a piece of a prompt) go without
-// this call, in a step of their own, or have their next row's token in chosen.
+// stride as it is), as the rows behind those have attended to nothing new.  Every request of
+// a call is verified: rows that are certain (a piece of a prompt) go without this call, in a
+// step of their own, or have their next row's token in chosen.
 typedef struct {
   int n_req, nodes, max_rows;                // as QTreePlan's
   int64_t parent_stride;
@@ -273,11 +273,12 @@ int qllama_tree_accept(const QTreeAccept *p, void *stream);
 // head is above 32, enter the products, as queries and weights do, as three 16-bit parts
 // that together are exact: what is left out of a product is below 1.001 x 2^-24 of it, as
 // much as rounding it to 32 bits leaves out.  width * page_size and rows * n_heads have to
-// be below 2^31 - 1024, n_req below 2^31 - 4096.  `nodes` is the number of rows of a request that the call is laid
-// out for (0: rows / n_req), the same that qllama_tree_attention_work is asked for; any
-// number of rows is right, other ones are slower.  Rows that no request has are left as they
-// were.  starts outside 0 .. rows count as the nearest inside; a row that two requests name
-// gets either result.  work: qllama_tree_attention_work bytes, 16-byte aligned.
+// be below 2^31 - 1024, n_req below 2^31 - 4096.  `nodes` is the number of rows of a request
+// that the call is laid out for (0: rows / n_req), the same that qllama_tree_attention_work
+// is asked for; any number of rows is right, other ones are slower.  Rows that no request
+// has are left as they were.  starts outside 0 .. rows count as the nearest inside; a row
+// that two requests name gets either result.  work: qllama_tree_attention_work bytes,
+// 16-byte aligned.
 typedef struct {
   int rows;                 // of q, o, lse and mask
   int n_req, n_heads, width, words, nodes;

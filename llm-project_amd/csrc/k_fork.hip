@@ -52,11 +52,11 @@ __device__ inline unsigned long long fork_rank(int covered, int i) { return (uns
 // The steps of a fork, each over all entries of the requests' tables.  Where there are few
 // requests with short tables one block takes all steps, a wave a request at a time; else every
 // step is a launch, with a block a request.  One block against six launches, whose enqueueing
-// takes the host 15 us more: 2 old and 2 new requests 8 us against 14 with 16 or 64 pages each,
-// 14 against 14 with 256, 36 against 22 with 1024; 16 and 16 10 against 15, 20 against 16, 55
-// against 23; 32 and 32 17 against 17, 32 against 17, and with 512 55 against 19; 256 and 256 of
-// 40 more than 100 against 20.  How many pages a request has the host does not know, only how
-// many its table has room for.
+// takes the host 15 us more, us with 16, 256 and 1024 pages each: 2 old and 2 new requests 8
+// against 14, 14 against 14, 36 against 22; 16 and 16 10 against 15, 20 against 16, 55 against 23;
+// 32 and 32 17 against 17, 32 against 17 (with 512: 55 against 19); 256 and 256 with 40 more than
+// 100 against 20.  How many pages a request has the host does not know, only how many its table
+// has room for.
 // Of what a step hands to the next: in the L2, also within one launch.
 template <typename T>
 __device__ inline T load(const T *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }

@@ -37,7 +37,7 @@
 //   32 of them, up to 64 rows                                  162 us     700 TFLOP/s in parts
 //   2 requests of up to 60000 tokens, f16, 48 rows             117-127 us 2.8 TB/s, 410 TFLOP/s in parts
 //   64 requests of up to 4100 tokens, int8, 7 rows             101-114 us 2.6 TB/s
-//   6 requests of up to 2048 tokens, f32, heads of 64, 200 rows in a chain  114-125 us  630 TFLOP/s in parts
+//   6 requests of up to 2048 tokens, f32, heads of 64, 200 rows in a chain  114-128 us  620 TFLOP/s in parts
 //   the same, heads of 128, bf16 117 us, f16 106, int8 119      640, 480, 630 TFLOP/s in parts
 //   1 request of 2060 tokens, bf16, 8 rows                     22 us
 // Measured and not kept: 32 columns a wave (queries and sums of both spill: 225 us against 144 at
@@ -176,7 +176,7 @@ __device__ inline bool odd_value(uint32_t x) {
 }
 
 // 8 floats as sums of three bf16 numbers, each rounded to nearest: exact, the second at most 2^-8 and the third 2^-17 of the
-// first.  ANY: the first has to be kept within bf16's range, which ends 2^-9 below a float's.
+// first.  ANY: the first has to be kept within bf16's range, which ends 2^-8 below a float's.
 typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
 template <bool ANY>
 __device__ inline Parts3 round3(const float (&x)[8]) {
@@ -197,6 +197,7 @@ __device__ inline Parts3 round3(const float (&x)[8]) {
   }
   return r;
 }
+
 // The dim of a head whose output is element c of an accumulator's row `lane` of 16.
 template <typename C>
 __device__ inline int dim_of(int c, int lane) { return C::F32 ? 64 * (c / 4) + 4 * lane + c % 4 : 16 * c + lane; }
